@@ -20,6 +20,7 @@ import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
 LIB_PATH = Path(os.environ.get("CCQ_LIB", Path(__file__).resolve().parent / "_lib" / "libccq_hip.so"))
 
 CCQ_F32, CCQ_F16, CCQ_BF16 = 0, 1, 2
+CCQ_Q_NONE, CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW = 0, 1, 2  # 8-bit row formats of ccq_rms_norm
 CCQ_EINVAL, CCQ_EUNSUPPORTED, CCQ_EWORKSPACE = -1, -2, -3
 CCQ_MOE_W4_NOALLOC_BYTES = 32 << 20  # the per-GPU scratch array of ccq_moe_w4_forward_noalloc
 
@@ -58,6 +59,14 @@ class ccq_fp8row_experts(ctypes.Structure):
         ("w_up", _vp), ("s_up", _vp),
         ("w_down", _vp), ("s_down", _vp),
         ("num_experts", _i64), ("hidden", _i64), ("inter", _i64),
+    ]
+
+
+class ccq_lora_adapters(ctypes.Structure):
+    _fields_ = [
+        ("a", _vp), ("b", _vp), ("scale", _vp), ("rank", _vp),
+        ("dtype", _int),
+        ("num_adapters", _i64), ("rank_max", _i64), ("in_features", _i64), ("out_features", _i64),
     ]
 
 
@@ -131,6 +140,12 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_fp8_block_dequant": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "ccq_fp8_block_linear_workspace_size": (_sz, [_i64, _i64]),
     "ccq_fp8_block_linear": (_int, [_vp, _int, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "ccq_fp8_block_linear_quantized": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
+    "ccq_rms_norm": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _int, ctypes.c_float, _vp, _i64, _vp, _int, _int, _vp,
+                            _vp, _i64, _i64, _vp]),
+    "ccq_lora_workspace_size": (_sz, [_i64, ctypes.POINTER(ccq_lora_adapters)]),
+    "ccq_lora_add": (_int, [_vp, _int, _i64, _vp, _vp, _int, _i64, _i64, ctypes.POINTER(ccq_lora_adapters), _vp, _sz,
+                            _vp]),
     "ccq_moe_fp8_workspace_size": (_sz, [_i64, _i64, ctypes.POINTER(ccq_fp8_experts)]),
     "ccq_moe_fp8_ffn": (_int, [_vp, _int, _vp, _vp, _vp, _int, _i64, _i64,
                                ctypes.POINTER(ccq_fp8_experts), _vp, _sz, _vp]),

@@ -25,7 +25,7 @@ from ccut._lib import call, lib
 
 BLOCK = 128
 
-__all__ = ["act_quant", "Fp8BlockWeights", "prepare", "unpack", "dequant", "linear"]
+__all__ = ["act_quant", "Fp8BlockWeights", "prepare", "unpack", "dequant", "linear", "linear_quantized"]
 
 
 def act_quant(x) -> tuple[torch.Tensor, torch.Tensor]:
@@ -128,3 +128,32 @@ def linear(weight, s_w, x, out_dtype: torch.dtype | None = None):
          y.data_ptr(), _dev.DTYPE_CODE[od], M, w.K, w.N, ws.data_ptr() if ws is not None else None, nbytes,
          _dev.stream_ptr(xd.device))
     return _dev.to_host(y) if host else y
+
+
+def linear_quantized(weight: Fp8BlockWeights, q: torch.Tensor, s: torch.Tensor,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`linear` on rows that are quantized already: ``q [..., K]`` e4m3
+    codes (uint8 or float8_e4m3fn) and ``s [..., K/128]`` float32 on the
+    device, from :func:`act_quant` or ``blocks.norm.rms_norm_fp8``."""
+    if q.dtype not in (torch.uint8, torch.float8_e4m3fn) or s.dtype != torch.float32:
+        raise ValueError(f"linear_quantized needs uint8 or float8_e4m3fn codes and float32 scales, got {q.dtype} "
+                         f"and {s.dtype}")
+    if out_dtype not in _dev.DTYPE_CODE:
+        raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    K = weight.K
+    if q.dim() < 1 or q.shape[-1] != K or tuple(s.shape) != (*q.shape[:-1], K // BLOCK):
+        raise ValueError(f"codes {tuple(q.shape)} and scales {tuple(s.shape)} must be [..., {K}] and "
+                         f"[..., {K // BLOCK}]")
+    if q.device != weight.w_tiled.device or s.device != q.device:
+        raise ValueError(f"codes on {q.device}, scales on {s.device}, weight on {weight.w_tiled.device}")
+    stream = _dev.stream_ptr(q.device)
+    if q.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return linear_quantized(weight, q, s, out_dtype)
+    q, s = q.contiguous(), s.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    y = torch.empty((*q.shape[:-1], weight.N), dtype=out_dtype, device=q.device)
+    call("ccq_fp8_block_linear_quantized", q.data_ptr(), s.data_ptr(), weight.w_tiled.data_ptr(),
+         weight.s_w.data_ptr(), y.data_ptr(), _dev.DTYPE_CODE[out_dtype], q.numel() // K, K, weight.N, stream)
+    return y

@@ -174,9 +174,19 @@ class LinearProj:
         self._w32 = w
         return w
 
-    def apply(self, x):
+    def apply(self, x, adapters=None, index=None):
         """``x [batch, in] @ W.T -> [batch, out]`` float32 (numpy in, numpy
-        out; a device tensor in, a device tensor out)."""
+        out; a device tensor in, a device tensor out).  With ``adapters``
+        (``quant.lora.LoraAdapters`` of this projection) and ``index [batch]``
+        (each row's adapter, negative for none), each row's low-rank product
+        is added to it."""
+        if (adapters is None) != (index is None):
+            raise ValueError(f"{self.name}: adapters and index come together")
+        if adapters is not None:
+            from ccut.quant import lora
+
+            xd = _f32_input(x) if _dev.is_host(x) else x
+            return _return(lora.add_(self.apply(xd), xd, adapters, _dev.to_device(index, torch.int64)), x)
         self._load()
         if self._method is None:
             return _return(f32_linear(_f32_input(x), self._w32), x)

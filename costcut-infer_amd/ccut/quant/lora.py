@@ -1,0 +1,138 @@
+"""Low-rank adapters of many requests at once beside one shared projection
+(``ccq_lora_add``): ``y[t] += scale[i] * B_i (A_i x[t])`` with ``i =
+index[t]``, in place on the projection's output -- ``awq.gemm``,
+``fp8_block.linear``, ``int8.int8_linear`` or ``LinearProj.apply`` (which
+takes the adapters itself).  Rows without an adapter are left as they are.
+Products and sums are float32 and y is rounded once.  The reference serves
+one request at a time and has no counterpart."""
+
+from __future__ import annotations
+
+import torch
+
+from ccut import _dev
+from ccut._lib import call, ccq_lora_adapters, lib
+
+__all__ = ["LoraAdapters", "add_"]
+
+MAX_ADAPTERS, MAX_RANK, MAX_TOKENS = 1024, 256, 65536
+
+
+class LoraAdapters:
+    """The adapters of one projection, stacked on the device: ``a [L, R, in]``
+    and ``b [L, out, R]`` (float16 or bfloat16), ``scale [L]`` (float32; None:
+    1 each), ``rank [L]`` (int32; None: R each) -- the ranks of an adapter
+    from ``rank[i]`` on are padding and are not read.  Dense tensors are
+    referred to as they are, so an adapter can be replaced in place (on the
+    stream that uses them); others are copied once."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale=None, rank=None):
+        if not a.is_cuda:
+            raise ValueError(f"Expected a cuda device, but got: {a.device}")
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"adapters must be a [L, R, in] and b [L, out, R], got {tuple(a.shape)} and "
+                             f"{tuple(b.shape)}")
+        if a.dtype != b.dtype or a.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"adapters must both be float16 or bfloat16, got {a.dtype} and {b.dtype}")
+        L, R, K = a.shape
+        if not (1 <= L <= MAX_ADAPTERS and 1 <= R <= MAX_RANK and K >= 1 and b.shape[1] >= 1):
+            raise ValueError(f"adapters a {tuple(a.shape)}, b {tuple(b.shape)}: need 1 to {MAX_ADAPTERS} adapters of "
+                             f"rank 1 to {MAX_RANK}, in and out at least 1")
+        scale = self._vector(scale, torch.float32, L, a.device, "scale")
+        rank = self._vector(rank, torch.int32, L, a.device, "rank")
+        if b.device != a.device:
+            raise ValueError(f"a on {a.device}, b on {b.device}")
+        self.a, self.b, self.scale, self.rank = a.contiguous(), b.contiguous(), scale, rank
+        self.num_adapters, self.rank_max, self.in_features, self.out_features = L, R, K, b.shape[1]
+        self.device = a.device
+        self._desc = ccq_lora_adapters(self.a.data_ptr(), self.b.data_ptr(),
+                                       scale.data_ptr() if scale is not None else None,
+                                       rank.data_ptr() if rank is not None else None, _dev.DTYPE_CODE[a.dtype],
+                                       L, R, K, b.shape[1])
+        self._bytes: dict[int, int] = {}
+
+    @staticmethod
+    def _vector(v, dtype: torch.dtype, L: int, device, what: str) -> torch.Tensor | None:
+        if v is None:
+            return None
+        t = v if isinstance(v, torch.Tensor) else torch.as_tensor(v)
+        if tuple(t.shape) != (L,):
+            raise ValueError(f"{what} must have one entry per adapter ({L}), got {tuple(t.shape)}")
+        return t.to(device=device, dtype=dtype).contiguous()
+
+    def workspace_size(self, T: int) -> int:
+        n = self._bytes.get(T)
+        if n is None:
+            n = self._bytes[T] = int(lib().ccq_lora_workspace_size(T, self._desc))
+        return n
+
+
+def _rows(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
+    if t.dtype not in _dev.DTYPE_CODE:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{what} must be [..., {width}], got {tuple(t.shape)}")
+    return t if t.dim() == 2 else t.reshape(-1, width)
+
+
+def _dense_rows(t: torch.Tensor) -> bool:
+    return t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) or t.numel() == 0
+
+
+def _overlap(y: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether rows of y and x share memory (column ranges of one buffer do
+    not, though their address ranges cross)."""
+    ye, xe = y.element_size(), x.element_size()
+    y0, x0 = y.data_ptr(), x.data_ptr()
+    T = y.shape[0]
+    yl, xl = (y.stride(0) * ye, x.stride(0) * xe) if T > 1 else (0, 0)
+    yw, xw = y.shape[1] * ye, x.shape[1] * xe
+    if y0 >= x0 + (T - 1) * xl + xw or x0 >= y0 + (T - 1) * yl + yw:
+        return False
+    if T <= 1 or yl != xl:
+        return True
+    d = (x0 - y0) % yl  # x's columns start d bytes behind y's in a row of the buffer
+    return d < yw or d + xw > yl
+
+
+def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.Tensor) -> torch.Tensor:
+    """``y[t] += scale[i] * (x[t] @ a[i].T) @ b[i].T`` with ``i = index[t]``,
+    in place; returns ``y``.  ``y [..., out]`` and ``x [..., in]`` (float32,
+    float16 or bfloat16 each, rows dense but with any row stride) and ``index
+    [...]`` (int64; other whole numbers are converted) are device tensors with
+    the same leading dimensions, at most 65536 rows.  An index outside [0, L)
+    means no adapter: that row is left as it is.  ``y`` must not overlap
+    ``x``.  Repeated calls give the same bits (no atomics)."""
+    stream = _dev.stream_ptr(y.device)
+    if y.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(y.device):
+            return add_(y, x, adapters, index)
+    dev = y.device
+    if x.device != dev or index.device != dev or adapters.device != dev:
+        raise ValueError(f"y on {dev}, x on {x.device}, index on {index.device}, adapters on {adapters.device}")
+    if x.shape[:-1] != y.shape[:-1] or index.shape != y.shape[:-1]:
+        raise ValueError(f"leading dimensions of y {tuple(y.shape)}, x {tuple(x.shape)} and index "
+                         f"{tuple(index.shape)} differ")
+    y2, x2 = _rows(y, adapters.out_features, "y"), _rows(x, adapters.in_features, "x")
+    if y2.data_ptr() != y.data_ptr() or not _dense_rows(y2):
+        raise ValueError("y must hold its rows one after the other, each of them dense (it is written in place)")
+    if not _dense_rows(x2):
+        x2 = x2.contiguous()
+    if index.dtype != torch.int64 or not index.is_contiguous():
+        if index.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+            raise ValueError(f"index must hold whole numbers, got {index.dtype}")
+        index = index.to(torch.int64).contiguous()
+    T = y2.shape[0]
+    if T > MAX_TOKENS:
+        raise ValueError(f"{T} rows: at most {MAX_TOKENS}")
+    if T == 0:
+        return y
+    if _overlap(y2, x2):
+        raise ValueError("y overlaps x")
+    nbytes = adapters.workspace_size(T)
+    # this call's own scratch, so that calls on several streams or in several graphs do not share it
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    call("ccq_lora_add", x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype], x2.stride(0) if T > 1 else x2.shape[1],
+         index.data_ptr(), y2.data_ptr(), _dev.DTYPE_CODE[y2.dtype], y2.stride(0) if T > 1 else y2.shape[1], T,
+         adapters._desc, ws.data_ptr(), nbytes, stream)
+    return y

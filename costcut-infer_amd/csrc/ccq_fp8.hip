@@ -1224,32 +1224,28 @@ extern "C" size_t ccq_fp8_block_linear_workspace_size(int64_t M, int64_t K) {
   return lin_layout(M, K).total;
 }
 
-extern "C" int ccq_fp8_block_linear(const void* x, int x_dtype, const uint8_t* w_tiled, const float* s_w, void* y,
-                                    int y_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  CCQ_REQUIRE(M >= 0 && K >= 0 && N >= 0, "ccq_fp8_block_linear: negative shape");
-  CCQ_REQUIRE(K % 128 == 0 && N % 128 == 0, "ccq_fp8_block_linear: need K %% 128 == 0 and N %% 128 == 0 (K=%lld N=%lld)",
+namespace {
+int check_block_linear(const char* name, const uint8_t* w_tiled, const float* s_w, const void* y, int y_dtype,
+                       int64_t M, int64_t K, int64_t N, bool& empty) {
+  CCQ_REQUIRE(M >= 0 && K >= 0 && N >= 0, "%s: negative shape", name);
+  CCQ_REQUIRE(K % 128 == 0 && N % 128 == 0, "%s: need K %% 128 == 0 and N %% 128 == 0 (K=%lld N=%lld)", name,
               (long long)K, (long long)N);
-  CCQ_REQUIRE(x_dtype == CCQ_F32 || x_dtype == CCQ_F16 || x_dtype == CCQ_BF16, "ccq_fp8_block_linear: bad x_dtype");
-  CCQ_REQUIRE(y_dtype == CCQ_F32 || y_dtype == CCQ_F16 || y_dtype == CCQ_BF16, "ccq_fp8_block_linear: bad y_dtype");
-  CCQ_REQUIRE(cdiv(M, F8_BM) * (N / 128) <= 0x7fffffff, "ccq_fp8_block_linear: M or N too large");
-  CCQ_REQUIRE(K == 0 || K >= 256, "ccq_fp8_block_linear: K=%lld < 256 (the kernel pipelines two 128-blocks)",
+  CCQ_REQUIRE(y_dtype == CCQ_F32 || y_dtype == CCQ_F16 || y_dtype == CCQ_BF16, "%s: bad y_dtype", name);
+  CCQ_REQUIRE(cdiv(M, F8_BM) * (N / 128) <= 0x7fffffff, "%s: M or N too large", name);
+  CCQ_REQUIRE(K == 0 || K >= 256, "%s: K=%lld < 256 (the kernel pipelines two 128-blocks)", name, (long long)K);
+  CCQ_REQUIRE(M * K < (int64_t)1 << 32, "%s: activations of %lld x %lld exceed 4 GiB", name, (long long)M,
               (long long)K);
-  CCQ_REQUIRE(M * K < (int64_t)1 << 32, "ccq_fp8_block_linear: activations of %lld x %lld exceed 4 GiB",
-              (long long)M, (long long)K);
-  if (M == 0 || N == 0) return 0;
-  CCQ_REQUIRE(K > 0, "ccq_fp8_block_linear: K == 0");
-  CCQ_REQUIRE(x && w_tiled && s_w && y, "ccq_fp8_block_linear: null pointer");
-  CCQ_REQUIRE(aligned(w_tiled, 16), "ccq_fp8_block_linear: w_tiled must be 16-byte aligned");
-  const LinLayout L = lin_layout(M, K);
-  CCQ_REQUIRE(workspace && workspace_bytes >= L.total && aligned(workspace, 256),
-              "ccq_fp8_block_linear: workspace of %zu bytes (256-byte aligned) needed, %zu given", L.total,
-              workspace_bytes);
-  hipStream_t st = as_stream(stream);
-  uint8_t* q = (uint8_t*)workspace + L.off_q;
-  float* s = (float*)((char*)workspace + L.off_s);
-  int rc = launch_act_quant(x, x_dtype, K, M, K, q, K, s, K / 128, st);
-  if (rc) return rc;
+  empty = M == 0 || N == 0;
+  if (empty) return 0;
+  CCQ_REQUIRE(K > 0, "%s: K == 0", name);
+  CCQ_REQUIRE(w_tiled && s_w && y, "%s: null pointer", name);
+  CCQ_REQUIRE(aligned(w_tiled, 16), "%s: w_tiled must be 16-byte aligned", name);
+  return 0;
+}
+
+// y = dequant(q, s) @ W^T on checked arguments
+int block_linear_gemm(const uint8_t* q, const float* s, const uint8_t* w_tiled, const float* s_w, void* y,
+                      int y_dtype, int64_t M, int64_t K, int64_t N, hipStream_t st) {
   Fp8GP p = {};
   p.a = q;
   p.lda = K;
@@ -1267,6 +1263,39 @@ extern "C" int ccq_fp8_block_linear(const void* x, int x_dtype, const uint8_t* w
   p.KB = (int)(K / 128);
   p.tiles = (int)cdiv(M, F8_BM);
   return launch_fp8_gemm<F8_STORE>(p, p.tiles, st);
+}
+}  // namespace
+
+extern "C" int ccq_fp8_block_linear(const void* x, int x_dtype, const uint8_t* w_tiled, const float* s_w, void* y,
+                                    int y_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  CCQ_REQUIRE(x_dtype == CCQ_F32 || x_dtype == CCQ_F16 || x_dtype == CCQ_BF16, "ccq_fp8_block_linear: bad x_dtype");
+  bool empty = false;
+  if (int rc = check_block_linear("ccq_fp8_block_linear", w_tiled, s_w, y, y_dtype, M, K, N, empty)) return rc;
+  if (empty) return 0;
+  CCQ_REQUIRE(x, "ccq_fp8_block_linear: null pointer");
+  const LinLayout L = lin_layout(M, K);
+  CCQ_REQUIRE(workspace && workspace_bytes >= L.total && aligned(workspace, 256),
+              "ccq_fp8_block_linear: workspace of %zu bytes (256-byte aligned) needed, %zu given", L.total,
+              workspace_bytes);
+  hipStream_t st = as_stream(stream);
+  uint8_t* q = (uint8_t*)workspace + L.off_q;
+  float* s = (float*)((char*)workspace + L.off_s);
+  int rc = launch_act_quant(x, x_dtype, K, M, K, q, K, s, K / 128, st);
+  if (rc) return rc;
+  return block_linear_gemm(q, s, w_tiled, s_w, y, y_dtype, M, K, N, st);
+}
+
+extern "C" int ccq_fp8_block_linear_quantized(const uint8_t* q, const float* s, const uint8_t* w_tiled,
+                                              const float* s_w, void* y, int y_dtype, int64_t M, int64_t K,
+                                              int64_t N, void* stream) {
+  bool empty = false;
+  if (int rc = check_block_linear("ccq_fp8_block_linear_quantized", w_tiled, s_w, y, y_dtype, M, K, N, empty))
+    return rc;
+  if (empty) return 0;
+  CCQ_REQUIRE(q && s, "ccq_fp8_block_linear_quantized: null pointer");
+  CCQ_REQUIRE(aligned(q, 16) && aligned(s, 4), "ccq_fp8_block_linear_quantized: q must be 16-byte aligned");
+  return block_linear_gemm(q, s, w_tiled, s_w, y, y_dtype, M, K, N, as_stream(stream));
 }
 
 // ------------------------------------------------------------ MoE FP8 --

@@ -35,6 +35,11 @@ extern "C" {
 #define CCQ_F16 1
 #define CCQ_BF16 2
 
+/* 8-bit row formats of ccq_rms_norm */
+#define CCQ_Q_NONE 0
+#define CCQ_Q_FP8_BLOCK 1 /* e4m3fn, a scale per row and 128 columns */
+#define CCQ_Q_INT8_ROW 2  /* int8, a scale per row */
+
 /* library version (major*10000 + minor*100 + patch) */
 int ccq_version(void);
 /* message of the last failed call on this thread ("" if none) */
@@ -514,6 +519,72 @@ int ccq_fp8_block_linear(const void* x, int x_dtype, const uint8_t* w_tiled,
                          const float* s_w, void* y, int y_dtype, int64_t M, int64_t K,
                          int64_t N, void* workspace, size_t workspace_bytes,
                          void* stream);
+
+/* ccq_fp8_block_linear on rows that are quantized already (ccq_fp8_act_quant
+ * or ccq_rms_norm): q [M, K] e4m3fn, 16-byte aligned, s [M, K/128]. */
+int ccq_fp8_block_linear_quantized(const uint8_t* q, const float* s, const uint8_t* w_tiled,
+                                   const float* s_w, void* y, int y_dtype, int64_t M, int64_t K,
+                                   int64_t N, void* stream);
+
+/* ------------------------------------------------------------------------
+ * RMS norm of rows with the residual's addition and 8-bit output rows: the
+ * input of the quantized linears (the reference norms in float32,
+ * blocks/norm.py:14, and hands float32 rows on)
+ * ---------------------------------------------------------------------- */
+
+/* Per row of H columns, in float32: s = x + residual (residual may be null),
+ * residual_out = s in x's type, rstd = 1 / sqrt(mean(s^2) + eps), p = s * w,
+ * y = p * rstd in y_dtype.
+ *   CCQ_Q_FP8_BLOCK (H % 128 == 0, q 8-byte aligned): per 128 columns
+ *     m = max(max|p|, 1e-30), q = RNE_e4m3(p * (448 / m)),
+ *     scale [rows, H/128] = m * rstd / 448: what ccq_fp8_block_linear
+ *     multiplies;
+ *   CCQ_Q_INT8_ROW: per row m as above, q = round-half-even(p * (127 / m)),
+ *     scale [rows] = m * rstd / 127: what ccq_int8_linear multiplies.
+ *     (ccq_int8_act_quant keeps the reference's factor, which saturates
+ *     almost every value; these codes use the int8 range.)
+ * A row with a NaN has NaN scales and NaN y; one with an infinity has NaN at
+ * it (in its block's or row's scale) and 0 elsewhere.
+ * x, residual, residual_out have x_dtype and row strides ldx, ldr, ldo (>= H,
+ * in elements; any element alignment); y, q and scale are dense.  Each of
+ * residual_out, y and (with CCQ_Q_NONE) q may be null.  residual_out may be
+ * x or residual itself with the same stride, no other overlap.
+ * 1 <= H <= 32768, eps > 0. */
+int ccq_rms_norm(const void* x, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
+                 const void* w, int w_dtype, float eps, void* residual_out, int64_t ldo,
+                 void* y, int y_dtype, int q_fmt, void* q, float* scale, int64_t rows, int64_t H,
+                 void* stream);
+
+/* ------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one shared projection (no
+ * counterpart in the reference, which serves one request at a time)
+ * ---------------------------------------------------------------------- */
+
+/* The adapters of one projection, stacked: a [L, R, K], b [L, N, R] in dtype
+ * (CCQ_F16 | CCQ_BF16), scale [L] float32 or null (1), rank [L] int32 or null
+ * (R): ranks from rank[i] on (clamped to [0, R]) are padding, not read.
+ * 1 <= L <= 1024, 1 <= R <= 256, K and N <= 2^20. */
+typedef struct ccq_lora_adapters {
+  const void* a;
+  const void* b;
+  const float* scale;
+  const int32_t* rank;
+  int dtype;
+  int64_t num_adapters, rank_max, in_features, out_features;
+} ccq_lora_adapters;
+
+/* Workspace of ccq_lora_add (tokens sorted by adapter, partial sums; no
+ * initial contents required).  Calls sharing one must not overlap in time. */
+size_t ccq_lora_workspace_size(int64_t T, const ccq_lora_adapters* ad);
+
+/* y[t, :] += scale[i] * (x[t, :] @ a[i]^T) @ b[i]^T with i = index[t], in
+ * float32, y rounded once; rows with index[t] outside [0, L) are left as they
+ * are (neither read nor written).  x and y each CCQ_F32 | CCQ_F16 | CCQ_BF16
+ * with row strides ldx >= K, ldy >= N in elements, any element alignment; y
+ * must not overlap x.  T <= 65536. */
+int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64_t* index, void* y, int y_dtype,
+                 int64_t ldy, int64_t T, const ccq_lora_adapters* ad, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 /* MoE experts, FP8 block: gate/up w [E][I, H] (tiled), s [E][I/128][H/128];
  * down w [E][H, I] (tiled), s [E][H/128][I/128]. */
