@@ -49,7 +49,7 @@ class LoraAdapters:
                                        scale.data_ptr() if scale is not None else None,
                                        rank.data_ptr() if rank is not None else None, _dev.DTYPE_CODE[a.dtype],
                                        L, R, K, b.shape[1])
-        self._bytes: dict[int, int] = {}
+        self._bytes: dict[tuple, int] = {}
 
     @staticmethod
     def _vector(v, dtype: torch.dtype, L: int, device, what: str) -> torch.Tensor | None:
@@ -60,10 +60,12 @@ class LoraAdapters:
             raise ValueError(f"{what} must have one entry per adapter ({L}), got {tuple(t.shape)}")
         return t.to(device=device, dtype=dtype).contiguous()
 
-    def workspace_size(self, T: int) -> int:
-        n = self._bytes.get(T)
+    def workspace_size(self, T: int, x_dtype: torch.dtype) -> int:
+        """Bytes of scratch that ``add_`` of T rows takes."""
+        n = self._bytes.get((T, x_dtype))
         if n is None:
-            n = self._bytes[T] = int(lib().ccq_lora_workspace_size(T, self._desc))
+            n = int(lib().ccq_lora_workspace_size(T, _dev.DTYPE_CODE[x_dtype], self._desc))
+            self._bytes[T, x_dtype] = n
         return n
 
 
@@ -129,10 +131,10 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
         return y
     if _overlap(y2, x2):
         raise ValueError("y overlaps x")
-    nbytes = adapters.workspace_size(T)
+    nbytes = adapters.workspace_size(T, x2.dtype)
     # this call's own scratch, so that calls on several streams or in several graphs do not share it
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     call("ccq_lora_add", x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype], x2.stride(0) if T > 1 else x2.shape[1],
          index.data_ptr(), y2.data_ptr(), _dev.DTYPE_CODE[y2.dtype], y2.stride(0) if T > 1 else y2.shape[1], T,
-         adapters._desc, ws.data_ptr(), nbytes, stream)
+         adapters._desc, ws.data_ptr() if ws is not None else None, nbytes, stream)
     return y

@@ -574,8 +574,9 @@ typedef struct ccq_lora_adapters {
 } ccq_lora_adapters;
 
 /* Workspace of ccq_lora_add (tokens sorted by adapter, partial sums; no
- * initial contents required).  Calls sharing one must not overlap in time. */
-size_t ccq_lora_workspace_size(int64_t T, const ccq_lora_adapters* ad);
+ * initial contents required), 0 for the batches that one kernel takes.  Calls
+ * sharing one must not overlap in time. */
+size_t ccq_lora_workspace_size(int64_t T, int x_dtype, const ccq_lora_adapters* ad);
 
 /* y[t, :] += scale[i] * (x[t, :] @ a[i]^T) @ b[i]^T with i = index[t], in
  * float32, y rounded once; rows with index[t] outside [0, L) are left as they

@@ -113,6 +113,15 @@ def test_most_adapters_and_tokens(gpu):
     _check(_run(c, gpu), c)
 
 
+@pytest.mark.parametrize("T", [40, 600, 1111])
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+def test_high_ranks_and_long_rows(gpu, T, types):
+    """Ranks and rows that go through two kernels at any number of tokens."""
+    for K, N, R in ((2056, 200, 256), (4100, 96, 130), (9000, 72, 40)):
+        c = _case(T, K, N, R, 3, *types, pattern="runs" if T > 600 else "mixed", ranks=T == 600)
+        _check(_run(c, gpu), c)
+
+
 def test_padded_ranks_are_not_read(gpu):
     """Ranks 0 to R; what is behind an adapter's rank is NaN."""
     for R, t in ((16, "bf16"), (40, "f16"), (128, "bf16")):

@@ -47,7 +47,7 @@ def test_empty_calls(lib):
     assert _norm(lib, rows=0) == 0
     ad = ccq_lora_adapters(256, 256, None, None, 2, 3, 16, 64, 48)
     assert lib.ccq_lora_add(P, 2, 64, P, P, 2, 48, 0, ad, None, 0, None) == 0
-    assert lib.ccq_lora_workspace_size(0, ad) == 0
+    assert lib.ccq_lora_workspace_size(0, 2, ad) == 0
     assert lib.ccq_fp8_block_linear_quantized(P, P, P, P, P, 2, 0, 256, 128, None) == 0
 
 
@@ -63,7 +63,7 @@ def test_empty_calls(lib):
 def test_lora(lib, kw, word):
     from ccut._lib import CCQ_EINVAL, ccq_lora_adapters, last_error
 
-    a = dict(x=P, x_dtype=2, ldx=64, index=P, y=P, y_dtype=2, ldy=48, T=5, ws=P, ws_bytes=1 << 30, a=256, b=256, dtype=2,
+    a = dict(x=P, x_dtype=2, ldx=64, index=P, y=P, y_dtype=2, ldy=48, T=600, ws=P, ws_bytes=1 << 30, a=256, b=256, dtype=2,
              L=3, R=16, K=64, N=48)
     a.update(kw)
     ad = ccq_lora_adapters(a["a"], a["b"], None, None, a["dtype"], a["L"], a["R"], a["K"], a["N"])
