@@ -20,6 +20,7 @@ namespace ccq {
 namespace {
 
 constexpr int LR_THREADS = 512, LR_WAVES = 8;
+constexpr int LE_THREADS = 256;  // of the expand kernel
 constexpr int LR_MAX_R = 256;
 constexpr int LR_MAX_L = 1024;
 constexpr int LR_SELF = 4096;   // most tokens that workgroups sort themselves
@@ -37,6 +38,7 @@ struct LoraP {
   const int32_t* meta;          // tiles of ccq_moe_align's schedule; null: workgroups sort
   float* p;                     // [S][T][Rp]
   int64_t ldx, ldy;
+  int64_t last_x, last_a, last_b;  // where the last 8 values of x, a and b begin
   int T, L, R, Rp, K, N;
   int S, kchunk;                // splits of K, K per split (a multiple of 32)
   int tiles, ncols;             // tiles of the grid, columns per workgroup
@@ -61,48 +63,40 @@ __device__ __forceinline__ f32x4 lr_mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// 8 values of a row of `len` from element k on, as loaded; past the end 0.
-// len % 8 == 0 (uniform): one load at any alignment, of a piece inside the
-// row where k is past the end.
+// 8 values from element i on of a buffer whose last 8 begin at `last`, as
+// loaded: one load at any element alignment, of those last 8 where i is past
+// them.  lr_fix then moves the values to their places and clears those from n
+// on; until then they may be other rows' values.
 template <int DT>
 struct Raw {
   u32x4 v[DT == CCQ_F32 ? 2 : 1];
 };
 template <int DT>
-__device__ __forceinline__ Raw<DT> lr_load(const void* base, int64_t row, int k, int len) {
+__device__ __forceinline__ Raw<DT> lr_load_whole(const void* base, int64_t i) {
   constexpr int E = DT == CCQ_F32 ? 4 : 2;
   Raw<DT> r;
-  const char* p = reinterpret_cast<const char*>(base) + row * E;
-  if (len % 8 == 0) {
-    __builtin_memcpy(&r, p + (int64_t)min(k, len - 8) * E, 8 * E);
-  } else if (k + 8 <= len) {
-    __builtin_memcpy(&r, p + (int64_t)k * E, 8 * E);
-  } else {
-    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) w[e] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < len) {
-        if constexpr (DT == CCQ_F32)
-          w[e] = reinterpret_cast<const uint32_t*>(p)[k + e];
-        else
-          w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[k + e] << (16 * (e & 1));
-      }
-  }
+  __builtin_memcpy(&r, reinterpret_cast<const char*>(base) + i * E, 8 * E);
   return r;
 }
 template <int DT>
-__device__ __forceinline__ Raw<DT> lr_load_whole(const void* base, int64_t row, int k) {
-  constexpr int E = DT == CCQ_F32 ? 4 : 2;
-  Raw<DT> r;
-  __builtin_memcpy(&r, reinterpret_cast<const char*>(base) + (row + k) * E, 8 * E);
-  return r;
+__device__ __forceinline__ Raw<DT> lr_load(const void* base, int64_t i, int64_t last) {
+  return lr_load_whole<DT>(base, i < last ? i : last);
 }
-// the values from element n (of 8) on as 0
 template <int DT>
-__device__ __forceinline__ void lr_mask(Raw<DT>& r, int n) {
+__device__ __forceinline__ void lr_fix(Raw<DT>& r, int64_t i, int64_t last, int n) {
+  constexpr int W = DT == CCQ_F32 ? 8 : 4;
+  const int s = i <= last ? 0 : i - last < 8 ? (int)(i - last) : 8;
   uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+  const int words = DT == CCQ_F32 ? s : s >> 1;
+#pragma unroll
+  for (int step = W / 2; step >= 1; step >>= 1)
+#pragma unroll
+    for (int e = 0; e < W; ++e) w[e] = words & step ? (e + step < W ? w[e + step] : 0u) : w[e];
+  if constexpr (DT != CCQ_F32) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) w[e] = s & 1 ? w[e] >> 16 | (e + 1 < W ? w[e + 1] << 16 : 0u) : w[e];
+  }
+  if (s >= 8) n = 0;
   if constexpr (DT == CCQ_F32) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = e < n ? w[e] : 0u;
@@ -201,6 +195,44 @@ __device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS<CH>& 
   __syncthreads();
 }
 
+// The same for up to 64 tokens and tiles of 16, by each wave for itself: lane t
+// holds token t.  Lane r < 16 returns the tile's row r (-1: padding).
+__device__ __forceinline__ int lr_find_tile_wave(const LoraP& p, int tile, int& adapter) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = lane < p.T ? p.index[lane] : -1;
+  const int key = i >= 0 && i < p.L ? (int)i : -1;
+  uint64_t same = __ballot(key >= 0);  // the tokens of this lane's adapter
+  for (int b = 0; (p.L - 1) >> b; ++b) {
+    const uint64_t m = __ballot((key >> b) & 1);
+    same &= (key >> b) & 1 ? m : ~m;
+  }
+  const bool head = key >= 0 && (same & ((1ull << lane) - 1)) == 0;
+  int n = head ? (__popcll(same) + 15) >> 4 : 0;  // tiles of this lane's adapter
+  int start;
+  if (__ballot(n > 1) == 0) {
+    start = __popcll(__ballot(head) & ((1ull << lane) - 1));
+  } else {
+    start = n;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(start, off, 64);
+      if (lane >= off) start += v;
+    }
+    start -= n;
+  }
+  const uint64_t hit = __ballot(head && tile >= start && tile < start + n);
+  adapter = -1;
+  if (hit == 0) return -1;
+  const int l = __builtin_ctzll(hit);
+  adapter = __builtin_amdgcn_readlane(key, l);
+  const int first = 16 * (tile - __builtin_amdgcn_readlane(start, l));
+  const uint64_t group = __ballot(key == adapter);
+  // token t of the adapter's rank j goes to lane j - first, the others to lane 63
+  const int j = __popcll(group & ((1ull << lane) - 1)) - first;
+  const bool in = key == adapter && j >= 0 && j < 16;
+  const int got = __builtin_amdgcn_ds_permute(4 * (in ? j : 63), lane);
+  return lane < min(16, __popcll(group) - first) ? got : -1;
+}
+
 // the same from a finished schedule
 template <int TM>
 __device__ void lr_read_tile(const LoraP& p, int tile, TileS<TM>& t) {
@@ -238,41 +270,87 @@ __device__ __forceinline__ void lr_multiply(const Raw<XT> (&xr)[MT], const Raw<W
   }
 }
 
-template <int XT, int WT, int MT, int RT>
-__device__ __forceinline__ void lr_shrink(const LoraP& p, const int64_t (&xrow)[MT], const int64_t (&arow)[RT], int k0,
-                                          int k1, f32x4 (&acc)[MT][RT]) {
-  constexpr int U = MT * RT >= 16 ? 1 : MT * RT >= 4 ? 2 : 4;  // k-steps whose loads are in flight together
+// U k-steps whose loads are in flight together, as often as they fit, then half as many
+template <int XT, int WT, int MT, int RT, int U>
+__device__ __forceinline__ void lr_steps(const LoraP& p, const int64_t (&xrow)[MT], const int64_t (&arow)[RT], int& k,
+                                         int k1, f32x4 (&acc)[MT][RT]) {
   const int g = (threadIdx.x >> 4) & 3;
-  int k = k0;
-  for (; k + 32 * U <= k1 && k + 32 * U <= p.K; k += 32 * U) {
+  for (; k + 32 * U <= k1; k += 32 * U) {
     Raw<XT> xr[U][MT];
     Raw<WT> ar[U][RT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) xr[u][m] = lr_load_whole<XT>(p.x, xrow[m], k + 32 * u + 8 * g);
+      for (int m = 0; m < MT; ++m) xr[u][m] = lr_load_whole<XT>(p.x, xrow[m] + k + 32 * u + 8 * g);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) ar[u][t] = lr_load_whole<WT>(p.a, arow[t], k + 32 * u + 8 * g);
+      for (int t = 0; t < RT; ++t) ar[u][t] = lr_load_whole<WT>(p.a, arow[t] + k + 32 * u + 8 * g);
     }
+    __builtin_amdgcn_sched_barrier(0);  // all of them before the first product
 #pragma unroll
     for (int u = 0; u < U; ++u) lr_multiply<XT, WT, MT, RT>(xr[u], ar[u], acc);
   }
-  for (; k < k1; k += 32) {
+  if constexpr (U > 1) lr_steps<XT, WT, MT, RT, U / 2>(p, xrow, arow, k, k1, acc);
+}
+
+template <int XT, int WT, int MT, int RT, int U>
+__device__ __forceinline__ void lr_shrink(const LoraP& p, const int64_t (&xrow)[MT], const int64_t (&arow)[RT], int k0,
+                                          int k1, f32x4 (&acc)[MT][RT]) {
+  const int g = (threadIdx.x >> 4) & 3;
+  int k = k0;
+  lr_steps<XT, WT, MT, RT, U>(p, xrow, arow, k, k1, acc);
+  if (k < k1) {  // the last, partial step of K
     const int kk = k + 8 * g;
     Raw<XT> xr[MT];
     Raw<WT> ar[RT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xr[m] = lr_load<XT>(p.x, xrow[m], kk, p.K);
+    for (int m = 0; m < MT; ++m) xr[m] = lr_load<XT>(p.x, xrow[m] + kk, p.last_x);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) ar[t] = lr_load<WT>(p.a, arow[t], kk, p.K);
-    if (k + 32 > p.K) {
+    for (int t = 0; t < RT; ++t) ar[t] = lr_load<WT>(p.a, arow[t] + kk, p.last_a);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) lr_mask<XT>(xr[m], p.K - kk);
+    for (int m = 0; m < MT; ++m) lr_fix<XT>(xr[m], xrow[m] + kk, p.last_x, p.K - kk);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) lr_mask<WT>(ar[t], p.K - kk);
-    }
+    for (int t = 0; t < RT; ++t) lr_fix<WT>(ar[t], arow[t] + kk, p.last_a, p.K - kk);
     lr_multiply<XT, WT, MT, RT>(xr, ar, acc);
   }
+}
+
+// Stages of whole 128-byte lines of x's rows, D - 1 of them loaded
+// ahead of the products: for the 64-token tiles, whose waves walk far in K.
+template <int XT, int WT, int MT, int RT, int D>
+__device__ __forceinline__ void lr_shrink_ring(const LoraP& p, const int64_t (&xrow)[MT], const int64_t (&arow)[RT],
+                                               int k0, int k1, f32x4 (&acc)[MT][RT]) {
+  const int g = (threadIdx.x >> 4) & 3;
+  constexpr int SU = XT == CCQ_F32 ? 1 : 2, SK = 32 * SU;
+  const int n = k1 > k0 ? (k1 - k0) / SK : 0;
+  Raw<XT> xr[D][SU][MT];
+  Raw<WT> ar[D][SU][RT];
+  auto load = [&](int s, int d) {
+    const int k = k0 + SK * s + 8 * g;
+#pragma unroll
+    for (int u = 0; u < SU; ++u) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xr[d][u][m] = lr_load_whole<XT>(p.x, xrow[m] + k + 32 * u);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) ar[d][u][t] = lr_load_whole<WT>(p.a, arow[t] + k + 32 * u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (n > 0) {
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d) load(min(d, n - 1), d);  // past the range: its last stage again, not multiplied
+    for (int s = 0; s < n; s += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        load(min(s + d + D - 1, n - 1), (d + D - 1) % D);
+        if (s + d < n) {
+#pragma unroll
+          for (int u = 0; u < SU; ++u) lr_multiply<XT, WT, MT, RT>(xr[d][u], ar[d][u], acc);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  lr_shrink<XT, WT, MT, RT, 1>(p, xrow, arow, k0 + SK * n, k1, acc);  // what is left: less than a stage
 }
 
 // ---------------------------------------------------------------- expand --
@@ -304,84 +382,93 @@ __device__ __forceinline__ void lr_split(const float (&v)[8], typename Half<WT>:
 // the power of two that brings a row whose largest finite |p| is m into [2^13, 2^14]
 __device__ __forceinline__ int lr_exponent(float m) { return m > 0.f ? min(max(13 - ilogbf(m), -100), 100) : 0; }
 
+// 16 bytes of a row of y from column n on (at any element alignment).  A piece
+// across the row's end is not loaded, and added to in place value by value.
+// YT: float32, or either 16-bit type (they differ in add_store alone).
+template <int YT>
+struct YPiece {
+  static constexpr int COLS = YT == CCQ_F32 ? 4 : 8;
+  u32x4 v;
+  __device__ __forceinline__ void load(const void* y, int64_t row, int n, int N) {
+    constexpr int E = YT == CCQ_F32 ? 4 : 2;
+    v = u32x4{0, 0, 0, 0};
+    if (n + COLS <= N) __builtin_memcpy(&v, reinterpret_cast<const char*>(y) + (row + n) * E, 16);
+  }
+  __device__ __forceinline__ void add_store(void* y, int y_dtype, int64_t row, int n, int N, const float (&d)[COLS]) {
+    constexpr int E = YT == CCQ_F32 ? 4 : 2;
+    char* at = reinterpret_cast<char*>(y) + (row + n) * E;
+    if (n + COLS <= N) {
+      u32x4 o;
+      if constexpr (YT == CCQ_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(__uint_as_float(v[e]) + d[e]);
+      } else if (y_dtype == CCQ_BF16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = bf16x2_bits(bf16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e], bf16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = f32_to_f16_bits(f16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e]) |
+                 f32_to_f16_bits(f16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]) << 16;
+      }
+      __builtin_memcpy(at, &o, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < COLS; ++e)
+        if (n + e < N) {
+          if constexpr (YT == CCQ_F32) {
+            reinterpret_cast<float*>(at)[e] += d[e];
+          } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(at) + e;
+            *h = (uint16_t)(y_dtype == CCQ_BF16 ? bf16x2_bits(bf16_bits_to_f32(*h) + d[e], 0.f)
+                                                : f32_to_f16_bits(f16_bits_to_f32(*h) + d[e]));
+          }
+        }
+    }
+  }
+};
+
 // Column of D row m of MFMA q in a block of 64: a lane's quads join to 16-byte
 // pieces of its token's row, four lanes to 64 contiguous bytes.
 template <int YT>
 __device__ __forceinline__ int lr_col(int q, int m) {
   return YT == CCQ_F32 ? 16 * q + m : 32 * (q >> 1) + 8 * (m >> 2) + 4 * (q & 1) + (m & 3);
 }
-
-// The lane's 16 values of y, block n0 of 64 columns
+// where piece i of lane group g begins, and its values among the lane's quads
 template <int YT>
-struct YBlock {
-  static constexpr int PIECES = YT == CCQ_F32 ? 4 : 2, COLS = YT == CCQ_F32 ? 4 : 8;
-  u32x4 v[PIECES];
-  __device__ __forceinline__ static int col(int piece, int g) { return YT == CCQ_F32 ? 16 * piece + 4 * g : 32 * piece + 8 * g; }
-  __device__ __forceinline__ void load(const void* y, int64_t row, int n0, int g, int N) {
-    constexpr int E = YT == CCQ_F32 ? 4 : 2;
+__device__ __forceinline__ int lr_piece_col(int i, int g) { return YT == CCQ_F32 ? 16 * i + 4 * g : 32 * i + 8 * g; }
+template <int YT>
+__device__ __forceinline__ void lr_store_pieces(const LoraP& p, YPiece<YT> (&y)[16 / YPiece<YT>::COLS], int64_t row,
+                                                int n0, int g, const f32x4 (&acc)[4], float f) {
+  constexpr int C = YPiece<YT>::COLS;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int n = n0 + col(i, g);
-      const char* at = reinterpret_cast<const char*>(y) + (row + n) * E;
-      if (n + COLS <= N) {
-        __builtin_memcpy(&v[i], at, 16);
-      } else {
-        v[i] = u32x4{0, 0, 0, 0};
+  for (int i = 0; i < 16 / C; ++i) {
+    float d[C];
 #pragma unroll
-        for (int e = 0; e < COLS; ++e)
-          if (n + e < N) {
-            if constexpr (YT == CCQ_F32)
-              v[i][e] = reinterpret_cast<const uint32_t*>(at)[e];
-            else
-              v[i][e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(at)[e] << (16 * (e & 1));
-          }
-      }
-    }
+    for (int e = 0; e < C; ++e) d[e] = acc[(C * i + e) / 4][e & 3] * f;
+    y[i].add_store(p.y, p.y_dtype, row, n0 + lr_piece_col<YT>(i, g), p.N, d);
   }
-  __device__ __forceinline__ void add_store(void* y, int64_t row, int n0, int g, int N, const f32x4 (&acc)[4], float f) {
-    constexpr int E = YT == CCQ_F32 ? 4 : 2;
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int n = n0 + col(i, g);
-      u32x4 o;
-      if constexpr (YT == CCQ_F32) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(__uint_as_float(v[i][e]) + acc[i][e] * f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4& d = acc[2 * i + (e >> 1)];
-          const uint32_t lo = v[i][e] & 0xFFFFu, hi = v[i][e] >> 16;
-          const float s0 = (YT == CCQ_BF16 ? bf16_bits_to_f32(lo) : f16_bits_to_f32(lo)) + d[2 * (e & 1)] * f;
-          const float s1 = (YT == CCQ_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi)) + d[2 * (e & 1) + 1] * f;
-          o[e] = YT == CCQ_BF16 ? bf16x2_bits(s0, s1) : f32_to_f16_bits(s0) | f32_to_f16_bits(s1) << 16;
-        }
-      }
-      char* at = reinterpret_cast<char*>(y) + (row + n) * E;
-      if (n + COLS <= N) {
-        __builtin_memcpy(at, &o, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < COLS; ++e)
-          if (n + e < N) {
-            if constexpr (YT == CCQ_F32)
-              reinterpret_cast<uint32_t*>(at)[e] = o[e];
-            else
-              reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-          }
-      }
-    }
-  }
-};
+}
 
-// B rows of the 64 columns from n0 on, ranks c + 8 g .. of MFMA q
-template <int WT, int YT>
-__device__ __forceinline__ void lr_load_b(const LoraP& p, int adapter, int rank, int n0, int c, Raw<WT> (&w)[4]) {
-  const int c16 = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+// B rows of 64 columns from n0 on, ranks c + 8 g .. (columns past the end
+// repeat the last one: not stored), and, in the last chunk, its part behind
+// the rank cleared: the padding there may hold anything.  col(q): the column
+// of this lane's row of MFMA q.
+template <int WT, typename F>
+__device__ __forceinline__ void lr_load_b(const LoraP& p, int adapter, int c, F col, Raw<WT> (&w)[4]) {
+  const int r = c + 8 * ((threadIdx.x >> 4) & 3);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int n = min(n0 + lr_col<YT>(q, c16), p.N - 1);  // columns past the end: not stored
-    w[q] = lr_load<WT>(p.b, ((int64_t)adapter * p.N + n) * p.R, c + 8 * g, p.R);
+  for (int q = 0; q < 4; ++q)
+    w[q] = lr_load<WT>(p.b, ((int64_t)adapter * p.N + min(col(q), p.N - 1)) * p.R + r, p.last_b);
+}
+template <int WT, typename F>
+__device__ __forceinline__ void lr_fix_b(const LoraP& p, int adapter, int rank, int c, F col, Raw<WT> (&w)[4]) {
+  const int r = c + 8 * ((threadIdx.x >> 4) & 3);
+  if (c + 32 > rank) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      lr_fix<WT>(w[q], ((int64_t)adapter * p.N + min(col(q), p.N - 1)) * p.R + r, p.last_b, rank - r);
   }
 }
 
@@ -394,20 +481,6 @@ __device__ __forceinline__ void lr_expand_step(const Raw<WT> (&w)[4], const type
 #pragma unroll
     for (int i = 0; i < PARTS; ++i)
       acc[q] = lr_mfma(__builtin_bit_cast(typename Half<WT>::vec, w[q]), pv[i], acc[q]);
-}
-
-template <int YT>
-__device__ __forceinline__ void lr_store(const LoraP& p, YBlock<YT>& y, int64_t row, int n0, int g,
-                                         const f32x4 (&acc)[4], float f) {
-  if constexpr (YT == CCQ_F32) {
-    y.add_store(p.y, row, n0, g, p.N, acc, f);
-  } else {  // both 16-bit types have one layout
-    if (p.y_dtype == CCQ_BF16) {
-      __builtin_bit_cast(YBlock<CCQ_BF16>, y).add_store(p.y, row, n0, g, p.N, acc, f);
-    } else {
-      __builtin_bit_cast(YBlock<CCQ_F16>, y).add_store(p.y, row, n0, g, p.N, acc, f);
-    }
-  }
 }
 
 // ------------------------------------------------------ one kernel (fused) --
@@ -425,14 +498,24 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   } u;
   __shared__ __align__(16) float ps[16][32 * RC + 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x % p.tiles, group = blockIdx.x / p.tiles;
-  lr_find_tile<16, 1>(p, tile, tl, u.sort);
-  const int adapter = tl.adapter;
+  // all workgroups of a tile on one XCD, whose L2 then holds its A
+  const int t8 = (p.tiles + 7) & ~7, tile = blockIdx.x % t8, group = blockIdx.x / t8;
+  if (tile >= p.tiles) return;
+  int adapter, own, tok;  // padding: the first row again, not stored
+  if (p.T <= 64) {
+    const int rows = lr_find_tile_wave(p, tile, adapter);
+    own = __shfl(rows, c16, 64);
+    tok = own >= 0 ? own : __shfl(rows, 0, 64);
+  } else {
+    lr_find_tile<16, 1>(p, tile, tl, u.sort);
+    adapter = tl.adapter;
+    own = tl.rows[c16];
+    tok = own >= 0 ? own : tl.rows[0];
+  }
   if (adapter < 0) return;
   const int rank = lr_rank(p, adapter);
   if (rank == 0) return;
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
-  const int own = tl.rows[c16], tok = own >= 0 ? own : tl.rows[0];  // padding: the first row again, not stored
   const int64_t xrow[1] = {(int64_t)tok * p.ldx}, yrow = (int64_t)tok * p.ldy;
   int64_t arow[RT];
 #pragma unroll
@@ -440,18 +523,19 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   const int end = min((group + 1) * p.ncols, p.N);
   int n0 = group * p.ncols + 64 * wave;
   Raw<WT> w[RC][4];
-  YBlock<YT> y;
+  YPiece<YT> y[16 / YPiece<YT>::COLS];
   auto fetch = [&]() {
 #pragma unroll
-    for (int c = 0; c < RC; ++c) lr_load_b<WT, YT>(p, adapter, rank, n0, 32 * c, w[c]);
-    y.load(p.y, yrow, n0, g, p.N);
+    for (int c = 0; c < RC; ++c) lr_load_b<WT>(p, adapter, 32 * c, [&](int q) { return n0 + lr_col<YT>(q, c16); }, w[c]);
+#pragma unroll
+    for (int i = 0; i < 16 / YPiece<YT>::COLS; ++i) y[i].load(p.y, yrow, n0 + lr_piece_col<YT>(i, g), p.N);
   };
   if (n0 < end) fetch();
   f32x4 acc[1][RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int k0 = wave * p.kchunk;
-  lr_shrink<XT, WT, 1, RT>(p, xrow, arow, k0, min(k0 + p.kchunk, p.K), acc);
+  lr_shrink<XT, WT, 1, RT, (RT == 1 ? 16 : RT == 8 ? 2 : RT == 4 ? 4 : 8) / (XT == CCQ_F32 ? 2 : 1)>(p, xrow, arow, k0, min(k0 + p.kchunk, p.K), acc);
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < RT; ++t) u.red[wave][t][lane] = acc[0][t];
@@ -500,13 +584,10 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
     for (int q = 0; q < 4; ++q) out[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
-      if (32 * c + 32 > rank) {  // the padding behind the rank may hold anything
-#pragma unroll
-        for (int q = 0; q < 4; ++q) lr_mask<WT>(w[c][q], rank - 32 * c - 8 * g);
-      }
+      lr_fix_b<WT>(p, adapter, rank, 32 * c, [&](int q) { return n0 + lr_col<YT>(q, c16); }, w[c]);
       lr_expand_step<WT, PARTS>(w[c], pv[c], out);
     }
-    if (own >= 0) lr_store<YT>(p, y, yrow, n0, g, out, down);
+    if (own >= 0) lr_store_pieces<YT>(p, y, yrow, n0, g, out, down);
     n0 += 64 * LR_WAVES;
     if (n0 >= end) break;
     fetch();
@@ -514,23 +595,37 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
 }
 
 // ------------------------------------------------------------ two kernels --
-// A tile's 16 MT tokens, RT * 16 ranks from 16 RT blockIdx.z on, K range of
-// one split, an eighth of it per wave.
-template <int XT, int WT, int MT, int RT>
+// A tile's 16 MT tokens, the K range of one split.  RH waves share a K part,
+// each with RT * 16 of the ranks (from 16 RT RH blockIdx.z on), so that a
+// wave's sums and its loads ahead fit its registers; the K parts' sums meet in
+// LDS.  An XCD takes neighbouring tiles, mostly of one adapter, at one pace
+// through K: its L2 serves A to all but the first of them.
+template <int XT, int WT, int MT, int RT, int RH>
 __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) {
   constexpr int TM = 16 * MT, CH = MT == 1 ? 1 : LR_SELF / LR_THREADS;
-  constexpr int PASS = MT * RT <= 8 ? MT : 8 / RT;  // row blocks whose sums are in LDS at once
+  constexpr int KP = LR_WAVES / RH;                          // K parts
+  constexpr int PASS = MT * RT * RH <= 8 ? MT : 8 / (RT * RH);  // row blocks whose sums are in LDS at once
   __shared__ TileS<TM> tl;
   __shared__ union {
     SortS<CH> sort;
-    f32x4 red[LR_WAVES][PASS][RT][64];
+    f32x4 red[KP][PASS][RH * RT][64];
   } u;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % p.S, tile = blockIdx.x / p.S;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+  const int per = (p.tiles + 7) >> 3, local = blockIdx.x >> 3, split = local % p.S;
+  const int tile = (blockIdx.x & 7) * per + local / p.S;
+  if (tile >= p.tiles) return;
   if (p.meta != nullptr) {
     lr_read_tile<TM>(p, tile, tl);
   } else {
-    lr_find_tile<TM, CH>(p, tile, tl, u.sort);
+    if (MT == 1 && p.T <= 64) {
+      int found;
+      const int rows = lr_find_tile_wave(p, tile, found);
+      if (threadIdx.x < TM) tl.rows[threadIdx.x] = rows;
+      if (threadIdx.x == 0) tl.adapter = found;
+      __syncthreads();
+    } else {
+      lr_find_tile<TM, CH>(p, tile, tl, u.sort);
+    }
     if (split == 0 && blockIdx.z == 0) {  // for the second kernel
       if (threadIdx.x < TM) p.tile_rows[(int64_t)tile * TM + threadIdx.x] = tl.rows[threadIdx.x];
       if (threadIdx.x == 0) p.tile_adapter[tile] = tl.adapter;
@@ -538,8 +633,9 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   }
   const int adapter = tl.adapter;
   if (adapter < 0) return;
-  const int rank = lr_rank(p, adapter), r0 = blockIdx.z * RT * 16;
-  if (r0 >= rank) return;
+  const int rank = lr_rank(p, adapter), rz = blockIdx.z * RH * RT * 16;
+  if (rz >= rank) return;
+  const int h = wave % RH, part = wave / RH, r0 = rz + h * RT * 16;
   int64_t xrow[MT], arow[RT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -553,24 +649,29 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int kw = (p.kchunk / 32 + LR_WAVES - 1) / LR_WAVES * 32;  // per wave
-  const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), k0 = ks + wave * kw;
-  lr_shrink<XT, WT, MT, RT>(p, xrow, arow, k0, min(k0 + kw, ke), acc);
+  const int kw = (p.kchunk / 32 + KP - 1) / KP * 32;  // per wave
+  const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), k0 = ks + part * kw, k1 = min(k0 + kw, ke);
+  if (r0 < rank) {
+    if constexpr (MT == 1)
+      lr_shrink<XT, WT, MT, RT, (RT == 8 ? 2 : RT == 4 ? 4 : 8) / (XT == CCQ_F32 ? 2 : 1)>(p, xrow, arow, k0, k1, acc);
+    else
+      lr_shrink_ring<XT, WT, MT, RT, RT == 1 ? 3 : 2>(p, xrow, arow, k0, k1, acc);
+  }
 #pragma unroll
   for (int m0 = 0; m0 < MT; m0 += PASS) {
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < PASS; ++m)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) u.red[wave][m][t][lane] = acc[m0 + m][t];
+      for (int t = 0; t < RT; ++t) u.red[part][m][h * RT + t][lane] = acc[m0 + m][t];
     __syncthreads();
-    for (int i = wave; i < PASS * RT; i += LR_WAVES) {
-      const int m = i / RT, t = i - m * RT;
-      if (r0 + 16 * t >= rank) continue;  // the workspace's rows end with the last used 16 ranks
+    for (int i = wave; i < PASS * RH * RT; i += LR_WAVES) {
+      const int m = i / (RH * RT), t = i - m * (RH * RT);
+      if (rz + 16 * t >= rank) continue;  // the workspace's rows end with the last used 16 ranks
       f32x4 s = u.red[0][m][t][lane];
 #pragma unroll
-      for (int k = 1; k < LR_WAVES; ++k) s += u.red[k][m][t][lane];
-      const int r = r0 + 16 * t + c16;
+      for (int k = 1; k < KP; ++k) s += u.red[k][m][t][lane];
+      const int r = rz + 16 * t + c16;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // D: column (rank) lane & 15, row (token) 4 (lane >> 4) + e
         const int id = tl.rows[16 * (m0 + m) + 4 * g + e];
@@ -580,16 +681,182 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   }
 }
 
+// The same for 64-token tiles of aligned rows, through LDS: a wave's load then
+// takes 8 rows x 128 bytes, whole lines, where the operand loads above ask for
+// half lines of 16 rows.  A stage holds 64 Q columns k of the 64 tokens and of
+// the RT * 16 ranks, copied by LDS DMA into a ring of D stages, D - 1 ahead;
+// each wave multiplies one step of 32 k (part) of it for RTW * 16 ranks (h).
+// In a line the 16-byte piece i of row r lies at i ^ (r & 7), so that the
+// operand reads of 8 neighbouring lanes cover all banks.
+template <int XT, int WT, int RT>
+struct TileShrink {
+  static constexpr int RTW = RT == 8 ? 2 : 1, RH = RT / RTW, KP = LR_WAVES / RH, Q = KP / 2;
+  static constexpr int SK = 64 * Q;                              // k of a stage
+  static constexpr int XL = Q * (XT == CCQ_F32 ? 2 : 1);         // lines of a row of x, of A: Q
+  static constexpr int X_BYTES = XL * 64 * 128, BYTES = X_BYTES + Q * 16 * RT * 128;
+  static constexpr int NI = BYTES / 1024 / LR_WAVES;             // copies of a wave per stage
+  static constexpr int FIT = 144 * 1024 / BYTES, D = FIT > 6 ? 6 : FIT;
+  static_assert(BYTES % (1024 * LR_WAVES) == 0 && D >= 2 && (D - 2) * NI < 64);
+  static_assert(D * BYTES >= KP * 4 * RT * 1024, "the partial sums reuse the ring");
+};
+
+template <int XT, int WT, int RT>
+__global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const LoraP p) {
+  using C = TileShrink<XT, WT, RT>;
+  constexpr int RTW = C::RTW, RH = C::RH, KP = C::KP, NI = C::NI, D = C::D;
+  constexpr int E = XT == CCQ_F32 ? 4 : 2;
+  __shared__ TileS<64> tl;
+  __shared__ __align__(16) union {
+    SortS<LR_SELF / LR_THREADS> sort;
+    char ring[D][C::BYTES];
+    f32x4 red[KP][4][RT][64];
+  } u;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+  const int per = (p.tiles + 7) >> 3, local = blockIdx.x >> 3, split = local % p.S;
+  const int tile = (blockIdx.x & 7) * per + local / p.S;
+  if (tile >= p.tiles) return;
+  if (p.meta != nullptr) {
+    lr_read_tile<64>(p, tile, tl);
+  } else {
+    lr_find_tile<64, LR_SELF / LR_THREADS>(p, tile, tl, u.sort);
+    if (split == 0 && blockIdx.z == 0) {  // for the second kernel
+      if (threadIdx.x < 64) p.tile_rows[(int64_t)tile * 64 + threadIdx.x] = tl.rows[threadIdx.x];
+      if (threadIdx.x == 0) p.tile_adapter[tile] = tl.adapter;
+    }
+  }
+  const int adapter = __builtin_amdgcn_readfirstlane(tl.adapter);
+  if (adapter < 0) return;
+  const int rank = __builtin_amdgcn_readfirstlane(lr_rank(p, adapter)), rz = blockIdx.z * RT * 16;
+  if (rz >= rank) return;
+  const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), stages = (ke - ks + C::SK - 1) / C::SK;
+
+  // copy i of the wave: 8 rows of one line, this lane piece `piece` of row `row`
+  uint32_t off[NI];   // bytes from the base below, at the split's first stage
+  const int piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = wave * NI + i;
+    if (c < C::X_BYTES / 1024) {
+      const int own = tl.rows[(c & 7) * 8 + (lane >> 3)];
+      off[i] = (uint32_t)((int64_t)(own >= 0 ? own : tl.rows[0]) * p.ldx * E) + (c >> 3) * 128 + 16 * piece;
+    } else {
+      const int a = c - C::X_BYTES / 1024, r = rz + (a % (2 * RT)) * 8 + (lane >> 3);
+      off[i] = (uint32_t)min(r, rank - 1) * (uint32_t)p.K * 2 + a / (2 * RT) * 128 + 16 * piece;
+    }
+  }
+  const char* xb = reinterpret_cast<const char*>(p.x) + (int64_t)ks * E;
+  const char* ab = reinterpret_cast<const char*>(p.a) + ((int64_t)adapter * p.R * p.K + ks) * 2;
+  const uint32_t lds0 = lds_addr(&u);
+  auto issue = [&](int s, int slot) {
+    const bool tail = ks + (s + 1) * C::SK > p.K;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = wave * NI + i;
+      const bool is_x = c < C::X_BYTES / 1024;
+      uint32_t o = off[i];
+      if (tail) {  // a piece past the end of its row: the row's first piece of the stage again, masked below
+        const int e = is_x ? E : 2, line = is_x ? c >> 3 : (c - C::X_BYTES / 1024) / (2 * RT);
+        if (ks + s * C::SK + (line * 128 + 16 * piece) / e >= p.K) o -= line * 128 + 16 * piece;
+      }
+      dma16((is_x ? xb + (int64_t)s * C::SK * E : ab + (int64_t)s * C::SK * 2), o, lds0 + slot * C::BYTES + c * 1024);
+    }
+  };
+  const int h = wave % RH, part = wave / RH;
+  f32x4 acc[4][RTW];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int t = 0; t < RTW; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  __syncthreads();  // the sort's LDS is free
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) issue(min(d, stages - 1), d);
+  int slot = 0;
+  for (int s = 0; s < stages; ++s) {
+    wait_vmcnt<(D - 2) * NI>();
+    lds_barrier();  // stage s is in LDS for all, and the slot before it is read out
+    issue(min(s + D - 1, stages - 1), slot == 0 ? D - 1 : slot - 1);  // past the range: not read
+    const char* st = u.ring[slot];
+    Raw<XT> xr[4];
+    Raw<WT> ar[RTW];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int row = 16 * m + c16;
+      if constexpr (XT == CCQ_F32) {
+        const char* line = st + part * 8192 + row * 128;
+        xr[m].v[0] = *reinterpret_cast<const u32x4*>(line + (((2 * g) ^ (row & 7)) * 16));
+        xr[m].v[1] = *reinterpret_cast<const u32x4*>(line + (((2 * g + 1) ^ (row & 7)) * 16));
+      } else {
+        xr[m].v[0] = *reinterpret_cast<const u32x4*>(st + (part >> 1) * 8192 + row * 128 +
+                                                     (((4 * (part & 1) + g) ^ (row & 7)) * 16));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RTW; ++t) {
+      const int row = 16 * (h * RTW + t) + c16;
+      ar[t].v[0] = *reinterpret_cast<const u32x4*>(st + C::X_BYTES + (part >> 1) * (16 * RT * 128) + row * 128 +
+                                                   (((4 * (part & 1) + g) ^ (row & 7)) * 16));
+    }
+    const int left = p.K - (ks + s * C::SK + 32 * part + 8 * g);
+    if (ks + (s + 1) * C::SK > p.K) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) lr_fix<XT>(xr[m], 0, 0, left);
+#pragma unroll
+      for (int t = 0; t < RTW; ++t) lr_fix<WT>(ar[t], 0, 0, left);
+    }
+    lr_multiply<XT, WT, 4, RTW>(xr, ar, acc);
+    slot = slot == D - 1 ? 0 : slot + 1;
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int t = 0; t < RTW; ++t) u.red[part][m][h * RTW + t][lane] = acc[m][t];
+  __syncthreads();
+  for (int i = wave; i < 4 * RT; i += LR_WAVES) {
+    const int m = i / RT, t = i % RT;
+    if (rz + 16 * t >= rank) continue;  // the workspace's rows end with the last used 16 ranks
+    f32x4 s = u.red[0][m][t][lane];
+#pragma unroll
+    for (int k = 1; k < KP; ++k) s += u.red[k][m][t][lane];
+    const int r = rz + 16 * t + c16;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // D: column (rank) lane & 15, row (token) 4 (lane >> 4) + e
+      const int id = tl.rows[16 * m + 4 * g + e];
+      if (id >= 0) p.p[((int64_t)split * p.T + id) * p.Rp + r] = r < rank ? s[e] : 0.f;
+    }
+  }
+}
+
+// Lanes of one wave hand each other values through LDS: the hardware keeps a
+// wave's LDS accesses in order, the fences keep the compiler from moving them
+// across.  They emit no instruction.
+__device__ __forceinline__ void lr_lane_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A tile's 16 MT tokens, ncols columns: p summed over the splits, scaled and
-// in parts in LDS; the waves take blocks of 64 columns.
+// in parts in LDS; a wave then takes 64 columns of 16 MP tokens at a time.  The
+// products' lanes hold 4 columns of 16 tokens each: they pass through the
+// wave's part of LDS into rows, so that y is read and written in whole lines
+// (8 lanes a row of 128 bytes).  y of the next step (and its weights, where one
+// chunk of 32 ranks is all) is loaded before the products of this one, the
+// first before p.
 template <int WT, int YT, int MT>
-__global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const LoraP p) {
+__global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand_kernel(const LoraP p) {
   using V = typename Half<WT>::vec;
-  constexpr int PARTS = WT == CCQ_F16 ? 2 : YT == CCQ_F32 ? 3 : 2, TM = 16 * MT;
+  constexpr int PARTS = WT == CCQ_F16 ? 2 : YT == CCQ_F32 ? 3 : 2, TM = 16 * MT, WAVES = LE_THREADS / 64;
+  constexpr int MP = MT < 2 ? MT : 2, PAIRS = MT / MP;
+  constexpr int E = YT == CCQ_F32 ? 4 : 2, COLS = 16 / E, RL = 64 / COLS;  // lanes of a row
+  constexpr int RI = 64 / RL, YN = 16 * MP / RI;                           // rows of an access, accesses of a step
   __shared__ TileS<TM> tl;
   __shared__ float downs[TM];
+  __shared__ __align__(16) float turn[WAVES][16 * MP][64 + 4];
   extern __shared__ __align__(16) uint16_t parts[];  // [PARTS][TM][ld]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+  const int yr = lane / RL, yc = lane % RL * COLS;  // this lane's row and columns of an access to y
   const int tile = blockIdx.x % p.tiles, group = blockIdx.x / p.tiles;
   lr_read_tile<TM>(p, tile, tl);
   const int adapter = tl.adapter;
@@ -598,93 +865,167 @@ __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const LoraP p) 
   if (rank == 0) return;
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
   const int rc = (rank + 31) / 32, r16 = (rank + 15) & ~15, ld = 32 * rc + 8;
-  {  // 8 threads a row, each every eighth piece of 8 ranks
-    const int row = threadIdx.x >> 3, j = threadIdx.x & 7;
-    const int id = row < TM ? tl.rows[row] : -1;
-    if (row < TM) {
-      float v[LR_MAX_R / 64][8];
-      float m = 0.f;
+  const int first = group * p.ncols + 64 * wave, end = min((group + 1) * p.ncols, p.N);
+  const int blocks = first < end ? (end - first + 64 * WAVES - 1) / (64 * WAVES) : 0, steps = blocks * PAIRS;
+  YPiece<YT> y[2][YN];
+  Raw<WT> w[4];
+  auto block_of = [&](int step) { return first + 64 * WAVES * (step / PAIRS); };  // step = block * PAIRS + pair
+  auto load_b = [&](int n0, int c, Raw<WT>(&v)[4]) {
+    lr_load_b<WT>(p, adapter, 32 * c, [&](int q) { return n0 + 16 * q + c16; }, v);
+  };
+  auto fetch = [&](int step, YPiece<YT>(&v)[YN]) {
+    const int m0 = (step % PAIRS) * MP;
 #pragma unroll
-      for (int i = 0; i < LR_MAX_R / 64; ++i) {
-        const int r = 64 * i + 8 * j;
+    for (int i = 0; i < YN; ++i) {
+      const int id = tl.rows[16 * m0 + RI * i + yr];
+      v[i].load(p.y, (int64_t)(id >= 0 ? id : tl.rows[0]) * p.ldy, block_of(step) + yc, p.N);
+    }
+  };
+  if (steps > 0) {
+    fetch(0, y[0]);
+    load_b(first, 0, w);
+  }
+  // 2, 4 or 8 threads a row (ranks up to 16, 128, 256), each every so manieth piece of 8 ranks
+  const int sh = r16 <= 16 ? 1 : r16 <= 128 ? 2 : 3, across = 8 << sh;
+#pragma unroll 1
+  for (int row = threadIdx.x >> sh; row < TM; row += LE_THREADS >> sh) {
+    const int j = threadIdx.x & ((1 << sh) - 1), id = tl.rows[row];
+    float v[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-        if (id >= 0 && r < r16) {
-          for (int s = 0; s < p.S; ++s) {
-            float o[8];
-            __builtin_memcpy(o, p.p + ((int64_t)s * p.T + id) * p.Rp + r, 32);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] += o[e];
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (id >= 0) {
+      const float* at = p.p + (int64_t)id * p.Rp + 8 * j;
+#pragma unroll 1
+      for (int s = 0; s < p.S; ++s, at += (int64_t)p.T * p.Rp) {
+        f32x4 o[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (across * i + 8 * j < r16) {
+            o[i][0] = *reinterpret_cast<const f32x4*>(at + across * i);
+            o[i][1] = *reinterpret_cast<const f32x4*>(at + across * i + 4);
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[i][e] = r + e < rank ? v[i][e] * scale : 0.f;
-            m = isfinite(v[i][e]) ? fmaxf(m, fabsf(v[i][e])) : m;
+        for (int i = 0; i < 4; ++i)
+          if (across * i + 8 * j < r16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] += o[i][e >> 2][e & 3];
           }
-        }
       }
-      float up = 1.f, down = 1.f;
-      if constexpr (WT == CCQ_F16) {
+    }
+    float m = 0.f;
 #pragma unroll
-        for (int off = 1; off < 8; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        const int ex = lr_exponent(m);
-        up = ldexpf(1.f, ex);
-        down = ldexpf(1.f, -ex);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = across * i + 8 * j + e < rank ? v[i][e] * scale : 0.f;
+        m = isfinite(v[i][e]) ? fmaxf(m, fabsf(v[i][e])) : m;
       }
-      if (j == 0) downs[row] = down;
+    float up = 1.f, down = 1.f;
+    if constexpr (WT == CCQ_F16) {
+      for (int off = 1; off < 1 << sh; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      const int ex = lr_exponent(m);
+      up = ldexpf(1.f, ex);
+      down = ldexpf(1.f, -ex);
+    }
+    if (j == 0) downs[row] = down;
+    for (int r = 8 * j, i = 0; i < 4; ++i, r += across) {
+      if (r < 32 * rc) {
+        V pv[PARTS];
+        float u[8];
 #pragma unroll
-      for (int i = 0; i < LR_MAX_R / 64; ++i) {
-        const int r = 64 * i + 8 * j;
-        if (r < 32 * rc) {
-          V pv[PARTS];
+        for (int e = 0; e < 8; ++e) u[e] = (i == 0 ? v[0][e] : i == 1 ? v[1][e] : i == 2 ? v[2][e] : v[3][e]) * up;
+        lr_split<WT, PARTS>(u, pv);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] *= up;
-          lr_split<WT, PARTS>(v[i], pv);
-#pragma unroll
-          for (int k = 0; k < PARTS; ++k) *reinterpret_cast<V*>(parts + (k * TM + row) * ld + r) = pv[k];
-        }
+        for (int k = 0; k < PARTS; ++k) *reinterpret_cast<V*>(parts + (k * TM + row) * ld + r) = pv[k];
       }
     }
   }
   __syncthreads();
-  int64_t yrow[MT];
-  bool own[MT];
+  float(*mine)[64 + 4] = turn[wave];
+  for (int s = 0; s < steps; s += 2) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int id = tl.rows[16 * m + c16];
-    own[m] = id >= 0;
-    yrow[m] = (int64_t)(id >= 0 ? id : tl.rows[0]) * p.ldy;
-  }
-  const int end = min((group + 1) * p.ncols, p.N);
-  for (int n0 = group * p.ncols + 64 * wave; n0 < end; n0 += 64 * LR_WAVES) {
-    YBlock<YT> y[MT];
-    f32x4 acc[MT][4];
+    for (int d = 0; d < 2; ++d) {
+      const int step = s + d;
+      if (step >= steps) break;
+      const int next = step + 1 < steps ? step + 1 : step;  // (the last one's again: not used)
+      fetch(next, y[d ^ 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      const int n0 = block_of(step), m0 = (step % PAIRS) * MP;
+      f32x4 acc[MP][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      y[m].load(p.y, yrow[m], n0, g, p.N);
+      for (int m = 0; m < MP; ++m)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) acc[m][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int c = 0; c < rc; ++c) {
-      Raw<WT> w[4];
-      lr_load_b<WT, YT>(p, adapter, rank, n0, 32 * c, w);
-      if (32 * c + 32 > rank) {  // the padding behind the rank may hold anything
+        for (int q = 0; q < 4; ++q) acc[m][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < rc; ++c) {
+        Raw<WT> after[4];  // the next chunk's, or the next step's first
+        load_b(c + 1 < rc ? n0 : block_of(next), c + 1 < rc ? c + 1 : 0, after);
+        __builtin_amdgcn_sched_barrier(0);
+        lr_fix_b<WT>(p, adapter, rank, 32 * c, [&](int q) { return n0 + 16 * q + c16; }, w);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) lr_mask<WT>(w[q], rank - 32 * c - 8 * g);
+        for (int m = 0; m < MP; ++m) {
+          V pv[PARTS];
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k)
+            pv[k] = *reinterpret_cast<const V*>(parts + (k * TM + 16 * (m0 + m) + c16) * ld + 32 * c + 8 * g);
+          lr_expand_step<WT, PARTS>(w, pv, acc[m]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = after[q];
       }
+      lr_lane_exchange();
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        V pv[PARTS];
+      for (int m = 0; m < MP; ++m)
 #pragma unroll
-        for (int k = 0; k < PARTS; ++k)
-          pv[k] = *reinterpret_cast<const V*>(parts + (k * TM + 16 * m + c16) * ld + 32 * c + 8 * g);
-        lr_expand_step<WT, PARTS>(w, pv, acc[m]);
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&mine[16 * m + c16][16 * q + 4 * g]) = acc[m][q];
+      lr_lane_exchange();
+#pragma unroll
+      for (int i = 0; i < YN; ++i) {
+        const int row = RI * i + yr, id = tl.rows[16 * m0 + row];
+        float add[COLS];
+        const float f = downs[16 * m0 + row];
+#pragma unroll
+        for (int e = 0; e < COLS; e += 4) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(&mine[row][yc + e]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) add[e + k] = v[k] * f;
+        }
+        if (id >= 0) y[d][i].add_store(p.y, p.y_dtype, (int64_t)id * p.ldy, n0 + yc, p.N, add);
       }
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (own[m]) lr_store<YT>(p, y[m], yrow[m], n0, g, acc[m], downs[16 * m + c16]);
   }
+}
+
+// Buffers of fewer than 8 values (no 16-byte load fits them): one thread per
+// value of y, sums in 64 bits.
+__device__ __forceinline__ float lr_value(const void* v, int64_t i, int dt) {
+  if (dt == CCQ_F32) return reinterpret_cast<const float*>(v)[i];
+  const uint32_t u = reinterpret_cast<const uint16_t*>(v)[i];
+  return dt == CCQ_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+}
+__global__ __launch_bounds__(256) void lora_tiny_kernel(const LoraP p, int x_dtype, int w_dtype) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t adapter = p.index[blockIdx.y];
+  if (n >= p.N || adapter < 0 || adapter >= p.L) return;
+  const int rank = lr_rank(p, (int)adapter);
+  if (rank == 0) return;
+  double sum = 0;
+  for (int r = 0; r < rank; ++r) {
+    double inner = 0;
+    for (int k = 0; k < p.K; ++k)
+      inner += (double)lr_value(p.x, blockIdx.y * p.ldx + k, x_dtype) *
+               (double)lr_value(p.a, (adapter * p.R + r) * p.K + k, w_dtype);
+    sum += inner * (double)lr_value(p.b, (adapter * p.N + n) * p.R + r, w_dtype);
+  }
+  const int64_t at = blockIdx.y * p.ldy + n;
+  const float v = (float)(lr_value(p.y, at, p.y_dtype) + sum * (p.scale != nullptr ? p.scale[adapter] : 1.f));
+  if (p.y_dtype == CCQ_F32)
+    reinterpret_cast<float*>(p.y)[at] = v;
+  else
+    reinterpret_cast<uint16_t*>(p.y)[at] =
+        (uint16_t)(p.y_dtype == CCQ_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
 }
 
 size_t a256l(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -705,22 +1046,25 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool one_type) {
   L.align = T > LR_SELF;
   L.tm = T <= LR_THREADS ? 16 : 64;
   L.tiles = ccq_moe_align_max_tiles(T, ad->num_adapters, L.tm);
-  // 8 waves x 64 columns for a workgroup, or a multiple where that still gives two workgroups per CU
+  // columns per workgroup: 64 for each wave, or a multiple where that still fills the CUs
+  const int64_t unit = L.fused ? 64 * LR_WAVES : LE_THREADS;
   const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm);
-  int64_t groups = cdiv(N, 512);
-  const int64_t want = cdiv(512, likely);
-  if (groups > want) groups = want;
-  L.ncols = cdiv(cdiv(N, groups), 512) * 512;
+  const int64_t want = (L.fused ? 256 : 768) / likely;
+  int64_t groups = cdiv(N, unit);
+  if (groups > want) groups = want < 1 ? 1 : want;
+  L.ncols = cdiv(cdiv(N, groups), unit) * unit;
   if (L.fused) {
     L.S = 1;
     L.kchunk = cdiv(cdiv(K, 32), LR_WAVES) * 32;
     return L;
   }
-  int64_t S = cdiv(512, likely);
+  int64_t S = 256 / L.tiles;  // one workgroup on a CU, all at once
   const int64_t most = cdiv(K, LR_WAVES * 64);
   S = S < most ? S : most;
   S = S < 8 ? S : 8;
-  L.kchunk = cdiv(cdiv(K, S), 32) * 32;
+  S = S < 1 ? 1 : S;
+  const int64_t step = L.tm == 16 ? 32 : 256;  // the largest stage of a 64-token tile
+  L.kchunk = cdiv(cdiv(K, S), step) * step;
   L.S = cdiv(K, L.kchunk);
   size_t o = 0;
   L.off_rows = o;
@@ -756,7 +1100,7 @@ int check_adapters(const ccq_lora_adapters* ad, const char* name) {
 template <int XT, int WT, int YT>
 void fused_launch(const LoraP& p, int64_t groups, hipStream_t st) {
   const int rt = (int)cdiv(p.R, 16);
-  const dim3 grid((unsigned)(p.tiles * groups)), block(LR_THREADS);
+  const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * groups)), block(LR_THREADS);
   if (rt <= 1)
     launch((lora_fused_kernel<XT, WT, YT, 1>), grid, block, 0, st, p);
   else if (rt <= 2)
@@ -778,21 +1122,40 @@ void fused_dispatch(const LoraP& p, int64_t groups, hipStream_t st) {
 template <int XT, int WT, int MT>
 void shrink_launch(const LoraP& p, hipStream_t st) {
   const int rt = (int)cdiv(p.R, 16);
-  const dim3 block(LR_THREADS);
-  const unsigned x = (unsigned)(p.tiles * p.S);
+  const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * p.S), 1, (unsigned)cdiv(rt, 8)), block(LR_THREADS);
   if (rt <= 1)
-    launch((lora_shrink_kernel<XT, WT, MT, 1>), dim3(x), block, 0, st, p);
+    launch((lora_shrink_kernel<XT, WT, MT, 1, 1>), grid, block, 0, st, p);
   else if (rt <= 2)
-    launch((lora_shrink_kernel<XT, WT, MT, 2>), dim3(x), block, 0, st, p);
+    launch((lora_shrink_kernel<XT, WT, MT, 2, 1>), grid, block, 0, st, p);
   else if (rt <= 4)
-    launch((lora_shrink_kernel<XT, WT, MT, 4>), dim3(x), block, 0, st, p);
+    launch((lora_shrink_kernel<XT, WT, MT, 4, 1>), grid, block, 0, st, p);
   else
-    launch((lora_shrink_kernel<XT, WT, MT, 8>), dim3(x, 1, (unsigned)cdiv(rt, 8)), block, 0, st, p);
+    launch((lora_shrink_kernel<XT, WT, MT, 4, 2>), grid, block, 0, st, p);
+}
+
+// 64-token tiles whose rows' 16-byte pieces are aligned
+template <int XT, int WT>
+void shrink_tile_launch(const LoraP& p, hipStream_t st) {
+  const int rt = (int)cdiv(p.R, 16);
+  const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * p.S), 1, (unsigned)cdiv(rt, 8)), block(LR_THREADS);
+  if (rt <= 1)
+    launch((lora_shrink_tile_kernel<XT, WT, 1>), grid, block, 0, st, p);
+  else if (rt <= 2)
+    launch((lora_shrink_tile_kernel<XT, WT, 2>), grid, block, 0, st, p);
+  else if (rt <= 4)
+    launch((lora_shrink_tile_kernel<XT, WT, 4>), grid, block, 0, st, p);
+  else
+    launch((lora_shrink_tile_kernel<XT, WT, 8>), grid, block, 0, st, p);
+}
+bool shrink_tile_ok(const LoraP& p, int x_dtype) {
+  const int64_t e = x_dtype == CCQ_F32 ? 4 : 2;
+  return p.K % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16) && p.ldx * e % 16 == 0 &&
+         ((int64_t)p.T * p.ldx) * e < ((int64_t)1 << 32);
 }
 
 template <int WT, int MT>
 void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
-  const dim3 grid((unsigned)(p.tiles * groups)), block(LR_THREADS);
+  const dim3 grid((unsigned)(p.tiles * groups)), block(LE_THREADS);
   const size_t ld = (size_t)cdiv(p.R, 32) * 32 + 8, part = ld * 16 * MT * 2;
   if (p.y_dtype == CCQ_F32)
     launch((lora_expand_kernel<WT, CCQ_F32, MT>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2), st, p);
@@ -802,7 +1165,14 @@ void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
 
 template <int WT, int MT>
 int two_launches(const LoraP& p, int x_dtype, int64_t groups, hipStream_t st) {
-  if (x_dtype == CCQ_BF16)
+  if (MT == 4 && shrink_tile_ok(p, x_dtype)) {
+    if (x_dtype == CCQ_BF16)
+      shrink_tile_launch<CCQ_BF16, WT>(p, st);
+    else if (x_dtype == CCQ_F16)
+      shrink_tile_launch<CCQ_F16, WT>(p, st);
+    else
+      shrink_tile_launch<CCQ_F32, WT>(p, st);
+  } else if (x_dtype == CCQ_BF16)
     shrink_launch<CCQ_BF16, WT, MT>(p, st);
   else if (x_dtype == CCQ_F16)
     shrink_launch<CCQ_F16, WT, MT>(p, st);
@@ -867,6 +1237,13 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
   p.tiles = (int)L.tiles;
   p.ncols = (int)L.ncols;
   p.y_dtype = y_dtype;
+  p.last_x = (T - 1) * ldx + p.K - 8;
+  p.last_a = ad->num_adapters * ad->rank_max * ad->in_features - 8;
+  p.last_b = ad->num_adapters * ad->rank_max * ad->out_features - 8;
+  if (p.last_x < 0 || p.last_a < 0 || p.last_b < 0) {
+    launch(lora_tiny_kernel, dim3((unsigned)cdiv(p.N, 256), (unsigned)T), dim3(256), 0, st, p, x_dtype, ad->dtype);
+    return launch_status("ccq_lora_add");
+  }
   if (L.fused) {
     if (ad->dtype == CCQ_BF16) {
       if (x_dtype == CCQ_F32)

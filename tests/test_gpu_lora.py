@@ -91,6 +91,15 @@ def test_inner_sizes(gpu, K):
         _check(_run(c, gpu), c)
 
 
+def test_smallest_buffers(gpu):
+    """Fewer values than one load takes, and barely as many."""
+    for T, K, N, R, L in ((1, 1, 1, 1, 1), (1, 7, 40, 3, 2), (1, 8, 40, 3, 2), (2, 3, 9, 5, 1), (3, 300, 1, 1, 7),
+                          (3, 300, 1, 1, 8), (5, 1, 77, 7, 1), (5, 2, 77, 4, 1), (2000, 1, 3, 1, 2), (700, 5, 2, 3, 2)):
+        for t in ("bf16", "f16", "f32"):
+            c = _case(T, K, N, R, L, t, "bf16" if t == "f32" else t, t)
+            _check(_run(c, gpu), c)
+
+
 @pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1000, 14336])
 def test_outer_sizes(gpu, N):
     for T, t in ((1, "bf16"), (20, "f16"), (5, "f32")):
