@@ -16,6 +16,7 @@ themselves (for a router or adapters beside a quantized projection).
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -40,67 +41,89 @@ class QuantizedRows(NamedTuple):
     residual: torch.Tensor | None
 
 
-def _rows(t: torch.Tensor, what: str, like: torch.Tensor) -> torch.Tensor:
-    """A [rows, H] view of ``t`` for the kernel, which takes row strides."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}; x is {like.dtype} "
-                         f"{tuple(like.shape)} on {like.device}")
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A [rows, H] view of ``t`` and its row stride (a single row's stride has
+    no meaning and may be any)."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+    if t.shape[0] <= 1:
+        return (t if t.stride(1) == 1 else t.contiguous()), t.shape[1]
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0)
 
 
-def _ld(t: torch.Tensor) -> int:
-    """The row stride (a single row's stride has no meaning and may be any)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _unlike(t: torch.Tensor, what: str, x: torch.Tensor) -> ValueError:
+    return ValueError(f"{what} is {t.dtype} {tuple(t.shape)} on {t.device}; x is {x.dtype} {tuple(x.shape)} on "
+                      f"{x.device}")
 
 
 def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, y_dtype, q_fmt: int):
-    if not x.is_cuda:
-        raise ValueError(f"Expected a cuda device, but got: {x.device}")
-    if x.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
+    index = x.get_device()
+    if not _dev.is_current(index):
+        with torch.cuda.device(index):
             return _norm(x, weight, eps, residual, residual_out, y_dtype, q_fmt)
-    if x.dtype not in _dev.DTYPE_CODE:
-        raise ValueError(f"rows must be float32, float16 or bfloat16, got {x.dtype}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_H:
-        raise ValueError(f"rows must be [..., H] with 1 <= H <= {MAX_H}, got {tuple(x.shape)}")
-    H = x.shape[-1]
+    dtype, shape = x.dtype, x.shape
+    code = _dev.DTYPE_CODE.get(dtype)
+    if code is None:
+        raise ValueError(f"rows must be float32, float16 or bfloat16, got {dtype}")
+    H = shape[-1] if shape else 0
+    if not 1 <= H <= MAX_H:
+        raise ValueError(f"rows must be [..., H] with 1 <= H <= {MAX_H}, got {tuple(shape)}")
     if q_fmt == CCQ_Q_FP8_BLOCK and H % 128:
         raise ValueError(f"FP8 rows need H % 128 == 0, got H={H}")
-    if not eps > 0 or eps == float("inf"):
+    if not 0 < eps < math.inf:
         raise ValueError(f"eps must be positive and finite, got {eps}")
-    if weight.shape != (H,) or weight.dtype not in _dev.DTYPE_CODE or weight.device != x.device:
+    wcode = _dev.DTYPE_CODE.get(weight.dtype)
+    if wcode is None or weight.shape != (H,) or weight.get_device() != index:
         raise ValueError(f"weight must be [{H}] float32, float16 or bfloat16 on {x.device}, got {weight.dtype} "
                          f"{tuple(weight.shape)} on {weight.device}")
-    weight = weight.contiguous()
-    x2 = _rows(x, "x", x)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    flat = len(shape) == 2
+    x2, ldx = (x, H) if flat and x.is_contiguous() else _rows(x)
     T = x2.shape[0]
-    r2 = o2 = None
+    rp = op = None
+    ldr = ldo = 0
     if residual is not None:
-        r2 = _rows(residual, "residual", x)
+        if residual.shape != shape or residual.dtype != dtype or residual.get_device() != index:
+            raise _unlike(residual, "residual", x)
+        r2, ldr = (residual, H) if flat and residual.is_contiguous() else _rows(residual)
+        rp = r2.data_ptr()
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        o2 = _rows(residual_out, "residual_out", x)
-        if o2.data_ptr() != residual_out.data_ptr():  # a copy, so not a view that could be written
-            raise ValueError("residual_out must hold its rows one after the other, each of them dense")
+            residual_out = _dev.empty_strided((T, H), (H, 1), dtype)
+            op, ldo = residual_out.data_ptr(), H
+            if not flat:
+                residual_out = residual_out.view(shape)
+        else:
+            if residual_out.shape != shape or residual_out.dtype != dtype or residual_out.get_device() != index:
+                raise _unlike(residual_out, "residual_out", x)
+            o2, ldo = _rows(residual_out)
+            op = o2.data_ptr()
+            if op != residual_out.data_ptr():  # a copy, so not a view that could be written
+                raise ValueError("residual_out must hold its rows one after the other, each of them dense")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    y = torch.empty(x.shape, dtype=y_dtype, device=x.device) if y_dtype is not None else None
-    q = scale = None
+    y = q = scale = yp = qp = sp = None
+    ycode = 0
+    if y_dtype is not None:
+        y = _dev.empty_strided((T, H), (H, 1), y_dtype)
+        yp, ycode = y.data_ptr(), _dev.DTYPE_CODE[y_dtype]
     if q_fmt == CCQ_Q_FP8_BLOCK:
-        q = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-        scale = torch.empty((*x.shape[:-1], H // 128), dtype=torch.float32, device=x.device)
+        q = _dev.empty_strided((T, H), (H, 1), torch.uint8)
+        scale = _dev.empty_strided((T, H >> 7), (H >> 7, 1), torch.float32)
+        qp, sp = q.data_ptr(), scale.data_ptr()
     elif q_fmt == CCQ_Q_INT8_ROW:
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    call("ccq_rms_norm", x2.data_ptr(), _dev.DTYPE_CODE[x.dtype], _ld(x2),
-         r2.data_ptr() if r2 is not None else None, _ld(r2) if r2 is not None else 0,
-         weight.data_ptr(), _dev.DTYPE_CODE[weight.dtype], eps,
-         o2.data_ptr() if o2 is not None else None, _ld(o2) if o2 is not None else 0,
-         y.data_ptr() if y is not None else None, _dev.DTYPE_CODE[y_dtype] if y is not None else 0, q_fmt,
-         q.data_ptr() if q is not None else None, scale.data_ptr() if scale is not None else None, T, H,
-         _dev.stream_ptr(x.device))
+        q = _dev.empty_strided((T, H), (H, 1), torch.int8)
+        scale = _dev.empty_strided((T,), (1,), torch.float32)
+        qp, sp = q.data_ptr(), scale.data_ptr()
+    call("ccq_rms_norm", x2.data_ptr(), code, ldx, rp, ldr, weight.data_ptr(), wcode, eps, op, ldo, yp, ycode, q_fmt,
+         qp, sp, T, H, _dev.raw_stream(index))
+    if not flat:
+        lead = shape[:-1]
+        y = y.view(shape) if y is not None else None
+        if q is not None:
+            q, scale = q.view(shape), scale.view(*lead, H >> 7) if q_fmt == CCQ_Q_FP8_BLOCK else scale.view(lead)
     return q, scale, y, residual_out
 
 

@@ -78,14 +78,14 @@ def _rows(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
 
 
 def _dense_rows(t: torch.Tensor) -> bool:
-    return t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) or t.numel() == 0
+    return t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1]
 
 
 def _overlap(y: torch.Tensor, x: torch.Tensor) -> bool:
     """Whether rows of y and x share memory (column ranges of one buffer do
     not, though their address ranges cross)."""
-    ye, xe = y.element_size(), x.element_size()
     y0, x0 = y.data_ptr(), x.data_ptr()
+    ye, xe = y.element_size(), x.element_size()
     T = y.shape[0]
     yl, xl = (y.stride(0) * ye, x.stride(0) * xe) if T > 1 else (0, 0)
     yw, xw = y.shape[1] * ye, x.shape[1] * xe
@@ -105,18 +105,19 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
     the same leading dimensions, at most 65536 rows.  An index outside [0, L)
     means no adapter: that row is left as it is.  ``y`` must not overlap
     ``x``.  Repeated calls give the same bits (no atomics)."""
-    stream = _dev.stream_ptr(y.device)
-    if y.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(y.device):
+    dev = y.get_device()
+    if not _dev.is_current(dev):
+        with torch.cuda.device(dev):
             return add_(y, x, adapters, index)
-    dev = y.device
-    if x.device != dev or index.device != dev or adapters.device != dev:
-        raise ValueError(f"y on {dev}, x on {x.device}, index on {index.device}, adapters on {adapters.device}")
-    if x.shape[:-1] != y.shape[:-1] or index.shape != y.shape[:-1]:
+    if x.get_device() != dev or index.get_device() != dev or adapters.device.index != dev:
+        raise ValueError(f"y on {y.device}, x on {x.device}, index on {index.device}, adapters on {adapters.device}")
+    lead = y.shape[:-1]
+    if x.shape[:-1] != lead or index.shape != lead:
         raise ValueError(f"leading dimensions of y {tuple(y.shape)}, x {tuple(x.shape)} and index "
                          f"{tuple(index.shape)} differ")
     y2, x2 = _rows(y, adapters.out_features, "y"), _rows(x, adapters.in_features, "x")
-    if y2.data_ptr() != y.data_ptr() or not _dense_rows(y2):
+    yp = y2.data_ptr()
+    if yp != y.data_ptr() or not _dense_rows(y2):
         raise ValueError("y must hold its rows one after the other, each of them dense (it is written in place)")
     if not _dense_rows(x2):
         x2 = x2.contiguous()
@@ -129,12 +130,14 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
         raise ValueError(f"{T} rows: at most {MAX_TOKENS}")
     if T == 0:
         return y
+    ldx, ldy = (x2.stride(0), y2.stride(0)) if T > 1 else (adapters.in_features, adapters.out_features)
     if _overlap(y2, x2):
         raise ValueError("y overlaps x")
     nbytes = adapters.workspace_size(T, x2.dtype)
-    # this call's own scratch, so that calls on several streams or in several graphs do not share it
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    call("ccq_lora_add", x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype], x2.stride(0) if T > 1 else x2.shape[1],
-         index.data_ptr(), y2.data_ptr(), _dev.DTYPE_CODE[y2.dtype], y2.stride(0) if T > 1 else y2.shape[1], T,
-         adapters._desc, ws.data_ptr() if ws is not None else None, nbytes, stream)
+    wp = None
+    if nbytes:  # this call's own scratch, so that calls on several streams or in several graphs do not share it
+        ws = _dev.empty_strided((nbytes,), (1,), torch.uint8)
+        wp = ws.data_ptr()
+    call("ccq_lora_add", x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype], ldx, index.data_ptr(), yp,
+         _dev.DTYPE_CODE[y2.dtype], ldy, T, adapters._desc, wp, nbytes, _dev.raw_stream(dev))
     return y

@@ -1048,7 +1048,7 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool one_type) {
   L.tiles = ccq_moe_align_max_tiles(T, ad->num_adapters, L.tm);
   // columns per workgroup: 64 for each wave, or a multiple where that still fills the CUs
   const int64_t unit = L.fused ? 64 * LR_WAVES : LE_THREADS;
-  const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm);
+  const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm) + (L.tiles - cdiv(T, L.tm)) / 2;
   const int64_t want = (L.fused ? 256 : 768) / likely;
   int64_t groups = cdiv(N, unit);
   if (groups > want) groups = want < 1 ? 1 : want;
@@ -1058,11 +1058,14 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool one_type) {
     L.kchunk = cdiv(cdiv(K, 32), LR_WAVES) * 32;
     return L;
   }
-  int64_t S = 256 / L.tiles;  // one workgroup on a CU, all at once
-  const int64_t most = cdiv(K, LR_WAVES * 64);
-  S = S < most ? S : most;
-  S = S < 8 ? S : 8;
-  S = S < 1 ? 1 : S;
+  // splits of K (one workgroup fits a CU): the fewest that keep the rounds of the CUs, each as long as its part of K
+  // and a start worth 512 k, within 5% of the shortest
+  const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
+  auto rounds = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512); };
+  double best = rounds(1);
+  for (int64_t s = 2; s <= most; ++s) best = rounds(s) < best ? rounds(s) : best;
+  int64_t S = 1;
+  while (rounds(S) > 1.05 * best) ++S;
   const int64_t step = L.tm == 16 ? 32 : 256;  // the largest stage of a 64-token tile
   L.kchunk = cdiv(cdiv(K, S), step) * step;
   L.S = cdiv(K, L.kchunk);
