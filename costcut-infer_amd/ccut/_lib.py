@@ -143,7 +143,7 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_fp8_block_linear_quantized": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
     "ccq_rms_norm": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _int, ctypes.c_float, _vp, _i64, _vp, _int, _int, _vp,
                             _vp, _i64, _i64, _vp]),
-    "ccq_lora_workspace_size": (_sz, [_i64, _int, ctypes.POINTER(ccq_lora_adapters)]),
+    "ccq_lora_workspace_size": (_sz, [_vp, _int, _i64, _i64, ctypes.POINTER(ccq_lora_adapters)]),
     "ccq_lora_add": (_int, [_vp, _int, _i64, _vp, _vp, _int, _i64, _i64, ctypes.POINTER(ccq_lora_adapters), _vp, _sz,
                             _vp]),
     "ccq_moe_fp8_workspace_size": (_sz, [_i64, _i64, ctypes.POINTER(ccq_fp8_experts)]),

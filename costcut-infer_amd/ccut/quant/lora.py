@@ -60,12 +60,12 @@ class LoraAdapters:
             raise ValueError(f"{what} must have one entry per adapter ({L}), got {tuple(t.shape)}")
         return t.to(device=device, dtype=dtype).contiguous()
 
-    def workspace_size(self, T: int, x_dtype: torch.dtype) -> int:
-        """Bytes of scratch that ``add_`` of T rows takes."""
-        n = self._bytes.get((T, x_dtype))
+    def workspace_size(self, xp: int, x_code: int, ldx: int, T: int) -> int:
+        """Bytes of scratch that ``add_`` takes for T rows of x at ``xp``."""
+        key = (T, x_code, ldx, xp & 15)
+        n = self._bytes.get(key)
         if n is None:
-            n = int(lib().ccq_lora_workspace_size(T, _dev.DTYPE_CODE[x_dtype], self._desc))
-            self._bytes[T, x_dtype] = n
+            n = self._bytes[key] = int(lib().ccq_lora_workspace_size(xp, x_code, ldx, T, self._desc))
         return n
 
 
@@ -133,11 +133,12 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
     ldx, ldy = (x2.stride(0), y2.stride(0)) if T > 1 else (adapters.in_features, adapters.out_features)
     if _overlap(y2, x2):
         raise ValueError("y overlaps x")
-    nbytes = adapters.workspace_size(T, x2.dtype)
+    xp, xcode = x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype]
+    nbytes = adapters.workspace_size(xp, xcode, ldx, T)
     wp = None
     if nbytes:  # this call's own scratch, so that calls on several streams or in several graphs do not share it
         ws = _dev.empty_strided((nbytes,), (1,), torch.uint8)
         wp = ws.data_ptr()
-    call("ccq_lora_add", x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype], ldx, index.data_ptr(), yp,
+    call("ccq_lora_add", xp, xcode, ldx, index.data_ptr(), yp,
          _dev.DTYPE_CODE[y2.dtype], ldy, T, adapters._desc, wp, nbytes, _dev.raw_stream(dev))
     return y

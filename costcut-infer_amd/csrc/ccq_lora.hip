@@ -126,14 +126,13 @@ struct TileS {
   int adapter, first;           // first: the tile's place among its adapter's
   int rows[TM];
 };
-template <int CH>
 struct SortS {
   int count[LR_MAX_L];
   int sum[LR_WAVES];
 };
 
 template <int TM, int CH>
-__device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS<CH>& s) {
+__device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int key[CH];
 #pragma unroll
@@ -465,7 +464,17 @@ __device__ __forceinline__ void lr_load_b(const LoraP& p, int adapter, int c, F 
 template <int WT, typename F>
 __device__ __forceinline__ void lr_fix_b(const LoraP& p, int adapter, int rank, int c, F col, Raw<WT> (&w)[4]) {
   const int r = c + 8 * ((threadIdx.x >> 4) & 3);
-  if (c + 32 > rank) {
+  if (c + 32 <= rank) return;
+  if (p.R % 8 == 0) {  // whole pieces: the same mask for all rows
+    uint32_t keep[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      keep[e] = (r + 2 * e < rank ? 0xFFFFu : 0u) | (r + 2 * e + 1 < rank ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[q].v[0][e] &= keep[e];
+  } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       lr_fix<WT>(w[q], ((int64_t)adapter * p.N + min(col(q), p.N - 1)) * p.R + r, p.last_b, rank - r);
@@ -484,63 +493,144 @@ __device__ __forceinline__ void lr_expand_step(const Raw<WT> (&w)[4], const type
 }
 
 // ------------------------------------------------------ one kernel (fused) --
-// A workgroup: a tile of 16 tokens, ncols columns.  Its 8 waves split K, add
-// their sums in LDS, and take blocks of 64 columns each; the first block's
-// weights and y are loaded before the first product.
+// A workgroup: a tile of 16 tokens, ncols columns.  The lines (64 k) of x and A
+// are dealt to its 8 waves, each copying its own into its part of LDS, D of
+// them ahead, and multiplying them without a barrier: a load that takes 8 rows
+// x 128 bytes reads 145 GB/s on a CU (131 KB by 8 waves, from L2), the
+// operands' own 16 rows x 64 bytes 40 GB/s.  The sums meet in LDS; the waves
+// then take blocks of 64 columns each, the first one's weights and y loaded
+// before the first product.  Rows are aligned to 16 bytes here.  In a line the
+// 16-byte piece i of row r lies at i ^ (r & 7), so that the operand reads of 8
+// neighbouring lanes cover all banks.
 template <int XT, int WT, int YT, int RT>
 __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   using V = typename Half<WT>::vec;
   constexpr int PARTS = WT == CCQ_F16 ? 2 : YT == CCQ_F32 ? 3 : 2, RC = (RT + 1) / 2;
+  constexpr int E = XT == CCQ_F32 ? 4 : 2, XL = E / 2;  // lines of x for 64 k
+  constexpr int BYTES = (XL + RT) * 2048, NI = BYTES / 1024, D = 18 * 1024 / BYTES;
+  static_assert(D >= 2 && D <= 4 && D * BYTES >= RT * 1024);
   __shared__ TileS<16> tl;
-  __shared__ union {
-    SortS<1> sort;
+  __shared__ __align__(16) union {
+    SortS sort;
+    char ring[LR_WAVES][D][BYTES];
     f32x4 red[LR_WAVES][RT][64];
   } u;
   __shared__ __align__(16) float ps[16][32 * RC + 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
   // all workgroups of a tile on one XCD, whose L2 then holds its A
   const int t8 = (p.tiles + 7) & ~7, tile = blockIdx.x % t8, group = blockIdx.x / t8;
   if (tile >= p.tiles) return;
-  int adapter, own, tok;  // padding: the first row again, not stored
+  int adapter, rows;  // lane r < 16: the tile's row r
   if (p.T <= 64) {
-    const int rows = lr_find_tile_wave(p, tile, adapter);
-    own = __shfl(rows, c16, 64);
-    tok = own >= 0 ? own : __shfl(rows, 0, 64);
+    rows = lr_find_tile_wave(p, tile, adapter);
   } else {
     lr_find_tile<16, 1>(p, tile, tl, u.sort);
     adapter = tl.adapter;
-    own = tl.rows[c16];
-    tok = own >= 0 ? own : tl.rows[0];
+    rows = tl.rows[c16];
   }
+  adapter = __builtin_amdgcn_readfirstlane(adapter);
   if (adapter < 0) return;
-  const int rank = lr_rank(p, adapter);
+  const int rank = __builtin_amdgcn_readfirstlane(lr_rank(p, adapter));
   if (rank == 0) return;
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
-  const int64_t xrow[1] = {(int64_t)tok * p.ldx}, yrow = (int64_t)tok * p.ldy;
-  int64_t arow[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) arow[t] = ((int64_t)adapter * p.R + min(16 * t + c16, rank - 1)) * p.K;
+  const int own = __shfl(rows, c16, 64), row0 = __shfl(rows, 0, 64);
+  const int64_t yrow = (int64_t)(own >= 0 ? own : row0) * p.ldy;  // padding: the first row again, not stored
+
   const int end = min((group + 1) * p.ncols, p.N);
   int n0 = group * p.ncols + 64 * wave;
+  auto col = [&](int q) { return n0 + lr_col<YT>(q, c16); };
   Raw<WT> w[RC][4];
   YPiece<YT> y[16 / YPiece<YT>::COLS];
   auto fetch = [&]() {
 #pragma unroll
-    for (int c = 0; c < RC; ++c) lr_load_b<WT>(p, adapter, 32 * c, [&](int q) { return n0 + lr_col<YT>(q, c16); }, w[c]);
+    for (int c = 0; c < RC; ++c) lr_load_b<WT>(p, adapter, 32 * c, col, w[c]);
 #pragma unroll
     for (int i = 0; i < 16 / YPiece<YT>::COLS; ++i) y[i].load(p.y, yrow, n0 + lr_piece_col<YT>(i, g), p.N);
   };
   if (n0 < end) fetch();
+  if (p.T > 64) __syncthreads();  // the sort's LDS is free
+
+  const int lines = (p.K + 63) / 64, n = lines > wave ? (lines - wave + LR_WAVES - 1) / LR_WAVES : 0;
+  const int piece = (lane & 7) ^ (lane >> 3);
+  uint32_t off[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = 8 * (i & 1) + (lane >> 3);
+    if (i < 2 * XL) {
+      const int id = __shfl(rows, r, 64);
+      off[i] = (uint32_t)((int64_t)(id >= 0 ? id : row0) * p.ldx * E) + (i >> 1) * 128 + 16 * piece;
+    } else {
+      off[i] = (uint32_t)min(16 * ((i >> 1) - XL) + r, rank - 1) * (uint32_t)p.K * 2 + 16 * piece;
+    }
+  }
+  const char* xb = reinterpret_cast<const char*>(p.x) + wave * 64 * E;
+  const char* ab = reinterpret_cast<const char*>(p.a) + ((int64_t)adapter * p.R * p.K + wave * 64) * 2;
+  const uint32_t lds0 = lds_addr(&u.ring[wave][0][0]);
+  auto issue = [&](int s, int slot) {
+    const int k = (s * LR_WAVES + wave) * 64;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t o = off[i];
+      if (k + 64 > p.K) {  // a piece past the end of its row: the line's first piece again, masked below
+        const int in = (i < 2 * XL ? ((i >> 1) * 128 + 16 * piece) / E : 8 * piece);
+        if (k + in >= p.K) o -= (i < 2 * XL ? (i >> 1) * 128 : 0) + 16 * piece;
+      }
+      dma16(i < 2 * XL ? xb + (int64_t)s * LR_WAVES * 64 * E : ab + (int64_t)s * LR_WAVES * 128, o,
+            lds0 + slot * BYTES + i * 1024);
+    }
+  };
   f32x4 acc[1][RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int k0 = wave * p.kchunk;
-  lr_shrink<XT, WT, 1, RT, (RT == 1 ? 16 : RT == 8 ? 2 : RT == 4 ? 4 : 8) / (XT == CCQ_F32 ? 2 : 1)>(p, xrow, arow, k0, min(k0 + p.kchunk, p.K), acc);
-  __syncthreads();
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < n) issue(d, d);
+  int slot = 0;
+  for (int s = 0; s < n; ++s) {
+    const int after = min(D, n - s) - 1;  // stages in flight behind this one
+    if (after == 0)
+      wait_vmcnt<0>();
+    else if (after == 1)
+      wait_vmcnt<NI>();
+    else if (after == 2)
+      wait_vmcnt<2 * NI>();
+    else
+      wait_vmcnt<3 * NI>();
+    asm volatile("" ::: "memory");
+    const char* st = u.ring[wave][slot];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Raw<XT> xr[1];
+      Raw<WT> ar[RT];
+      if constexpr (XT == CCQ_F32) {
+        const char* line = st + h * 2048 + c16 * 128;
+        xr[0].v[0] = *reinterpret_cast<const u32x4*>(line + (((2 * g) ^ (c16 & 7)) * 16));
+        xr[0].v[1] = *reinterpret_cast<const u32x4*>(line + (((2 * g + 1) ^ (c16 & 7)) * 16));
+      } else {
+        xr[0].v[0] = *reinterpret_cast<const u32x4*>(st + c16 * 128 + (((4 * h + g) ^ (c16 & 7)) * 16));
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        ar[t].v[0] = *reinterpret_cast<const u32x4*>(st + (XL + t) * 2048 + c16 * 128 + (((4 * h + g) ^ (c16 & 7)) * 16));
+      const int left = p.K - ((s * LR_WAVES + wave) * 64 + 32 * h + 8 * g);
+      if ((s * LR_WAVES + wave) * 64 + 64 > p.K) {
+        lr_fix<XT>(xr[0], 0, 0, left);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) lr_fix<WT>(ar[t], 0, 0, left);
+      }
+      lr_multiply<XT, WT, 1, RT>(xr, ar, acc);
+    }
+    if (s + D < n) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read out
+      issue(s + D, slot);
+    }
+    slot = slot == D - 1 ? 0 : slot + 1;
+  }
+  lds_barrier();
 #pragma unroll
   for (int t = 0; t < RT; ++t) u.red[wave][t][lane] = acc[0][t];
   for (int i = threadIdx.x; i < 16 * (32 * RC - 16 * RT); i += LR_THREADS) ps[i & 15][16 * RT + (i >> 4)] = 0.f;
-  __syncthreads();
+  lds_barrier();
   for (int t = wave; t < RT; t += LR_WAVES) {
     f32x4 s = u.red[0][t][lane];
 #pragma unroll
@@ -549,7 +639,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) ps[4 * g + i][16 * t + c16] = 16 * t + c16 < rank ? s[i] * scale : 0.f;
   }
-  __syncthreads();
+  lds_barrier();
   if (n0 >= end) return;
   V pv[RC][PARTS];
   float down = 1.f;
@@ -584,7 +674,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
     for (int q = 0; q < 4; ++q) out[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
-      lr_fix_b<WT>(p, adapter, rank, 32 * c, [&](int q) { return n0 + lr_col<YT>(q, c16); }, w[c]);
+      lr_fix_b<WT>(p, adapter, rank, 32 * c, col, w[c]);
       lr_expand_step<WT, PARTS>(w[c], pv[c], out);
     }
     if (own >= 0) lr_store_pieces<YT>(p, y, yrow, n0, g, out, down);
@@ -607,7 +697,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   constexpr int PASS = MT * RT * RH <= 8 ? MT : 8 / (RT * RH);  // row blocks whose sums are in LDS at once
   __shared__ TileS<TM> tl;
   __shared__ union {
-    SortS<CH> sort;
+    SortS sort;
     f32x4 red[KP][PASS][RH * RT][64];
   } u;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
@@ -707,7 +797,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
   constexpr int E = XT == CCQ_F32 ? 4 : 2;
   __shared__ TileS<64> tl;
   __shared__ __align__(16) union {
-    SortS<LR_SELF / LR_THREADS> sort;
+    SortS sort;
     char ring[D][C::BYTES];
     f32x4 red[KP][4][RT][64];
   } u;
@@ -1036,16 +1126,18 @@ struct LoraPlan {
   size_t off_rows, off_tile, off_meta, off_counts, off_align, off_p, total;
 };
 
-constexpr int64_t LR_FUSED_BYTES = 512 << 10;  // of one adapter's A
+constexpr int64_t LR_FUSED_BYTES = 256 << 10;  // of a tile's x and A that each workgroup of one kernel reads
 
-LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool one_type) {
+// lines: lora_lines, one_type: x float32 or of A's type
+LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_type) {
   LoraPlan L = {};
   const int64_t K = ad->in_features, N = ad->out_features, R = ad->rank_max;
   L.Rp = cdiv(R, 16) * 16;
-  L.fused = one_type && T <= LR_THREADS && R <= 128 && L.Rp * K * 2 <= LR_FUSED_BYTES;
+  L.fused = lines && one_type && T <= LR_THREADS && R <= 32 && (16 + L.Rp) * K * 2 <= LR_FUSED_BYTES;
   L.align = T > LR_SELF;
   L.tm = T <= LR_THREADS ? 16 : 64;
   L.tiles = ccq_moe_align_max_tiles(T, ad->num_adapters, L.tm);
+  if (L.tiles > T) L.tiles = T;  // every tile has a token
   // columns per workgroup: 64 for each wave, or a multiple where that still fills the CUs
   const int64_t unit = L.fused ? 64 * LR_WAVES : LE_THREADS;
   const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm) + (L.tiles - cdiv(T, L.tm)) / 2;
@@ -1102,16 +1194,11 @@ int check_adapters(const ccq_lora_adapters* ad, const char* name) {
 
 template <int XT, int WT, int YT>
 void fused_launch(const LoraP& p, int64_t groups, hipStream_t st) {
-  const int rt = (int)cdiv(p.R, 16);
   const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * groups)), block(LR_THREADS);
-  if (rt <= 1)
+  if (p.R <= 16)
     launch((lora_fused_kernel<XT, WT, YT, 1>), grid, block, 0, st, p);
-  else if (rt <= 2)
-    launch((lora_fused_kernel<XT, WT, YT, 2>), grid, block, 0, st, p);
-  else if (rt <= 4)
-    launch((lora_fused_kernel<XT, WT, YT, 4>), grid, block, 0, st, p);
   else
-    launch((lora_fused_kernel<XT, WT, YT, 8>), grid, block, 0, st, p);
+    launch((lora_fused_kernel<XT, WT, YT, 2>), grid, block, 0, st, p);
 }
 
 template <int XT, int WT>
@@ -1150,12 +1237,6 @@ void shrink_tile_launch(const LoraP& p, hipStream_t st) {
   else
     launch((lora_shrink_tile_kernel<XT, WT, 8>), grid, block, 0, st, p);
 }
-bool shrink_tile_ok(const LoraP& p, int x_dtype) {
-  const int64_t e = x_dtype == CCQ_F32 ? 4 : 2;
-  return p.K % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16) && p.ldx * e % 16 == 0 &&
-         ((int64_t)p.T * p.ldx) * e < ((int64_t)1 << 32);
-}
-
 template <int WT, int MT>
 void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
   const dim3 grid((unsigned)(p.tiles * groups)), block(LE_THREADS);
@@ -1167,8 +1248,8 @@ void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
 }
 
 template <int WT, int MT>
-int two_launches(const LoraP& p, int x_dtype, int64_t groups, hipStream_t st) {
-  if (MT == 4 && shrink_tile_ok(p, x_dtype)) {
+int two_launches(const LoraP& p, int x_dtype, bool lines, int64_t groups, hipStream_t st) {
+  if (MT == 4 && lines) {
     if (x_dtype == CCQ_BF16)
       shrink_tile_launch<CCQ_BF16, WT>(p, st);
     else if (x_dtype == CCQ_F16)
@@ -1187,6 +1268,12 @@ int two_launches(const LoraP& p, int x_dtype, int64_t groups, hipStream_t st) {
 }
 
 bool lora_float_code(int dt) { return dt == CCQ_F32 || dt == CCQ_F16 || dt == CCQ_BF16; }
+// rows of x and A aligned to 16 bytes, x within 32-bit offsets
+bool lora_lines(const void* x, int x_dtype, int64_t ldx, int64_t T, const ccq_lora_adapters* ad) {
+  const int64_t e = x_dtype == CCQ_F32 ? 4 : 2;
+  return ad->in_features % 8 == 0 && aligned(x, 16) && aligned(ad->a, 16) && ldx * e % 16 == 0 &&
+         ldx <= ((int64_t)1 << 32) / (T * e) - 1;
+}
 bool lora_one_type(int x_dtype, const ccq_lora_adapters* ad) { return x_dtype == CCQ_F32 || x_dtype == ad->dtype; }
 
 }  // namespace
@@ -1195,9 +1282,10 @@ bool lora_one_type(int x_dtype, const ccq_lora_adapters* ad) { return x_dtype ==
 
 using namespace ccq;
 
-extern "C" size_t ccq_lora_workspace_size(int64_t T, int x_dtype, const ccq_lora_adapters* ad) {
+extern "C" size_t ccq_lora_workspace_size(const void* x, int x_dtype, int64_t ldx, int64_t T,
+                                          const ccq_lora_adapters* ad) {
   if (T <= 0 || T > 65536 || !lora_float_code(x_dtype) || check_adapters(ad, "ccq_lora_workspace_size")) return 0;
-  return lora_plan(T, ad, lora_one_type(x_dtype, ad)).total;
+  return lora_plan(T, ad, lora_lines(x, x_dtype, ldx, T, ad), lora_one_type(x_dtype, ad)).total;
 }
 
 extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64_t* index, void* y, int y_dtype,
@@ -1213,7 +1301,8 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
   CCQ_REQUIRE(aligned(x, x_dtype == CCQ_F32 ? 4 : 2) && aligned(y, y_dtype == CCQ_F32 ? 4 : 2) && aligned(index, 8) &&
                   aligned(ad->a, 2) && aligned(ad->b, 2) && aligned(ad->scale, 4) && aligned(ad->rank, 4),
               "ccq_lora_add: a pointer is not aligned to its elements");
-  const LoraPlan L = lora_plan(T, ad, lora_one_type(x_dtype, ad));
+  const bool lines = lora_lines(x, x_dtype, ldx, T, ad);
+  const LoraPlan L = lora_plan(T, ad, lines, lora_one_type(x_dtype, ad));
   CCQ_REQUIRE(L.total == 0 || (workspace && workspace_bytes >= L.total && aligned(workspace, 256)),
               "ccq_lora_add: workspace of %zu bytes (256-byte aligned) needed, %zu given", L.total, workspace_bytes);
   hipStream_t st = as_stream(stream);
@@ -1271,8 +1360,8 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
     if (rc) return rc;
   }
   if (ad->dtype == CCQ_BF16)
-    return L.tm == 16 ? two_launches<CCQ_BF16, 1>(p, x_dtype, groups, st)
-                      : two_launches<CCQ_BF16, 4>(p, x_dtype, groups, st);
-  return L.tm == 16 ? two_launches<CCQ_F16, 1>(p, x_dtype, groups, st)
-                    : two_launches<CCQ_F16, 4>(p, x_dtype, groups, st);
+    return L.tm == 16 ? two_launches<CCQ_BF16, 1>(p, x_dtype, lines, groups, st)
+                      : two_launches<CCQ_BF16, 4>(p, x_dtype, lines, groups, st);
+  return L.tm == 16 ? two_launches<CCQ_F16, 1>(p, x_dtype, lines, groups, st)
+                    : two_launches<CCQ_F16, 4>(p, x_dtype, lines, groups, st);
 }

@@ -573,10 +573,12 @@ typedef struct ccq_lora_adapters {
   int64_t num_adapters, rank_max, in_features, out_features;
 } ccq_lora_adapters;
 
-/* Workspace of ccq_lora_add (tokens sorted by adapter, partial sums; no
- * initial contents required), 0 for the batches that one kernel takes.  Calls
- * sharing one must not overlap in time. */
-size_t ccq_lora_workspace_size(int64_t T, int x_dtype, const ccq_lora_adapters* ad);
+/* Workspace of ccq_lora_add on these rows (tokens sorted by adapter, partial
+ * sums; no initial contents required), 0 for the batches that one kernel
+ * takes: few tokens, low ranks, and x and a aligned to 16 bytes in each row.
+ * x is not read.  Calls sharing one must not overlap in time. */
+size_t ccq_lora_workspace_size(const void* x, int x_dtype, int64_t ldx, int64_t T,
+                               const ccq_lora_adapters* ad);
 
 /* y[t, :] += scale[i] * (x[t, :] @ a[i]^T) @ b[i]^T with i = index[t], in
  * float32, y rounded once; rows with index[t] outside [0, L) are left as they

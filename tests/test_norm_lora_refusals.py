@@ -47,7 +47,7 @@ def test_empty_calls(lib):
     assert _norm(lib, rows=0) == 0
     ad = ccq_lora_adapters(256, 256, None, None, 2, 3, 16, 64, 48)
     assert lib.ccq_lora_add(P, 2, 64, P, P, 2, 48, 0, ad, None, 0, None) == 0
-    assert lib.ccq_lora_workspace_size(0, 2, ad) == 0
+    assert lib.ccq_lora_workspace_size(P, 2, 64, 0, ad) == 0
     assert lib.ccq_fp8_block_linear_quantized(P, P, P, P, P, 2, 0, 256, 128, None) == 0
 
 
