@@ -34,7 +34,8 @@ struct LoraP {
   const float* scale;
   const int32_t* rank;
   int32_t* tile_rows;           // [tiles][TM], -1: padding
-  int32_t* tile_adapter;        // [tiles], -1: no such tile
+  int32_t* tile_adapter;        // [tiles], of ccq_moe_align's schedule
+  int4* tile_info;              // [tiles], for the second kernel: adapter (-1: no such tile), rank, bits of the scale
   const int32_t* meta;          // tiles of ccq_moe_align's schedule; null: workgroups sort
   float* p;                     // [S][T][Rp]
   int64_t ldx, ldy;
@@ -117,6 +118,18 @@ __device__ __forceinline__ int lr_rank(const LoraP& p, int adapter) {
   return p.rank != nullptr ? min(max(p.rank[adapter], 0), p.R) : p.R;
 }
 
+// inclusive sum over the lanes up to this one: within rows of 16 lanes, then
+// the rows' last lanes carried on
+__device__ __forceinline__ int lr_wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // -------------------------------------------------------------- the tile --
 // Tile `tile` of the tokens sorted by adapter (tokens in order within one),
 // each adapter's run padded to whole tiles of TM: its adapter (-1: there is no
@@ -157,15 +170,11 @@ __device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS& s) {
   // tiles before an adapter: each thread takes two neighbouring adapters
   const int n0 = 2 * tid < p.L ? (s.count[2 * tid] + TM - 1) / TM : 0;
   const int n1 = 2 * tid + 1 < p.L ? (s.count[2 * tid + 1] + TM - 1) / TM : 0;
-  int sum = n0 + n1;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int v = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += v;
-  }
+  int sum = lr_wave_scan(n0 + n1);
   if (lane == 63) s.sum[wave] = sum;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) sum += s.sum[w];
+#pragma unroll
+  for (int w = 0; w < LR_WAVES - 1; ++w) sum += w < wave ? s.sum[w] : 0;
   const int start = sum - n0 - n1;
   if (tile >= start && tile < start + n0) {
     t.adapter = 2 * tid;
@@ -183,7 +192,8 @@ __device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS& s) {
   if (lane == 0) s.sum[wave] = mine;  // the sums of above were read before the last barrier
   __syncthreads();
   int pos = -t.first * TM;
-  for (int w = 0; w < wave; ++w) pos += s.sum[w];
+#pragma unroll
+  for (int w = 0; w < LR_WAVES - 1; ++w) pos += w < wave ? s.sum[w] : 0;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const uint64_t m = __ballot(key[c] == adapter);
@@ -211,12 +221,7 @@ __device__ __forceinline__ int lr_find_tile_wave(const LoraP& p, int tile, int& 
   if (__ballot(n > 1) == 0) {
     start = __popcll(__ballot(head) & ((1ull << lane) - 1));
   } else {
-    start = n;
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(start, off, 64);
-      if (lane >= off) start += v;
-    }
-    start -= n;
+    start = lr_wave_scan(n) - n;
   }
   const uint64_t hit = __ballot(head && tile >= start && tile < start + n);
   adapter = -1;
@@ -239,6 +244,13 @@ __device__ void lr_read_tile(const LoraP& p, int tile, TileS<TM>& t) {
   if (threadIdx.x < TM) t.rows[threadIdx.x] = none ? -1 : p.tile_rows[(int64_t)tile * TM + threadIdx.x];
   if (threadIdx.x == 0) t.adapter = none ? -1 : p.tile_adapter[tile];
   __syncthreads();
+}
+
+// what the second kernel needs of a tile in one load
+__device__ __forceinline__ void lr_write_info(const LoraP& p, int tile, int adapter, int rank) {
+  if (threadIdx.x == 0)
+    p.tile_info[tile] = make_int4(rank > 0 ? adapter : -1, rank,
+                                  __float_as_int(adapter >= 0 && p.scale != nullptr ? p.scale[adapter] : 1.f), 0);
 }
 
 // ---------------------------------------------------------------- shrink --
@@ -716,14 +728,13 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
     } else {
       lr_find_tile<TM, CH>(p, tile, tl, u.sort);
     }
-    if (split == 0 && blockIdx.z == 0) {  // for the second kernel
-      if (threadIdx.x < TM) p.tile_rows[(int64_t)tile * TM + threadIdx.x] = tl.rows[threadIdx.x];
-      if (threadIdx.x == 0) p.tile_adapter[tile] = tl.adapter;
-    }
+    if (split == 0 && blockIdx.z == 0 && threadIdx.x < TM)  // for the second kernel
+      p.tile_rows[(int64_t)tile * TM + threadIdx.x] = tl.rows[threadIdx.x];
   }
   const int adapter = tl.adapter;
-  if (adapter < 0) return;
-  const int rank = lr_rank(p, adapter), rz = blockIdx.z * RH * RT * 16;
+  const int rank = adapter < 0 ? 0 : lr_rank(p, adapter);
+  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank);
+  const int rz = blockIdx.z * RH * RT * 16;
   if (rz >= rank) return;
   const int h = wave % RH, part = wave / RH, r0 = rz + h * RT * 16;
   int64_t xrow[MT], arow[RT];
@@ -809,14 +820,13 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
     lr_read_tile<64>(p, tile, tl);
   } else {
     lr_find_tile<64, LR_SELF / LR_THREADS>(p, tile, tl, u.sort);
-    if (split == 0 && blockIdx.z == 0) {  // for the second kernel
-      if (threadIdx.x < 64) p.tile_rows[(int64_t)tile * 64 + threadIdx.x] = tl.rows[threadIdx.x];
-      if (threadIdx.x == 0) p.tile_adapter[tile] = tl.adapter;
-    }
+    if (split == 0 && blockIdx.z == 0 && threadIdx.x < 64)  // for the second kernel
+      p.tile_rows[(int64_t)tile * 64 + threadIdx.x] = tl.rows[threadIdx.x];
   }
   const int adapter = __builtin_amdgcn_readfirstlane(tl.adapter);
-  if (adapter < 0) return;
-  const int rank = __builtin_amdgcn_readfirstlane(lr_rank(p, adapter)), rz = blockIdx.z * RT * 16;
+  const int rank = __builtin_amdgcn_readfirstlane(adapter < 0 ? 0 : lr_rank(p, adapter));
+  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank);
+  const int rz = blockIdx.z * RT * 16;
   if (rz >= rank) return;
   const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), stages = (ke - ks + C::SK - 1) / C::SK;
 
@@ -948,12 +958,12 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
   const int yr = lane / RL, yc = lane % RL * COLS;  // this lane's row and columns of an access to y
   const int tile = blockIdx.x % p.tiles, group = blockIdx.x / p.tiles;
-  lr_read_tile<TM>(p, tile, tl);
-  const int adapter = tl.adapter;
+  const int4 info = p.tile_info[tile];
+  if (threadIdx.x < TM) tl.rows[threadIdx.x] = p.tile_rows[(int64_t)tile * TM + threadIdx.x];
+  __syncthreads();
+  const int adapter = info.x, rank = info.y;
   if (adapter < 0) return;
-  const int rank = lr_rank(p, adapter);
-  if (rank == 0) return;
-  const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
+  const float scale = __int_as_float(info.z);
   const int rc = (rank + 31) / 32, r16 = (rank + 15) & ~15, ld = 32 * rc + 8;
   const int first = group * p.ncols + 64 * wave, end = min((group + 1) * p.ncols, p.N);
   const int blocks = first < end ? (end - first + 64 * WAVES - 1) / (64 * WAVES) : 0, steps = blocks * PAIRS;
@@ -985,23 +995,32 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-    if (id >= 0) {
-      const float* at = p.p + (int64_t)id * p.Rp + 8 * j;
+    const float* at = p.p + (int64_t)(id >= 0 ? id : tl.rows[0]) * p.Rp + 8 * j;
+    const int64_t step = (int64_t)p.T * p.Rp;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {  // two pieces of four splits at once
+      if (across * i >= r16) break;
 #pragma unroll 1
-      for (int s = 0; s < p.S; ++s, at += (int64_t)p.T * p.Rp) {
-        f32x4 o[4][2];
+      for (int s = 0; s < p.S; s += 4) {
+        f32x4 o[2][4][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (across * i + 8 * j < r16) {
-            o[i][0] = *reinterpret_cast<const f32x4*>(at + across * i);
-            o[i][1] = *reinterpret_cast<const f32x4*>(at + across * i + 4);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // (past the splits or the ranks: one of those again, not added)
+            const float* from = at + min(s + k, p.S - 1) * step + (across * (i + h) + 8 * j < r16 ? across * (i + h) : 0);
+            if (8 * j < r16) {
+              o[h][k][0] = *reinterpret_cast<const f32x4*>(from);
+              o[h][k][1] = *reinterpret_cast<const f32x4*>(from + 4);
+            }
           }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (across * i + 8 * j < r16) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] += o[i][e >> 2][e & 3];
-          }
+          for (int k = 0; k < 4; ++k)
+            if (s + k < p.S) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[i + h][e] += o[h][k][e >> 2][e & 3];
+            }
       }
     }
     float m = 0.f;
@@ -1009,7 +1028,7 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[i][e] = across * i + 8 * j + e < rank ? v[i][e] * scale : 0.f;
+        v[i][e] = id >= 0 && across * i + 8 * j + e < rank ? v[i][e] * scale : 0.f;
         m = isfinite(v[i][e]) ? fmaxf(m, fabsf(v[i][e])) : m;
       }
     float up = 1.f, down = 1.f;
@@ -1123,7 +1142,7 @@ size_t a256l(size_t b) { return (b + 255) & ~(size_t)255; }
 struct LoraPlan {
   bool fused, align;
   int64_t tm, tiles, S, kchunk, Rp, ncols;
-  size_t off_rows, off_tile, off_meta, off_counts, off_align, off_p, total;
+  size_t off_rows, off_tile, off_info, off_meta, off_counts, off_align, off_p, total;
 };
 
 constexpr int64_t LR_FUSED_BYTES = 256 << 10;  // of a tile's x and A that each workgroup of one kernel reads
@@ -1164,8 +1183,10 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   size_t o = 0;
   L.off_rows = o;
   o += a256l((size_t)L.tiles * L.tm * 4);
+  L.off_info = o;
+  o += a256l((size_t)L.tiles * sizeof(int4));
   L.off_tile = o;
-  o += a256l((size_t)L.tiles * 4);
+  if (L.align) o += a256l((size_t)L.tiles * 4);
   L.off_meta = o;
   o += 256;
   L.off_counts = o;
@@ -1352,6 +1373,7 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
   }
   p.tile_rows = (int32_t*)(ws + L.off_rows);
   p.tile_adapter = (int32_t*)(ws + L.off_tile);
+  p.tile_info = (int4*)(ws + L.off_info);
   p.p = (float*)(ws + L.off_p);
   if (L.align) {
     p.meta = (const int32_t*)(ws + L.off_meta);
