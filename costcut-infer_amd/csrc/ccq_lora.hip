@@ -791,7 +791,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
 // operand reads of 8 neighbouring lanes cover all banks.
 template <int XT, int WT, int RT>
 struct TileShrink {
-  static constexpr int RTW = RT == 8 ? 2 : 1, RH = RT / RTW, KP = LR_WAVES / RH, Q = KP / 2;
+  static constexpr int RTW = RT == 8 ? 4 : RT == 4 ? 2 : 1, RH = RT / RTW, KP = LR_WAVES / RH, Q = KP / 2;
   static constexpr int SK = 64 * Q;                              // k of a stage
   static constexpr int XL = Q * (XT == CCQ_F32 ? 2 : 1);         // lines of a row of x, of A: Q
   static constexpr int X_BYTES = XL * 64 * 128, BYTES = X_BYTES + Q * 16 * RT * 128;
@@ -1160,7 +1160,11 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   // columns per workgroup: 64 for each wave, or a multiple where that still fills the CUs
   const int64_t unit = L.fused ? 64 * LR_WAVES : LE_THREADS;
   const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm) + (L.tiles - cdiv(T, L.tm)) / 2;
-  const int64_t want = (L.fused ? 256 : 768) / likely;
+  // (a workgroup of one kernel fills a CU; three of the expand kernel fit, two above 64 ranks.  Fewer workgroups with
+  // more columns each are slower, T=4096 N=4096 R=128: 8 groups of 512 columns 34 us, 6 of 768 43; so is a second
+  // round for a few of them, 49, when there are more tiles than likely)
+  const int64_t slots = L.fused ? 256 : R <= 64 ? 768 : 512;
+  const int64_t want = L.fused ? slots / likely : (slots + likely / 2) / likely;
   int64_t groups = cdiv(N, unit);
   if (groups > want) groups = want < 1 ? 1 : want;
   L.ncols = cdiv(cdiv(N, groups), unit) * unit;
