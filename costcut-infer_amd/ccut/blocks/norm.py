@@ -22,7 +22,10 @@ from typing import NamedTuple
 import torch
 
 from ccut import _dev
-from ccut._lib import CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW, CCQ_Q_NONE, call
+from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream
+from ccut._lib import CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW, CCQ_Q_NONE, check, lib
+
+_U8, _I8, _F32 = torch.uint8, torch.int8, torch.float32
 
 __all__ = ["rms_norm", "rms_norm_fp8", "rms_norm_int8", "QuantizedRows"]
 
@@ -58,45 +61,47 @@ def _unlike(t: torch.Tensor, what: str, x: torch.Tensor) -> ValueError:
                       f"{x.device}")
 
 
-def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, y_dtype, q_fmt: int):
+def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, normed: bool, y_dtype, q_fmt: int):
+    # (a decode call is 3 us on the GPU: what is asked of torch here is what counts)
     index = x.get_device()
-    if not _dev.is_current(index):
+    if not is_current(index):
         with torch.cuda.device(index):
-            return _norm(x, weight, eps, residual, residual_out, y_dtype, q_fmt)
+            return _norm(x, weight, eps, residual, residual_out, normed, y_dtype, q_fmt)
     dtype, shape = x.dtype, x.shape
-    code = _dev.DTYPE_CODE.get(dtype)
+    code = DTYPE_CODE.get(dtype)
     if code is None:
         raise ValueError(f"rows must be float32, float16 or bfloat16, got {dtype}")
     H = shape[-1] if shape else 0
     if not 1 <= H <= MAX_H:
         raise ValueError(f"rows must be [..., H] with 1 <= H <= {MAX_H}, got {tuple(shape)}")
-    if q_fmt == CCQ_Q_FP8_BLOCK and H % 128:
+    if q_fmt == CCQ_Q_FP8_BLOCK and H & 127:
         raise ValueError(f"FP8 rows need H % 128 == 0, got H={H}")
     if not 0 < eps < math.inf:
         raise ValueError(f"eps must be positive and finite, got {eps}")
-    wcode = _dev.DTYPE_CODE.get(weight.dtype)
-    if wcode is None or weight.shape != (H,) or weight.get_device() != index:
+    wcode = DTYPE_CODE.get(weight.dtype)
+    if wcode is None or weight.dim() != 1 or weight.numel() != H or weight.get_device() != index:
         raise ValueError(f"weight must be [{H}] float32, float16 or bfloat16 on {x.device}, got {weight.dtype} "
                          f"{tuple(weight.shape)} on {weight.device}")
     if not weight.is_contiguous():
         weight = weight.contiguous()
     flat = len(shape) == 2
     x2, ldx = (x, H) if flat and x.is_contiguous() else _rows(x)
-    T = x2.shape[0]
-    rp = op = None
-    ldr = ldo = 0
+    T = shape[0] if flat else x2.shape[0]
+    size, strides = (T, H), (H, 1)
+    rp = op = yp = qp = sp = q = scale = y = None
+    ldr = ldo = ycode = 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype != dtype or residual.get_device() != index:
+        if residual.dtype != dtype or residual.shape != shape or residual.get_device() != index:
             raise _unlike(residual, "residual", x)
         r2, ldr = (residual, H) if flat and residual.is_contiguous() else _rows(residual)
         rp = r2.data_ptr()
         if residual_out is None:
-            residual_out = _dev.empty_strided((T, H), (H, 1), dtype)
+            residual_out = empty_strided(size, strides, dtype)
             op, ldo = residual_out.data_ptr(), H
             if not flat:
                 residual_out = residual_out.view(shape)
         else:
-            if residual_out.shape != shape or residual_out.dtype != dtype or residual_out.get_device() != index:
+            if residual_out.dtype != dtype or residual_out.shape != shape or residual_out.get_device() != index:
                 raise _unlike(residual_out, "residual_out", x)
             o2, ldo = _rows(residual_out)
             op = o2.data_ptr()
@@ -104,27 +109,28 @@ def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, y_dtype, 
                 raise ValueError("residual_out must hold its rows one after the other, each of them dense")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    y = q = scale = yp = qp = sp = None
-    ycode = 0
-    if y_dtype is not None:
-        y = _dev.empty_strided((T, H), (H, 1), y_dtype)
-        yp, ycode = y.data_ptr(), _dev.DTYPE_CODE[y_dtype]
+    if normed:
+        ycode = code if y_dtype is None else DTYPE_CODE[y_dtype]
+        y = empty_strided(size, strides, y_dtype or dtype)
+        yp = y.data_ptr()
     if q_fmt == CCQ_Q_FP8_BLOCK:
-        q = _dev.empty_strided((T, H), (H, 1), torch.uint8)
-        scale = _dev.empty_strided((T, H >> 7), (H >> 7, 1), torch.float32)
+        q = empty_strided(size, strides, _U8)
+        scale = empty_strided((T, H >> 7), (H >> 7, 1), _F32)
         qp, sp = q.data_ptr(), scale.data_ptr()
     elif q_fmt == CCQ_Q_INT8_ROW:
-        q = _dev.empty_strided((T, H), (H, 1), torch.int8)
-        scale = _dev.empty_strided((T,), (1,), torch.float32)
+        q = empty_strided(size, strides, _I8)
+        scale = empty_strided((T,), (1,), _F32)
         qp, sp = q.data_ptr(), scale.data_ptr()
-    call("ccq_rms_norm", x2.data_ptr(), code, ldx, rp, ldr, weight.data_ptr(), wcode, eps, op, ldo, yp, ycode, q_fmt,
-         qp, sp, T, H, _dev.raw_stream(index))
+    rc = lib().ccq_rms_norm(x2.data_ptr(), code, ldx, rp, ldr, weight.data_ptr(), wcode, eps, op, ldo, yp, ycode, q_fmt,
+                            qp, sp, T, H, raw_stream(index))
+    if rc:
+        check(rc, "ccq_rms_norm")
     if not flat:
-        lead = shape[:-1]
         y = y.view(shape) if y is not None else None
         if q is not None:
-            q, scale = q.view(shape), scale.view(*lead, H >> 7) if q_fmt == CCQ_Q_FP8_BLOCK else scale.view(lead)
-    return q, scale, y, residual_out
+            q = q.view(shape)
+            scale = scale.view(*shape[:-1], H >> 7) if q_fmt == CCQ_Q_FP8_BLOCK else scale.view(shape[:-1])
+    return QuantizedRows(q, scale, y, residual_out)
 
 
 def rms_norm(x, weight, eps: float = 1e-6, *, residual=None, residual_out: torch.Tensor | None = None,
@@ -140,12 +146,11 @@ def rms_norm(x, weight, eps: float = 1e-6, *, residual=None, residual_out: torch
 
         if residual_out is not None:
             raise ValueError("residual_out is for device rows")
-        _, _, y, s = _norm(up(x), up(weight), eps, up(residual), None, torch.float32, CCQ_Q_NONE)
+        _, _, y, s = _norm(up(x), up(weight), eps, up(residual), None, True, None, CCQ_Q_NONE)
         return _dev.to_host(y) if s is None else (_dev.to_host(y), _dev.to_host(s))
-    y_dtype = out_dtype or x.dtype
-    if y_dtype not in _dev.DTYPE_CODE:
-        raise ValueError(f"rows must be float32, float16 or bfloat16, got {y_dtype}")
-    _, _, y, s = _norm(x, weight, eps, residual, residual_out, y_dtype, CCQ_Q_NONE)
+    if out_dtype is not None and out_dtype not in DTYPE_CODE:
+        raise ValueError(f"rows must be float32, float16 or bfloat16, got {out_dtype}")
+    _, _, y, s = _norm(x, weight, eps, residual, residual_out, True, out_dtype, CCQ_Q_NONE)
     return y if s is None else (y, s)
 
 
@@ -154,8 +159,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, re
     """:func:`rms_norm` of device rows (H % 128 == 0) to e4m3 codes with a
     scale per row and 128 columns; ``normed`` returns the normalized rows
     (x's type) beside them, from the same pass."""
-    return QuantizedRows(*_norm(x, weight, eps, residual, residual_out, x.dtype if normed else None,
-                                CCQ_Q_FP8_BLOCK))
+    return _norm(x, weight, eps, residual, residual_out, normed, None, CCQ_Q_FP8_BLOCK)
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residual: torch.Tensor | None = None,
@@ -164,5 +168,4 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, r
     (``amax / 127``; ``quant.int8.quantize_per_token`` keeps the reference's
     factor, which saturates almost every value); ``normed`` as in
     :func:`rms_norm_fp8`."""
-    return QuantizedRows(*_norm(x, weight, eps, residual, residual_out, x.dtype if normed else None,
-                                CCQ_Q_INT8_ROW))
+    return _norm(x, weight, eps, residual, residual_out, normed, None, CCQ_Q_INT8_ROW)

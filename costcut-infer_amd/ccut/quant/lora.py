@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 
 from ccut import _dev
-from ccut._lib import call, ccq_lora_adapters, lib
+from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream
+from ccut._lib import ccq_lora_adapters, check, lib
 
 __all__ = ["LoraAdapters", "add_"]
 
@@ -44,10 +45,10 @@ class LoraAdapters:
             raise ValueError(f"a on {a.device}, b on {b.device}")
         self.a, self.b, self.scale, self.rank = a.contiguous(), b.contiguous(), scale, rank
         self.num_adapters, self.rank_max, self.in_features, self.out_features = L, R, K, b.shape[1]
-        self.device = a.device
+        self.device, self._index = a.device, a.get_device()
         self._desc = ccq_lora_adapters(self.a.data_ptr(), self.b.data_ptr(),
                                        scale.data_ptr() if scale is not None else None,
-                                       rank.data_ptr() if rank is not None else None, _dev.DTYPE_CODE[a.dtype],
+                                       rank.data_ptr() if rank is not None else None, DTYPE_CODE[a.dtype],
                                        L, R, K, b.shape[1])
         self._bytes: dict[tuple, int] = {}
 
@@ -70,7 +71,7 @@ class LoraAdapters:
 
 
 def _rows(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
-    if t.dtype not in _dev.DTYPE_CODE:
+    if t.dtype not in DTYPE_CODE:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError(f"{what} must be [..., {width}], got {tuple(t.shape)}")
@@ -81,19 +82,16 @@ def _dense_rows(t: torch.Tensor) -> bool:
     return t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1]
 
 
-def _overlap(y: torch.Tensor, x: torch.Tensor) -> bool:
-    """Whether rows of y and x share memory (column ranges of one buffer do
-    not, though their address ranges cross)."""
-    y0, x0 = y.data_ptr(), x.data_ptr()
-    ye, xe = y.element_size(), x.element_size()
-    T = y.shape[0]
-    yl, xl = (y.stride(0) * ye, x.stride(0) * xe) if T > 1 else (0, 0)
-    yw, xw = y.shape[1] * ye, x.shape[1] * xe
-    if y0 >= x0 + (T - 1) * xl + xw or x0 >= y0 + (T - 1) * yl + yw:
+def _overlap(yp: int, ycode: int, ldy: int, N: int, xp: int, xcode: int, ldx: int, K: int, T: int) -> bool:
+    """Whether T rows of y (N values at yp, stride ldy) and x share memory;
+    column ranges of one buffer do not, though their address ranges cross."""
+    ye, xe = (2 if ycode else 4), (2 if xcode else 4)
+    yl, xl, yw, xw = ldy * ye, ldx * xe, N * ye, K * xe
+    if yp >= xp + (T - 1) * xl + xw or xp >= yp + (T - 1) * yl + yw:
         return False
     if T <= 1 or yl != xl:
         return True
-    d = (x0 - y0) % yl  # x's columns start d bytes behind y's in a row of the buffer
+    d = (xp - yp) % yl  # x's columns start d bytes behind y's in a row of the buffer
     return d < yw or d + xw > yl
 
 
@@ -106,18 +104,17 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
     means no adapter: that row is left as it is.  ``y`` must not overlap
     ``x``.  Repeated calls give the same bits (no atomics)."""
     dev = y.get_device()
-    if not _dev.is_current(dev):
+    if not is_current(dev):
         with torch.cuda.device(dev):
             return add_(y, x, adapters, index)
-    if x.get_device() != dev or index.get_device() != dev or adapters.device.index != dev:
+    if x.get_device() != dev or index.get_device() != dev or adapters._index != dev:
         raise ValueError(f"y on {y.device}, x on {x.device}, index on {index.device}, adapters on {adapters.device}")
-    lead = y.shape[:-1]
-    if x.shape[:-1] != lead or index.shape != lead:
+    if x.shape[:-1] != index.shape or y.shape[:-1] != index.shape:
         raise ValueError(f"leading dimensions of y {tuple(y.shape)}, x {tuple(x.shape)} and index "
                          f"{tuple(index.shape)} differ")
     y2, x2 = _rows(y, adapters.out_features, "y"), _rows(x, adapters.in_features, "x")
     yp = y2.data_ptr()
-    if yp != y.data_ptr() or not _dense_rows(y2):
+    if y2 is not y and yp != y.data_ptr() or not _dense_rows(y2):
         raise ValueError("y must hold its rows one after the other, each of them dense (it is written in place)")
     if not _dense_rows(x2):
         x2 = x2.contiguous()
@@ -131,14 +128,16 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
     if T == 0:
         return y
     ldx, ldy = (x2.stride(0), y2.stride(0)) if T > 1 else (adapters.in_features, adapters.out_features)
-    if _overlap(y2, x2):
+    xp, xcode, ycode = x2.data_ptr(), DTYPE_CODE[x2.dtype], DTYPE_CODE[y2.dtype]
+    if _overlap(yp, ycode, ldy, adapters.out_features, xp, xcode, ldx, adapters.in_features, T):
         raise ValueError("y overlaps x")
-    xp, xcode = x2.data_ptr(), _dev.DTYPE_CODE[x2.dtype]
     nbytes = adapters.workspace_size(xp, xcode, ldx, T)
     wp = None
     if nbytes:  # this call's own scratch, so that calls on several streams or in several graphs do not share it
-        ws = _dev.empty_strided((nbytes,), (1,), torch.uint8)
+        ws = empty_strided((nbytes,), (1,), torch.uint8)
         wp = ws.data_ptr()
-    call("ccq_lora_add", xp, xcode, ldx, index.data_ptr(), yp,
-         _dev.DTYPE_CODE[y2.dtype], ldy, T, adapters._desc, wp, nbytes, _dev.raw_stream(dev))
+    rc = lib().ccq_lora_add(xp, xcode, ldx, index.data_ptr(), yp, ycode, ldy, T, adapters._desc, wp, nbytes,
+                            raw_stream(dev))
+    if rc:
+        check(rc, "ccq_lora_add")
     return y

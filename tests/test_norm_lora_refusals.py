@@ -105,16 +105,24 @@ def test_host_tensors():
 
 def test_overlap_of_views():
     """Which views of one buffer count as overlapping."""
-    from ccut.quant.lora import _overlap
+    from ccut import _dev
+    from ccut.quant import lora
+
+    def over(y, x):
+        return lora._overlap(y.data_ptr(), _dev.DTYPE_CODE[y.dtype], y.stride(0), y.shape[1], x.data_ptr(),
+                             _dev.DTYPE_CODE[x.dtype], x.stride(0), x.shape[1], y.shape[0])
 
     buf = torch.zeros((6, 100))
-    assert not _overlap(buf[:, :40], buf[:, 40:])
-    assert not _overlap(buf[:, 60:], buf[:, :60])
-    assert _overlap(buf[:, :41], buf[:, 40:])
-    assert _overlap(buf[:, 30:70], buf[:, :31])
-    assert _overlap(buf, buf)
-    assert not _overlap(buf[:3], buf[3:])
-    assert _overlap(buf[:4], buf[3:])
-    assert not _overlap(buf[1:4, 50:], buf[2:5, :50])
-    assert _overlap(buf[:1, :40], buf[:1, 39:])
-    assert not _overlap(torch.zeros((6, 40)), torch.zeros((6, 40)))
+    assert not over(buf[:, :40], buf[:, 40:])
+    assert not over(buf[:, 60:], buf[:, :60])
+    assert over(buf[:, :41], buf[:, 40:])
+    assert over(buf[:, 30:70], buf[:, :31])
+    assert over(buf, buf)
+    assert not over(buf[:3], buf[3:])
+    assert over(buf[:3], buf[2:5])
+    assert not over(buf[1:4, 50:], buf[2:5, :50])
+    assert over(buf[:1, :40], buf[:1, 39:])
+    assert not over(torch.zeros((6, 40)), torch.zeros((6, 40)))
+    half = buf.view(torch.float16)  # 200 columns of half the size
+    assert not over(half[:, :80], buf[:, 40:])
+    assert over(half[:, :81], buf[:, 40:])
