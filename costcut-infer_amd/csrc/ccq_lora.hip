@@ -390,8 +390,11 @@ __device__ __forceinline__ void lr_split(const float (&v)[8], typename Half<WT>:
   }
 }
 
-// the power of two that brings a row whose largest finite |p| is m into [2^13, 2^14]
-__device__ __forceinline__ int lr_exponent(float m) { return m > 0.f ? min(max(13 - ilogbf(m), -100), 100) : 0; }
+// k such that 2^k brings a row whose largest finite |p| is m into [2^13, 2^14]
+__device__ __forceinline__ int lr_exponent(float m) {
+  return m > 0.f ? min(max(14 - __builtin_amdgcn_frexp_expf(m), -100), 100) : 0;
+}
+__device__ __forceinline__ float lr_pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 
 // 16 bytes of a row of y from column n on (at any element alignment).  A piece
 // across the row's end is not loaded, and added to in place value by value.
@@ -560,7 +563,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
     for (int i = 0; i < 16 / YPiece<YT>::COLS; ++i) y[i].load(p.y, yrow, n0 + lr_piece_col<YT>(i, g), p.N);
   };
   if (n0 < end) fetch();
-  if (p.T > 64) __syncthreads();  // the sort's LDS is free
+  if (p.T > 64) lds_barrier();  // the sort's LDS is free
 
   const int lines = (p.K + 63) / 64, n = lines > wave ? (lines - wave + LR_WAVES - 1) / LR_WAVES : 0;
   const int piece = (lane & 7) ^ (lane >> 3);
@@ -570,7 +573,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
     const int r = 8 * (i & 1) + (lane >> 3);
     if (i < 2 * XL) {
       const int id = __shfl(rows, r, 64);
-      off[i] = (uint32_t)((int64_t)(id >= 0 ? id : row0) * p.ldx * E) + (i >> 1) * 128 + 16 * piece;
+      off[i] = (uint32_t)(id >= 0 ? id : row0) * ((uint32_t)p.ldx * E) + (i >> 1) * 128 + 16 * piece;
     } else {
       off[i] = (uint32_t)min(16 * ((i >> 1) - XL) + r, rank - 1) * (uint32_t)p.K * 2 + 16 * piece;
     }
@@ -670,8 +673,8 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
       m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       const int ex = lr_exponent(m);
-      const float up = ldexpf(1.f, ex);
-      down = ldexpf(1.f, -ex);
+      const float up = lr_pow2(ex);
+      down = lr_pow2(-ex);
 #pragma unroll
       for (int c = 0; c < RC; ++c)
 #pragma unroll
@@ -838,7 +841,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
     const int c = wave * NI + i;
     if (c < C::X_BYTES / 1024) {
       const int own = tl.rows[(c & 7) * 8 + (lane >> 3)];
-      off[i] = (uint32_t)((int64_t)(own >= 0 ? own : tl.rows[0]) * p.ldx * E) + (c >> 3) * 128 + 16 * piece;
+      off[i] = (uint32_t)(own >= 0 ? own : tl.rows[0]) * ((uint32_t)p.ldx * E) + (c >> 3) * 128 + 16 * piece;
     } else {
       const int a = c - C::X_BYTES / 1024, r = rz + (a % (2 * RT)) * 8 + (lane >> 3);
       off[i] = (uint32_t)min(r, rank - 1) * (uint32_t)p.K * 2 + a / (2 * RT) * 128 + 16 * piece;
@@ -1035,8 +1038,8 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
     if constexpr (WT == CCQ_F16) {
       for (int off = 1; off < 1 << sh; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
       const int ex = lr_exponent(m);
-      up = ldexpf(1.f, ex);
-      down = ldexpf(1.f, -ex);
+      up = lr_pow2(ex);
+      down = lr_pow2(-ex);
     }
     if (j == 0) downs[row] = down;
     for (int r = 8 * j, i = 0; i < 4; ++i, r += across) {
