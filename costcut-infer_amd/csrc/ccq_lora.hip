@@ -15,6 +15,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace ccq {
 
 namespace {
@@ -279,6 +281,16 @@ __device__ __forceinline__ void lr_multiply(const Raw<XT> (&xr)[MT], const Raw<W
           acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(lr_f32<XT>(xr[m], e), av, acc[m][t], 0, 0, 0);
       }
   }
+}
+
+// Tile and split of a workgroup of the shrink kernels: tiles dealt to the XCDs
+// one by one, all splits of one together.  (Runs of tiles on an XCD would share
+// A in its L2, but the tiles that the grid has beyond the real ones then idle
+// whole XCDs: T=64 K=14336 R=128, 16 tiles of at most 20, 24 us against 15.)
+__device__ __forceinline__ int lr_tile_of(const LoraP& p, int& split) {
+  const int local = blockIdx.x >> 3, t = local / p.S;
+  split = local - t * p.S;
+  return t * 8 + (blockIdx.x & 7);
 }
 
 // U k-steps whose loads are in flight together, as often as they fit, then half as many
@@ -703,8 +715,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
 // A tile's 16 MT tokens, the K range of one split.  RH waves share a K part,
 // each with RT * 16 of the ranks (from 16 RT RH blockIdx.z on), so that a
 // wave's sums and its loads ahead fit its registers; the K parts' sums meet in
-// LDS.  An XCD takes neighbouring tiles, mostly of one adapter, at one pace
-// through K: its L2 serves A to all but the first of them.
+// LDS.
 template <int XT, int WT, int MT, int RT, int RH>
 __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) {
   constexpr int TM = 16 * MT, CH = MT == 1 ? 1 : LR_SELF / LR_THREADS;
@@ -716,8 +727,8 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
     f32x4 red[KP][PASS][RH * RT][64];
   } u;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
-  const int per = (p.tiles + 7) >> 3, local = blockIdx.x >> 3, split = local % p.S;
-  const int tile = (blockIdx.x & 7) * per + local / p.S;
+  int split;
+  const int tile = lr_tile_of(p, split);
   if (tile >= p.tiles) return;
   if (p.meta != nullptr) {
     lr_read_tile<TM>(p, tile, tl);
@@ -816,8 +827,8 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
     f32x4 red[KP][4][RT][64];
   } u;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
-  const int per = (p.tiles + 7) >> 3, local = blockIdx.x >> 3, split = local % p.S;
-  const int tile = (blockIdx.x & 7) * per + local / p.S;
+  int split;
+  const int tile = lr_tile_of(p, split);
   if (tile >= p.tiles) return;
   if (p.meta != nullptr) {
     lr_read_tile<64>(p, tile, tl);
@@ -988,10 +999,14 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
     fetch(0, y[0]);
     load_b(first, 0, w);
   }
-  // 2, 4 or 8 threads a row (ranks up to 16, 128, 256), each every so manieth piece of 8 ranks
+  // 2, 4 or 8 threads a row (ranks up to 16, 128, 256), each every so manieth piece of 8 ranks.  A tile of 16 rows
+  // leaves threads: they share the splits, each row's first threads adding the shares in order.
   const int sh = r16 <= 16 ? 1 : r16 <= 128 ? 2 : 3, across = 8 << sh;
+  const int shares = MT == 1 ? LE_THREADS >> (sh + 4) : 1, share = MT == 1 ? threadIdx.x >> (sh + 4) : 0;
+  const int per = p.S <= 4 ? p.S : (p.S + shares - 1) / shares, s0 = share * per, s1 = min(s0 + per, p.S);
+  float* shared = reinterpret_cast<float*>(parts + PARTS * TM * ld);  // [shares][16][r16]
 #pragma unroll 1
-  for (int row = threadIdx.x >> sh; row < TM; row += LE_THREADS >> sh) {
+  for (int row = MT == 1 ? (threadIdx.x >> sh) & 15 : threadIdx.x >> sh; row < TM; row += LE_THREADS >> sh) {
     const int j = threadIdx.x & ((1 << sh) - 1), id = tl.rows[row];
     float v[4][8];
 #pragma unroll
@@ -1004,13 +1019,13 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
     for (int i = 0; i < 4; i += 2) {  // two pieces of four splits at once
       if (across * i >= r16) break;
 #pragma unroll 1
-      for (int s = 0; s < p.S; s += 4) {
+      for (int s = s0; s < s1; s += 4) {
         f32x4 o[2][4][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // (past the splits or the ranks: one of those again, not added)
-            const float* from = at + min(s + k, p.S - 1) * step + (across * (i + h) + 8 * j < r16 ? across * (i + h) : 0);
+            const float* from = at + min(s + k, s1 - 1) * step + (across * (i + h) + 8 * j < r16 ? across * (i + h) : 0);
             if (8 * j < r16) {
               o[h][k][0] = *reinterpret_cast<const f32x4*>(from);
               o[h][k][1] = *reinterpret_cast<const f32x4*>(from + 4);
@@ -1020,11 +1035,33 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (s + k < p.S) {
+            if (s + k < s1) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[i + h][e] += o[h][k][e >> 2][e & 3];
             }
       }
+    }
+    if constexpr (MT == 1) {
+      if (p.S > 4) {  // else the first share is all
+        for (int r = 8 * j, i = 0; i < 4; ++i, r += across)
+          if (r < r16 && share > 0) {
+            float* to = shared + (share * 16 + row) * r16 + r;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = i == 0 ? v[0][e] : i == 1 ? v[1][e] : i == 2 ? v[2][e] : v[3][e];
+          }
+        lds_barrier();
+        if (share == 0) {
+          for (int k = 1; k < shares; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (across * i + 8 * j < r16) {
+                const float* from = shared + (k * 16 + row) * r16 + across * i + 8 * j;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] += from[e];
+              }
+        }
+      }
+      if (share > 0) break;
     }
     float m = 0.f;
 #pragma unroll
@@ -1176,14 +1213,20 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
     L.kchunk = cdiv(cdiv(K, 32), LR_WAVES) * 32;
     return L;
   }
-  // splits of K (one workgroup fits a CU): the fewest that keep the rounds of the CUs, each as long as its part of K
-  // and a start worth 512 k, within 5% of the shortest
-  const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
-  auto rounds = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512); };
-  double best = rounds(1);
-  for (int64_t s = 2; s <= most; ++s) best = rounds(s) < best ? rounds(s) : best;
+  // splits of K: for 16-token tiles (whose A is read once) as many as give every CU a workgroup; else (one workgroup
+  // fits a CU) the fewest that keep the rounds of the CUs, each as long as its part of K and a start worth 512 k,
+  // within 5% of the shortest
   int64_t S = 1;
-  while (rounds(S) > 1.05 * best) ++S;
+  if (L.tm == 16) {
+    S = 256 / likely < cdiv(K, 256) ? 256 / likely : cdiv(K, 256);
+    S = S < 1 ? 1 : S > 32 ? 32 : S;
+  } else {
+    const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
+    auto rounds = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512); };
+    double best = rounds(1);
+    for (int64_t s = 2; s <= most; ++s) best = rounds(s) < best ? rounds(s) : best;
+    while (rounds(S) > 1.05 * best) ++S;
+  }
   const int64_t step = L.tm == 16 ? 32 : 256;  // the largest stage of a 64-token tile
   L.kchunk = cdiv(cdiv(K, S), step) * step;
   L.S = cdiv(K, L.kchunk);
@@ -1269,10 +1312,12 @@ template <int WT, int MT>
 void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
   const dim3 grid((unsigned)(p.tiles * groups)), block(LE_THREADS);
   const size_t ld = (size_t)cdiv(p.R, 32) * 32 + 8, part = ld * 16 * MT * 2;
+  const int shares = LE_THREADS / 16 / (p.R <= 16 ? 2 : p.R <= 128 ? 4 : 8);  // (at most: an adapter's own rank may be lower)
+  const size_t shared = MT == 1 && p.S > 4 ? (size_t)std::max(shares, 4) * 16 * cdiv(p.R, 16) * 16 * 4 : 0;
   if (p.y_dtype == CCQ_F32)
-    launch((lora_expand_kernel<WT, CCQ_F32, MT>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2), st, p);
+    launch((lora_expand_kernel<WT, CCQ_F32, MT>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2) + shared, st, p);
   else
-    launch((lora_expand_kernel<WT, CCQ_BF16, MT>), grid, block, part * 2, st, p);
+    launch((lora_expand_kernel<WT, CCQ_BF16, MT>), grid, block, part * 2 + shared, st, p);
 }
 
 template <int WT, int MT>
