@@ -56,6 +56,19 @@ def is_current(index: int) -> bool:
     return index == torch._C._cuda_getDevice()
 
 
+def rows_overlap(yp: int, ycode: int, ldy: int, N: int, xp: int, xcode: int, ldx: int, K: int, T: int) -> bool:
+    """Whether T rows of y (N values at yp, stride ldy) and x share memory;
+    column ranges of one buffer do not, though their address ranges cross."""
+    ye, xe = (2 if ycode else 4), (2 if xcode else 4)
+    yl, xl, yw, xw = ldy * ye, ldx * xe, N * ye, K * xe
+    if yp >= xp + (T - 1) * xl + xw or xp >= yp + (T - 1) * yl + yw:
+        return False
+    if T <= 1 or yl != xl:
+        return True
+    d = (xp - yp) % yl  # x's columns start d bytes behind y's in a row of the buffer
+    return d < yw or d + xw > yl
+
+
 def is_host(a) -> bool:
     return not (isinstance(a, torch.Tensor) and a.is_cuda)
 

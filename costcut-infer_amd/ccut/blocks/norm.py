@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from ccut import _dev
-from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream
+from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream, rows_overlap
 from ccut._lib import CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW, CCQ_Q_NONE, check, lib
 
 _U8, _I8, _F32 = torch.uint8, torch.int8, torch.float32
@@ -107,6 +107,9 @@ def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, normed: b
             op = o2.data_ptr()
             if op != residual_out.data_ptr():  # a copy, so not a view that could be written
                 raise ValueError("residual_out must hold its rows one after the other, each of them dense")
+            for p, ld in ((x2.data_ptr(), ldx), (rp, ldr)):
+                if (p, ld) != (op, ldo) and rows_overlap(op, code, ldo, H, p, code, ld, H, T):
+                    raise ValueError("residual_out overlaps x or residual and is neither")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     if normed:
@@ -138,7 +141,8 @@ def rms_norm(x, weight, eps: float = 1e-6, *, residual=None, residual_out: torch
     """``y = s * rsqrt(mean(s^2) + eps) * weight`` with ``s = x + residual``
     over the last dimension, computed in float32; returns ``y`` (``out_dtype``,
     default x's), or ``(y, s)`` where a residual is given (``s`` in x's type,
-    written to ``residual_out``, which may be ``residual`` or ``x``).  Host
+    written to ``residual_out``, which may be ``residual`` or ``x`` but no
+    other view of their memory).  Host
     arrays are uploaded as float32 and numpy float32 is returned."""
     if _dev.is_host(x):
         def up(a):

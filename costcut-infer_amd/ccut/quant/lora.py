@@ -12,6 +12,7 @@ import torch
 
 from ccut import _dev
 from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream
+from ccut._dev import rows_overlap as _overlap
 from ccut._lib import ccq_lora_adapters, check, lib
 
 __all__ = ["LoraAdapters", "add_"]
@@ -66,6 +67,8 @@ class LoraAdapters:
         key = (T, x_code, ldx, xp & 15)
         n = self._bytes.get(key)
         if n is None:
+            if len(self._bytes) >= 4096:
+                self._bytes.clear()
             n = self._bytes[key] = int(lib().ccq_lora_workspace_size(xp, x_code, ldx, T, self._desc))
         return n
 
@@ -80,19 +83,6 @@ def _rows(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
 
 def _dense_rows(t: torch.Tensor) -> bool:
     return t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1]
-
-
-def _overlap(yp: int, ycode: int, ldy: int, N: int, xp: int, xcode: int, ldx: int, K: int, T: int) -> bool:
-    """Whether T rows of y (N values at yp, stride ldy) and x share memory;
-    column ranges of one buffer do not, though their address ranges cross."""
-    ye, xe = (2 if ycode else 4), (2 if xcode else 4)
-    yl, xl, yw, xw = ldy * ye, ldx * xe, N * ye, K * xe
-    if yp >= xp + (T - 1) * xl + xw or xp >= yp + (T - 1) * yl + yw:
-        return False
-    if T <= 1 or yl != xl:
-        return True
-    d = (xp - yp) % yl  # x's columns start d bytes behind y's in a row of the buffer
-    return d < yw or d + xw > yl
 
 
 def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.Tensor) -> torch.Tensor:

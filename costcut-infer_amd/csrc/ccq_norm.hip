@@ -18,6 +18,7 @@ namespace ccq {
 
 namespace {
 
+constexpr int NORM_GRID_BITS = 21;     // workgroups of a grid row: a launch takes fewer than 2^32 threads in x
 constexpr float kNormTiny = 1e-30f;  // 127 or 448 over it is finite
 
 struct NormP {
@@ -117,8 +118,9 @@ template <int XT, int QF, int WAVES, int VPT>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel(const NormP p) {
   constexpr int THREADS = 64 * WAVES;
   const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
-  if (WAVES == 1 && row >= p.rows) return;
+  const int64_t group = ((int64_t)blockIdx.y << NORM_GRID_BITS) + blockIdx.x;
+  const int64_t row = WAVES == 1 ? group * 4 + (threadIdx.x >> 6) : group;
+  if (row >= p.rows) return;
   float v[VPT][8], m[VPT];
   float sum = 0.f;
 #pragma unroll
@@ -222,7 +224,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
 
 template <int XT, int QF>
 int norm_launch(const NormP& p, hipStream_t st) {
-  const dim3 one((unsigned)cdiv(p.rows, 4)), row((unsigned)p.rows);
+  auto grid = [](int64_t groups) {
+    const int64_t most = (int64_t)1 << NORM_GRID_BITS;
+    return dim3((unsigned)(groups < most ? groups : most), (unsigned)cdiv(groups, most));
+  };
+  const dim3 one = grid(cdiv(p.rows, 4)), row = grid(p.rows);
   if (p.H <= 512)
     launch((rms_norm_kernel<XT, QF, 1, 1>), one, dim3(256), 0, st, p);
   else if (p.H <= 2048)

@@ -241,3 +241,31 @@ def test_refusals(gpu):
         with pytest.raises(ValueError):
             f()
             print(f"call {i} was not refused")
+
+
+def test_very_many_rows(gpu):
+    """More rows than one dimension of a launch takes."""
+    from ccut.blocks import norm
+
+    for T, H in ((2 ** 23 + 1037, 2), (2 ** 21 + 37, 520)):
+        x = torch.randn((T, H), generator=torch.Generator(device=gpu).manual_seed(H), device=gpu).bfloat16()
+        w = torch.linspace(0.5, 1.5, H, device=gpu)
+        got = norm.rms_norm_int8(x, w, EPS, normed=True)
+        for t in range(0, T, 2 ** 20):
+            part = norm.rms_norm_int8(x[t:t + 2 ** 20], w, EPS, normed=True)
+            assert all(torch.equal(a[t:t + 2 ** 20], b) for a, b in zip(got[:3], part[:3])), f"rows from {t}"
+        tail = slice(T - 40, T)
+        _check(norm.QuantizedRows(*(t[tail] for t in got[:3]), None), x[tail].cpu(), w.cpu(), None, "int8", True)
+
+
+def test_sum_over_another_view_is_refused(gpu):
+    from ccut.blocks import norm
+
+    buf, w = torch.zeros((8, 512), device=gpu), torch.ones(256, device=gpu)
+    x, r = buf[:4, :256], torch.zeros((4, 256), device=gpu)
+    for out in (buf[1:5, :256], buf[:4, 1:257], buf[:4].view(8, 256)[:4]):
+        for a, b in ((x, r), (r, x)):
+            with pytest.raises(ValueError, match="overlaps"):
+                norm.rms_norm_int8(a, w, residual=b, residual_out=out)
+    for out in (buf[:4, 256:], buf[4:, :256], x, r):
+        assert norm.rms_norm_int8(x, w, residual=r, residual_out=out).residual is out
