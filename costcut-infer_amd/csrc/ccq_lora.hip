@@ -1147,28 +1147,34 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
   }
 }
 
-// Buffers of fewer than 8 values (no 16-byte load fits them): one thread per
-// value of y, sums in 64 bits.
+// Buffers of fewer than 8 values (no 16-byte load fits them), so K, N or both
+// are below 8: a workgroup forms a token's p, a wave for each rank, then takes
+// its 256 columns.  Sums in 64 bits.
 __device__ __forceinline__ float lr_value(const void* v, int64_t i, int dt) {
   if (dt == CCQ_F32) return reinterpret_cast<const float*>(v)[i];
   const uint32_t u = reinterpret_cast<const uint16_t*>(v)[i];
   return dt == CCQ_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
 }
 __global__ __launch_bounds__(256) void lora_tiny_kernel(const LoraP p, int x_dtype, int w_dtype) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t adapter = p.index[blockIdx.y];
-  if (n >= p.N || adapter < 0 || adapter >= p.L) return;
-  const int rank = lr_rank(p, (int)adapter);
+  __shared__ double ps[LR_MAX_R];
+  const int64_t token = blockIdx.x, n = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int64_t adapter = p.index[token];
+  if (adapter < 0 || adapter >= p.L) return;
+  const int rank = lr_rank(p, (int)adapter), lane = threadIdx.x & 63;
   if (rank == 0) return;
-  double sum = 0;
-  for (int r = 0; r < rank; ++r) {
-    double inner = 0;
-    for (int k = 0; k < p.K; ++k)
-      inner += (double)lr_value(p.x, blockIdx.y * p.ldx + k, x_dtype) *
-               (double)lr_value(p.a, (adapter * p.R + r) * p.K + k, w_dtype);
-    sum += inner * (double)lr_value(p.b, (adapter * p.N + n) * p.R + r, w_dtype);
+  for (int r = threadIdx.x >> 6; r < rank; r += 4) {
+    double sum = 0;
+    for (int k = lane; k < p.K; k += 64)
+      sum += (double)lr_value(p.x, token * p.ldx + k, x_dtype) *
+             (double)lr_value(p.a, (adapter * p.R + r) * p.K + k, w_dtype);
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (lane == 0) ps[r] = sum;
   }
-  const int64_t at = blockIdx.y * p.ldy + n;
+  __syncthreads();
+  if (n >= p.N) return;
+  double sum = 0;
+  for (int r = 0; r < rank; ++r) sum += ps[r] * (double)lr_value(p.b, (adapter * p.N + n) * p.R + r, w_dtype);
+  const int64_t at = token * p.ldy + n;
   const float v = (float)(lr_value(p.y, at, p.y_dtype) + sum * (p.scale != nullptr ? p.scale[adapter] : 1.f));
   if (p.y_dtype == CCQ_F32)
     reinterpret_cast<float*>(p.y)[at] = v;
@@ -1406,7 +1412,7 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
   p.last_a = ad->num_adapters * ad->rank_max * ad->in_features - 8;
   p.last_b = ad->num_adapters * ad->rank_max * ad->out_features - 8;
   if (p.last_x < 0 || p.last_a < 0 || p.last_b < 0) {
-    launch(lora_tiny_kernel, dim3((unsigned)cdiv(p.N, 256), (unsigned)T), dim3(256), 0, st, p, x_dtype, ad->dtype);
+    launch(lora_tiny_kernel, dim3((unsigned)T, (unsigned)cdiv(p.N, 256)), dim3(256), 0, st, p, x_dtype, ad->dtype);
     return launch_status("ccq_lora_add");
   }
   if (L.fused) {

@@ -394,3 +394,128 @@ def test_beside_quantized_projections(gpu):
 def on_norm(x, w, res):
     s = (x.float() + res.float()).double()
     return s / (s.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+
+
+@pytest.mark.parametrize("T", [300, 600, 1111, 4500])
+def test_views_of_many_rows(gpu, T):
+    """Rows at odd offsets and strides for every number of tokens, K a multiple
+    of 8 and not, with guards around y."""
+    from ccut.quant import lora
+
+    for K, N, off, R, t in ((96, 77, 1, 16, "bf16"), (256, 264, 8, 40, "f16"), (100, 64, 3, 130, "bf16"),
+                            (64, 72, 1, 8, "f32")):
+        c = _case(T, K, N, R, 4, t, "bf16" if t == "f32" else t, t, ranks=True)
+        big = torch.full((T + 2, K + N + 20), 5.0, dtype=DT[t], device=gpu)
+        xs, ys = big[1:-1, off:off + K], big[1:-1, off + K:off + K + N]
+        xs.copy_(c["x"].to(gpu))
+        ys.copy_(c["y"].to(gpu))
+        before = big.clone()
+        lora.add_(ys, xs, _adapters(c, gpu), c["index"].to(gpu))
+        _check(ys, c)
+        ys.copy_(c["y"].to(gpu))
+        assert torch.equal(big, before)
+
+
+def test_smallest_buffers_many_tokens(gpu):
+    """Adapters of a few values beside many tokens, long rows or wide ones."""
+    for T, K, N, R, L in ((65536, 40, 1, 1, 1), (4100, 2000, 7, 1, 1), (3000, 1, 700, 7, 1), (4, 1, 3000, 256, 5),
+                          (1, 7, 100, 200, 3)):
+        for t in ("bf16", "f32"):
+            c = _case(T, K, N, R, L, t, "bf16", t)
+            _check(_run(c, gpu), c)
+
+
+def test_far_inputs(gpu):
+    """Rows of x beyond 2^32 bytes, for the tiles of few and of many tokens."""
+    from ccut.quant import lora
+
+    buf = torch.empty(36000 * 65536 + 64, dtype=torch.bfloat16, device=gpu)
+    for T, ld in ((36000, 65536), (300, 7864320)):
+        c = _case(T, 64, 40, 8, 3, "bf16", "bf16", "bf16")
+        xs = buf[8:8 + T * ld].view(T, ld)[:, :64]
+        assert (T - 1) * ld * 2 > 2 ** 32
+        xs.copy_(c["x"].to(gpu))
+        y = c["y"].to(gpu)
+        lora.add_(y, xs, _adapters(c, gpu), c["index"].to(gpu))
+        _check(y, c)
+
+
+@pytest.mark.parametrize("T", [6, 200, 900])
+def test_one_stack_on_two_streams(gpu, T):
+    """The same adapters, rows and index in calls that run at once."""
+    from ccut.quant import lora
+
+    c = _case(T, 640, 300, 24, 5, "bf16", "bf16", "bf16")
+    ad, x, index = _adapters(c, gpu), c["x"].to(gpu), c["index"].to(gpu)
+    want = _run(c, gpu)
+    _check(want, c)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(4):
+        ys = [c["y"].to(gpu) for _ in range(6)]
+        torch.cuda.synchronize()
+        for n, y in enumerate(ys):
+            with torch.cuda.stream(streams[n & 1]):
+                lora.add_(y, x, ad, index)
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in ys), f"turn {turn}"
+
+
+@pytest.mark.parametrize("T", [1, 48, 700])
+def test_captured_chain(gpu, T):
+    """Norm, 8-bit projection and adapters in one graph, the residual in
+    place, replayed on new rows with eager work between."""
+    from ccut import workloads
+    from ccut.blocks import norm
+    from ccut.quant import fp8_block, lora
+
+    H, N, R, L = 512, 384, 16, 4
+    g = torch.Generator(device=gpu).manual_seed(T)
+    w = 1 + 0.1 * torch.randn(H, generator=g, device=gpu)
+    wq, ws = workloads.fp8_block_weights(1, N, H, 1, gpu)
+    lin = fp8_block.prepare(wq[0], ws[0], H)
+    c = _case(T, H, N, R, L, "bf16", "bf16", "bf16")
+    ad = _adapters(c, gpu)
+
+    def layer(x, res, index):
+        q, scale, y, _ = norm.rms_norm_fp8(x, w, residual=res, residual_out=res, normed=True)
+        return lora.add_(fp8_block.linear_quantized(lin, q, scale), y, ad, index)
+
+    rows = [[torch.randn((T, H), generator=g, device=gpu).bfloat16() for _ in range(2)] +
+            [torch.randint(-1, L, (T,), generator=g, device=gpu)] for _ in range(3)]
+    held = [t.clone() for t in rows[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(*held)
+    for n in (1, 0, 2, 1):
+        for to, src in zip(held, rows[n]):
+            to.copy_(src)
+        graph.replay()
+        again = [t.clone() for t in rows[n]]
+        want = layer(*again)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(held[1], again[1]), f"rows {n}"
+
+
+def test_rows_quantized_already_refusals(gpu):
+    from ccut import workloads
+    from ccut.quant import fp8_block
+
+    wq, ws = workloads.fp8_block_weights(1, 128, 256, 1, gpu)
+    lin = fp8_block.prepare(wq[0], ws[0], 256)
+    q, s = torch.zeros((3, 256), dtype=torch.uint8, device=gpu), torch.ones((3, 2), device=gpu)
+    for f in (lambda: fp8_block.linear_quantized(lin, q.float(), s), lambda: fp8_block.linear_quantized(lin, q, s.half()),
+              lambda: fp8_block.linear_quantized(lin, q[:, :128], s), lambda: fp8_block.linear_quantized(lin, q, s[:2]),
+              lambda: fp8_block.linear_quantized(lin, q, s[:, :1]), lambda: fp8_block.linear_quantized(lin, q.cpu(), s),
+              lambda: fp8_block.linear_quantized(lin, q, s.cpu()),
+              lambda: fp8_block.linear_quantized(lin, q, s, torch.float64)):
+        with pytest.raises(ValueError):
+            f()
+    assert fp8_block.linear_quantized(lin, q[:0], s[:0]).shape == (0, 128)
+    big = torch.randint(0, 100, (7, 300), dtype=torch.uint8, device=gpu)  # codes at an odd address and stride
+    got = fp8_block.linear_quantized(lin, big[:, 3:259], torch.ones((7, 2), device=gpu), torch.float32)
+    want = fp8_block.linear_quantized(lin, big[:, 3:259].clone(), torch.ones((7, 2), device=gpu), torch.float32)
+    assert torch.equal(got, want)
+    one = fp8_block.linear_quantized(lin, big[0, 3:259].view(torch.float8_e4m3fn), torch.ones(2, device=gpu),
+                                     torch.float32)
+    assert one.shape == (128,)
