@@ -135,7 +135,8 @@ __device__ __forceinline__ int lr_wave_scan(int v) {
 // -------------------------------------------------------------- the tile --
 // Tile `tile` of the tokens sorted by adapter (tokens in order within one),
 // each adapter's run padded to whole tiles of TM: its adapter (-1: there is no
-// such tile) and token ids.  Wave w holds tokens 64 (w CH + c) + lane.
+// such tile) and token ids.  Wave w holds tokens 64 (w CH + c) + lane;
+// pick(number of tiles) is the tile.
 template <int TM>
 struct TileS {
   int adapter, first;           // first: the tile's place among its adapter's
@@ -146,8 +147,8 @@ struct SortS {
   int sum[LR_WAVES];
 };
 
-template <int TM, int CH>
-__device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS& s) {
+template <int TM, int CH, class Pick>
+__device__ void lr_find_tile(const LoraP& p, Pick pick, TileS<TM>& t, SortS& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int key[CH];
 #pragma unroll
@@ -177,6 +178,10 @@ __device__ void lr_find_tile(const LoraP& p, int tile, TileS<TM>& t, SortS& s) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < LR_WAVES - 1; ++w) sum += w < wave ? s.sum[w] : 0;
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < LR_WAVES; ++w) total += s.sum[w];
+  const int tile = pick(total);
   const int start = sum - n0 - n1;
   if (tile >= start && tile < start + n0) {
     t.adapter = 2 * tid;
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   if (p.T <= 64) {
     rows = lr_find_tile_wave(p, tile, adapter);
   } else {
-    lr_find_tile<16, 1>(p, tile, tl, u.sort);
+    lr_find_tile<16, 1>(p, [&](int) { return tile; }, tl, u.sort);
     adapter = tl.adapter;
     rows = tl.rows[c16];
   }
@@ -740,7 +745,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
       if (threadIdx.x == 0) tl.adapter = found;
       __syncthreads();
     } else {
-      lr_find_tile<TM, CH>(p, tile, tl, u.sort);
+      lr_find_tile<TM, CH>(p, [&](int) { return tile; }, tl, u.sort);
     }
     if (split == 0 && blockIdx.z == 0 && threadIdx.x < TM)  // for the second kernel
       p.tile_rows[(int64_t)tile * TM + threadIdx.x] = tl.rows[threadIdx.x];
@@ -827,16 +832,30 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
     f32x4 red[KP][4][RT][64];
   } u;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
-  int split;
-  const int tile = lr_tile_of(p, split);
-  if (tile >= p.tiles) return;
+  // the tiles' K ranges, range by range, in eight parts of one size, one to an
+  // XCD: its L2 then reads few adapters' A, and of those one range each
+  int split = 0, tile = -1, total = 0;
+  auto pick = [&](int count) {
+    total = count;
+    const int xcd = blockIdx.x & 7, all = count * p.S, from = (int)((int64_t)xcd * all >> 3);
+    const int at = from + (blockIdx.x >> 3);
+    if (at < (int)((int64_t)(xcd + 1) * all >> 3)) {
+      split = at / count;
+      tile = at - split * count;
+    }
+    return tile;
+  };
   if (p.meta != nullptr) {
-    lr_read_tile<64>(p, tile, tl);
+    pick(p.meta[0]);
+    if (tile >= 0) lr_read_tile<64>(p, tile, tl);
   } else {
-    lr_find_tile<64, LR_SELF / LR_THREADS>(p, tile, tl, u.sort);
-    if (split == 0 && blockIdx.z == 0 && threadIdx.x < 64)  // for the second kernel
+    lr_find_tile<64, LR_SELF / LR_THREADS>(p, pick, tl, u.sort);
+    if (tile >= 0 && split == 0 && blockIdx.z == 0 && threadIdx.x < 64)  // for the second kernel
       p.tile_rows[(int64_t)tile * 64 + threadIdx.x] = tl.rows[threadIdx.x];
   }
+  if (blockIdx.x == 0 && blockIdx.z == 0)  // no such tiles
+    for (int i = total + threadIdx.x; i < p.tiles; i += LR_THREADS) p.tile_info[i] = make_int4(-1, 0, 0, 0);
+  if (tile < 0) return;
   const int adapter = __builtin_amdgcn_readfirstlane(tl.adapter);
   const int rank = __builtin_amdgcn_readfirstlane(adapter < 0 ? 0 : lr_rank(p, adapter));
   if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank);
@@ -958,11 +977,14 @@ __device__ __forceinline__ void lr_lane_exchange() {
 // (8 lanes a row of 128 bytes).  y of the next step (and its weights, where one
 // chunk of 32 ranks is all) is loaded before the products of this one, the
 // first before p.
-template <int WT, int YT, int MT>
-__global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand_kernel(const LoraP p) {
+template <int WT, int YT, int MT, int KEEP>
+__global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 ? 4 : 8) ? 2 : 3) void lora_expand_kernel(
+    const LoraP p) {
   using V = typename Half<WT>::vec;
   constexpr int PARTS = WT == CCQ_F16 ? 2 : YT == CCQ_F32 ? 3 : 2, TM = 16 * MT, WAVES = LE_THREADS / 64;
   constexpr int MP = MT < 2 ? MT : 2, PAIRS = MT / MP;
+  constexpr bool STREAM = KEEP > 4;
+  constexpr int SLOTS = !STREAM ? KEEP : YT == CCQ_F32 ? 2 : 4;
   constexpr int E = YT == CCQ_F32 ? 4 : 2, COLS = 16 / E, RL = 64 / COLS;  // lanes of a row
   constexpr int RI = 64 / RL, YN = 16 * MP / RI;                           // rows of an access, accesses of a step
   __shared__ TileS<TM> tl;
@@ -982,7 +1004,7 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
   const int first = group * p.ncols + 64 * wave, end = min((group + 1) * p.ncols, p.N);
   const int blocks = first < end ? (end - first + 64 * WAVES - 1) / (64 * WAVES) : 0, steps = blocks * PAIRS;
   YPiece<YT> y[2][YN];
-  Raw<WT> w[4];
+  Raw<WT> w[SLOTS][4];  // the block's weights in chunks of 32 ranks
   auto block_of = [&](int step) { return first + 64 * WAVES * (step / PAIRS); };  // step = block * PAIRS + pair
   auto load_b = [&](int n0, int c, Raw<WT>(&v)[4]) {
     lr_load_b<WT>(p, adapter, 32 * c, [&](int q) { return n0 + 16 * q + c16; }, v);
@@ -997,7 +1019,9 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
   };
   if (steps > 0) {
     fetch(0, y[0]);
-    load_b(first, 0, w);
+#pragma unroll
+    for (int c = 0; c < SLOTS; ++c)
+      if (c < rc) load_b(first, c, w[c]);
   }
   // 2, 4 or 8 threads a row (ranks up to 16, 128, 256), each every so manieth piece of 8 ranks.  A tile of 16 rows
   // leaves threads: they share the splits, each row's first threads adding the shares in order.
@@ -1107,22 +1131,28 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 ? 2 : 3) void lora_expand
       for (int m = 0; m < MP; ++m)
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[m][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const bool fresh = PAIRS == 1 || d == 0, last = PAIRS == 1 || d == 1;  // of the block's pairs
 #pragma unroll 1
-      for (int c = 0; c < rc; ++c) {
-        Raw<WT> after[4];  // the next chunk's, or the next step's first
-        load_b(c + 1 < rc ? n0 : block_of(next), c + 1 < rc ? c + 1 : 0, after);
-        __builtin_amdgcn_sched_barrier(0);
-        lr_fix_b<WT>(p, adapter, rank, 32 * c, [&](int q) { return n0 + 16 * q + c16; }, w);
+      for (int c0 = 0; c0 < (STREAM ? rc : 1); c0 += SLOTS) {
 #pragma unroll
-        for (int m = 0; m < MP; ++m) {
-          V pv[PARTS];
+        for (int j = 0; j < SLOTS; ++j) {
+          const int c = c0 + j;
+          if (c < rc) {
+            if (STREAM || fresh) lr_fix_b<WT>(p, adapter, rank, 32 * c, [&](int q) { return n0 + 16 * q + c16; }, w[j]);
 #pragma unroll
-          for (int k = 0; k < PARTS; ++k)
-            pv[k] = *reinterpret_cast<const V*>(parts + (k * TM + 16 * (m0 + m) + c16) * ld + 32 * c + 8 * g);
-          lr_expand_step<WT, PARTS>(w, pv, acc[m]);
+            for (int m = 0; m < MP; ++m) {
+              V pv[PARTS];
+#pragma unroll
+              for (int k = 0; k < PARTS; ++k)
+                pv[k] = *reinterpret_cast<const V*>(parts + (k * TM + 16 * (m0 + m) + c16) * ld + 32 * c + 8 * g);
+              lr_expand_step<WT, PARTS>(w[j], pv, acc[m]);
+            }
+          }
+          if (STREAM && c + SLOTS < rc)
+            load_b(n0, c + SLOTS, w[j]);
+          else if ((STREAM || last) && c0 + SLOTS >= rc && j < rc && step + 1 < steps)
+            load_b(block_of(step + 1), j, w[j]);
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = after[q];
       }
       lr_lane_exchange();
 #pragma unroll
@@ -1314,16 +1344,16 @@ void shrink_tile_launch(const LoraP& p, hipStream_t st) {
   else
     launch((lora_shrink_tile_kernel<XT, WT, 8>), grid, block, 0, st, p);
 }
-template <int WT, int MT>
+template <int WT, int MT, int KEEP>
 void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
   const dim3 grid((unsigned)(p.tiles * groups)), block(LE_THREADS);
   const size_t ld = (size_t)cdiv(p.R, 32) * 32 + 8, part = ld * 16 * MT * 2;
   const int shares = LE_THREADS / 16 / (p.R <= 16 ? 2 : p.R <= 128 ? 4 : 8);  // (at most: an adapter's own rank may be lower)
   const size_t shared = MT == 1 && p.S > 4 ? (size_t)std::max(shares, 4) * 16 * cdiv(p.R, 16) * 16 * 4 : 0;
   if (p.y_dtype == CCQ_F32)
-    launch((lora_expand_kernel<WT, CCQ_F32, MT>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2) + shared, st, p);
+    launch((lora_expand_kernel<WT, CCQ_F32, MT, KEEP>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2) + shared, st, p);
   else
-    launch((lora_expand_kernel<WT, CCQ_BF16, MT>), grid, block, part * 2 + shared, st, p);
+    launch((lora_expand_kernel<WT, CCQ_BF16, MT, KEEP>), grid, block, part * 2 + shared, st, p);
 }
 
 template <int WT, int MT>
@@ -1342,7 +1372,14 @@ int two_launches(const LoraP& p, int x_dtype, bool lines, int64_t groups, hipStr
   else
     shrink_launch<CCQ_F32, WT, MT>(p, st);
   if (int rc = launch_status("ccq_lora_add (shrink)")) return rc;
-  expand_launch<WT, MT>(p, groups, st);
+  if (p.R <= 32)
+    expand_launch<WT, MT, 1>(p, groups, st);
+  else if (p.R <= 64)
+    expand_launch<WT, MT, 2>(p, groups, st);
+  else if (p.R <= 128)
+    expand_launch<WT, MT, 4>(p, groups, st);
+  else
+    expand_launch<WT, MT, 8>(p, groups, st);
   return launch_status("ccq_lora_add (expand)");
 }
 
