@@ -53,10 +53,12 @@ struct Half;
 template <>
 struct Half<CCQ_BF16> {
   using vec = bf16x8;
+  using quad = __bf16 __attribute__((ext_vector_type(4)));
 };
 template <>
 struct Half<CCQ_F16> {
   using vec = f16x8;
+  using quad = _Float16 __attribute__((ext_vector_type(4)));
 };
 
 __device__ __forceinline__ f32x4 lr_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -385,10 +387,10 @@ __device__ __forceinline__ void lr_shrink_ring(const LoraP& p, const int64_t (&x
 // p in parts of the weights' type, most significant first, whose sum is p to
 // 16 (two parts of bf16), 24 (three) or 22 bits of the row's largest (two of
 // f16, the row scaled by a power of two into its range).
-template <int WT, int PARTS>
-__device__ __forceinline__ void lr_split(const float (&v)[8], typename Half<WT>::vec (&out)[PARTS]) {
+template <int WT, int PARTS, int N, class V>
+__device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < N; ++e) {
     float rest = v[e];
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
@@ -1017,105 +1019,95 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
       v[i].load(p.y, (int64_t)(id >= 0 ? id : tl.rows[0]) * p.ldy, block_of(step) + yc, p.N);
     }
   };
+  // 4 ranks a lane, as many lanes a row as its ranks take.  A tile of 16 rows may leave waves: they share the splits,
+  // the first ones adding the shares in order.
+  const int lp = r16 <= 16 ? 2 : r16 <= 32 ? 3 : r16 <= 64 ? 4 : r16 <= 128 ? 5 : 6;
+  const int j = threadIdx.x & ((1 << lp) - 1), sub = threadIdx.x >> lp;
+  const bool spare = MT == 1 && lp < 4;
+  const int share = spare ? __builtin_amdgcn_readfirstlane(sub >> 4) : 0, shares = spare ? 16 >> lp : 1;
+  const int per = p.S <= 4 ? p.S : (p.S + shares - 1) / shares, s0 = share * per, s1 = min(s0 + per, p.S);
+  const int rows = spare ? 16 : LE_THREADS >> lp, passes = TM / rows, row0 = spare ? sub & 15 : sub;
+  float* shared = reinterpret_cast<float*>(parts + PARTS * TM * ld);  // [shares][16][r16]
+  const char* pb = reinterpret_cast<const char*>(p.p);
+  const int64_t pstep = (int64_t)p.T * p.Rp * 4;
+  constexpr int HELD = MT > 1 && (KEEP == 1 || KEEP == 4 && YT == CCQ_F32) ? 8 : 16;  // (more would spill)
+  constexpr int U = MT == 1 ? 1 : KEEP == 1 || HELD == 8 ? 2 : 4, KS = HELD / U;  // passes and splits whose loads are in flight together
+  f32x4 o[U][KS];
+  auto load_p = [&](int pass, int s) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (pass + u < passes) {
+        const int id = tl.rows[(pass + u) * rows + row0];
+        const uint32_t off = ((uint32_t)(id >= 0 ? id : tl.rows[0]) * (uint32_t)p.Rp + (4 * j < r16 ? 4 * j : 0)) * 4;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          if (s + k < s1) o[u][k] = *reinterpret_cast<const f32x4*>(pb + (s + k) * pstep + off);
+      }
+  };
+  load_p(0, s0);
   if (steps > 0) {
     fetch(0, y[0]);
 #pragma unroll
     for (int c = 0; c < SLOTS; ++c)
       if (c < rc) load_b(first, c, w[c]);
   }
-  // 2, 4 or 8 threads a row (ranks up to 16, 128, 256), each every so manieth piece of 8 ranks.  A tile of 16 rows
-  // leaves threads: they share the splits, each row's first threads adding the shares in order.
-  const int sh = r16 <= 16 ? 1 : r16 <= 128 ? 2 : 3, across = 8 << sh;
-  const int shares = MT == 1 ? LE_THREADS >> (sh + 4) : 1, share = MT == 1 ? threadIdx.x >> (sh + 4) : 0;
-  const int per = p.S <= 4 ? p.S : (p.S + shares - 1) / shares, s0 = share * per, s1 = min(s0 + per, p.S);
-  float* shared = reinterpret_cast<float*>(parts + PARTS * TM * ld);  // [shares][16][r16]
 #pragma unroll 1
-  for (int row = MT == 1 ? (threadIdx.x >> sh) & 15 : threadIdx.x >> sh; row < TM; row += LE_THREADS >> sh) {
-    const int j = threadIdx.x & ((1 << sh) - 1), id = tl.rows[row];
-    float v[4][8];
+  for (int pass = 0; pass < passes; pass += U) {
+    f32x4 sum[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-    const float* at = p.p + (int64_t)(id >= 0 ? id : tl.rows[0]) * p.Rp + 8 * j;
-    const int64_t step = (int64_t)p.T * p.Rp;
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {  // two pieces of four splits at once
-      if (across * i >= r16) break;
+    for (int u = 0; u < U; ++u) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-      for (int s = s0; s < s1; s += 4) {
-        f32x4 o[2][4][2];
+    for (int s = s0; s < s1; s += KS) {
+      if (s > s0) load_p(pass, s);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int k = 0; k < KS; ++k)
+        if (s + k < s1) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // (past the splits or the ranks: one of those again, not added)
-            const float* from = at + min(s + k, s1 - 1) * step + (across * (i + h) + 8 * j < r16 ? across * (i + h) : 0);
-            if (8 * j < r16) {
-              o[h][k][0] = *reinterpret_cast<const f32x4*>(from);
-              o[h][k][1] = *reinterpret_cast<const f32x4*>(from + 4);
-            }
-          }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (s + k < s1) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[i + h][e] += o[h][k][e >> 2][e & 3];
-            }
-      }
-    }
-    if constexpr (MT == 1) {
-      if (p.S > 4) {  // else the first share is all
-        for (int r = 8 * j, i = 0; i < 4; ++i, r += across)
-          if (r < r16 && share > 0) {
-            float* to = shared + (share * 16 + row) * r16 + r;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) to[e] = i == 0 ? v[0][e] : i == 1 ? v[1][e] : i == 2 ? v[2][e] : v[3][e];
-          }
-        lds_barrier();
-        if (share == 0) {
-          for (int k = 1; k < shares; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (across * i + 8 * j < r16) {
-                const float* from = shared + (k * 16 + row) * r16 + across * i + 8 * j;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] += from[e];
-              }
+          for (int u = 0; u < U; ++u) sum[u] += o[u][k];
         }
+    }
+    if (pass + U < passes) load_p(pass + U, s0);
+    if constexpr (MT == 1) {
+      if (spare && p.S > 4) {  // else the first share is all
+        if (share > 0 && 4 * j < r16) *reinterpret_cast<f32x4*>(shared + (share * 16 + row0) * r16 + 4 * j) = sum[0];
+        lds_barrier();
+        if (share == 0 && 4 * j < r16)
+          for (int k = 1; k < shares; ++k) sum[0] += *reinterpret_cast<const f32x4*>(shared + (k * 16 + row0) * r16 + 4 * j);
       }
       if (share > 0) break;
     }
-    float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int u = 0; u < U; ++u) {
+      if (pass + u >= passes) break;
+      const int row = (pass + u) * rows + row0, id = tl.rows[row];
+      float v[4], m = 0.f, up = 1.f, down = 1.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[i][e] = id >= 0 && across * i + 8 * j + e < rank ? v[i][e] * scale : 0.f;
-        m = isfinite(v[i][e]) ? fmaxf(m, fabsf(v[i][e])) : m;
+      for (int e = 0; e < 4; ++e) {
+        v[e] = id >= 0 && 4 * j + e < rank ? sum[u][e] * scale : 0.f;
+        m = isfinite(v[e]) ? fmaxf(m, fabsf(v[e])) : m;
       }
-    float up = 1.f, down = 1.f;
-    if constexpr (WT == CCQ_F16) {
-      for (int off = 1; off < 1 << sh; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      const int ex = lr_exponent(m);
-      up = lr_pow2(ex);
-      down = lr_pow2(-ex);
-    }
-    if (j == 0) downs[row] = down;
-    for (int r = 8 * j, i = 0; i < 4; ++i, r += across) {
-      if (r < 32 * rc) {
-        V pv[PARTS];
-        float u[8];
+      if constexpr (WT == CCQ_F16) {
+        for (int off = 1; off < 1 << lp; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        const int ex = lr_exponent(m);
+        up = lr_pow2(ex);
+        down = lr_pow2(-ex);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = (i == 0 ? v[0][e] : i == 1 ? v[1][e] : i == 2 ? v[2][e] : v[3][e]) * up;
-        lr_split<WT, PARTS>(u, pv);
+        for (int e = 0; e < 4; ++e) v[e] *= up;
+      }
+      if (j == 0) downs[row] = down;
+      if (4 * j < 32 * rc) {
+        typename Half<WT>::quad pv[PARTS];
+        lr_split<WT, PARTS>(v, pv);
 #pragma unroll
-        for (int k = 0; k < PARTS; ++k) *reinterpret_cast<V*>(parts + (k * TM + row) * ld + r) = pv[k];
+        for (int k = 0; k < PARTS; ++k) {
+          uint16_t* to = parts + (k * TM + row) * ld + 4 * j;
+          *reinterpret_cast<typename Half<WT>::quad*>(to) = pv[k];
+          if (r16 == 16) *reinterpret_cast<uint64_t*>(to + 16) = 0;  // the chunk's other half
+        }
       }
     }
   }
-  __syncthreads();
+  lds_barrier();
   float(*mine)[64 + 4] = turn[wave];
   for (int s = 0; s < steps; s += 2) {
 #pragma unroll
@@ -1348,8 +1340,7 @@ template <int WT, int MT, int KEEP>
 void expand_launch(const LoraP& p, int64_t groups, hipStream_t st) {
   const dim3 grid((unsigned)(p.tiles * groups)), block(LE_THREADS);
   const size_t ld = (size_t)cdiv(p.R, 32) * 32 + 8, part = ld * 16 * MT * 2;
-  const int shares = LE_THREADS / 16 / (p.R <= 16 ? 2 : p.R <= 128 ? 4 : 8);  // (at most: an adapter's own rank may be lower)
-  const size_t shared = MT == 1 && p.S > 4 ? (size_t)std::max(shares, 4) * 16 * cdiv(p.R, 16) * 16 * 4 : 0;
+  const size_t shared = MT == 1 && p.S > 4 ? 4 * 16 * 16 * 4 : 0;  // 4 shares of up to 16 ranks, 2 of up to 32
   if (p.y_dtype == CCQ_F32)
     launch((lora_expand_kernel<WT, CCQ_F32, MT, KEEP>), grid, block, part * (WT == CCQ_BF16 ? 3 : 2) + shared, st, p);
   else
