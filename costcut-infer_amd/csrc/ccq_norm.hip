@@ -18,7 +18,8 @@ namespace ccq {
 
 namespace {
 
-constexpr int NORM_GRID_BITS = 21;     // workgroups of a grid row: a launch takes fewer than 2^32 threads in x
+constexpr int64_t NORM_ROWS = 1 << 21;  // of a launch, which takes fewer than 2^32 threads (a second grid dimension
+                                        // for the others costs each call 0.2 to 0.35 us)
 constexpr float kNormTiny = 1e-30f;  // 127 or 448 over it is finite
 
 struct NormP {
@@ -118,9 +119,8 @@ template <int XT, int QF, int WAVES, int VPT>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel(const NormP p) {
   constexpr int THREADS = 64 * WAVES;
   const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t group = ((int64_t)blockIdx.y << NORM_GRID_BITS) + blockIdx.x;
-  const int64_t row = WAVES == 1 ? group * 4 + (threadIdx.x >> 6) : group;
-  if (row >= p.rows) return;
+  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (WAVES == 1 && row >= p.rows) return;
   float v[VPT][8], m[VPT];
   float sum = 0.f;
 #pragma unroll
@@ -224,11 +224,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
 
 template <int XT, int QF>
 int norm_launch(const NormP& p, hipStream_t st) {
-  auto grid = [](int64_t groups) {
-    const int64_t most = (int64_t)1 << NORM_GRID_BITS;
-    return dim3((unsigned)(groups < most ? groups : most), (unsigned)cdiv(groups, most));
-  };
-  const dim3 one = grid(cdiv(p.rows, 4)), row = grid(p.rows);
+  const dim3 one((unsigned)cdiv(p.rows, 4)), row((unsigned)p.rows);
   if (p.H <= 512)
     launch((rms_norm_kernel<XT, QF, 1, 1>), one, dim3(256), 0, st, p);
   else if (p.H <= 2048)
@@ -280,9 +276,17 @@ extern "C" int ccq_rms_norm(const void* x, int x_dtype, int64_t ldx, const void*
                   aligned(scale, 4),
               "ccq_rms_norm: a pointer is not aligned to its elements");
   CCQ_REQUIRE(q_fmt != CCQ_Q_FP8_BLOCK || aligned(q, 8), "ccq_rms_norm: q must be 8-byte aligned");
-  NormP p = {x, residual, w, residual_out, y, (uint8_t*)q, scale, ldx, ldr, ldo, rows, (int)H, w_dtype, y_dtype, eps};
   hipStream_t st = as_stream(stream);
-  if (x_dtype == CCQ_BF16) return norm_dispatch<CCQ_BF16>(q_fmt, p, st);
-  if (x_dtype == CCQ_F16) return norm_dispatch<CCQ_F16>(q_fmt, p, st);
-  return norm_dispatch<CCQ_F32>(q_fmt, p, st);
+  const size_t ye = y_dtype == CCQ_F32 ? 4 : 2;
+  auto at = [](const void* b, int64_t i, size_t size) { return b == nullptr ? nullptr : (char*)b + i * size; };
+  for (int64_t r = 0; r < rows; r += NORM_ROWS) {
+    const NormP p = {at(x, r * ldx, e), at(residual, r * ldr, e), w, at(residual_out, r * ldo, e), at(y, r * H, ye),
+                     (uint8_t*)at(q, r * H, 1), (float*)at(scale, r * (q_fmt == CCQ_Q_FP8_BLOCK ? H >> 7 : 1), 4),
+                     ldx, ldr, ldo, rows - r < NORM_ROWS ? rows - r : NORM_ROWS, (int)H, w_dtype, y_dtype, eps};
+    const int rc = x_dtype == CCQ_BF16  ? norm_dispatch<CCQ_BF16>(q_fmt, p, st)
+                   : x_dtype == CCQ_F16 ? norm_dispatch<CCQ_F16>(q_fmt, p, st)
+                                        : norm_dispatch<CCQ_F32>(q_fmt, p, st);
+    if (rc) return rc;
+  }
+  return 0;
 }

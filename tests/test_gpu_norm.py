@@ -244,7 +244,7 @@ def test_refusals(gpu):
 
 
 def test_very_many_rows(gpu):
-    """More rows than one dimension of a launch takes."""
+    """More rows than one launch takes."""
     from ccut.blocks import norm
 
     for T, H in ((2 ** 23 + 1037, 2), (2 ** 21 + 37, 520)):
@@ -256,6 +256,15 @@ def test_very_many_rows(gpu):
             assert all(torch.equal(a[t:t + 2 ** 20], b) for a, b in zip(got[:3], part[:3])), f"rows from {t}"
         tail = slice(T - 40, T)
         _check(norm.QuantizedRows(*(t[tail] for t in got[:3]), None), x[tail].cpu(), w.cpu(), None, "int8", True)
+
+    T, H = 2 ** 21 + 37, 128  # FP8, strided rows, the sum in place
+    buf = torch.randn((T, 2 * H + 8), generator=torch.Generator(device=gpu).manual_seed(1), device=gpu).half()
+    x, res = buf[:, :H], buf[:, H:2 * H]
+    before, w = res.clone(), torch.linspace(0.5, 1.5, H, device=gpu)
+    got = norm.rms_norm_fp8(x, w, EPS, residual=res, residual_out=res, normed=True)
+    for rows in (slice(0, 50), slice(2 ** 21 - 20, T)):
+        part = norm.QuantizedRows(*(t[rows] for t in got))
+        _check(part, x[rows].cpu(), w.cpu(), before[rows].cpu(), "fp8", True)
 
 
 def test_sum_over_another_view_is_refused(gpu):
