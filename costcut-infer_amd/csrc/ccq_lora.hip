@@ -1213,7 +1213,7 @@ struct LoraPlan {
   size_t off_rows, off_tile, off_info, off_meta, off_counts, off_align, off_p, total;
 };
 
-constexpr int64_t LR_FUSED_BYTES = 256 << 10;  // of a tile's x and A that each workgroup of one kernel reads
+constexpr int64_t LR_FUSED_BYTES = 384 << 10;  // of a tile's x and A that each workgroup of one kernel reads
 
 // lines: lora_lines, one_type: x float32 or of A's type
 LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_type) {

@@ -113,8 +113,9 @@ __device__ __forceinline__ void store8_any(int dt, void* p, int64_t i, int n, co
 }
 
 // Columns 8 (t + THREADS i) .. + 7 of a row are vector i of its thread t; a
-// row is held in registers, so x, residual and w are read once.  WAVES waves
-// work on a row: one (four rows in a workgroup, no barrier), four or sixteen.
+// row is held in registers, so x, residual and w are read once and HBM bounds
+// long batches.  WAVES waves work on a row; one wave's workgroup takes four
+// rows and needs no barrier.
 template <int XT, int QF, int WAVES, int VPT>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel(const NormP p) {
   constexpr int THREADS = 64 * WAVES;
@@ -222,17 +223,35 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
   }
 }
 
+// By the row's length, so that its threads hold one vector or two: longer
+// chains of loads cost more than idle threads (GPU time in us, bf16 with a
+// residual to FP8, 4096 rows; waves x vectors):
+//   H = 512 1x1 5.8, 4x1 6.8; 1024 2x1 7.9, 4x1 9.1; 2048 4x1 14.8, 1x4 15.0;
+//   7168 8x2 40.4 (5.1 TB/s), 16x1 42.4, 4x4 45.8; 2000 rows of 16384
+//   16x2 45, 16x4 58.
+// Up to 512 rows do not fill the CUs, and latency counts: one vector a thread
+// (1 row of 4096 8x1 2.8, 4x2 3.7, 4096 rows 23.6 and 22.5; 1 row of 7168
+// 16x1 3.4, 8x2 3.8, 4x4 5.8).
 template <int XT, int QF>
 int norm_launch(const NormP& p, hipStream_t st) {
   const dim3 one((unsigned)cdiv(p.rows, 4)), row((unsigned)p.rows);
+  const bool few = p.rows <= 512;
   if (p.H <= 512)
     launch((rms_norm_kernel<XT, QF, 1, 1>), one, dim3(256), 0, st, p);
+  else if (p.H <= 1024)
+    launch((rms_norm_kernel<XT, QF, 2, 1>), row, dim3(128), 0, st, p);
   else if (p.H <= 2048)
     launch((rms_norm_kernel<XT, QF, 4, 1>), row, dim3(256), 0, st, p);
+  else if (p.H <= 4096 && few)
+    launch((rms_norm_kernel<XT, QF, 8, 1>), row, dim3(512), 0, st, p);
   else if (p.H <= 4096)
     launch((rms_norm_kernel<XT, QF, 4, 2>), row, dim3(256), 0, st, p);
+  else if (p.H <= 8192 && few)
+    launch((rms_norm_kernel<XT, QF, 16, 1>), row, dim3(1024), 0, st, p);
   else if (p.H <= 8192)
-    launch((rms_norm_kernel<XT, QF, 4, 4>), row, dim3(256), 0, st, p);
+    launch((rms_norm_kernel<XT, QF, 8, 2>), row, dim3(512), 0, st, p);
+  else if (p.H <= 16384)
+    launch((rms_norm_kernel<XT, QF, 16, 2>), row, dim3(1024), 0, st, p);
   else
     launch((rms_norm_kernel<XT, QF, 16, 4>), row, dim3(1024), 0, st, p);
   return launch_status("ccq_rms_norm");
