@@ -92,7 +92,8 @@ def add_(y: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, index: torch.
     [...]`` (int64; other whole numbers are converted) are device tensors with
     the same leading dimensions, at most 65536 rows.  An index outside [0, L)
     means no adapter: that row is left as it is.  ``y`` must not overlap
-    ``x``.  Repeated calls give the same bits (no atomics)."""
+    ``x``.  Repeated calls give the same bits (sums have a fixed
+    order)."""
     dev = y.get_device()
     if not is_current(dev):
         with torch.cuda.device(dev):

@@ -11,6 +11,15 @@
 // Few tokens: one kernel does both, each workgroup forming p anew for its
 // columns.  Else two kernels, p's partial sums (K split over workgroups)
 // passing through the workspace and added in the splits' order.
+//
+// p stays float32 between the products.  The second one takes it in parts of
+// the weights' type (lr_split) whose sum is p to 16 bits or more, so that y's
+// own rounding is the only one that shows; sums are float32 everywhere.
+//
+// What bounds it: prompts, y read and written once and x read once (T=2048
+// K=4096 N=14336 R=16: 134 MB, 34 us, 4.1 TB/s); a batch of few tokens, the
+// chain index -> tile -> A, x, B, y -> LDS -> store, 6 to 9 us in one kernel,
+// 11 to 16 in two.
 #include "ccq_common.h"
 
 #include <math.h>
@@ -25,7 +34,8 @@ constexpr int LR_THREADS = 512, LR_WAVES = 8;
 constexpr int LE_THREADS = 256;  // of the expand kernel
 constexpr int LR_MAX_R = 256;
 constexpr int LR_MAX_L = 1024;
-constexpr int LR_SELF = 4096;   // most tokens that workgroups sort themselves
+constexpr int LR_SELF = 4096;   // most tokens that workgroups sort themselves: 8 a thread (T=4096 K=N=2048 R=16 21.8 us,
+                                // behind the schedule's own launch 26.0; T=1100 15.6 and 18.4)
 
 struct LoraP {
   const void* x;
@@ -810,6 +820,10 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
 // each wave multiplies one step of 32 k (part) of it for RTW * 16 ranks (h).
 // In a line the 16-byte piece i of row r lies at i ^ (r & 7), so that the
 // operand reads of 8 neighbouring lanes cover all banks.
+// T=4096 K=14336 R=128: 47 us, 2.4 TB/s of x; 34 us with x in the last level
+// cache, 27 us at R=16.  A, two thirds of a stage, comes from L2; more stages
+// ahead, x and A copied by waves of their own, and other orders of the stages
+// left the time as it is.
 template <int XT, int WT, int RT>
 struct TileShrink {
   static constexpr int RTW = RT == 8 ? 4 : RT == 4 ? 2 : 1, RH = RT / RTW, KP = LR_WAVES / RH, Q = KP / 2;
@@ -976,9 +990,14 @@ __device__ __forceinline__ void lr_lane_exchange() {
 // in parts in LDS; a wave then takes 64 columns of 16 MP tokens at a time.  The
 // products' lanes hold 4 columns of 16 tokens each: they pass through the
 // wave's part of LDS into rows, so that y is read and written in whole lines
-// (8 lanes a row of 128 bytes).  y of the next step (and its weights, where one
-// chunk of 32 ranks is all) is loaded before the products of this one, the
-// first before p.
+// (8 lanes a row of 128 bytes).  A block's weights, up to KEEP chunks of 32
+// ranks, stay in registers for all tokens of the tile, each chunk replaced by
+// the next block's behind its last product (more than 128 ranks pass through
+// as a stream); y of the next step is loaded before the products of this one.
+// p's loads go first: a wave waits for its loads in order, and those of y come
+// from HBM.  T=2048 N=14336 R=16: 25.7 us for 117 MB of y (4.6 TB/s; 27.5 with
+// y before p, 30.1 with the weights loaded step by step).  T=4096 N=4096
+// R=128: 30.4 us, 10 of them until p of three splits is in LDS.
 template <int WT, int YT, int MT, int KEEP>
 __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 ? 4 : 8) ? 2 : 3) void lora_expand_kernel(
     const LoraP p) {
@@ -1213,7 +1232,11 @@ struct LoraPlan {
   size_t off_rows, off_tile, off_info, off_meta, off_counts, off_align, off_p, total;
 };
 
-constexpr int64_t LR_FUSED_BYTES = 384 << 10;  // of a tile's x and A that each workgroup of one kernel reads
+// Of a tile's x and A, which each workgroup of the one kernel reads.  One
+// kernel and two, in us: T=16 K=4096 N=14336 R=16 (256 KiB) 8.6 and 11.8, T=64
+// K=N=4096 R=32 (384) 8.3 and 10.4, T=1 K=N=8192 R=16 (512) 10.2 and 9.3, T=16
+// K=14336 N=4096 R=16 (896) 14.3 and 10.8.
+constexpr int64_t LR_FUSED_BYTES = 384 << 10;
 
 // lines: lora_lines, one_type: x float32 or of A's type
 LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_type) {
@@ -1222,16 +1245,18 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   L.Rp = cdiv(R, 16) * 16;
   L.fused = lines && one_type && T <= LR_THREADS && R <= 32 && (16 + L.Rp) * K * 2 <= LR_FUSED_BYTES;
   L.align = T > LR_SELF;
+  // tiles of 16 up to a token a thread of the sort (T=256 K=N=4096 R=64 14.3 us, by tiles of 64 19.0; T=512 18.6 and
+  // 20.0), of 64 above, which read A a quarter as often
   L.tm = T <= LR_THREADS ? 16 : 64;
   L.tiles = ccq_moe_align_max_tiles(T, ad->num_adapters, L.tm);
   if (L.tiles > T) L.tiles = T;  // every tile has a token
   // columns per workgroup: 64 for each wave, or a multiple where that still fills the CUs
   const int64_t unit = L.fused ? 64 * LR_WAVES : LE_THREADS;
   const int64_t likely = L.tm == 16 ? L.tiles : cdiv(T, L.tm) + (L.tiles - cdiv(T, L.tm)) / 2;
-  // (a workgroup of one kernel fills a CU; three of the expand kernel fit, two above 64 ranks.  Fewer workgroups with
-  // more columns each are slower, T=4096 N=4096 R=128: 8 groups of 512 columns 34 us, 6 of 768 43; so is a second
-  // round for a few of them, 49, when there are more tiles than likely)
-  const int64_t slots = L.fused ? 256 : R <= 64 ? 768 : 512;
+  // (a workgroup of one kernel fills a CU; three, two or one of the expand kernel fit, by registers and LDS.  A second
+  // round for a part of them is what costs: T=2048 N=14336 R=64 35 us by groups for two a CU, 46 for three; T=4096
+  // N=4096 R=256 59 for one, 70 for two; T=4096 N=4096 R=128 34 by 8 groups of 512 columns, 43 by 6 of 768)
+  const int64_t slots = L.fused ? 256 : L.tm == 16 ? (R <= 64 ? 768 : 512) : R <= 32 ? 768 : R <= 128 ? 512 : 256;
   const int64_t want = L.fused ? slots / likely : (slots + likely / 2) / likely;
   int64_t groups = cdiv(N, unit);
   if (groups > want) groups = want < 1 ? 1 : want;
@@ -1242,18 +1267,20 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
     return L;
   }
   // splits of K: for 16-token tiles (whose A is read once) as many as give every CU a workgroup; else (one workgroup
-  // fits a CU) the fewest that keep the rounds of the CUs, each as long as its part of K and a start worth 512 k,
-  // within 5% of the shortest
+  // fits a CU) the fewest within 5% of the shortest time, in units of a k: the rounds of the CUs, each as long as its
+  // part of K and a start worth 512, and each split's p, which every group of columns reads (T=1000 K=N=4096 R=128
+  // 32.2 us, without this term 33.8; R=200 46 and 50)
   int64_t S = 1;
   if (L.tm == 16) {
     S = 256 / likely < cdiv(K, 256) ? 256 / likely : cdiv(K, 256);
     S = S < 1 ? 1 : S > 32 ? 32 : S;
   } else {
     const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
-    auto rounds = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512); };
-    double best = rounds(1);
-    for (int64_t s = 2; s <= most; ++s) best = rounds(s) < best ? rounds(s) : best;
-    while (rounds(S) > 1.05 * best) ++S;
+    const int64_t part = R < 64 ? R : R < 128 ? 64 : 128;
+    auto time = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512) + (double)(s * part); };
+    double best = time(1);
+    for (int64_t s = 2; s <= most; ++s) best = time(s) < best ? time(s) : best;
+    while (time(S) > 1.05 * best) ++S;
   }
   const int64_t step = L.tm == 16 ? 32 : 256;  // the largest stage of a 64-token tile
   L.kchunk = cdiv(cdiv(K, S), step) * step;
