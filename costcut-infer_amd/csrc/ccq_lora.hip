@@ -1010,7 +1010,9 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
   constexpr int RI = 64 / RL, YN = 16 * MP / RI;                           // rows of an access, accesses of a step
   __shared__ TileS<TM> tl;
   __shared__ float downs[TM];
-  __shared__ __align__(16) float turn[WAVES][16 * MP][64 + 4];
+  // (with half of it two workgroups of three parts and 128 ranks fit a CU: T=3020 N=5152 float32 68 -> 50 us)
+  constexpr int TURN = YT == CCQ_F32 && KEEP == 4 && MT > 1 ? 1 : MP;  // row blocks that turn at once
+  __shared__ __align__(16) float turn[WAVES][16 * TURN][64 + 4];
   extern __shared__ __align__(16) uint16_t parts[];  // [PARTS][TM][ld]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
   const int yr = lane / RL, yc = lane % RL * COLS;  // this lane's row and columns of an access to y
@@ -1165,24 +1167,27 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
             load_b(block_of(step + 1), j, w[j]);
         }
       }
-      lr_lane_exchange();
 #pragma unroll
-      for (int m = 0; m < MP; ++m)
+      for (int h = 0; h < MP; h += TURN) {
+        lr_lane_exchange();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&mine[16 * m + c16][16 * q + 4 * g]) = acc[m][q];
-      lr_lane_exchange();
+        for (int m = 0; m < TURN; ++m)
 #pragma unroll
-      for (int i = 0; i < YN; ++i) {
-        const int row = RI * i + yr, id = tl.rows[16 * m0 + row];
-        float add[COLS];
-        const float f = downs[16 * m0 + row];
+          for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&mine[16 * m + c16][16 * q + 4 * g]) = acc[h + m][q];
+        lr_lane_exchange();
 #pragma unroll
-        for (int e = 0; e < COLS; e += 4) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(&mine[row][yc + e]);
+        for (int i = 0; i < YN * TURN / MP; ++i) {
+          const int at = h * YN / MP + i, row = RI * i + yr, id = tl.rows[16 * (m0 + h) + row];
+          float add[COLS];
+          const float f = downs[16 * (m0 + h) + row];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) add[e + k] = v[k] * f;
+          for (int e = 0; e < COLS; e += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(&mine[row][yc + e]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add[e + k] = v[k] * f;
+          }
+          if (id >= 0) y[d][at].add_store(p.y, p.y_dtype, (int64_t)id * p.ldy, n0 + yc, p.N, add);
         }
-        if (id >= 0) y[d][i].add_store(p.y, p.y_dtype, (int64_t)id * p.ldy, n0 + yc, p.N, add);
       }
     }
   }
@@ -1239,7 +1244,7 @@ struct LoraPlan {
 constexpr int64_t LR_FUSED_BYTES = 384 << 10;
 
 // lines: lora_lines, one_type: x float32 or of A's type
-LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_type) {
+LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_type, bool x32) {
   LoraPlan L = {};
   const int64_t K = ad->in_features, N = ad->out_features, R = ad->rank_max;
   L.Rp = cdiv(R, 16) * 16;
@@ -1266,18 +1271,22 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
     L.kchunk = cdiv(cdiv(K, 32), LR_WAVES) * 32;
     return L;
   }
-  // splits of K: for 16-token tiles (whose A is read once) as many as give every CU a workgroup; else (one workgroup
-  // fits a CU) the fewest within 5% of the shortest time, in units of a k: the rounds of the CUs, each as long as its
-  // part of K and a start worth 512, and each split's p, which every group of columns reads (T=1000 K=N=4096 R=128
-  // 32.2 us, without this term 33.8; R=200 46 and 50)
+  // splits of K: for 16-token tiles (whose A is read once) as many as give every CU a workgroup, and no more than where
+  // p's reading grows faster than K's parts shrink (S^2 R = 3.5 K: T=100 K=4560 N=400 R=128 10 splits 18.1 us, 18 20.6; T=30
+  // K=N=8192 R=256 10 27.4, 32 33.8); else (one workgroup fits a CU) the fewest within 5% of the shortest time, in units of
+  // a k: the rounds of the CUs, each as long as its part of K and a start worth 512, and each split's p, which every
+  // group of columns reads (T=1000 K=N=4096 R=128 32.2 us, without this term 33.8; R=200 46 and 50).  float32 x takes
+  // four times as long a k (its products are the 32-bit ones; T=1051 K=2352 R=128 48 us, at 16-bit costs 61).
   int64_t S = 1;
   if (L.tm == 16) {
     S = 256 / likely < cdiv(K, 256) ? 256 / likely : cdiv(K, 256);
-    S = S < 1 ? 1 : S > 32 ? 32 : S;
+    S = S > 32 ? 32 : S;
+    while (S > 1 && 2 * S * S * L.Rp > 7 * K) --S;
+    S = S < 1 ? 1 : S;
   } else {
     const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
-    const int64_t part = R < 64 ? R : R < 128 ? 64 : 128;
-    auto time = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + 512) + (double)(s * part); };
+    const int64_t part = (R < 64 ? R : R < 128 ? 64 : 128) / (x32 ? 4 : 1), start = x32 ? 128 : 512;
+    auto time = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + start) + (double)(s * part); };
     double best = time(1);
     for (int64_t s = 2; s <= most; ++s) best = time(s) < best ? time(s) : best;
     while (time(S) > 1.05 * best) ++S;
@@ -1419,7 +1428,7 @@ using namespace ccq;
 extern "C" size_t ccq_lora_workspace_size(const void* x, int x_dtype, int64_t ldx, int64_t T,
                                           const ccq_lora_adapters* ad) {
   if (T <= 0 || T > 65536 || !lora_float_code(x_dtype) || check_adapters(ad, "ccq_lora_workspace_size")) return 0;
-  return lora_plan(T, ad, lora_lines(x, x_dtype, ldx, T, ad), lora_one_type(x_dtype, ad)).total;
+  return lora_plan(T, ad, lora_lines(x, x_dtype, ldx, T, ad), lora_one_type(x_dtype, ad), x_dtype == CCQ_F32).total;
 }
 
 extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64_t* index, void* y, int y_dtype,
@@ -1436,7 +1445,7 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
                   aligned(ad->a, 2) && aligned(ad->b, 2) && aligned(ad->scale, 4) && aligned(ad->rank, 4),
               "ccq_lora_add: a pointer is not aligned to its elements");
   const bool lines = lora_lines(x, x_dtype, ldx, T, ad);
-  const LoraPlan L = lora_plan(T, ad, lines, lora_one_type(x_dtype, ad));
+  const LoraPlan L = lora_plan(T, ad, lines, lora_one_type(x_dtype, ad), x_dtype == CCQ_F32);
   CCQ_REQUIRE(L.total == 0 || (workspace && workspace_bytes >= L.total && aligned(workspace, 256)),
               "ccq_lora_add: workspace of %zu bytes (256-byte aligned) needed, %zu given", L.total, workspace_bytes);
   hipStream_t st = as_stream(stream);
