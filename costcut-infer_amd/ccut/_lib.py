@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -68,6 +69,9 @@ class ccq_lora_adapters(ctypes.Structure):
         ("dtype", _int),
         ("num_adapters", _i64), ("rank_max", _i64), ("in_features", _i64), ("out_features", _i64),
     ]
+
+
+RMS_NORM_ARGS = struct.Struct("@8P5q4if4x")  # ccq_rms_norm_args
 
 
 # name -> (restype, argtypes); the order follows include/ccq.h
@@ -143,6 +147,7 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_fp8_block_linear_quantized": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
     "ccq_rms_norm": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _int, ctypes.c_float, _vp, _i64, _vp, _int, _int, _vp,
                             _vp, _i64, _i64, _vp]),
+    "ccq_rms_norm_packed": (_int, [ctypes.c_char_p]),  # RMS_NORM_ARGS.pack(...)
     "ccq_lora_workspace_size": (_sz, [_vp, _int, _i64, _i64, ctypes.POINTER(ccq_lora_adapters)]),
     "ccq_lora_add": (_int, [_vp, _int, _i64, _vp, _vp, _int, _i64, _i64, ctypes.POINTER(ccq_lora_adapters), _vp, _sz,
                             _vp]),

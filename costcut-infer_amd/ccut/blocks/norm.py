@@ -16,20 +16,21 @@ themselves (for a router or adapters beside a quantized projection).
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple
 
 import torch
 
 from ccut import _dev
 from ccut._dev import DTYPE_CODE, empty_strided, is_current, raw_stream, rows_overlap
-from ccut._lib import CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW, CCQ_Q_NONE, check, lib
+from ccut._lib import CCQ_Q_FP8_BLOCK, CCQ_Q_INT8_ROW, CCQ_Q_NONE, RMS_NORM_ARGS, check, lib
 
 _U8, _I8, _F32 = torch.uint8, torch.int8, torch.float32
+_pack = RMS_NORM_ARGS.pack
 
 __all__ = ["rms_norm", "rms_norm_fp8", "rms_norm_int8", "QuantizedRows"]
 
 MAX_H = 32768
+MAX_EPS = 3.4e38  # a float32
 
 
 class QuantizedRows(NamedTuple):
@@ -76,7 +77,7 @@ def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, normed: b
         raise ValueError(f"rows must be [..., H] with 1 <= H <= {MAX_H}, got {tuple(shape)}")
     if q_fmt == CCQ_Q_FP8_BLOCK and H & 127:
         raise ValueError(f"FP8 rows need H % 128 == 0, got H={H}")
-    if not 0 < eps < math.inf:
+    if not 0 < eps < MAX_EPS:
         raise ValueError(f"eps must be positive and finite, got {eps}")
     wcode = DTYPE_CODE.get(weight.dtype)
     if wcode is None or weight.dim() != 1 or weight.numel() != H or weight.get_device() != index:
@@ -88,8 +89,8 @@ def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, normed: b
     x2, ldx = (x, H) if flat and x.is_contiguous() else _rows(x)
     T = shape[0] if flat else x2.shape[0]
     size, strides = (T, H), (H, 1)
-    rp = op = yp = qp = sp = q = scale = y = None
-    ldr = ldo = ycode = 0
+    q = scale = y = None
+    rp = op = yp = qp = sp = ldr = ldo = ycode = 0
     if residual is not None:
         if residual.dtype != dtype or residual.shape != shape or residual.get_device() != index:
             raise _unlike(residual, "residual", x)
@@ -124,8 +125,8 @@ def _norm(x: torch.Tensor, weight, eps: float, residual, residual_out, normed: b
         q = empty_strided(size, strides, _I8)
         scale = empty_strided((T,), (1,), _F32)
         qp, sp = q.data_ptr(), scale.data_ptr()
-    rc = lib().ccq_rms_norm(x2.data_ptr(), code, ldx, rp, ldr, weight.data_ptr(), wcode, eps, op, ldo, yp, ycode, q_fmt,
-                            qp, sp, T, H, raw_stream(index))
+    rc = lib().ccq_rms_norm_packed(_pack(x2.data_ptr(), rp, weight.data_ptr(), op, yp, qp, sp, raw_stream(index), ldx,
+                                         ldr, ldo, T, H, code, wcode, ycode, q_fmt, eps))
     if rc:
         check(rc, "ccq_rms_norm")
     if not flat:

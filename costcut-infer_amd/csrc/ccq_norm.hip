@@ -313,3 +313,9 @@ extern "C" int ccq_rms_norm(const void* x, int x_dtype, int64_t ldx, const void*
   }
   return 0;
 }
+
+extern "C" int ccq_rms_norm_packed(const ccq_rms_norm_args* a) {
+  CCQ_REQUIRE(a != nullptr, "ccq_rms_norm_packed: null arguments");
+  return ccq_rms_norm(a->x, a->x_dtype, a->ldx, a->residual, a->ldr, a->w, a->w_dtype, a->eps, a->residual_out, a->ldo,
+                      a->y, a->y_dtype, a->q_fmt, a->q, a->scale, a->rows, a->H, a->stream);
+}

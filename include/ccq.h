@@ -555,6 +555,23 @@ int ccq_rms_norm(const void* x, int x_dtype, int64_t ldx, const void* residual, 
                  void* y, int y_dtype, int q_fmt, void* q, float* scale, int64_t rows, int64_t H,
                  void* stream);
 
+/* ccq_rms_norm's arguments in one block, for callers that pay for each argument
+ * of a call: from Python 18 of them take 1.6 us, a packed block 0.45. */
+typedef struct ccq_rms_norm_args {
+  const void* x;
+  const void* residual;
+  const void* w;
+  void* residual_out;
+  void* y;
+  void* q;
+  float* scale;
+  void* stream;
+  int64_t ldx, ldr, ldo, rows, H;
+  int x_dtype, w_dtype, y_dtype, q_fmt;
+  float eps;
+} ccq_rms_norm_args;
+int ccq_rms_norm_packed(const ccq_rms_norm_args* args);
+
 /* ------------------------------------------------------------------------
  * Low-rank adapters of many requests beside one shared projection (no
  * counterpart in the reference, which serves one request at a time)

@@ -126,3 +126,24 @@ def test_overlap_of_views():
     half = buf.view(torch.float16)  # 200 columns of half the size
     assert not over(half[:, :80], buf[:, 40:])
     assert over(half[:, :81], buf[:, 40:])
+
+
+def test_rms_norm_packed(lib):
+    """The arguments in one block reach the same checks, each from its place."""
+    from ccut._lib import CCQ_EINVAL, RMS_NORM_ARGS, last_error
+
+    def call(**kw):
+        a = dict(x=256, residual=0, w=256, residual_out=0, y=0, q=256, scale=256, stream=0, ldx=256, ldr=0, ldo=0, rows=2,
+                 H=256, x_dtype=2, w_dtype=2, y_dtype=0, q_fmt=1, eps=1e-6)
+        a.update(kw)
+        return lib.ccq_rms_norm_packed(RMS_NORM_ARGS.pack(*a.values()))
+
+    assert RMS_NORM_ARGS.size == 128
+    assert call(rows=0) == 0
+    for kw, word in [(dict(rows=-1), "rows"), (dict(H=200), "multiple of 128"), (dict(x_dtype=3), "x_dtype"),
+                     (dict(w_dtype=-1), "w_dtype"), (dict(y=256, y_dtype=9), "y_dtype"), (dict(q_fmt=3), "q_fmt"),
+                     (dict(eps=0.0), "eps"), (dict(ldx=255), "stride"), (dict(residual=256, ldr=255), "stride"),
+                     (dict(residual_out=256, ldo=0), "stride"), (dict(x=0), "null"), (dict(w=0), "null"),
+                     (dict(q=0), "null"), (dict(scale=0), "null"), (dict(x=257), "aligned"), (dict(q=260), "8-byte")]:
+        assert call(**kw) == CCQ_EINVAL and word in last_error(), kw
+    assert lib.ccq_rms_norm_packed(None) == CCQ_EINVAL and "null" in last_error()
