@@ -47,13 +47,14 @@ struct LoraP {
   const int32_t* rank;
   int32_t* tile_rows;           // [tiles][TM], -1: padding
   int32_t* tile_adapter;        // [tiles], of ccq_moe_align's schedule
-  int4* tile_info;              // [tiles], for the second kernel: adapter (-1: no such tile), rank, bits of the scale
+  int4* tile_info;              // [tiles], for the second kernel: adapter (-1: no such tile), rank, bits of the scale, splits
   const int32_t* meta;          // tiles of ccq_moe_align's schedule; null: workgroups sort
   float* p;                     // [S][T][Rp]
   int64_t ldx, ldy;
   int64_t last_x, last_a, last_b;  // where the last 8 values of x, a and b begin
   int T, L, R, Rp, K, N;
   int S, kchunk;                // splits of K, K per split (a multiple of 32)
+  int few, S_few, kchunk_few;   // those of the 64-token shrink for up to `few` tiles
   int tiles, ncols;             // tiles of the grid, columns per workgroup
   int y_dtype;
 };
@@ -266,10 +267,10 @@ __device__ void lr_read_tile(const LoraP& p, int tile, TileS<TM>& t) {
 }
 
 // what the second kernel needs of a tile in one load
-__device__ __forceinline__ void lr_write_info(const LoraP& p, int tile, int adapter, int rank) {
+__device__ __forceinline__ void lr_write_info(const LoraP& p, int tile, int adapter, int rank, int splits) {
   if (threadIdx.x == 0)
     p.tile_info[tile] = make_int4(rank > 0 ? adapter : -1, rank,
-                                  __float_as_int(adapter >= 0 && p.scale != nullptr ? p.scale[adapter] : 1.f), 0);
+                                  __float_as_int(adapter >= 0 && p.scale != nullptr ? p.scale[adapter] : 1.f), splits);
 }
 
 // ---------------------------------------------------------------- shrink --
@@ -764,7 +765,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   }
   const int adapter = tl.adapter;
   const int rank = adapter < 0 ? 0 : lr_rank(p, adapter);
-  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank);
+  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank, p.S);
   const int rz = blockIdx.z * RH * RT * 16;
   if (rz >= rank) return;
   const int h = wave % RH, part = wave / RH, r0 = rz + h * RT * 16;
@@ -820,10 +821,10 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
 // each wave multiplies one step of 32 k (part) of it for RTW * 16 ranks (h).
 // In a line the 16-byte piece i of row r lies at i ^ (r & 7), so that the
 // operand reads of 8 neighbouring lanes cover all banks.
-// T=4096 K=14336 R=128: 47 us, 2.4 TB/s of x; 34 us with x in the last level
-// cache, 27 us at R=16.  A, two thirds of a stage, comes from L2; more stages
-// ahead, x and A copied by waves of their own, and other orders of the stages
-// left the time as it is.
+// T=4096 K=14336 R=128: 42.6 us, 2.6 TB/s of x (47 by three splits; then 34
+// with x in the last level cache, 27 at R=16).  A, two thirds of a stage, comes
+// from L2; more stages ahead, x and A copied by waves of their own, and other
+// orders of the stages left the time as it is.
 template <int XT, int WT, int RT>
 struct TileShrink {
   static constexpr int RTW = RT == 8 ? 4 : RT == 4 ? 2 : 1, RH = RT / RTW, KP = LR_WAVES / RH, Q = KP / 2;
@@ -850,10 +851,14 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
   // the tiles' K ranges, range by range, in eight parts of one size, one to an
   // XCD: its L2 then reads few adapters' A, and of those one range each
-  int split = 0, tile = -1, total = 0;
+  int split = 0, tile = -1, total = 0, S = p.S, kchunk = p.kchunk;
   auto pick = [&](int count) {
     total = count;
-    const int xcd = blockIdx.x & 7, all = count * p.S, from = (int)((int64_t)xcd * all >> 3);
+    if (count <= p.few) {
+      S = p.S_few;
+      kchunk = p.kchunk_few;
+    }
+    const int xcd = blockIdx.x & 7, all = count * S, from = (int)((int64_t)xcd * all >> 3);
     const int at = from + (blockIdx.x >> 3);
     if (at < (int)((int64_t)(xcd + 1) * all >> 3)) {
       split = at / count;
@@ -874,10 +879,10 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
   if (tile < 0) return;
   const int adapter = __builtin_amdgcn_readfirstlane(tl.adapter);
   const int rank = __builtin_amdgcn_readfirstlane(adapter < 0 ? 0 : lr_rank(p, adapter));
-  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank);
+  if (split == 0 && blockIdx.z == 0) lr_write_info(p, tile, adapter, rank, S);
   const int rz = blockIdx.z * RT * 16;
   if (rz >= rank) return;
-  const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), stages = (ke - ks + C::SK - 1) / C::SK;
+  const int ks = split * kchunk, ke = min(ks + kchunk, p.K), stages = (ke - ks + C::SK - 1) / C::SK;
 
   // copy i of the wave: 8 rows of one line, this lane piece `piece` of row `row`
   uint32_t off[NI];   // bytes from the base below, at the split's first stage
@@ -997,7 +1002,7 @@ __device__ __forceinline__ void lr_lane_exchange() {
 // p's loads go first: a wave waits for its loads in order, and those of y come
 // from HBM.  T=2048 N=14336 R=16: 25.7 us for 117 MB of y (4.6 TB/s; 27.5 with
 // y before p, 30.1 with the weights loaded step by step).  T=4096 N=4096
-// R=128: 30.4 us, 10 of them until p of three splits is in LDS.
+// R=128: 30.8 us, 10 of them until p of its splits is in LDS.
 template <int WT, int YT, int MT, int KEEP>
 __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 ? 4 : 8) ? 2 : 3) void lora_expand_kernel(
     const LoraP p) {
@@ -1046,7 +1051,8 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
   const int j = threadIdx.x & ((1 << lp) - 1), sub = threadIdx.x >> lp;
   const bool spare = MT == 1 && lp < 4;
   const int share = spare ? __builtin_amdgcn_readfirstlane(sub >> 4) : 0, shares = spare ? 16 >> lp : 1;
-  const int per = p.S <= 4 ? p.S : (p.S + shares - 1) / shares, s0 = share * per, s1 = min(s0 + per, p.S);
+  const int S = __builtin_amdgcn_readfirstlane(info.w);
+  const int per = S <= 4 ? S : (S + shares - 1) / shares, s0 = share * per, s1 = min(s0 + per, S);
   const int rows = spare ? 16 : LE_THREADS >> lp, passes = TM / rows, row0 = spare ? sub & 15 : sub;
   float* shared = reinterpret_cast<float*>(parts + PARTS * TM * ld);  // [shares][16][r16]
   const char* pb = reinterpret_cast<const char*>(p.p);
@@ -1089,7 +1095,7 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
     }
     if (pass + U < passes) load_p(pass + U, s0);
     if constexpr (MT == 1) {
-      if (spare && p.S > 4) {  // else the first share is all
+      if (spare && S > 4) {  // else the first share is all
         if (share > 0 && 4 * j < r16) *reinterpret_cast<f32x4*>(shared + (share * 16 + row0) * r16 + 4 * j) = sum[0];
         lds_barrier();
         if (share == 0 && 4 * j < r16)
@@ -1234,6 +1240,7 @@ size_t a256l(size_t b) { return (b + 255) & ~(size_t)255; }
 struct LoraPlan {
   bool fused, align;
   int64_t tm, tiles, S, kchunk, Rp, ncols;
+  int64_t few, S_few, kchunk_few;  // as in LoraP
   size_t off_rows, off_tile, off_info, off_meta, off_counts, off_align, off_p, total;
 };
 
@@ -1286,10 +1293,23 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   } else {
     const int64_t most = cdiv(K, LR_WAVES * 64) < 8 ? cdiv(K, LR_WAVES * 64) : 8;
     const int64_t part = (R < 64 ? R : R < 128 ? 64 : 128) / (x32 ? 4 : 1), start = x32 ? 128 : 512;
-    auto time = [&](int64_t s) { return (double)cdiv(likely * s, 256) * ((double)K / s + start) + (double)(s * part); };
-    double best = time(1);
-    for (int64_t s = 2; s <= most; ++s) best = time(s) < best ? time(s) : best;
-    while (time(S) > 1.05 * best) ++S;
+    auto splits = [&](int64_t tiles) {
+      auto time = [&](int64_t s) { return (double)cdiv(tiles * s, 256) * ((double)K / s + start) + (double)(s * part); };
+      double best = time(1);
+      for (int64_t s = 2; s <= most; ++s) best = time(s) < best ? time(s) : best;
+      int64_t s = 1;
+      while (time(s) > 1.05 * best) ++s;
+      return s;
+    };
+    S = splits(likely);
+    // where few tiles are padding the kernel, which counts them, may take more in as many rounds (T=4096 K=14336 R=128,
+    // 62 tiles of at most 68: 4 splits 42.6 us, 3 46.9)
+    const int64_t least = cdiv(T, L.tm), S_few = lines ? splits(least) : S;
+    if (S_few > S) {
+      L.kchunk_few = cdiv(cdiv(K, S_few), 256) * 256;
+      L.S_few = cdiv(K, L.kchunk_few);
+      L.few = cdiv(least * L.S_few, 256) * 256 / L.S_few;
+    }
   }
   const int64_t step = L.tm == 16 ? 32 : 256;  // the largest stage of a 64-token tile
   L.kchunk = cdiv(cdiv(K, S), step) * step;
@@ -1308,7 +1328,7 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   L.off_align = o;
   if (L.align) o += a256l(align_scratch_bytes(T, ad->num_adapters));
   L.off_p = o;
-  o += a256l((size_t)L.S * T * L.Rp * 4);
+  o += a256l((size_t)std::max(L.S, L.S_few) * T * L.Rp * 4);
   L.total = o;
   return L;
 }
@@ -1362,7 +1382,7 @@ void shrink_launch(const LoraP& p, hipStream_t st) {
 template <int XT, int WT>
 void shrink_tile_launch(const LoraP& p, hipStream_t st) {
   const int rt = (int)cdiv(p.R, 16);
-  const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * p.S), 1, (unsigned)cdiv(rt, 8)), block(LR_THREADS);
+  const dim3 grid((unsigned)(((p.tiles + 7) & ~7) * std::max(p.S, p.S_few)), 1, (unsigned)cdiv(rt, 8)), block(LR_THREADS);
   if (rt <= 1)
     launch((lora_shrink_tile_kernel<XT, WT, 1>), grid, block, 0, st, p);
   else if (rt <= 2)
@@ -1469,6 +1489,9 @@ extern "C" int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64
   p.N = (int)ad->out_features;
   p.S = (int)L.S;
   p.kchunk = (int)L.kchunk;
+  p.few = (int)L.few;
+  p.S_few = (int)L.S_few;
+  p.kchunk_few = (int)L.kchunk_few;
   p.tiles = (int)L.tiles;
   p.ncols = (int)L.ncols;
   p.y_dtype = y_dtype;

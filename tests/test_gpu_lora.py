@@ -519,3 +519,12 @@ def test_rows_quantized_already_refusals(gpu):
     one = fp8_block.linear_quantized(lin, big[0, 3:259].view(torch.float8_e4m3fn), torch.ones(2, device=gpu),
                                      torch.float32)
     assert one.shape == (128,)
+
+
+@pytest.mark.parametrize("T,K,R,L", [(2048, 4096, 16, 8), (4096, 2048, 128, 6), (1500, 3600, 40, 20)])
+@pytest.mark.parametrize("pattern", ["one", "runs", "mixed", "none"])
+def test_splits_by_the_number_of_tiles(gpu, T, K, R, L, pattern):
+    """Tiles without padding, with some, with as much as there can be, and none."""
+    for types in (("bf16", "bf16", "bf16"), ("f32", "f16", "f32")):
+        c = _case(T, K, 40, R, L, *types, pattern=pattern)
+        _check(_run(c, gpu), c)
