@@ -420,9 +420,12 @@ __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
   }
 }
 
-// k such that 2^k brings a row whose largest finite |p| is m into [2^13, 2^14]
+// k such that 2^k brings a row whose largest finite |p| is m into [2^13, 2^14],
+// from -114 (m near 2^128) on, up to what lr_pow2 holds of 2^k and 2^-k: below
+// 2^-112 m stays smaller (2^-126 becomes 1), and the parts, which end at 2^-24,
+// still hold 22 bits of it.
 __device__ __forceinline__ int lr_exponent(float m) {
-  return m > 0.f ? min(max(14 - __builtin_amdgcn_frexp_expf(m), -100), 100) : 0;
+  return m > 0.f ? min(14 - __builtin_amdgcn_frexp_expf(m), 126) : 0;
 }
 __device__ __forceinline__ float lr_pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 

@@ -528,3 +528,22 @@ def test_splits_by_the_number_of_tiles(gpu, T, K, R, L, pattern):
     for types in (("bf16", "bf16", "bf16"), ("f32", "f16", "f32")):
         c = _case(T, K, 40, R, L, *types, pattern=pattern)
         _check(_run(c, gpu), c)
+
+
+def _factor(c, f):
+    """The adapters' products times f, and y with them."""
+    c["scale"] = torch.where(torch.arange(c["a"].shape[0]) % 2 == 0, 1.0, -0.75) * f
+    c["y"] = (c["y"].double() * f).to(c["y"].dtype)
+    return c
+
+
+@pytest.mark.parametrize("power", [110, 116, 120, 122, -100, -108, -114, -120])
+@pytest.mark.parametrize("T,K,R", [(5, 64, 16), (40, 200, 40), (600, 72, 24), (600, 75, 130)])
+def test_products_over_the_float32_range(gpu, T, K, R, power):
+    """Scaled inner products near both ends of float32's range.  (Parts in
+    bfloat16 end at 2^-133: products below 2^-107 keep fewer bits there.)"""
+    for types in (("f32", "f16", "f32"), ("f16", "f16", "f32"), ("f32", "bf16", "f32"), ("bf16", "bf16", "f32")):
+        if types[1] == "bf16" and power < -100:
+            continue
+        c = _factor(_case(T, K, 72, R, 3, *types), 2.0 ** power)
+        _check(_run(c, gpu), c)
