@@ -397,7 +397,10 @@ __device__ __forceinline__ void lr_shrink_ring(const LoraP& p, const int64_t (&x
 // ---------------------------------------------------------------- expand --
 // p in parts of the weights' type, most significant first, whose sum is p to
 // 16 (two parts of bf16), 24 (three) or 22 bits of the row's largest (two of
-// f16, the row scaled by a power of two into its range).
+// f16, the row scaled by a power of two into its range).  Parts in bf16 end at
+// 2^-133: a p below 2^-107 keeps fewer bits of three.  A finite p that rounds
+// to infinity in bf16 gives that type's largest value and the rest (2^-8 of p
+// or less, so two parts still hold 16 bits).
 template <int WT, int PARTS, int N, class V>
 __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
 #pragma unroll
@@ -407,7 +410,9 @@ __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
     for (int i = 0; i < PARTS; ++i) {
       float h;
       if constexpr (WT == CCQ_BF16) {
-        const __bf16 b = (__bf16)rest;
+        constexpr float most = 0x1.FEp127f;
+        const float in = i == 0 && isfinite(rest) ? fminf(fmaxf(rest, -most), most) : rest;
+        const __bf16 b = (__bf16)in;
         out[i][e] = b;
         h = (float)b;
       } else {

@@ -547,3 +547,19 @@ def test_products_over_the_float32_range(gpu, T, K, R, power):
             continue
         c = _factor(_case(T, K, 72, R, 3, *types), 2.0 ** power)
         _check(_run(c, gpu), c)
+
+
+@pytest.mark.parametrize("T,R", [(5, 16), (40, 40), (600, 24)])
+def test_largest_products(gpu, T, R):
+    """Inner products that round to infinity in bfloat16 and are finite in
+    float32: 2^127 (2 - 2^-8) and more."""
+    for ydt in ("f32", "bf16"):
+        c = _case(T, 64, 72, R, 2, "f32", "bf16", ydt, scale=False)
+        c["x"].zero_()
+        c["x"][:, 3] = torch.where(torch.arange(T) % 3 == 0, -1.0, 1.0) * torch.linspace(3.3896e38, 3.4028e38, T)
+        c["a"].zero_()
+        c["a"][:, ::5, 3] = 1.0
+        c["b"] = torch.zeros_like(c["b"])
+        c["b"][:, :, 0] = torch.linspace(-0.75, 0.75, 72).bfloat16()  # 0 among them
+        c["b"][:, 36, 0] = 0.0
+        _check(_run(c, gpu), c)
