@@ -185,7 +185,9 @@ class LinearProj:
         if adapters is not None:
             from ccut.quant import lora
 
-            xd = _f32_input(x) if _dev.is_host(x) else x
+            # the adapters take float rows of the current device as they are; others are converted, as apply does
+            as_is = not _dev.is_host(x) and x.dtype in _dev.DTYPE_CODE and _dev.is_current(x.get_device())
+            xd = x if as_is else _f32_input(x)
             return _return(lora.add_(self.apply(xd), xd, adapters, _dev.to_device(index, torch.int64)), x)
         self._load()
         if self._method is None:

@@ -563,3 +563,24 @@ def test_largest_products(gpu, T, R):
         c["b"][:, :, 0] = torch.linspace(-0.75, 0.75, 72).bfloat16()  # 0 among them
         c["b"][:, 36, 0] = 0.0
         _check(_run(c, gpu), c)
+
+
+def test_projection_with_adapters_takes_what_it_takes_without(gpu):
+    """Rows of any type that ``apply`` converts, an index of any whole
+    numbers."""
+    from ccut.quant.linear import FakeWeightReader, LinearProj
+
+    T, K, N = 9, 64, 48
+    c = _case(T, K, N, 8, 3, "f32", "bf16", "f32")
+    ad = _adapters(c, gpu)
+    rng = np.random.default_rng(1)
+    wf = rng.standard_normal((N, K)).astype(np.float32)
+    proj = LinearProj(0, "proj", N, K, FakeWeightReader({(0, "proj"): wf.tobytes()}, {(0, "proj"): (N, K, "F32")}), None)
+    for x in (c["x"].to(gpu), c["x"].to(gpu).double(), c["x"].numpy().astype(np.float64),
+              torch.randint(-4, 5, (T, K), device=gpu)):
+        plain = torch.as_tensor(proj.apply(x)).cpu()
+        want = dict(c, x=torch.as_tensor(x).cpu().float(), y=plain)
+        for index in (c["index"].to(gpu), c["index"].tolist(), c["index"].numpy().astype(np.int16)):
+            _check(torch.as_tensor(proj.apply(x, adapters=ad, index=index)), want)
+    none = np.zeros((0, K), np.float32)
+    assert proj.apply(none).shape == proj.apply(none, adapters=ad, index=[]).shape == (0, N)
