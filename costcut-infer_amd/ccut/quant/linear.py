@@ -178,8 +178,8 @@ class LinearProj:
         """``x [batch, in] @ W.T -> [batch, out]`` float32 (numpy in, numpy
         out; a device tensor in, a device tensor out).  With ``adapters``
         (``quant.lora.LoraAdapters`` of this projection) and ``index [batch]``
-        (each row's adapter, negative for none), each row's low-rank product
-        is added to it."""
+        (each row's adapter, negative for none; whole numbers), each row's
+        low-rank product is added to it."""
         if (adapters is None) != (index is None):
             raise ValueError(f"{self.name}: adapters and index come together")
         if adapters is not None:
@@ -188,7 +188,10 @@ class LinearProj:
             # the adapters take float rows of the current device as they are; others are converted, as apply does
             as_is = not _dev.is_host(x) and x.dtype in _dev.DTYPE_CODE and _dev.is_current(x.get_device())
             xd = x if as_is else _f32_input(x)
-            return _return(lora.add_(self.apply(xd), xd, adapters, _dev.to_device(index, torch.int64)), x)
+            index = _dev.to_device(index)
+            if index.numel() and (index.is_floating_point() or index.is_complex() or index.dtype == torch.bool):
+                raise ValueError(f"{self.name}: index must hold whole numbers, got {index.dtype}")
+            return _return(lora.add_(self.apply(xd), xd, adapters, index.to(torch.int64)), x)
         self._load()
         if self._method is None:
             return _return(f32_linear(_f32_input(x), self._w32), x)

@@ -567,7 +567,7 @@ def test_largest_products(gpu, T, R):
 
 def test_projection_with_adapters_takes_what_it_takes_without(gpu):
     """Rows of any type that ``apply`` converts, an index of any whole
-    numbers."""
+    numbers; one that would be cut to whole numbers is refused."""
     from ccut.quant.linear import FakeWeightReader, LinearProj
 
     T, K, N = 9, 64, 48
@@ -582,5 +582,8 @@ def test_projection_with_adapters_takes_what_it_takes_without(gpu):
         want = dict(c, x=torch.as_tensor(x).cpu().float(), y=plain)
         for index in (c["index"].to(gpu), c["index"].tolist(), c["index"].numpy().astype(np.int16)):
             _check(torch.as_tensor(proj.apply(x, adapters=ad, index=index)), want)
+    for index in (c["index"].numpy().astype(np.float32), c["index"].to(gpu).double(), c["index"].numpy() >= 0):
+        with pytest.raises(ValueError, match="whole numbers"):
+            proj.apply(c["x"].numpy(), adapters=ad, index=index)
     none = np.zeros((0, K), np.float32)
     assert proj.apply(none).shape == proj.apply(none, adapters=ad, index=[]).shape == (0, N)
