@@ -35,16 +35,30 @@ def stream_ptr(device: torch.device | None = None) -> int:
     if device is not None and device not in _GPUS and device.type != "cuda":
         raise ValueError(f"Expected a cuda device, but got: {device}")
     index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
-    return torch._C._cuda_getCurrentRawStream(index)
+    return raw_stream(index)
 
 
-# A tensor of uninitialised memory on the current device, by (shape, strides,
-# dtype): 0.8 us, torch.empty 1.3-1.6 (a decode call with three outputs takes
-# 3-5 us on the GPU)
-empty_strided = torch._C._dynamo.guards._empty_strided_cuda
+def _empty_strided(size, strides, dtype: torch.dtype) -> torch.Tensor:
+    return torch.empty_strided(size, strides, dtype=dtype, device="cuda")
 
 
-raw_stream = torch._C._cuda_getCurrentRawStream  # of a device's index: what stream_ptr asks
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _current_device() -> int:
+    return torch.cuda.current_device()
+
+
+# Short cuts inside torch, where this torch has them (one built for the CPU
+# lacks some, and they carry no promise), else the public calls above.
+# empty_strided: a tensor of uninitialised memory on the current device, by
+# (shape, strides, dtype): 0.8 us, torch.empty 1.3-1.6 (a decode call with three
+# outputs takes 3-5 us on the GPU).
+_guards = getattr(getattr(torch._C, "_dynamo", None), "guards", None)
+empty_strided = getattr(_guards, "_empty_strided_cuda", _empty_strided)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)  # of a device's index: what stream_ptr asks
+current_device = getattr(torch._C, "_cuda_getDevice", _current_device)
 
 
 def is_current(index: int) -> bool:
@@ -53,7 +67,7 @@ def is_current(index: int) -> bool:
     initialised: 0.15 us, ``torch.cuda.current_device()`` 0.25."""
     if index < 0:
         raise ValueError("Expected a cuda device, but got: cpu")
-    return index == torch._C._cuda_getDevice()
+    return index == current_device()
 
 
 def rows_overlap(yp: int, ycode: int, ldy: int, N: int, xp: int, xcode: int, ldx: int, K: int, T: int) -> bool:

@@ -278,3 +278,23 @@ def test_sum_over_another_view_is_refused(gpu):
                 norm.rms_norm_int8(a, w, residual=b, residual_out=out)
     for out in (buf[:4, 256:], buf[4:, :256], x, r):
         assert norm.rms_norm_int8(x, w, residual=r, residual_out=out).residual is out
+
+
+def test_public_allocation_and_stream_calls(gpu, monkeypatch):
+    """The calls that stand in for torch's internal short cuts give the same
+    rows, on a stream of their own too."""
+    from ccut import _dev
+    from ccut.blocks import norm
+
+    x, w, r = (t.to(gpu) for t in _case(9, 256, torch.bfloat16, True))
+    want = norm.rms_norm_fp8(x, w, EPS, residual=r, normed=True)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        assert _dev._raw_stream(0) == _dev.raw_stream(0) == st.cuda_stream
+        monkeypatch.setattr(norm, "empty_strided", _dev._empty_strided)
+        monkeypatch.setattr(norm, "raw_stream", _dev._raw_stream)
+        monkeypatch.setattr(_dev, "current_device", _dev._current_device)
+        got = norm.rms_norm_fp8(x, w, EPS, residual=r, normed=True)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

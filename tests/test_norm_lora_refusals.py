@@ -147,3 +147,36 @@ def test_rms_norm_packed(lib):
                      (dict(q=0), "null"), (dict(scale=0), "null"), (dict(x=257), "aligned"), (dict(q=260), "8-byte")]:
         assert call(**kw) == CCQ_EINVAL and word in last_error(), kw
     assert lib.ccq_rms_norm_packed(None) == CCQ_EINVAL and "null" in last_error()
+
+
+def test_without_torch_internals():
+    """A torch that lacks the internal short cuts (one built for the CPU, or
+    another release) still imports the package, on which host-only code
+    stands, and allocates by the public calls."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+del torch._C._dynamo.guards._empty_strided_cuda
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import ccut.blocks.norm, ccut.quant.lora, ccut.quant.registry
+from ccut import _dev
+made = []
+torch.empty_strided = lambda *a, **k: made.append((a, k))
+_dev.empty_strided((2, 3), (3, 1), torch.float32)
+assert made == [(((2, 3), (3, 1)), dict(dtype=torch.float32, device="cuda"))], made
+torch.cuda.current_device = lambda: 5
+assert _dev.is_current(5) and not _dev.is_current(0)
+torch.cuda.current_stream = lambda device: type("S", (), dict(cuda_stream=100 + device))
+assert _dev.raw_stream(3) == 103 and _dev.stream_ptr(torch.device("cuda", 2)) == 102
+print("ok")
+"""
+    pkg = Path(__file__).resolve().parents[1] / "costcut-infer_amd"
+    r = subprocess.run([sys.executable, "-c", code, str(pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]
