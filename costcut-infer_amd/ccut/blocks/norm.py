@@ -144,8 +144,12 @@ def rms_norm(x, weight, eps: float = 1e-6, *, residual=None, residual_out: torch
     default x's), or ``(y, s)`` where a residual is given (``s`` in x's type,
     written to ``residual_out``, which may be ``residual`` or ``x`` but no
     other view of their memory).  Host
-    arrays are uploaded as float32 and numpy float32 is returned."""
+    arrays are uploaded as float32 and numpy float32 is returned, no other
+    ``out_dtype``."""
     if _dev.is_host(x):
+        if out_dtype not in (None, torch.float32):
+            raise ValueError(f"host rows are returned as float32, not {out_dtype}")
+
         def up(a):
             return a if a is None else _dev.to_device(a, torch.float32)
 

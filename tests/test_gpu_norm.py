@@ -298,3 +298,16 @@ def test_public_allocation_and_stream_calls(gpu, monkeypatch):
         got = norm.rms_norm_fp8(x, w, EPS, residual=r, normed=True)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_host_rows_are_returned_as_float32(gpu):
+    """Another type for host rows is refused, not left out."""
+    from ccut.blocks import norm
+
+    x, w = torch.randn(3, 40), torch.ones(40)
+    y = norm.rms_norm(x.numpy(), w.numpy(), EPS, out_dtype=torch.float32)
+    assert y.dtype.name == "float32"
+    _close(torch.from_numpy(y), on.rms_norm(x, w, EPS)[3])
+    for dt in (torch.float16, torch.bfloat16, torch.float64):
+        with pytest.raises(ValueError, match="float32"):
+            norm.rms_norm(x.numpy(), w.numpy(), EPS, out_dtype=dt)
