@@ -311,3 +311,54 @@ def test_host_rows_are_returned_as_float32(gpu):
     for dt in (torch.float16, torch.bfloat16, torch.float64):
         with pytest.raises(ValueError, match="float32"):
             norm.rms_norm(x.numpy(), w.numpy(), EPS, out_dtype=dt)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H", [2049, 2176, 4095, 4096, 4097, 7168, 8191, 8192])
+def test_both_sides_of_the_row_count_rule(gpu, H, dt):
+    """More than 512 rows take two vectors a thread, fewer one, for rows of
+    2049 to 8192: every output format on both."""
+    from ccut.blocks import norm
+
+    for T in (512, 513, 530):
+        x, w, r = _case(T, H, DT[dt], T != 513)
+        xd, wd, rd = x.to(gpu), w.to(gpu), None if r is None else r.to(gpu)
+        _check(norm.rms_norm_int8(xd, wd, EPS, residual=rd, normed=True), x, w, r, "int8", True)
+        if H % 128 == 0:
+            _check(norm.rms_norm_fp8(xd, wd, EPS, residual=rd, normed=True), x, w, r, "fp8", True)
+        y = on.rms_norm(x, w, EPS, r)[3]
+        got = norm.rms_norm(xd, wd, EPS, residual=rd)
+        _close(got if r is None else got[0], y, x.dtype)
+
+
+@pytest.mark.parametrize("H", [9000, 16384, 16385, 20000])
+def test_long_rows(gpu, H):
+    """The two instances above 8192 columns, few rows and many."""
+    from ccut.blocks import norm
+
+    for T, dt in ((3, "f32"), (600, "bf16"), (40, "f16")):
+        x, w, r = _case(T, H, DT[dt], True)
+        xd, wd, rd = x.to(gpu), w.to(gpu), r.to(gpu)
+        _check(norm.rms_norm_int8(xd, wd, EPS, residual=rd, normed=True), x, w, r, "int8", True)
+        if H % 128 == 0:
+            _check(norm.rms_norm_fp8(xd, wd, EPS, residual=rd, normed=True), x, w, r, "fp8", True)
+
+
+def test_rows_whose_squares_overflow(gpu):
+    """Finite values whose squares leave float32: the row's statistics are
+    infinite, so y and the scales are 0, with the codes as defined."""
+    from ccut.blocks import norm
+
+    x, w, _ = _case(4, 1024, torch.float32, False)
+    x[1] *= 1e25
+    x[2, 700] = 1e30
+    for f, rows in ((norm.rms_norm_fp8, on.fp8_rows), (norm.rms_norm_int8, on.int8_rows)):
+        got = f(x.to(gpu), w.to(gpu), EPS, normed=True)
+        _, p, rstd, y = on.rms_norm(x, w, EPS)
+        q, scale = rows(p, rstd)
+        assert torch.equal(got.q.cpu(), q)
+        for t in (1, 2):
+            assert (got.scale[t] == 0).all() and (got.y[t] == 0).all()
+        for t in (0, 3):
+            _close(got.scale[t], scale[t])
+            _close(got.y[t], y[t])
