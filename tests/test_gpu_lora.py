@@ -587,3 +587,34 @@ def test_projection_with_adapters_takes_what_it_takes_without(gpu):
             proj.apply(c["x"].numpy(), adapters=ad, index=index)
     none = np.zeros((0, K), np.float32)
     assert proj.apply(none).shape == proj.apply(none, adapters=ad, index=[]).shape == (0, N)
+
+
+@pytest.mark.parametrize("K", [2048, 4104, 3601])
+@pytest.mark.parametrize("T", [4097, 5000, 8192])
+def test_splits_above_the_self_sorted_batches(gpu, T, K):
+    """K in several parts behind the schedule's own launch: whole and partial
+    last stages, rows that are not aligned, few and many tiles (5000 tokens of
+    40 adapters take another number of parts for each)."""
+    for R, L, pattern, types in ((16, 3, "runs", ("bf16", "bf16", "bf16")), (64, 40, "one", ("f16", "f16", "f16")),
+                                 (64, 40, "mixed", ("f16", "f16", "f32")), (128, 7, "runs", ("f32", "bf16", "f32")),
+                                 (200, 40, "runs", ("bf16", "bf16", "f32")), (32, 40, "one", ("f32", "f16", "f32")),
+                                 (16, 5, "none", ("bf16", "bf16", "bf16"))):
+        c = _case(T, K, 40, R, L, *types, pattern=pattern, ranks=R == 64 and pattern == "mixed")
+        _check(_run(c, gpu), c)
+
+
+def test_far_inputs_of_one_copy_base(gpu):
+    """Rows of x between 2^31 and 2^32 bytes behind the first, as 32-bit
+    offsets of aligned copies, for tiles of few tokens in one kernel and of
+    many.  x begins 2^31 bytes into its buffer, which holds any such offset."""
+    from ccut.quant import lora
+
+    buf = torch.empty(3 * 2 ** 30 + 2 ** 22, dtype=torch.bfloat16, device=gpu)
+    for T, ld in ((16, 130000000), (700, 2900000), (5000, 420000)):
+        c = _case(T, 128, 40, 16, 3, "bf16", "bf16", "bf16")
+        assert 2 ** 31 < (T - 1) * ld * 2 and (ld + 1) * T * 2 <= 2 ** 32 and ld % 8 == 0
+        xs = buf[2 ** 30:2 ** 30 + T * ld].view(T, ld)[:, :128]
+        xs.copy_(c["x"].to(gpu))
+        y = c["y"].to(gpu)
+        lora.add_(y, xs, _adapters(c, gpu), c["index"].to(gpu))
+        _check(y, c)
