@@ -398,9 +398,10 @@ __device__ __forceinline__ void lr_shrink_ring(const LoraP& p, const int64_t (&x
 // p in parts of the weights' type, most significant first, whose sum is p to
 // 16 (two parts of bf16), 24 (three) or 22 bits of the row's largest (two of
 // f16, the row scaled by a power of two into its range).  Parts in bf16 end at
-// 2^-133: a p below 2^-107 keeps fewer bits of three.  A finite p that rounds
-// to infinity in bf16 gives that type's largest value and the rest (2^-8 of p
-// or less, so two parts still hold 16 bits).
+// 2^-133, so a p below 2^-105 keeps fewer bits of three; they are taken of p / 4
+// (LR_DOWN), since a p of 2^128 (1 - 2^-9) and more rounds to infinity in bf16.
+template <int WT>
+constexpr float LR_DOWN = WT == CCQ_BF16 ? 4.f : 1.f;
 template <int WT, int PARTS, int N, class V>
 __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
 #pragma unroll
@@ -410,9 +411,7 @@ __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
     for (int i = 0; i < PARTS; ++i) {
       float h;
       if constexpr (WT == CCQ_BF16) {
-        constexpr float most = 0x1.FEp127f;
-        const float in = i == 0 && isfinite(rest) ? fminf(fmaxf(rest, -most), most) : rest;
-        const __bf16 b = (__bf16)in;
+        const __bf16 b = (__bf16)rest;
         out[i][e] = b;
         h = (float)b;
       } else {
@@ -585,7 +584,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   if (adapter < 0) return;
   const int rank = __builtin_amdgcn_readfirstlane(lr_rank(p, adapter));
   if (rank == 0) return;
-  const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
+  const float scale = (p.scale != nullptr ? p.scale[adapter] : 1.f) / LR_DOWN<WT>;
   const int own = __shfl(rows, c16, 64), row0 = __shfl(rows, 0, 64);
   const int64_t yrow = (int64_t)(own >= 0 ? own : row0) * p.ldy;  // padding: the first row again, not stored
 
@@ -695,7 +694,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
   lds_barrier();
   if (n0 >= end) return;
   V pv[RC][PARTS];
-  float down = 1.f;
+  float down = LR_DOWN<WT>;
   {
     float v[RC][8];
 #pragma unroll
@@ -1035,7 +1034,7 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
   __syncthreads();
   const int adapter = info.x, rank = info.y;
   if (adapter < 0) return;
-  const float scale = __int_as_float(info.z);
+  const float scale = __int_as_float(info.z) / LR_DOWN<WT>;
   const int rc = (rank + 31) / 32, r16 = (rank + 15) & ~15, ld = 32 * rc + 8;
   const int first = group * p.ncols + 64 * wave, end = min((group + 1) * p.ncols, p.N);
   const int blocks = first < end ? (end - first + 64 * WAVES - 1) / (64 * WAVES) : 0, steps = blocks * PAIRS;
@@ -1115,7 +1114,7 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
     for (int u = 0; u < U; ++u) {
       if (pass + u >= passes) break;
       const int row = (pass + u) * rows + row0, id = tl.rows[row];
-      float v[4], m = 0.f, up = 1.f, down = 1.f;
+      float v[4], m = 0.f, up = 1.f, down = LR_DOWN<WT>;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = id >= 0 && 4 * j + e < rank ? sum[u][e] * scale : 0.f;
