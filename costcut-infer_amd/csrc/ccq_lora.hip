@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ccq {
 
@@ -424,6 +425,16 @@ __device__ __forceinline__ void lr_split(const float (&v)[N], V (&out)[PARTS]) {
   }
 }
 
+// the value whose parts lie `stride` values apart
+template <int WT, int PARTS>
+__device__ __forceinline__ float lr_join(const uint16_t* parts, int stride) {
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i)
+    v += WT == CCQ_BF16 ? bf16_bits_to_f32(parts[i * stride]) : f16_bits_to_f32(parts[i * stride]);
+  return v;
+}
+
 // k such that 2^k brings a row whose largest finite |p| is m into [2^13, 2^14],
 // from -114 (m near 2^128) on, up to what lr_pow2 holds of 2^k and 2^-k: below
 // 2^-112 m stays smaller (2^-126 becomes 1), and the parts, which end at 2^-24,
@@ -435,7 +446,7 @@ __device__ __forceinline__ float lr_pow2(int k) { return __uint_as_float((uint32
 
 // 16 bytes of a row of y from column n on (at any element alignment).  A piece
 // across the row's end is not loaded, and added to in place value by value.
-// YT: float32, or either 16-bit type (they differ in add_store alone).
+// YT: float32, or either 16-bit type (they differ in the sums alone).
 template <int YT>
 struct YPiece {
   static constexpr int COLS = YT == CCQ_F32 ? 4 : 8;
@@ -445,24 +456,33 @@ struct YPiece {
     v = u32x4{0, 0, 0, 0};
     if (n + COLS <= N) __builtin_memcpy(&v, reinterpret_cast<const char*>(y) + (row + n) * E, 16);
   }
+  // the piece with d added; DT: y's type
+  template <int DT>
+  __device__ __forceinline__ u32x4 sum(const float (&d)[COLS]) const {
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == CCQ_F32)
+        o[e] = __float_as_uint(__uint_as_float(v[e]) + d[e]);
+      else if constexpr (DT == CCQ_BF16)
+        o[e] = bf16x2_bits(bf16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e], bf16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]);
+      else
+        o[e] = f32_to_f16_bits(f16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e]) |
+               f32_to_f16_bits(f16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]) << 16;
+    }
+    return o;
+  }
   __device__ __forceinline__ void add_store(void* y, int y_dtype, int64_t row, int n, int N, const float (&d)[COLS]) {
     constexpr int E = YT == CCQ_F32 ? 4 : 2;
     char* at = reinterpret_cast<char*>(y) + (row + n) * E;
     if (n + COLS <= N) {
       u32x4 o;
-      if constexpr (YT == CCQ_F32) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(__uint_as_float(v[e]) + d[e]);
-      } else if (y_dtype == CCQ_BF16) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = bf16x2_bits(bf16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e], bf16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = f32_to_f16_bits(f16_bits_to_f32(v[e] & 0xFFFFu) + d[2 * e]) |
-                 f32_to_f16_bits(f16_bits_to_f32(v[e] >> 16) + d[2 * e + 1]) << 16;
-      }
+      if constexpr (YT == CCQ_F32)
+        o = sum<CCQ_F32>(d);
+      else if (y_dtype == CCQ_BF16)
+        o = sum<CCQ_BF16>(d);
+      else
+        o = sum<CCQ_F16>(d);
       __builtin_memcpy(at, &o, 16);
     } else {
 #pragma unroll
@@ -489,16 +509,79 @@ __device__ __forceinline__ int lr_col(int q, int m) {
 // where piece i of lane group g begins, and its values among the lane's quads
 template <int YT>
 __device__ __forceinline__ int lr_piece_col(int i, int g) { return YT == CCQ_F32 ? 16 * i + 4 * g : 32 * i + 8 * g; }
+// Lanes of one wave hand each other values through LDS: the hardware keeps a
+// wave's LDS accesses in order, the fences keep the compiler from moving them
+// across.  They emit no instruction.
+__device__ __forceinline__ void lr_lane_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// An infinite weight times p's parts is NaN where these differ in sign or one
+// is 0.  Where a column has such a weight, its sums that are NaN are formed anew
+// from whole p(row, r): `sums` holds the wave's 64 columns from n0 on, a row of
+// them for each of ROWS tokens.  (p joined from f16 parts is 0 below 2^-38 of
+// its row's largest.)  The lane and the scan of b one by one: what is alive in
+// the kernels' loops leaves few registers.  The check of the sums costs T=16
+// K=4096 N=14336 R=16 0.2 of 8.4 us and T=4096 N=4096 R=128 0.1 of 71.7 a call;
+// x that is NaN throughout, which scans b for nothing, takes 44 -> 154 us there
+// with K=2048.
+template <int WT, int ROWS, class F>
+__device__ __forceinline__ void lr_whole_sums(const LoraP& p, int adapter, int rank, int n0, float (*sums)[64 + 4], F whole) {
+  const int lane = lane_id_here();
+  const uint16_t* b = reinterpret_cast<const uint16_t*>(p.b) + ((int64_t)adapter * p.N + min(n0 + lane, p.N - 1)) * p.R;
+  bool inf = false;
+#pragma unroll 1
+  for (int r = 0; r < rank; ++r) inf |= (b[r] & 0x7FFF) == (WT == CCQ_BF16 ? 0x7F80 : 0x7C00);
+  if (!inf) return;
+#pragma unroll 1
+  for (int i = 0; i < ROWS; ++i) {
+    if (sums[i][lane] == sums[i][lane]) continue;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < rank; ++r)
+      sum = fmaf(whole(i, r), WT == CCQ_BF16 ? bf16_bits_to_f32(b[r]) : f16_bits_to_f32(b[r]), sum);
+    sums[i][lane] = sum;
+  }
+}
+
+// not a number if one of acc is none (or where their products leave the range)
+__device__ __forceinline__ float lr_nan_of(const f32x4 (&acc)[4]) {
+  float t = 0.f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) t = fmaf(acc[q][2], acc[q][3], fmaf(acc[q][0], acc[q][1], t));
+  return t;
+}
+
+// (The branches between whole and ragged blocks and between the types stand once,
+// around all pieces: a kernel of a few us pays for the code that it steps over.
+// T=16 K=4096 N=14336 R=16 9.4 us on the GPU by branches in each piece, 9.2 so.)
 template <int YT>
 __device__ __forceinline__ void lr_store_pieces(const LoraP& p, YPiece<YT> (&y)[16 / YPiece<YT>::COLS], int64_t row,
                                                 int n0, int g, const f32x4 (&acc)[4], float f) {
-  constexpr int C = YPiece<YT>::COLS;
+  constexpr int C = YPiece<YT>::COLS, E = YT == CCQ_F32 ? 4 : 2;
+  float d[16 / C][C];
 #pragma unroll
-  for (int i = 0; i < 16 / C; ++i) {
-    float d[C];
+  for (int i = 0; i < 16; ++i) d[i / C][i % C] = acc[i / 4][i & 3] * f;
+  if (__builtin_expect(n0 + 64 <= p.N, 1)) {
+    char* at = reinterpret_cast<char*>(p.y) + (row + n0 + lr_piece_col<YT>(0, g)) * E;
+    auto store = [&](auto dt) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) d[e] = acc[(C * i + e) / 4][e & 3] * f;
-    y[i].add_store(p.y, p.y_dtype, row, n0 + lr_piece_col<YT>(i, g), p.N, d);
+      for (int i = 0; i < 16 / C; ++i) {
+        const u32x4 o = y[i].template sum<decltype(dt)::value>(d[i]);
+        __builtin_memcpy(at + lr_piece_col<YT>(i, 0) * E, &o, 16);
+      }
+    };
+    if constexpr (YT == CCQ_F32)
+      store(std::integral_constant<int, CCQ_F32>{});
+    else if (p.y_dtype == CCQ_BF16)
+      store(std::integral_constant<int, CCQ_BF16>{});
+    else
+      store(std::integral_constant<int, CCQ_F16>{});
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16 / C; ++i) y[i].add_store(p.y, p.y_dtype, row, n0 + lr_piece_col<YT>(i, g), p.N, d[i]);
   }
 }
 
@@ -728,6 +811,20 @@ __global__ __launch_bounds__(LR_THREADS) void lora_fused_kernel(const LoraP p) {
     for (int c = 0; c < RC; ++c) {
       lr_fix_b<WT>(p, adapter, rank, 32 * c, col, w[c]);
       lr_expand_step<WT, PARTS>(w[c], pv[c], out);
+    }
+    const float nan = lr_nan_of(out);
+    if (__builtin_expect(__any(nan != nan), 0)) {
+      // in the wave's part of the ring (p is not scaled here in f16, and the new sums are not finite)
+      float(*mine)[64 + 4] = reinterpret_cast<float(*)[64 + 4]>(u.ring[wave][0]);
+      lr_lane_exchange();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(&mine[c16][lr_col<YT>(q, 4 * g)]) = out[q];
+      lr_lane_exchange();
+      lr_whole_sums<WT, 16>(p, adapter, rank, n0, mine, [&](int i, int r) { return ps[i][r]; });
+      lr_lane_exchange();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) out[q] = *reinterpret_cast<const f32x4*>(&mine[c16][lr_col<YT>(q, 4 * g)]);
     }
     if (own >= 0) lr_store_pieces<YT>(p, y, yrow, n0, g, out, down);
     n0 += 64 * LR_WAVES;
@@ -989,15 +1086,6 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_tile_kernel(const Lora
   }
 }
 
-// Lanes of one wave hand each other values through LDS: the hardware keeps a
-// wave's LDS accesses in order, the fences keep the compiler from moving them
-// across.  They emit no instruction.
-__device__ __forceinline__ void lr_lane_exchange() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // A tile's 16 MT tokens, ncols columns: p summed over the splits, scaled and
 // in parts in LDS; a wave then takes 64 columns of 16 MP tokens at a time.  The
 // products' lanes hold 4 columns of 16 tokens each: they pass through the
@@ -1187,7 +1275,16 @@ __global__ __launch_bounds__(LE_THREADS, YT == CCQ_F32 || KEEP * MT >= (MT == 1 
         for (int m = 0; m < TURN; ++m)
 #pragma unroll
           for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&mine[16 * m + c16][16 * q + 4 * g]) = acc[h + m][q];
+        float nan = 0.f;
+#pragma unroll
+        for (int m = 0; m < TURN; ++m) nan += lr_nan_of(acc[h + m]);
         lr_lane_exchange();
+        if (__builtin_expect(__any(nan != nan), 0)) {
+          const uint16_t* of = parts + 16 * (m0 + h) * ld;
+          lr_whole_sums<WT, 16 * TURN>(p, adapter, rank, n0, mine,
+                                       [&](int i, int r) { return lr_join<WT, PARTS>(of + i * ld + r, TM * ld); });
+          lr_lane_exchange();
+        }
 #pragma unroll
         for (int i = 0; i < YN * TURN / MP; ++i) {
           const int at = h * YN / MP + i, row = RI * i + yr, id = tl.rows[16 * (m0 + h) + row];

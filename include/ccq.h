@@ -599,7 +599,8 @@ size_t ccq_lora_workspace_size(const void* x, int x_dtype, int64_t ldx, int64_t 
 
 /* y[t, :] += scale[i] * (x[t, :] @ a[i]^T) @ b[i]^T with i = index[t], in
  * float32, y rounded once; rows with index[t] outside [0, L) are left as they
- * are (neither read nor written).  x and y each CCQ_F32 | CCQ_F16 | CCQ_BF16
+ * are (neither read nor written).  Infinities and NaN in x, a and b give what
+ * these products give, in their own rows and columns.  x and y each CCQ_F32 | CCQ_F16 | CCQ_BF16
  * with row strides ldx >= K, ldy >= N in elements, any element alignment; y
  * must not overlap x.  T <= 65536. */
 int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64_t* index, void* y, int y_dtype,

@@ -618,3 +618,23 @@ def test_far_inputs_of_one_copy_base(gpu):
         y = c["y"].to(gpu)
         lora.add_(y, xs, _adapters(c, gpu), c["index"].to(gpu))
         _check(y, c)
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+@pytest.mark.parametrize("T,K,R", [(5, 64, 16), (70, 128, 32), (90, 200, 40), (600, 72, 24), (600, 75, 130)])
+def test_infinite_weights(gpu, T, K, R, types):
+    """Infinities in b give what the whole products give: infinities of the
+    product's sign, NaN only where two of them differ or the product is 0."""
+    c = _case(T, K, 200, R, 3, *types)
+    c["x"][1] = 0.0
+    c["index"][1] = 2
+    for i, n, r, v in ((0, 0, 0, "inf"), (0, 69, R - 1, "-inf"), (2, 7, 3, "inf"), (2, 7, 8, "inf"), (2, 199, 1, "-inf")):
+        c["b"][i, n, r] = float(v)
+    y = _run(c, gpu).cpu()
+    ref, bound = ol.add(c["y"], c["x"], c["a"], c["b"], c["index"], c["scale"], c["rank"])
+    fine = torch.isfinite(ref)
+    off, tol = (y.double() - ref).abs(), bound(c["y"].dtype, c["a"].dtype)
+    assert (off[fine] <= tol[fine]).all(), f"worst {(off / tol)[fine].max():.3f} of the bound"
+    assert torch.equal(y.isnan(), ref.isnan())
+    assert torch.equal(y[ref.isinf()].double(), ref[ref.isinf()])
+    assert ref.isinf().any() and ref[1].isnan().any()
