@@ -24,7 +24,7 @@ class LoraAdapters:
     """The adapters of one projection, stacked on the device: ``a [L, R, in]``
     and ``b [L, out, R]`` (float16 or bfloat16), ``scale [L]`` (float32; None:
     1 each), ``rank [L]`` (int32; None: R each) -- the ranks of an adapter
-    from ``rank[i]`` on are padding and are not read.  Dense tensors are
+    from ``rank[i]`` on are padding, and what they hold is not used.  Dense tensors are
     referred to as they are, so an adapter can be replaced in place (on the
     stream that uses them); others are copied once."""
 

@@ -357,7 +357,8 @@ __device__ __forceinline__ void lr_shrink(const LoraP& p, const int64_t (&xrow)[
 }
 
 // Stages of whole 128-byte lines of x's rows, D - 1 of them loaded
-// ahead of the products: for the 64-token tiles, whose waves walk far in K.
+// ahead of the products: for the 64-token tiles of rows that are not aligned,
+// whose waves walk far in K.
 template <int XT, int WT, int MT, int RT, int D>
 __device__ __forceinline__ void lr_shrink_ring(const LoraP& p, const int64_t (&xrow)[MT], const int64_t (&arow)[RT],
                                                int k0, int k1, f32x4 (&acc)[MT][RT]) {
@@ -890,7 +891,7 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const LoraP p) 
   const int ks = split * p.kchunk, ke = min(ks + p.kchunk, p.K), k0 = ks + part * kw, k1 = min(k0 + kw, ke);
   if (r0 < rank) {
     if constexpr (MT == 1)
-      lr_shrink<XT, WT, MT, RT, (RT == 8 ? 2 : RT == 4 ? 4 : 8) / (XT == CCQ_F32 ? 2 : 1)>(p, xrow, arow, k0, k1, acc);
+      lr_shrink<XT, WT, MT, RT, (RT == 4 ? 4 : 8) / (XT == CCQ_F32 ? 2 : 1)>(p, xrow, arow, k0, k1, acc);
     else
       lr_shrink_ring<XT, WT, MT, RT, RT == 1 ? 3 : 2>(p, xrow, arow, k0, k1, acc);
   }
@@ -1379,7 +1380,6 @@ LoraPlan lora_plan(int64_t T, const ccq_lora_adapters* ad, bool lines, bool one_
   L.ncols = cdiv(cdiv(N, groups), unit) * unit;
   if (L.fused) {
     L.S = 1;
-    L.kchunk = cdiv(cdiv(K, 32), LR_WAVES) * 32;
     return L;
   }
   // splits of K: for 16-token tiles (whose A is read once) as many as give every CU a workgroup, and no more than where

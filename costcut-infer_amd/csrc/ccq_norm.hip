@@ -227,8 +227,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rms_norm_kernel
   }
 }
 
-// By the row's length, so that its threads hold one vector or two: longer
-// chains of loads cost more than idle threads (GPU time in us, bf16 with a
+// By the row's length, so that its threads hold one vector or two (four above
+// 16384, where a workgroup has no more threads): longer chains of loads cost
+// more than idle threads (GPU time in us, bf16 with a
 // residual to FP8, 4096 rows; waves x vectors):
 //   H = 512 1x1 5.8, 4x1 6.8; 1024 2x1 7.9, 4x1 9.1; 2048 4x1 14.8, 1x4 15.0;
 //   7168 8x2 40.4 (5.1 TB/s), 16x1 42.4, 4x4 45.8; 2000 rows of 16384

@@ -544,7 +544,9 @@ int ccq_fp8_block_linear_quantized(const uint8_t* q, const float* s, const uint8
  *     (ccq_int8_act_quant keeps the reference's factor, which saturates
  *     almost every value; these codes use the int8 range.)
  * A row with a NaN has NaN scales and NaN y; one with an infinity has NaN at
- * it (in its block's or row's scale) and 0 elsewhere.
+ * it (in its block's or row's scale) and 0 elsewhere.  The statistics are
+ * float32: a finite row whose sum of squares leaves its range (|s| about 1e19)
+ * has rstd 0, so y and scales of 0.
  * x, residual, residual_out have x_dtype and row strides ldx, ldr, ldo (>= H,
  * in elements; any element alignment); y, q and scale are dense.  Each of
  * residual_out, y and (with CCQ_Q_NONE) q may be null.  residual_out may be
@@ -579,7 +581,8 @@ int ccq_rms_norm_packed(const ccq_rms_norm_args* args);
 
 /* The adapters of one projection, stacked: a [L, R, K], b [L, N, R] in dtype
  * (CCQ_F16 | CCQ_BF16), scale [L] float32 or null (1), rank [L] int32 or null
- * (R): ranks from rank[i] on (clamped to [0, R]) are padding, not read.
+ * (R): what a and b hold for ranks from rank[i] on (clamped to [0, R]) is
+ * padding and not used.
  * 1 <= L <= 1024, 1 <= R <= 256, K and N <= 2^20. */
 typedef struct ccq_lora_adapters {
   const void* a;
@@ -600,9 +603,9 @@ size_t ccq_lora_workspace_size(const void* x, int x_dtype, int64_t ldx, int64_t 
 /* y[t, :] += scale[i] * (x[t, :] @ a[i]^T) @ b[i]^T with i = index[t], in
  * float32, y rounded once; rows with index[t] outside [0, L) are left as they
  * are (neither read nor written).  Infinities and NaN in x, a and b give what
- * these products give, in their own rows and columns.  x and y each CCQ_F32 | CCQ_F16 | CCQ_BF16
- * with row strides ldx >= K, ldy >= N in elements, any element alignment; y
- * must not overlap x.  T <= 65536. */
+ * these products give, in their own rows and columns.  x and y each CCQ_F32 |
+ * CCQ_F16 | CCQ_BF16 with row strides ldx >= K, ldy >= N in elements, any
+ * element alignment; y must not overlap x.  T <= 65536. */
 int ccq_lora_add(const void* x, int x_dtype, int64_t ldx, const int64_t* index, void* y, int y_dtype,
                  int64_t ldy, int64_t T, const ccq_lora_adapters* ad, void* workspace,
                  size_t workspace_bytes, void* stream);
