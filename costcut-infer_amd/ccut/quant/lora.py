@@ -24,9 +24,13 @@ class LoraAdapters:
     """The adapters of one projection, stacked on the device: ``a [L, R, in]``
     and ``b [L, out, R]`` (float16 or bfloat16), ``scale [L]`` (float32; None:
     1 each), ``rank [L]`` (int32; None: R each) -- the ranks of an adapter
-    from ``rank[i]`` on are padding, and what they hold is not used.  Dense tensors are
-    referred to as they are, so an adapter can be replaced in place (on the
-    stream that uses them); others are copied once."""
+    from ``rank[i]`` on are padding, and what they hold is not used.  Dense
+    tensors are referred to as they are, so an adapter can be replaced by
+    writing into them (on the stream that uses them); others are copied once.
+    The tensors themselves stay those of the construction."""
+
+    _FIXED = frozenset(("a", "b", "scale", "rank", "num_adapters", "rank_max", "in_features", "out_features", "device",
+                        "_index", "_desc", "_held"))
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale=None, rank=None):
         if not a.is_cuda:
@@ -44,14 +48,18 @@ class LoraAdapters:
         rank = self._vector(rank, torch.int32, L, a.device, "rank")
         if b.device != a.device:
             raise ValueError(f"a on {a.device}, b on {b.device}")
-        self.a, self.b, self.scale, self.rank = a.contiguous(), b.contiguous(), scale, rank
-        self.num_adapters, self.rank_max, self.in_features, self.out_features = L, R, K, b.shape[1]
-        self.device, self._index = a.device, a.get_device()
-        self._desc = ccq_lora_adapters(self.a.data_ptr(), self.b.data_ptr(),
-                                       scale.data_ptr() if scale is not None else None,
-                                       rank.data_ptr() if rank is not None else None, DTYPE_CODE[a.dtype],
-                                       L, R, K, b.shape[1])
-        self._bytes: dict[tuple, int] = {}
+        a, b = a.contiguous(), b.contiguous()
+        desc = ccq_lora_adapters(a.data_ptr(), b.data_ptr(), scale.data_ptr() if scale is not None else None,
+                                 rank.data_ptr() if rank is not None else None, DTYPE_CODE[a.dtype], L, R, K, b.shape[1])
+        self.__dict__.update(a=a, b=b, scale=scale, rank=rank, num_adapters=L, rank_max=R, in_features=K,
+                             out_features=b.shape[1], device=a.device, _index=a.get_device(), _desc=desc, _bytes={},
+                             _held=[t.untyped_storage() for t in (a, b, scale, rank) if t is not None])
+
+    def __setattr__(self, name: str, value) -> None:
+        # the descriptor holds the tensors' addresses: another tensor in their place would not be the one that is read
+        if name in self._FIXED:
+            raise AttributeError(f"{name}: adapters are replaced by writing into their tensors")
+        super().__setattr__(name, value)
 
     @staticmethod
     def _vector(v, dtype: torch.dtype, L: int, device, what: str) -> torch.Tensor | None:

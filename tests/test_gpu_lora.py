@@ -638,3 +638,22 @@ def test_infinite_weights(gpu, T, K, R, types):
     assert torch.equal(y.isnan(), ref.isnan())
     assert torch.equal(y[ref.isinf()].double(), ref[ref.isinf()])
     assert ref.isinf().any() and ref[1].isnan().any()
+
+
+def test_stacks_are_not_exchanged(gpu):
+    """Another tensor in the place of a stack is refused (the calls would read
+    the old one); the memory that the calls read lives as long as the handle."""
+    from ccut.quant import lora
+
+    c = _case(30, 128, 96, 16, 3, "bf16", "bf16", "bf16", ranks=True)
+    ad = _adapters(c, gpu)
+    for name in ("a", "b", "scale", "rank", "in_features"):
+        with pytest.raises(AttributeError, match="writing into"):
+            setattr(ad, name, getattr(ad, name))
+    ad.label = "q_proj"
+    ad.label = "k_proj"
+    kept = [t.clone() for t in (ad.a, ad.b)]
+    ad.a.data, ad.b.data = torch.zeros_like(kept[0]), torch.zeros_like(kept[1])  # their old memory is not handed out
+    for _ in range(4):
+        torch.full_like(kept[0], float("nan")), torch.full_like(kept[1], float("nan"))
+    _check(lora.add_(c["y"].to(gpu), c["x"].to(gpu), ad, c["index"].to(gpu)), c)
