@@ -657,3 +657,28 @@ def test_stacks_are_not_exchanged(gpu):
     for _ in range(4):
         torch.full_like(kept[0], float("nan")), torch.full_like(kept[1], float("nan"))
     _check(lora.add_(c["y"].to(gpu), c["x"].to(gpu), ad, c["index"].to(gpu)), c)
+
+
+def test_captured_above_the_self_sorted_batches(gpu):
+    """A captured call of more than 4096 tokens, K in parts, replayed on other
+    rows and other numbers of tiles with eager work between the replays."""
+    from ccut.quant import lora
+
+    T, K, N, R, L = 5000, 2048, 72, 24, 40
+    cs = [_case(T, K, N, R, L, "bf16", "bf16", "bf16", seed=s, pattern=p) for s, p in
+          enumerate(("one", "mixed", "none", "runs"))]
+    ad = _adapters(cs[0], gpu)
+    x, y, index = (cs[0][k].to(gpu) for k in ("x", "y", "index"))
+    lora.add_(y, x, ad, index)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lora.add_(y, x, ad, index)
+    for n in (1, 0, 3, 2, 0):
+        for to, k in ((x, "x"), (y, "y"), (index, "index")):
+            to.copy_(cs[n][k].to(gpu))
+        graph.replay()
+        want = lora.add_(cs[n]["y"].to(gpu), cs[n]["x"].to(gpu), ad, cs[n]["index"].to(gpu))
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), f"rows {n}"
+        _check(y, dict(cs[n], a=cs[0]["a"], b=cs[0]["b"], scale=cs[0]["scale"]))
