@@ -17,13 +17,15 @@ or CUDA tensors (staying on the device).
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from ccut import _dev
-from ccut._lib import call, ccq_fp8_experts, ccq_fp8row_experts, ccq_w4_experts, lib
-from ccut.quant import awq
+from ccut._dev import empty_strided, is_current, raw_stream
+from ccut._lib import ACTIVATIONS, call, ccq_fp8_experts, ccq_fp8row_experts, ccq_w4_experts, check, lib
+from ccut.quant import awq, dense
 
 __all__ = [
     "topk_softmax",
@@ -39,6 +41,14 @@ __all__ = [
     "moe_forward_fp8",
     "Fp8RowExperts",
     "moe_ffn_fp8row",
+    "Permutation",
+    "moe_permute",
+    "moe_permute_backward",
+    "moe_unpermute",
+    "moe_unpermute_backward",
+    "DenseExperts",
+    "moe_ffn_dense",
+    "moe_forward_dense",
 ]
 
 _MODE_SOFTMAX_ALL, _MODE_TOPK_THEN_SOFTMAX, _MODE_RAW_EXP, _MODE_PLAIN, _MODE_ROUTE_NORM = 0, 1, 2, 3, 4
@@ -651,3 +661,240 @@ def moe_ffn_fp8row(x, ids, weights, experts: Fp8RowExperts, out_dtype: torch.dty
         call("ccq_moe_fp8row_ffn", xd.data_ptr(), ids.data_ptr(), wts.data_ptr(), y.data_ptr(),
              _dev.DTYPE_CODE[out_dtype], T, k, desc, ws.data_ptr(), nbytes, _dev.stream_ptr(xd.device))
     return y
+
+
+# ---------------------------------------------------------------------------
+# tokens sorted by expert and back, and experts in 16 bits on the sorted rows
+# ---------------------------------------------------------------------------
+
+MAX_ASSIGNMENTS, MAX_SLOTS, MAX_SORT_EXPERTS = 1 << 20, 64, 1024
+
+
+class Permutation(NamedTuple):
+    """Where :func:`moe_permute` put the assignments: ``position [T, k]``
+    (int32) the row of each, ``~row`` for one whose expert is outside
+    ``[0, E)`` (behind all others); ``offsets [E + 1]`` (int32) each
+    expert's first row, and the end of the last."""
+
+    position: torch.Tensor
+    offsets: torch.Tensor
+
+
+def _float_rows(t: torch.Tensor, what: str, index: int) -> tuple[torch.Tensor, int]:
+    if t.dtype not in _dev.DTYPE_CODE or t.dim() != 2 or t.shape[1] < 1 or t.get_device() != index:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16 rows [n, H] on cuda:{index}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    if t.shape[0] <= 1:
+        return (t if t.stride(1) == 1 else t.contiguous()), t.shape[1]
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _positions(plan: Permutation, index: int) -> torch.Tensor:
+    p = plan.position
+    if p.dtype != torch.int32 or p.dim() != 2 or p.get_device() != index:
+        raise ValueError(f"plan.position must be int32 [T, k] on cuda:{index}, got {p.dtype} {tuple(p.shape)} on "
+                         f"{p.device}")
+    return p if p.is_contiguous() else p.contiguous()
+
+
+def _routing_weights(weights: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
+    if weights.shape != position.shape or weights.device != position.device or not weights.is_floating_point():
+        raise ValueError(f"weights must be floats {tuple(position.shape)} on {position.device}, got {weights.dtype} "
+                         f"{tuple(weights.shape)} on {weights.device}")
+    return weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
+
+
+def moe_permute(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, Permutation]:
+    """Each token's row once for each of its experts, sorted by expert
+    (tokens and slots in order within one): ``x [T, H]`` (float32, float16 or
+    bfloat16, any row stride) and ``ids [T, k]`` (int64; other whole numbers
+    are converted) on the device -> ``(rows [T * k, H], Permutation)``.
+    Assignments whose id is outside ``[0, num_experts)`` are left out; as many
+    rows of zeros stand at the end.  ``T * k <= 2^20``, ``k <= 64``, at most
+    1024 experts."""
+    index = x.get_device()
+    if not is_current(index):
+        with torch.cuda.device(index):
+            return moe_permute(x, ids, num_experts)
+    x2, ldx = _float_rows(x, "x", index)
+    T, H = x2.shape
+    if ids.dim() != 2 or ids.shape[0] != T or ids.get_device() != index:
+        raise ValueError(f"ids must be [{T}, k] on {x.device}, got {tuple(ids.shape)} on {ids.device}")
+    k = ids.shape[1]
+    if not 1 <= k <= MAX_SLOTS or T * k > MAX_ASSIGNMENTS or not 1 <= num_experts <= MAX_SORT_EXPERTS:
+        raise ValueError(f"{T} tokens of {k} of {num_experts} experts: need 1 <= k <= {MAX_SLOTS}, T * k <= "
+                         f"{MAX_ASSIGNMENTS}, 1 to {MAX_SORT_EXPERTS} experts")
+    if ids.dtype != torch.int64 or not ids.is_contiguous():
+        if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+            raise ValueError(f"ids must hold whole numbers, got {ids.dtype}")
+        ids = ids.to(torch.int64).contiguous()
+    rows = empty_strided((T * k, H), (H, 1), x.dtype)
+    position = empty_strided((T, k), (k, 1), torch.int32)
+    offsets = empty_strided((num_experts + 1,), (1,), torch.int32)
+    handle = lib()
+    nbytes = handle.ccq_moe_permute_workspace_size(T, k, num_experts)
+    sp = 0
+    if nbytes:  # this call's own, so that calls on several streams or in several graphs do not share it
+        scratch = empty_strided((nbytes,), (1,), torch.uint8)
+        sp = scratch.data_ptr()
+    rc = handle.ccq_moe_permute(x2.data_ptr(), _dev.DTYPE_CODE[x.dtype], ldx, ids.data_ptr(), rows.data_ptr(),
+                                position.data_ptr(), offsets.data_ptr(), T, k, num_experts, H, sp, nbytes,
+                                raw_stream(index))
+    if rc:
+        check(rc, "ccq_moe_permute")
+    return rows, Permutation(position, offsets)
+
+
+def moe_unpermute(rows: torch.Tensor, plan: Permutation, weights: torch.Tensor | None = None,
+                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Sorted rows back to their tokens: ``y[t] = sum_s weights[t, s] *
+    rows[plan.position[t, s]]`` (``weights [T, k]``, None: 1 each), float32
+    sums in slot order, rounded once to ``out_dtype`` (default: rows').
+    Left-out assignments contribute nothing."""
+    index = rows.get_device()
+    if not is_current(index):
+        with torch.cuda.device(index):
+            return moe_unpermute(rows, plan, weights, out_dtype)
+    r2, ldr = _float_rows(rows, "rows", index)
+    position = _positions(plan, index)
+    T, k = position.shape
+    H = r2.shape[1]
+    if not 1 <= k <= MAX_SLOTS or r2.shape[0] != T * k or T * k > MAX_ASSIGNMENTS:
+        raise ValueError(f"rows {tuple(rows.shape)} and position {tuple(position.shape)}: need T * k rows, k <= "
+                         f"{MAX_SLOTS}, T * k <= {MAX_ASSIGNMENTS}")
+    out_dtype = out_dtype or rows.dtype
+    if out_dtype not in _dev.DTYPE_CODE:
+        raise ValueError(f"y must be float32, float16 or bfloat16, got {out_dtype}")
+    wp = 0
+    if weights is not None:
+        weights = _routing_weights(weights, position)
+        wp = weights.data_ptr()
+    y = empty_strided((T, H), (H, 1), out_dtype)
+    rc = lib().ccq_moe_unpermute(r2.data_ptr(), _dev.DTYPE_CODE[rows.dtype], ldr, T * k, position.data_ptr(), wp,
+                                 y.data_ptr(), _dev.DTYPE_CODE[out_dtype], T, k, H, raw_stream(index))
+    if rc:
+        check(rc, "ccq_moe_unpermute")
+    return y
+
+
+def moe_permute_backward(d_rows: torch.Tensor, plan: Permutation) -> torch.Tensor:
+    """The gradient of ``x`` in :func:`moe_permute` from that of its rows:
+    each token's kept rows added in float32, rounded once."""
+    return moe_unpermute(d_rows, plan)
+
+
+def moe_unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, plan: Permutation, weights: torch.Tensor
+                           ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of ``rows`` and ``weights`` in :func:`moe_unpermute`
+    from that of its result: ``d_rows[position[t, s]] = weights[t, s] *
+    dy[t]`` (zeros for left-out assignments, rows' type) and ``d_weights
+    [T, k] = <rows[position[t, s]], dy[t]>`` (float32, 0 for left-out ones).
+    ``dy [T, H]`` and ``rows [T * k, H]`` are of one type."""
+    index = rows.get_device()
+    if not is_current(index):
+        with torch.cuda.device(index):
+            return moe_unpermute_backward(dy, rows, plan, weights)
+    r2, ldr = _float_rows(rows, "rows", index)
+    g2, ldy = _float_rows(dy, "dy", index)
+    position = _positions(plan, index)
+    T, k = position.shape
+    H = r2.shape[1]
+    if not 1 <= k <= MAX_SLOTS or r2.shape[0] != T * k or T * k > MAX_ASSIGNMENTS:
+        raise ValueError(f"rows {tuple(rows.shape)} and position {tuple(position.shape)}: need T * k rows, k <= "
+                         f"{MAX_SLOTS}, T * k <= {MAX_ASSIGNMENTS}")
+    if dy.dtype != rows.dtype or tuple(dy.shape) != (T, H):
+        raise ValueError(f"dy must be {rows.dtype} [{T}, {H}], got {dy.dtype} {tuple(dy.shape)}")
+    weights = _routing_weights(weights, position)
+    d_rows = empty_strided((T * k, H), (H, 1), rows.dtype)
+    d_weights = empty_strided((T, k), (k, 1), torch.float32)
+    rc = lib().ccq_moe_unpermute_grad(g2.data_ptr(), ldy, r2.data_ptr(), ldr, _dev.DTYPE_CODE[rows.dtype], T * k,
+                                      position.data_ptr(), weights.data_ptr(), d_rows.data_ptr(), d_weights.data_ptr(),
+                                      T, k, H, raw_stream(index))
+    if rc:
+        check(rc, "ccq_moe_unpermute_grad")
+    return d_rows, d_weights
+
+
+@dataclass
+class DenseExperts:
+    """All experts of one MoE layer in 16 bits, resident in HBM: ``w_gate_up
+    [E, 2I, H]`` (each expert's gate rows, then its up rows), ``w_down
+    [E, H, I]``, both float16 or both bfloat16, and where the model has them
+    the biases ``b_gate_up [E, 2I]`` and ``b_down [E, H]``."""
+
+    w_gate_up: torch.Tensor
+    w_down: torch.Tensor
+    b_gate_up: torch.Tensor | None = None
+    b_down: torch.Tensor | None = None
+    act: str = "silu"
+
+    def __post_init__(self):
+        gu, d = self.w_gate_up, self.w_down
+        if gu.dim() != 3 or d.dim() != 3 or gu.shape[0] != d.shape[0] or (d.shape[1], 2 * d.shape[2]) != (
+                gu.shape[2], gu.shape[1]):
+            raise ValueError(f"w_gate_up [E, 2I, H] and w_down [E, H, I] disagree: {tuple(gu.shape)}, "
+                             f"{tuple(d.shape)}")
+        if gu.dtype != d.dtype or gu.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"experts must be float16 or bfloat16, got {gu.dtype} and {d.dtype}")
+        if self.act not in ACTIVATIONS:
+            raise ValueError(f"act={self.act!r}: one of {', '.join(map(repr, ACTIVATIONS))}")
+        for b, w, what in ((self.b_gate_up, gu, "b_gate_up"), (self.b_down, d, "b_down")):
+            if b is not None and b.shape != w.shape[:-1]:
+                raise ValueError(f"{what} must be {tuple(w.shape[:-1])}, got {tuple(b.shape)}")
+
+    @staticmethod
+    def from_stacks(gate, up, down, act: str = "silu") -> "DenseExperts":
+        """``gate``, ``up [E, I, H]`` and ``down [E, H, I]`` (row = output
+        channel, as checkpoints store them), host or device."""
+        g, u, d = (_dev.to_device(t) for t in (gate, up, down))
+        return DenseExperts(torch.cat([g, u], 1), d, act=act)
+
+    @property
+    def num_experts(self) -> int:
+        return self.w_down.shape[0]
+
+    @property
+    def hidden(self) -> int:
+        return self.w_down.shape[1]
+
+    @property
+    def inter(self) -> int:
+        return self.w_down.shape[2]
+
+    @property
+    def bytes_per_expert(self) -> int:
+        """Bytes of one expert's weights: the algorithmic traffic of reading
+        it once."""
+        return 6 * self.hidden * self.inter
+
+
+def moe_ffn_dense(x: torch.Tensor, ids, weights, experts: DenseExperts, out_dtype: torch.dtype | None = None, *,
+                  shared=None, shared_gate: float = 1.0) -> torch.Tensor:
+    """Expert FFN + weighted combine for already-routed tokens on 16-bit
+    experts: tokens sorted by expert, the gated gate/up product, the down
+    product and the weighted sum (:func:`moe_permute`,
+    ``quant.dense.linear_grouped`` twice, :func:`moe_unpermute`).  ``x
+    [T, H]`` of the experts' type; the rows between the steps are of that
+    type too.  ``shared`` ([T, H], the shared expert's output): ``shared_gate
+    * shared`` is added to the sum, in float32."""
+    if x.dtype != experts.w_down.dtype or x.dim() != 2 or x.shape[1] != experts.hidden:
+        raise ValueError(f"x must be {experts.w_down.dtype} [T, {experts.hidden}], got {x.dtype} {tuple(x.shape)}")
+    rows, plan = moe_permute(x, _dev.to_device(ids), experts.num_experts)
+    h = dense.linear_grouped(rows, plan.offsets, experts.w_gate_up, experts.b_gate_up, act=experts.act, gated=True)
+    down = dense.linear_grouped(h, plan.offsets, experts.w_down, experts.b_down)
+    weights = _dev.to_device(weights, torch.float32)
+    if shared is None:
+        return moe_unpermute(down, plan, weights, out_dtype)
+    y = moe_unpermute(down, plan, weights, torch.float32)
+    shared_expert_add(y, _shared_rows(shared, *y.shape, y.device), shared_gate)
+    return y.to(out_dtype or x.dtype)
+
+
+def moe_forward_dense(x: torch.Tensor, router_logits, experts: DenseExperts, top_k: int, norm_topk_prob: bool = True,
+                      out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Routed MoE layer on 16-bit experts: ``topk_softmax`` then
+    :func:`moe_ffn_dense`."""
+    w, ids = topk_softmax(router_logits, top_k, norm_topk_prob)
+    return moe_ffn_dense(x, ids, w, experts, out_dtype)

@@ -8,10 +8,11 @@ routed experts, the experts' FFN with the weighted combine, the shared expert
 and the metrics.  The expert weights come from ``reader`` in one of two ways:
 
 * ``reader.experts(layer)`` returning a whole layer in device format
-  (``W4Experts``, ``Fp8Experts`` or ``Fp8RowExperts``): one fused call
-  (``moe_ffn_w4`` / ``moe_ffn_fp8`` / ``moe_ffn_fp8row``); activations go
-  to the int4 kernels as bfloat16, to the per-row FP8 kernels (the
-  reference checkpoint's own format) as float32.
+  (``W4Experts``, ``Fp8Experts``, ``Fp8RowExperts`` or ``DenseExperts``):
+  one call (``moe_ffn_w4`` / ``moe_ffn_fp8`` / ``moe_ffn_fp8row`` /
+  ``moe_ffn_dense``); activations go to the int4 kernels as bfloat16, to the
+  per-row FP8 kernels (the reference checkpoint's own format) as float32, to
+  16-bit experts in their type.
 * otherwise ``reader.get(layer, eid, timeout)`` per routed expert returning
   float32 ``(w_gate [hidden, inter], w_up [hidden, inter], w_down [inter,
   hidden])``, the orientation ``expert_ffn`` takes, then ``expert_ffn``
@@ -199,9 +200,13 @@ class ExpertPipeline:
             out = moe.moe_ffn_fp8row(xd, ids, weights, ex, out_dtype=torch.float32, shared=s_out,
                                      shared_gate=shared_gate)
             shared_done = True
+        elif isinstance(ex, moe.DenseExperts):
+            out = moe.moe_ffn_dense(xd.to(ex.w_down.dtype), ids, weights, ex, out_dtype=torch.float32, shared=s_out,
+                                    shared_gate=shared_gate)
+            shared_done = True
         elif ex is not None:
             raise TypeError(f"reader.experts({layer}) returned {type(ex).__name__}, "
-                            "expected W4Experts, Fp8Experts or Fp8RowExperts")
+                            "expected W4Experts, Fp8Experts, Fp8RowExperts or DenseExperts")
         else:
             out, shared_done = self._per_expert(layer, xd, ids, weights, flat_ids, s_out, shared_gate)
         if s_out is not None and not shared_done:

@@ -1,0 +1,542 @@
+// Tokens sorted by expert and back, and the gradients of both.
+//
+// Assignment a = t k + s gives token t to expert ids[a]; key(a) is that expert,
+// or E where ids[a] is outside [0, E).  The order is by (key, a):
+//   position[a] = #{a' : (key(a'), a') < (key(a), a)}, as ~row where key(a) = E,
+//   offsets[e]  = #{a' : key(a') < e},  e = 0 .. E,
+//   permute     rows[position[t, s]] = x[t], zero from row offsets[E] on,
+//   unpermute   y[t] = sum_s weights[t, s] rows[position[t, s]]  (kept s, in order, float32),
+//   its gradient  d_rows[position[t, s]] = weights[t, s] dy[t],
+//                 d_weights[t, s] = sum_h rows[position[t, s], h] dy[t, h]  (float32).
+// The gradient of permute is unpermute without weights.
+//
+// A permutation of no arithmetic to speak of: bytes bound it.  Everything goes by
+// tokens, so that a token's row is read once and its k rows are written (or read)
+// from there, 16 bytes a lane.
+#include "ccq_common.h"
+
+namespace ccq {
+
+namespace {
+
+constexpr int PM_THREADS = 256, PM_WAVES = 4;
+constexpr int PM_MAX_E = 1024;
+constexpr int PM_MAX_K = 64;
+constexpr int64_t PM_MAX_N = 1 << 20;  // assignments: their numbers and their keys share 32 bits
+constexpr int PM_SHIFT = 20;
+constexpr int PM_OWN = 256;            // most assignments of a workgroup
+constexpr int PM_CHUNKS = 128;         // most rows of the table of counts
+constexpr int PM_SELF = 4096;          // most assignments that every workgroup ranks its own among by itself
+
+struct PermP {
+  const void* x;
+  const int64_t* ids;
+  void* rows;
+  int32_t* position;
+  int32_t* offsets;
+  int32_t* table;                      // [chunks][E + 1] counts
+  int64_t ldx;                         // bytes
+  int64_t T;
+  int n, k, E, H, esize;
+  int tokens;                          // of a workgroup
+  int row_threads;                     // threads on one row, a power of two
+  int chunk, chunks;                   // assignments of a table row (whole workgroups), table rows
+};
+
+__device__ __forceinline__ uint32_t pm_key(const PermP& p, int a) {
+  const int64_t id = p.ids[a];
+  return id >= 0 && id < p.E ? (uint32_t)id : (uint32_t)p.E;
+}
+
+// inclusive sum over the lanes up to this one
+__device__ __forceinline__ int pm_scan(int v) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(v, m, 64);
+    v += lane >= m ? o : 0;
+  }
+  return v;
+}
+
+// s.total (counts by key) -> s.start (rows before a key), by all threads
+struct PermS {
+  int total[PM_MAX_E + 1], start[PM_MAX_E + 1], before[PM_MAX_E + 1];
+  int sum[PM_WAVES];
+  uint32_t own[PM_OWN];
+  int rank[PM_OWN];
+};
+__device__ __forceinline__ void pm_starts(const PermP& p, PermS& s) {
+  constexpr int PER = (PM_MAX_E + 1 + PM_THREADS - 1) / PM_THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int v[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = tid * PER + i;
+    v[i] = e <= p.E ? s.total[e] : 0;
+    sum += v[i];
+  }
+  int at = pm_scan(sum);
+  if (lane == 63) s.sum[wave] = at;
+  __syncthreads();
+  at -= sum;
+#pragma unroll
+  for (int w = 0; w < PM_WAVES - 1; ++w) at += w < wave ? s.sum[w] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = tid * PER + i;
+    if (e <= p.E) s.start[e] = at;
+    at += v[i];
+  }
+  __syncthreads();
+}
+
+// columns of the table, all rows and those before `chunk`
+__device__ __forceinline__ void pm_columns(const PermP& p, PermS& s, int chunk) {
+  for (int e = threadIdx.x; e <= p.E; e += PM_THREADS) {
+    int total = 0, before = 0;
+    for (int c = 0; c < p.chunks; ++c) {
+      const int v = p.table[(int64_t)c * (p.E + 1) + e];
+      total += v;
+      before += c < chunk ? v : 0;
+    }
+    s.total[e] = total;
+    s.before[e] = before;
+  }
+  __syncthreads();
+  pm_starts(p, s);
+}
+
+__device__ __forceinline__ void pm_count(const PermP& p, int* count, int from, int to) {
+  for (int e = threadIdx.x; e <= p.E; e += PM_THREADS) count[e] = 0;
+  __syncthreads();
+  for (int a = from + threadIdx.x; a < to; a += PM_THREADS) atomicAdd(&count[pm_key(p, a)], 1);
+  __syncthreads();
+}
+
+// Counts of each expert in each chunk of the assignments, for batches above
+// PM_SELF.
+__global__ __launch_bounds__(PM_THREADS) void permute_count_kernel(const PermP p) {
+  __shared__ int count[PM_MAX_E + 1];
+  const int from = blockIdx.x * p.chunk;
+  pm_count(p, count, from, min(from + p.chunk, p.n));
+  for (int e = threadIdx.x; e <= p.E; e += PM_THREADS) p.table[(int64_t)blockIdx.x * (p.E + 1) + e] = count[e];
+}
+
+// One 16-byte piece of a row, at any alignment of the elements (a row's last
+// piece ends with the row and may repeat some of the one before).
+__device__ __forceinline__ u32x4 pm_load(const char* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+__device__ __forceinline__ void pm_store(char* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
+
+// Workgroup b sorts and copies `tokens` tokens; the last one writes the
+// offsets.  A workgroup needs the rank of its own few assignments only, which
+// it finds by comparing them with all others (TABLE: with those of its chunk,
+// the counts of the chunks before giving the rest): a ballot a comparison, no
+// sort, and for a decode batch no second launch.
+template <bool TABLE>
+__global__ __launch_bounds__(PM_THREADS) void permute_kernel(const PermP p) {
+  __shared__ PermS s;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (blockIdx.x == gridDim.x - 1) {
+    if constexpr (TABLE) {
+      pm_columns(p, s, 0);
+    } else {
+      pm_count(p, s.total, 0, p.n);
+      pm_starts(p, s);
+    }
+    for (int e = tid; e <= p.E; e += PM_THREADS) p.offsets[e] = s.start[e];
+    return;
+  }
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
+  const int tokens = (int)imin64(p.tokens, p.T - t0);
+  const int a0 = (int)t0 * p.k, own = tokens * p.k;
+  for (int j = tid; j < own; j += PM_THREADS) {
+    s.own[j] = pm_key(p, a0 + j) << PM_SHIFT | (uint32_t)(a0 + j);
+    s.rank[j] = 0;
+  }
+  const int chunk = TABLE ? a0 / p.chunk : 0;
+  const int from = TABLE ? chunk * p.chunk : 0, to = TABLE ? min(from + p.chunk, p.n) : p.n;
+  if constexpr (TABLE) pm_columns(p, s, chunk);  // waits for all threads
+  else __syncthreads();
+  for (int base = from; base < to; base += 4 * PM_THREADS) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = base + i * PM_THREADS + tid;
+      c[i] = a < to ? pm_key(p, a) << PM_SHIFT | (uint32_t)a : ~0u;
+    }
+    for (int j = 0; j < own; ++j) {
+      const uint32_t mine = __builtin_amdgcn_readfirstlane(s.own[j]);
+      const uint32_t low = TABLE ? mine >> PM_SHIFT << PM_SHIFT : 0u;  // of the same key, or of all
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) count += __builtin_popcountll(__ballot(c[i] - low < mine - low));
+      if (lane == 0 && count) atomicAdd(&s.rank[j], count);
+    }
+  }
+  __syncthreads();
+  for (int j = tid; j < own; j += PM_THREADS) {
+    const uint32_t key = s.own[j] >> PM_SHIFT;
+    const int row = s.rank[j] + (TABLE ? s.start[key] + s.before[key] : 0);
+    s.rank[j] = (int)key == p.E ? ~row : row;
+    p.position[a0 + j] = s.rank[j];
+  }
+  __syncthreads();
+  const int64_t width = (int64_t)p.H * p.esize;
+  const char* x = reinterpret_cast<const char*>(p.x) + t0 * p.ldx;
+  char* rows = reinterpret_cast<char*>(p.rows);
+  if (width < 16) {
+    for (int j = tid; j < own; j += PM_THREADS) {
+      const int at = s.rank[j];
+      char* row = rows + (int64_t)(at < 0 ? ~at : at) * width;
+      for (int b = 0; b < width; b += 2)
+        *reinterpret_cast<uint16_t*>(row + b) =
+            at < 0 ? (uint16_t)0 : *reinterpret_cast<const uint16_t*>(x + j / p.k * p.ldx + b);
+    }
+    return;
+  }
+  const int side = p.row_threads, first = tid / side;
+  for (int t = first; t < tokens; t += PM_THREADS / side)
+    for (int64_t b = 16 * (tid & (side - 1)); b < width; b += 16 * side) {
+      const int64_t at = b + 16 <= width ? b : width - 16;
+      const u32x4 v = pm_load(x + t * p.ldx + at);
+      for (int i = 0; i < p.k; ++i) {
+        const int row = s.rank[t * p.k + i];
+        pm_store(rows + (int64_t)(row < 0 ? ~row : row) * width + at, row < 0 ? u32x4{0, 0, 0, 0} : v);
+      }
+    }
+}
+
+// --------------------------------------------------------------- and back --
+struct UnpermP {
+  const void* rows;
+  const int32_t* position;
+  const float* weights;  // or null
+  const void* dy;        // gradients only
+  void* out;             // y, or d_rows
+  float* d_weights;
+  int64_t ldr, ldy, R, T;  // strides in elements
+  int k, H;
+  int y_dtype;
+  int row_threads;
+};
+
+template <int DT>
+constexpr int kPiece = DT == CCQ_F32 ? 4 : 8;  // elements of 16 bytes
+
+template <int DT>
+__device__ __forceinline__ void pm_floats(u32x4 b, float (&v)[kPiece<DT>]) {
+#pragma unroll
+  for (int e = 0; e < kPiece<DT>; ++e) {
+    if constexpr (DT == CCQ_F32) {
+      v[e] = __uint_as_float(b[e]);
+    } else {
+      const uint32_t u = (b[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+      v[e] = DT == CCQ_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pm_pair(int dt, float a, float b) {
+  return dt == CCQ_BF16 ? bf16x2_bits(a, b) : f32_to_f16_bits(a) | f32_to_f16_bits(b) << 16;
+}
+template <int N>
+__device__ __forceinline__ void pm_store_floats(int dt, void* y, int64_t i, const float (&v)[N]) {
+  if (dt == CCQ_F32) {
+    __builtin_memcpy(reinterpret_cast<float*>(y) + i, v, 4 * N);
+  } else {
+    uint32_t b[N / 2];
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) b[e] = pm_pair(dt, v[2 * e], v[2 * e + 1]);
+    __builtin_memcpy(reinterpret_cast<uint16_t*>(y) + i, b, 2 * N);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float pm_one(const void* p, int64_t i) {
+  if constexpr (DT == CCQ_F32) return reinterpret_cast<const float*>(p)[i];
+  const uint32_t u = reinterpret_cast<const uint16_t*>(p)[i];
+  return DT == CCQ_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+}
+__device__ __forceinline__ void pm_store_one(int dt, void* y, int64_t i, float v) {
+  if (dt == CCQ_F32)
+    reinterpret_cast<float*>(y)[i] = v;
+  else
+    reinterpret_cast<uint16_t*>(y)[i] = (uint16_t)(dt == CCQ_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
+}
+
+// A thread adds one piece of a token's rows, eight of them in flight.
+template <int DT>
+__global__ __launch_bounds__(PM_THREADS) void unpermute_kernel(const UnpermP p) {
+  constexpr int N = kPiece<DT>;
+  const int side = p.row_threads, first = threadIdx.x / side;
+  const int64_t t = (int64_t)blockIdx.x * (PM_THREADS / side) + first;
+  if (t >= p.T) return;
+  const int32_t* position = p.position + t * p.k;
+  const float* weights = p.weights != nullptr ? p.weights + t * p.k : nullptr;
+  const int c = threadIdx.x & (side - 1);
+  if (p.H < N) {
+    if (c < p.H) {
+      float sum = 0.f;
+      for (int s = 0; s < p.k; ++s) {
+        const int at = position[s];
+        if (at < 0 || at >= p.R) continue;
+        const float v = pm_one<DT>(p.rows, at * p.ldr + c);
+        sum = weights != nullptr ? fmaf(v, weights[s], sum) : sum + v;
+      }
+      pm_store_one(p.y_dtype, p.out, t * p.H + c, sum);
+    }
+    return;
+  }
+  for (int h = c * N; h < p.H; h += side * N) {
+    const int i = min(h, p.H - N);
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = 0.f;
+    for (int s0 = 0; s0 < p.k; s0 += 8) {
+      u32x4 b[8];
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = s0 + j < p.k ? position[s0 + j] : -1;
+        const bool kept = at >= 0 && at < p.R;
+        b[j] = kept ? pm_load(reinterpret_cast<const char*>(p.rows) + (at * p.ldr + i) * (DT == CCQ_F32 ? 4 : 2))
+                    : u32x4{0, 0, 0, 0};
+        w[j] = !kept ? 0.f : weights != nullptr ? weights[s0 + j] : 1.f;  // (0 times the zeros above, whatever the weight)
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v[N];
+        pm_floats<DT>(b[j], v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] = fmaf(v[e], w[j], sum[e]);
+      }
+    }
+    pm_store_floats(p.y_dtype, p.out, t * p.H + i, sum);
+  }
+}
+
+// WAVES waves on a token: each piece of dy is read once, multiplied into the
+// token's rows' gradients and with the rows themselves; the products' sums are
+// joined over the lanes at the end (always in the same order).
+template <int DT, int WAVES>
+__global__ __launch_bounds__(PM_THREADS) void unpermute_grad_kernel(const UnpermP p) {
+  constexpr int N = kPiece<DT>, TOKENS = PM_WAVES / WAVES;
+  __shared__ float part[PM_WAVES][8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = (int64_t)blockIdx.x * TOKENS + wave / WAVES;
+  const bool there = t < p.T;
+  const int c = (wave % WAVES) * 64 + lane;
+  constexpr int64_t E = DT == CCQ_F32 ? 4 : 2;
+  for (int s0 = 0; s0 < p.k; s0 += 8) {
+    float sum[8], w[8];
+    int at[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum[j] = 0.f;
+      const bool slot = there && s0 + j < p.k;
+      at[j] = slot ? p.position[t * p.k + s0 + j] : INT32_MIN;
+      w[j] = slot ? p.weights[t * p.k + s0 + j] : 0.f;
+    }
+    if (there) {
+      if (p.H < N) {
+        if (c < p.H) {
+          const float g = pm_one<DT>(p.dy, t * p.ldy + c);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int row = at[j] < 0 ? ~at[j] : at[j];
+            if (row >= p.R) continue;
+            if (at[j] >= 0) sum[j] = pm_one<DT>(p.rows, row * p.ldr + c) * g;
+            pm_store_one(DT, p.out, (int64_t)row * p.H + c, at[j] >= 0 ? w[j] * g : 0.f);
+          }
+        }
+      } else {
+        for (int h = c * N; h < p.H; h += WAVES * 64 * N) {
+          const int i = min(h, p.H - N);
+          const u32x4 gb = pm_load(reinterpret_cast<const char*>(p.dy) + (t * p.ldy + i) * E);
+          u32x4 rb[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            rb[j] = at[j] >= 0 && at[j] < p.R ? pm_load(reinterpret_cast<const char*>(p.rows) + (at[j] * p.ldr + i) * E)
+                                              : u32x4{0, 0, 0, 0};
+          float g[N];
+          pm_floats<DT>(gb, g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int row = at[j] < 0 ? ~at[j] : at[j];
+            if (row >= p.R) continue;
+            float r[N], o[N];
+            pm_floats<DT>(rb[j], r);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              o[e] = at[j] >= 0 ? w[j] * g[e] : 0.f;
+              // (a row's last piece counts what the piece before it does not have)
+              if (at[j] >= 0 && e >= h - i) sum[j] = fmaf(r[e], g[e], sum[j]);
+            }
+            pm_store_floats(DT, p.out, (int64_t)row * p.H + i, o);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int m = 32; m; m >>= 1) sum[j] += wave_shfl_xor(sum[j], m);
+    if constexpr (WAVES > 1) {
+      if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[wave][j] = sum[j];
+      __syncthreads();
+      if (wave % WAVES == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int v = 1; v < WAVES; ++v) sum[j] += part[wave + v][j];
+      __syncthreads();
+    }
+    if (there && c == 0)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (s0 + j < p.k) p.d_weights[t * p.k + s0 + j] = sum[j];
+  }
+}
+
+// threads on a row: whole waves' worth of its pieces, at least 16
+int row_threads(int64_t bytes) {
+  int t = 16;
+  while (t < PM_THREADS && t * 16 < bytes) t *= 2;
+  return t;
+}
+
+int64_t esize(int dt) { return dt == CCQ_F32 ? 4 : 2; }
+
+int check_sizes(const char* what, int dtype, int64_t T, int64_t k, int64_t H) {
+  CCQ_REQUIRE(dtype == CCQ_F32 || dtype == CCQ_F16 || dtype == CCQ_BF16, "%s: dtype %d", what, dtype);
+  CCQ_REQUIRE(k >= 1 && k <= PM_MAX_K, "%s: k=%lld, 1 to %d", what, (long long)k, PM_MAX_K);
+  CCQ_REQUIRE(T >= 0 && T <= PM_MAX_N && T * k <= PM_MAX_N, "%s: T=%lld tokens of %lld experts: at most 2^20 in all", what, (long long)T,
+              (long long)k);
+  CCQ_REQUIRE(H >= 1 && H <= 1 << 20, "%s: H=%lld, 1 to 2^20", what, (long long)H);
+  return 0;
+}
+
+void plan_permute(PermP& p, int64_t T, int64_t k) {
+  p.n = (int)(T * k);
+  p.tokens = (int)(T <= 1024 ? 1 : T <= 4096 ? 4 : 8);
+  while (p.tokens * k > PM_OWN) p.tokens /= 2;
+  const int unit = (int)(p.tokens * k);
+  const int least = p.n / PM_CHUNKS > 512 ? p.n / PM_CHUNKS : 512;
+  p.chunk = (int)(cdiv(least, unit) * unit);
+  p.chunks = (int)cdiv(p.n, p.chunk);
+}
+
+}  // namespace
+
+}  // namespace ccq
+
+using namespace ccq;
+
+extern "C" size_t ccq_moe_permute_workspace_size(int64_t T, int64_t k, int64_t num_experts) {
+  if (T < 1 || T > PM_MAX_N || k < 1 || k > PM_MAX_K || num_experts < 1 || num_experts > PM_MAX_E ||
+      T * k > PM_MAX_N || T * k <= PM_SELF)
+    return 0;
+  PermP p;
+  plan_permute(p, T, k);
+  return (size_t)p.chunks * (num_experts + 1) * 4;
+}
+
+extern "C" int ccq_moe_permute(const void* x, int dtype, int64_t ldx, const int64_t* ids, void* rows, int32_t* position,
+                               int32_t* offsets, int64_t T, int64_t k, int64_t num_experts, int64_t H, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  const char* what = "ccq_moe_permute";
+  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
+  CCQ_REQUIRE(num_experts >= 1 && num_experts <= PM_MAX_E, "%s: num_experts=%lld, 1 to %d", what, (long long)num_experts,
+              PM_MAX_E);
+  CCQ_REQUIRE(T <= 1 || ldx >= H, "%s: row stride %lld of rows of %lld", what, (long long)ldx, (long long)H);
+  CCQ_REQUIRE(offsets != nullptr && (T == 0 || (x && ids && rows && position)), "%s: null pointer", what);
+  const size_t e = (size_t)esize(dtype);
+  CCQ_REQUIRE(aligned(x, e) && aligned(rows, e) && aligned(ids, 8) && aligned(position, 4) && aligned(offsets, 4),
+              "%s: pointers must be aligned to their elements", what);
+  const size_t need = ccq_moe_permute_workspace_size(T, k, num_experts);
+  CCQ_REQUIRE(need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
+              "%s: workspace of %zu bytes needed", what, need);
+  PermP p = {x, ids, rows, position, offsets, reinterpret_cast<int32_t*>(workspace), ldx * (int64_t)e, T};
+  plan_permute(p, T, k);
+  p.k = (int)k;
+  p.E = (int)num_experts;
+  p.H = (int)H;
+  p.esize = (int)e;
+  p.row_threads = row_threads(H * (int64_t)e);
+  const dim3 grid((uint32_t)(cdiv(T, p.tokens) + 1));
+  if (need) {
+    launch(permute_count_kernel, dim3((uint32_t)p.chunks), dim3(PM_THREADS), 0, as_stream(stream), p);
+    if (int rc = launch_status(what)) return rc;
+    launch(permute_kernel<true>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  } else {
+    launch(permute_kernel<false>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  }
+  return launch_status(what);
+}
+
+extern "C" int ccq_moe_unpermute(const void* rows, int dtype, int64_t ldr, int64_t num_rows, const int32_t* position,
+                                 const float* weights, void* y, int y_dtype, int64_t T, int64_t k, int64_t H,
+                                 void* stream) {
+  const char* what = "ccq_moe_unpermute";
+  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
+  CCQ_REQUIRE(y_dtype == CCQ_F32 || y_dtype == CCQ_F16 || y_dtype == CCQ_BF16, "%s: y_dtype %d", what, y_dtype);
+  CCQ_REQUIRE(num_rows >= 0 && (num_rows <= 1 || ldr >= H), "%s: %lld rows of %lld, stride %lld", what,
+              (long long)num_rows, (long long)H, (long long)ldr);
+  if (T == 0) return 0;
+  CCQ_REQUIRE((rows || num_rows == 0) && position && y, "%s: null pointer", what);
+  CCQ_REQUIRE(aligned(rows, (size_t)esize(dtype)) && aligned(position, 4) && aligned(weights, 4) &&
+                  aligned(y, (size_t)esize(y_dtype)),
+              "%s: pointers must be aligned to their elements", what);
+  UnpermP p = {rows, position, weights, nullptr, y, nullptr, ldr, 0, num_rows, T, (int)k, (int)H, y_dtype,
+               row_threads(H * esize(dtype))};
+  const dim3 grid((uint32_t)cdiv(T, PM_THREADS / p.row_threads));
+  if (dtype == CCQ_BF16)
+    launch(unpermute_kernel<CCQ_BF16>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  else if (dtype == CCQ_F16)
+    launch(unpermute_kernel<CCQ_F16>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  else
+    launch(unpermute_kernel<CCQ_F32>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  return launch_status(what);
+}
+
+namespace ccq {
+namespace {
+template <int WAVES>
+void launch_grad(int dtype, const UnpermP& p, hipStream_t st) {
+  const dim3 grid((uint32_t)cdiv(p.T, PM_WAVES / WAVES));
+  if (dtype == CCQ_BF16)
+    launch(unpermute_grad_kernel<CCQ_BF16, WAVES>, grid, dim3(PM_THREADS), 0, st, p);
+  else if (dtype == CCQ_F16)
+    launch(unpermute_grad_kernel<CCQ_F16, WAVES>, grid, dim3(PM_THREADS), 0, st, p);
+  else
+    launch(unpermute_grad_kernel<CCQ_F32, WAVES>, grid, dim3(PM_THREADS), 0, st, p);
+}
+}  // namespace
+}  // namespace ccq
+
+extern "C" int ccq_moe_unpermute_grad(const void* dy, int64_t ldy, const void* rows, int64_t ldr, int dtype,
+                                      int64_t num_rows, const int32_t* position, const float* weights, void* d_rows,
+                                      float* d_weights, int64_t T, int64_t k, int64_t H, void* stream) {
+  const char* what = "ccq_moe_unpermute_grad";
+  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
+  CCQ_REQUIRE(num_rows >= 0 && (num_rows <= 1 || ldr >= H) && (T <= 1 || ldy >= H),
+              "%s: %lld rows of %lld, strides %lld and %lld", what, (long long)num_rows, (long long)H, (long long)ldr,
+              (long long)ldy);
+  if (T == 0) return 0;
+  CCQ_REQUIRE(dy && rows && position && weights && d_rows && d_weights, "%s: null pointer", what);
+  const size_t e = (size_t)esize(dtype);
+  CCQ_REQUIRE(aligned(dy, e) && aligned(rows, e) && aligned(d_rows, e) && aligned(position, 4) && aligned(weights, 4) &&
+                  aligned(d_weights, 4),
+              "%s: pointers must be aligned to their elements", what);
+  const UnpermP p = {rows, position, weights, dy, d_rows, d_weights, ldr, ldy, num_rows, T, (int)k, (int)H, dtype, 0};
+  if (T >= 1024)
+    launch_grad<1>(dtype, p, as_stream(stream));
+  else
+    launch_grad<4>(dtype, p, as_stream(stream));
+  return launch_status(what);
+}

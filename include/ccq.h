@@ -737,6 +737,88 @@ int ccq_moe_f32_ffn(const float* x, const int64_t* ids, const float* weights,
                     int64_t num_experts, int64_t hidden, int64_t inter, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Tokens sorted by expert and back, with gradients (the grouping that
+ * moe_combine does per expert, blocks/moe.py:163-172, as operators)
+ * ---------------------------------------------------------------------- */
+
+/* Workspace of ccq_moe_permute (counts; no initial contents required), 0 for
+ * the batches that one kernel sorts.  Calls sharing one must not overlap. */
+size_t ccq_moe_permute_workspace_size(int64_t T, int64_t k, int64_t num_experts);
+
+/* The assignments (token t, slot s), a = t k + s, in the order of (expert, a),
+ * those with ids outside [0, num_experts) behind all others:
+ * position [T, k] the row of each assignment, ~row for those left out;
+ * offsets [num_experts + 1] the first row of each expert, and the end;
+ * rows [T k, H] the tokens' rows in that order, zeros from row
+ * offsets[num_experts] on.  x [T, H] of dtype (CCQ_F32 | CCQ_F16 | CCQ_BF16) with
+ * row stride ldx, ids [T, k] int64.  T k <= 2^20, k <= 64, H <= 2^20,
+ * num_experts <= 1024; any element alignment; rows must not overlap x. */
+int ccq_moe_permute(const void* x, int dtype, int64_t ldx, const int64_t* ids, void* rows, int32_t* position,
+                    int32_t* offsets, int64_t T, int64_t k, int64_t num_experts, int64_t H, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* y[t] = sum over s of weights[t, s] * rows[position[t, s]] (weights null: 1
+ * each), float32 sums in slot order, y [T, H] of y_dtype rounded once; positions
+ * outside [0, num_rows) contribute nothing.  rows [num_rows, H] of dtype, row
+ * stride ldr.  Without weights also the gradient of x in ccq_moe_permute, rows
+ * being that of its rows. */
+int ccq_moe_unpermute(const void* rows, int dtype, int64_t ldr, int64_t num_rows, const int32_t* position,
+                      const float* weights, void* y, int y_dtype, int64_t T, int64_t k, int64_t H, void* stream);
+
+/* The gradients of ccq_moe_unpermute from dy [T, H]: d_rows [num_rows, H] (dense)
+ * in row position[t, s] weights[t, s] * dy[t] rounded once, zeros in row r where
+ * the position is ~r; d_weights [T, k] the float32 products of rows and dy, 0
+ * where the position is negative.  rows, dy and d_rows of dtype, row strides ldr
+ * and ldy; each row of d_rows is written by the position that names it. */
+int ccq_moe_unpermute_grad(const void* dy, int64_t ldy, const void* rows, int64_t ldr, int dtype, int64_t num_rows,
+                           const int32_t* position, const float* weights, void* d_rows, float* d_weights, int64_t T,
+                           int64_t k, int64_t H, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Linears with 16-bit weights, the epilogue in the product's kernel
+ * ---------------------------------------------------------------------- */
+#define CCQ_ACT_NONE 0
+#define CCQ_ACT_RELU 1
+#define CCQ_ACT_GELU 2      /* z Phi(z) */
+#define CCQ_ACT_GELU_TANH 3 /* its approximation by tanh */
+#define CCQ_ACT_SILU 4
+
+/* x [M, K] and w [W, K] of dtype (CCQ_F16 | CCQ_BF16), W = N, or 2N where gated;
+ * bias [W] of bias_dtype or null; residual [M, N] of y_dtype or null; y [M, N] of
+ * y_dtype; row strides ldx, ldr, ldy in elements, w dense, any element alignment.
+ * Grouped: w [num_experts, W, K], bias [num_experts, W], offsets
+ * [num_experts + 1].  residual may be y; y must not overlap x or another view of
+ * residual.  M, K, N <= 2^20, num_experts <= 1024. */
+typedef struct ccq_dense_args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* residual;
+  void* y;
+  const int32_t* offsets;
+  void* workspace;
+  void* stream;
+  size_t workspace_bytes;
+  int64_t ldx, ldr, ldy, M, K, N, num_experts;
+  int dtype, bias_dtype, y_dtype, act, gated;
+} ccq_dense_args;
+
+/* Workspace of ccq_dense_linear for these arguments (partial sums of K's
+ * splits; no initial contents required), 0 where K is not split.  Calls sharing
+ * one must not overlap in time. */
+size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args);
+
+/* z = x w^T + bias; y = act(z) + residual, gated: y = act(z[:, :N]) * z[:, N:] +
+ * residual; products, sums and the epilogue in float32, y rounded once. */
+int ccq_dense_linear(const ccq_dense_args* args);
+
+/* ccq_dense_linear where rows offsets[e] .. offsets[e + 1] - 1 of x take w[e] and
+ * bias[e] (offsets within [0, M] and rising, as ccq_moe_permute makes them; read
+ * on the device); rows of y from offsets[num_experts] on are zeros.  Takes no
+ * workspace. */
+int ccq_dense_linear_grouped(const ccq_dense_args* args);
+
 #ifdef __cplusplus
 }
 #endif
