@@ -16,6 +16,7 @@
 #include "ccq_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ccq {
 
@@ -322,105 +323,148 @@ __global__ __launch_bounds__(FEW_THREADS) void dense_few_kernel(const DenseP p) 
 
 // ---------------------------------------------------------------- tiles --
 // BM rows of x by BN rows of w (gated: 16 of the gate's and 16 of the up half's in
-// turn), 64 columns of K a stage, two stages in LDS.  A stage's rows are 128
-// bytes, their eight 16-byte pieces XORed with the row's low bits, so that the 8
-// rows that one cycle of an operand's read touches lie in different banks.
-// DMA: stages are copied into LDS by the load itself, the next one while this one
-// is multiplied (x, w and their rows aligned to 16 bytes); else through registers,
-// at any alignment.
+// turn), 64 columns of K a stage.  Rows in LDS are 128 bytes, their eight 16-byte
+// pieces XORed with the row's low bits, so that the lanes which one cycle of an
+// operand's read serves lie in different banks (no conflicts in the counters).
 constexpr int DN_BK = 64;
 
-template <int DT, int BM, int BN, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const DenseP p) {
-  using Vec = typename DnVec<DT>::type;
-  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = BM + BN;
-  constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  constexpr int STAGE = ROWS * 128;
-  constexpr int LOADS = ROWS / 8 / WAVES;  // pieces of a thread
-  static_assert(ROWS % (8 * WAVES) == 0 && BM % 8 == 0 && FN % 2 == 0, "whole pieces, pairs of groups");
-  __shared__ __align__(16) char lds[2][STAGE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-
+struct DnPlace {  // a workgroup's tile
   DnTile t;
-  int nt, split = 0;
+  int n0;         // first column
+  int split;
+};
+
+// The tile of this workgroup: neighbouring tiles on one XCD, eight row tiles side
+// by side, so that its workgroups share rows of both operands in its L2.
+template <int BM>
+__device__ __forceinline__ DnPlace dn_place(const DenseP& p, int columns) {
+  DnPlace w = {};
   if (p.offsets != nullptr) {
     int at = 0;
-    t = dn_find_tile<BM>(p, [&](int total) {
+    w.t = dn_find_tile<BM>(p, [&](int total) {
       const int all = total * p.ntiles;
       if ((int)blockIdx.x >= all) return -1;
       at = xcd_remap(blockIdx.x, all);
       return at / p.ntiles;
     });
-    if (t.expert < 0) return;
-    nt = at % p.ntiles;
-  } else {
-    const int all = p.mtiles * p.ntiles * p.splits;
-    const int id = xcd_remap(blockIdx.x, all), tiles = p.mtiles * p.ntiles;
-    split = id / tiles;
-    // eight row tiles side by side, so that the workgroups of an XCD share rows of both operands
-    const int at = id % tiles, band = at / (8 * p.ntiles), inside = at % (8 * p.ntiles);
-    const int high = min(8, p.mtiles - 8 * band);
-    const int mt = 8 * band + inside % high;
-    nt = inside / high;
-    t = DnTile{0, (int64_t)mt * BM, (int)imin64(BM, p.M - (int64_t)mt * BM)};
+    w.n0 = at % p.ntiles * columns;
+    return w;
   }
-  const int columns = p.gated ? BN / 2 : BN, n0 = nt * columns;
-  if (t.expert == p.E) {
-    dn_zero(p, t, n0, columns, THREADS);
+  const int tiles = p.mtiles * p.ntiles, id = xcd_remap(blockIdx.x, tiles * p.splits);
+  w.split = id / tiles;
+  const int at = id % tiles, band = at / (8 * p.ntiles), inside = at % (8 * p.ntiles);
+  const int high = min(8, p.mtiles - 8 * band), mt = 8 * band + inside % high;
+  w.n0 = inside / high * columns;
+  w.t = DnTile{0, (int64_t)mt * BM, (int)imin64(BM, p.M - (int64_t)mt * BM)};
+  return w;
+}
+
+// row `q` of a tile's rows of w, as a row of w from row n0 on
+__device__ __forceinline__ int64_t dn_wrow(const DenseP& p, int n0, int q) {
+  const int n = p.gated ? (q >> 5) * 16 + (q & 15) : q;
+  return (int64_t)min(n, p.N - 1 - n0) + (p.gated && q & 16 ? p.N : 0);
+}
+
+// The sums of a wave's FN x FM groups to y, or to the splits' sums: group (i, j)
+// holds rows w0 + 16 i .. of the tile's w and row m0 + 16 j + lane % 16 of its x.
+// They go through the wave's own piece of LDS, 16 rows at a time, so that rows of y
+// are read and written in whole lines and the epilogue's code stands here once a
+// group of rows (in place it took the accumulators' registers).
+template <int FN>
+constexpr int kScratch = 16 * (4 * FN + 1) * 16;  // bytes; a row's 4 FN quads and one, so that 16 rows start in 16 banks
+template <int FM, int FN>
+__device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
+                                         char* scratch) {
+  constexpr int LINE = 4 * FN + 1;
+  const int lane = lane_id();
+  f32x4* own = reinterpret_cast<f32x4*>(scratch);
+  const bool paired = p.gated && p.part == nullptr;
+  const int quads = paired ? 2 * FN : 4 * FN;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) own[(lane & 15) * LINE + 4 * i + (lane >> 4)] = acc[i][j];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+    for (int at = lane; at < 16 * quads; at += 64) {
+      const int r = at / quads, c = at - r * quads, row = m0 + 16 * j + r;
+      if (row >= w.t.rows) break;
+      if (paired) {
+        const f32x4* q = own + r * LINE + (c & 3) + 8 * (c >> 2);
+        dn_finish(p, w.t.row + row, w.t.expert, w.n0 + w0 / 2 + 4 * c, q[0], q[4]);
+      } else if (p.part == nullptr) {
+        dn_finish(p, w.t.row + row, w.t.expert, w.n0 + w0 + 4 * c, own[r * LINE + c], f32x4{0.f, 0.f, 0.f, 0.f});
+      } else {
+        const int q = w0 + 4 * c, n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q);
+        if (n < p.N)
+          dn_store4(CCQ_F32, p.part, ((int64_t)w.split * p.M + w.t.row + row) * p.W + n + (p.gated && q & 16 ? p.N : 0),
+                    p.N - n, own[r * LINE + c]);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// x and w aligned to 16 bytes in every row.  A stage's x and w are a unit each in
+// a ring of five units of LDS, copied there by the loads themselves.  A stage is
+// multiplied in two halves of 32 columns; each half's operands are read from LDS
+// while the half before is multiplied, so the one barrier of a stage stands
+// between its halves: behind it, all of this stage is in registers, its two units
+// are free, and the next stage is in LDS.  Copies are spread over the products
+// (64 of them at once fill the address unit and hold up the waves that issue
+// them): w of the stage after the next follows the barrier, its x, into the ring's
+// fifth unit, the first half of the next stage, so x is two stages ahead.
+// 256 x 256, 4096 x 14336 x 4096: 327 us, 1470 TFLOP/s; the matrix unit is busy in
+// 76 % of the cycles, at 1.75 GHz of 2.4: power bounds it.  (Two whole stages, the
+// copies at once: 423 us; spread: 344; 32x32x16 products: 347 us, fewer cycles at
+// a lower clock.)
+template <int DT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const DenseP p) {
+  using Vec = typename DnVec<DT>::type;
+  constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  constexpr int UNIT = (BM > BN ? BM : BN) * 128;
+  constexpr int LX = BM / (8 * WAVES), LW = (BN + 8 * WAVES - 1) / (8 * WAVES);  // copies of a wave: 8 rows each
+  constexpr int NM = FM * FN, NR = FM + FN;                                      // products and reads of a half
+  static_assert(TM % 16 == 0 && TN % 16 == 0 && BM % (8 * WAVES) == 0 && 8 * WAVES * LW * 128 <= UNIT, "whole units");
+  static_assert(NM >= 2 * NR && NM >= 4 * LW, "reads and copies fit between the products");
+  __shared__ __align__(16) char lds[5 * UNIT];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int columns = p.gated ? BN / 2 : BN;
+  const DnPlace w = dn_place<BM>(p, columns);
+  if (w.t.expert < 0) return;
+  if (w.t.expert == p.E) {
+    dn_zero(p, w.t, w.n0, columns, 64 * WAVES);
     return;
   }
-  const int kfrom = split * p.kchunk, kto = min(p.K, kfrom + p.kchunk);
-  const uint16_t* xb = reinterpret_cast<const uint16_t*>(p.x) + t.row * p.ldx;
-  const uint16_t* wb = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)t.expert * p.W + n0) * p.K;
+  const int kfrom = w.split * p.kchunk, kto = min(p.K, kfrom + p.kchunk);
+  const int stages = (kto - kfrom + DN_BK - 1) / DN_BK, whole = (kto - kfrom) / DN_BK;
+  const uint16_t* xb = reinterpret_cast<const uint16_t*>(p.x) + w.t.row * p.ldx + kfrom;
+  const uint16_t* wb = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)w.t.expert * p.W + w.n0) * p.K + kfrom;
 
-  // piece i of a thread: row 8 (wave + WAVES i) + lane / 8 of the stage, LDS piece lane % 8
+  // copy i of a wave: rows 8 (wave + WAVES i) + lane / 8 of the unit, LDS piece lane % 8
   const int piece = (lane & 7) ^ (lane >> 3);  // its columns 8 piece .. + 7 (the row's low bits are lane / 8)
-  int64_t from[LOADS];                         // in elements, from xb or wb
+  uint32_t xo[LX], wo[LW];                     // in bytes, from xb and wb (rows past the tile's: its last one again)
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int row = 8 * (wave + WAVES * i) + (lane >> 3);
-    if (row < BM) {
-      from[i] = (int64_t)min(row, t.rows - 1) * p.ldx + 8 * piece;
-    } else {
-      const int q = row - BM, n = p.gated ? (q >> 5) * 16 + (q & 15) : q;
-      from[i] = ((int64_t)min(n, p.N - 1 - n0) + (p.gated && q & 16 ? p.N : 0)) * p.K + 8 * piece;
-    }
-  }
-  uint32_t voff[LOADS];
+  for (int i = 0; i < LX; ++i)
+    xo[i] = (uint32_t)(2 * (min(8 * (wave + WAVES * i) + (lane >> 3), w.t.rows - 1) * p.ldx + 8 * piece));
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) voff[i] = (uint32_t)(2 * from[i]);
-  const uint32_t lds0 = lds_addr(&lds[0][0]);
-
-  auto stage_dma = [&](int k0, int b) {
-    const uint32_t to = lds0 + b * STAGE + wave * 1024;
-    if (k0 + DN_BK <= kto) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const bool isx = WAVES * i + WAVES <= BM / 8 || (WAVES * i < BM / 8 && wave + WAVES * i < BM / 8);
-        dma16((isx ? xb : wb) + k0, voff[i], to + i * WAVES * 1024);
-      }
-    } else {  // K ends inside: zeros from there on, in both operands
-      const bool valid = k0 + 8 * piece < kto;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const bool isx = WAVES * i + WAVES <= BM / 8 || (WAVES * i < BM / 8 && wave + WAVES * i < BM / 8);
-        if (valid)
-          dma16((isx ? xb : wb) + k0, voff[i], to + i * WAVES * 1024);
-        else
-          *reinterpret_cast<u32x4*>(&lds[b][(wave + i * WAVES) * 1024 + lane * 16]) = u32x4{0, 0, 0, 0};
-      }
-    }
+  for (int i = 0; i < LW; ++i)
+    wo[i] = (uint32_t)(2 * (dn_wrow(p, w.n0, min(8 * (wave + WAVES * i) + (lane >> 3), BN - 1)) * p.K + 8 * piece));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(&lds[0])) + wave * 1024;
+  auto copy_x = [&](int i, int s, int unit) { dma16(xb + s * DN_BK, xo[i], lds0 + unit + i * WAVES * 1024); };
+  auto copy_w = [&](int i, int s, int unit) { dma16(wb + s * DN_BK, wo[i], lds0 + unit + i * WAVES * 1024); };
+  // the last stage, where K ends inside it: zeros from there on, in both operands
+  const bool valid = (stages - 1) * DN_BK + 8 * piece < kto - kfrom;
+  auto zero = [&](int i, int unit) {
+    *reinterpret_cast<u32x4*>(&lds[unit + (wave + i * WAVES) * 1024 + lane * 16]) = u32x4{0, 0, 0, 0};
   };
-  auto stage_load = [&](int k0, u32x4 (&v)[LOADS]) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const bool isx = 8 * (wave + WAVES * i) < BM;
-      v[i] = dn_load8<false>((isx ? xb : wb) + from[i] - 8 * piece, k0 + 8 * piece, kto);
-    }
+  auto last_x = [&](int i, int unit) {
+    if (valid) copy_x(i, stages - 1, unit);
+    else zero(i, unit);
   };
-  auto stage_store = [&](int b, const u32x4 (&v)[LOADS]) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) *reinterpret_cast<u32x4*>(&lds[b][(wave + i * WAVES) * 1024 + lane * 16]) = v[i];
+  auto last_w = [&](int i, int unit) {
+    if (valid) copy_w(i, stages - 1, unit);
+    else zero(i, unit);
   };
 
   f32x4 acc[FN][FM];
@@ -428,67 +472,156 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const Dense
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Half {
+    Vec x[FM], w[FN];
+  };
+  Half even, odd;  // operands of a stage's first and second 32 columns
   const int m0 = wave / WN * TM, w0 = wave % WN * TN;
-  const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;  // of the stage's first 32 columns; the others': ^ 64
-  const uint32_t xat = (m0 + (lane & 15)) * 128, wat = (BM + w0 + (lane & 15)) * 128;
+  const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;  // of the first 32 columns; the others': ^ 64
+  const uint32_t xat = (m0 + (lane & 15)) * 128 + swz, wat = (w0 + (lane & 15)) * 128 + swz;
+  auto read = [&](Half& h, int r, uint32_t xa, uint32_t wa) {  // in the order in which the products take them
+    if (r == 0)
+      h.w[0] = *reinterpret_cast<const Vec*>(&lds[wa]);
+    else if (r <= FM)
+      h.x[r - 1] = *reinterpret_cast<const Vec*>(&lds[xa + (r - 1) * 2048]);
+    else
+      h.w[r - FM] = *reinterpret_cast<const Vec*>(&lds[wa + (r - FM) * 2048]);
+  };
+  auto ring = [](int u) { return u >= 5 * UNIT ? u - 5 * UNIT : u; };
+  int ux = 0;  // the unit of this stage's x; its w is in the next one, the next stage in the two after that
+  // COPY: of stage s + 2, 1 whole, 2 the last one; NEXT: there is a stage s + 1
+  auto stage = [&](auto copy, auto next, int s) {
+    constexpr int COPY = decltype(copy)::value;
+    constexpr bool NEXT = decltype(next)::value;
+    const int uw = ring(ux + UNIT), nx = ring(ux + 2 * UNIT), nw = ring(ux + 3 * UNIT), free = ring(ux + 4 * UNIT);
+    {
+      const uint32_t xa = (xat + ux) ^ 64, wa = (wat + uw) ^ 64;
+#pragma unroll
+      for (int q = 0; q < NM; ++q) {
+        if (q % 2 == 0 && q / 2 < NR) read(odd, q / 2, xa, wa);
+        if (COPY && q % (NM / LX) == NM / LX / 2) {
+          if constexpr (COPY == 1) copy_x(q / (NM / LX), s + 2, free);
+          else last_x(q / (NM / LX), free);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        acc[q / FM][q % FM] = dn_mfma(even.w[q / FM], even.x[q % FM], acc[q / FM][q % FM]);
+      }
+    }
+    if constexpr (NEXT) {
+      wait_vmcnt<COPY == 1 ? LX : 0>();  // all but the copies just issued
+      lds_barrier();
+    }
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+      if (NEXT && q % 2 == 0 && q / 2 < NR) read(even, q / 2, xat + nx, wat + nw);
+      if (COPY && q % 2 == 0 && q / 2 < LW) {
+        if constexpr (COPY == 1) copy_w(q / 2, s + 2, ux);
+        else last_w(q / 2, ux);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      acc[q / FM][q % FM] = dn_mfma(odd.w[q / FM], odd.x[q % FM], acc[q / FM][q % FM]);
+    }
+    ux = nx;
+  };
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    if (b < whole) {
+#pragma unroll
+      for (int i = 0; i < LX; ++i) copy_x(i, b, 2 * b * UNIT);
+#pragma unroll
+      for (int i = 0; i < LW; ++i) copy_w(i, b, (2 * b + 1) * UNIT);
+    } else if (b < stages) {
+#pragma unroll
+      for (int i = 0; i < LX; ++i) last_x(i, 2 * b * UNIT);
+#pragma unroll
+      for (int i = 0; i < LW; ++i) last_w(i, (2 * b + 1) * UNIT);
+    }
+  }
+  if (whole >= 2) wait_vmcnt<LX + LW>();
+  else wait_vmcnt<0>();
+  lds_barrier();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(even, r, xat, wat + UNIT);
+  constexpr std::integral_constant<int, 0> none{};
+  constexpr std::integral_constant<int, 1> full{};
+  constexpr std::integral_constant<int, 2> end{};
+  int s = 0;
+  for (; s + 2 < whole; ++s) stage(full, std::true_type{}, s);
+  if (s + 2 < stages) stage(end, std::true_type{}, s++);
+  if (s + 1 < stages) stage(none, std::true_type{}, s++);
+  stage(none, std::false_type{}, s);
+  __syncthreads();  // (the waves' scratch lies in the ring)
+  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
+}
 
-  auto multiply = [&](int b) {
+// The same product for rows at any alignment: stages pass through registers, two
+// of them in LDS.
+template <int DT>
+__global__ __launch_bounds__(256, 2) void dense_ragged_kernel(const DenseP p) {
+  using Vec = typename DnVec<DT>::type;
+  constexpr int B = 128, WAVES = 4, FM = 4, FN = 4, LOADS = B / 8 / WAVES, UNIT = B * 128;
+  __shared__ __align__(16) char lds[2][2 * UNIT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int columns = p.gated ? B / 2 : B;
+  const DnPlace w = dn_place<B>(p, columns);
+  if (w.t.expert < 0) return;
+  if (w.t.expert == p.E) {
+    dn_zero(p, w.t, w.n0, columns, 64 * WAVES);
+    return;
+  }
+  const int kfrom = w.split * p.kchunk, kto = min(p.K, kfrom + p.kchunk);
+  const int stages = (kto - kfrom + DN_BK - 1) / DN_BK;
+  const int piece = (lane & 7) ^ (lane >> 3);
+  const uint16_t *x[LOADS], *wr[LOADS];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint32_t o = swz ^ (64 * s);
-      Vec xv[FM], wv[FN];
+  for (int i = 0; i < LOADS; ++i) {
+    const int row = 8 * (wave + WAVES * i) + (lane >> 3);
+    x[i] = reinterpret_cast<const uint16_t*>(p.x) + (w.t.row + min(row, w.t.rows - 1)) * p.ldx;
+    wr[i] = reinterpret_cast<const uint16_t*>(p.w) +
+            ((int64_t)w.t.expert * p.W + w.n0 + dn_wrow(p, w.n0, row)) * p.K;
+  }
+  f32x4 acc[FN][FM];
 #pragma unroll
-      for (int j = 0; j < FM; ++j) xv[j] = *reinterpret_cast<const Vec*>(&lds[b][xat + o + j * 2048]);
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) wv[i] = *reinterpret_cast<const Vec*>(&lds[b][wat + o + i * 2048]);
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int m0 = wave / 2 * 64, w0 = wave % 2 * 64;
+  const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;
+  const uint32_t xat = (m0 + (lane & 15)) * 128 + swz, wat = UNIT + (w0 + (lane & 15)) * 128 + swz;
+  u32x4 xv[LOADS], wv[LOADS];
+  auto load = [&](int s) {
+    const int k = kfrom + s * DN_BK + 8 * piece;
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = dn_mfma(wv[i], xv[j], acc[i][j]);
+    for (int i = 0; i < LOADS; ++i) {
+      xv[i] = dn_load8<false>(x[i], k, kto);
+      wv[i] = dn_load8<false>(wr[i], k, kto);
     }
   };
-
-  const int stages = (kto - kfrom + DN_BK - 1) / DN_BK;
-  if constexpr (DMA) {
-    stage_dma(kfrom, 0);
-    for (int s = 0; s < stages; ++s) {
-      wait_vmcnt<0>();   // this wave's pieces of stage s are there,
-      lds_barrier();     // all waves' are, and all have multiplied stage s - 1
-      if (s + 1 < stages) stage_dma(kfrom + (s + 1) * DN_BK, (s + 1) & 1);
-      multiply(s & 1);
+  load(0);
+  for (int s = 0; s < stages; ++s) {
+    char* to = &lds[s & 1][wave * 1024 + lane * 16];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      *reinterpret_cast<u32x4*>(to + i * WAVES * 1024) = xv[i];
+      *reinterpret_cast<u32x4*>(to + UNIT + i * WAVES * 1024) = wv[i];
     }
-  } else {
-    u32x4 v[LOADS];
-    stage_load(kfrom, v);
-    for (int s = 0; s < stages; ++s) {
-      stage_store(s & 1, v);
-      __syncthreads();
-      if (s + 1 < stages) stage_load(kfrom + (s + 1) * DN_BK, v);
-      multiply(s & 1);
-    }
-  }
-
+    __syncthreads();
+    if (s + 1 < stages) load(s + 1);
 #pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int row = m0 + 16 * j + (lane & 15);
-    if (row >= t.rows) continue;
-    if (p.part != nullptr) {
-      float* part = p.part + ((int64_t)split * p.M + t.row + row) * p.W;
+    for (int h = 0; h < 2; ++h) {
+      Vec xf[FM], wf[FN];
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const int q = w0 + 16 * i, n = n0 + (p.gated ? (q >> 5) * 16 : q) + 4 * (lane >> 4);
-        if (n < p.N) dn_store4(CCQ_F32, part, n + (p.gated && q & 16 ? p.N : 0), p.N - n, acc[i][j]);
-      }
-    } else if (p.gated) {
+      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const Vec*>(&lds[s & 1][(xat ^ (64 * h)) + j * 2048]);
 #pragma unroll
-      for (int i = 0; i < FN; i += 2)
-        dn_finish(p, t.row + row, t.expert, n0 + (w0 + 16 * i) / 2 + 4 * (lane >> 4), acc[i][j], acc[i + 1][j]);
-    } else {
+      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const Vec*>(&lds[s & 1][(wat ^ (64 * h)) + i * 2048]);
 #pragma unroll
       for (int i = 0; i < FN; ++i)
-        dn_finish(p, t.row + row, t.expert, n0 + w0 + 16 * i + 4 * (lane >> 4), acc[i][j], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = dn_mfma(wf[i], xf[j], acc[i][j]);
     }
   }
+  __syncthreads();
+  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[0][wave * kScratch<FN>]);
 }
 
 // The splits' sums added in order, and the epilogue.
@@ -575,11 +708,11 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
     return launch_status(what);
   }
   if (q.bm == 256)
-    launch(dense_tile_kernel<DT, 256, 256, 2, 4, true>, dim3((uint32_t)grid), dim3(512), 0, st, p);
+    launch(dense_tile_kernel<DT, 256, 256, 4, 2>, dim3((uint32_t)grid), dim3(512), 0, st, p);
   else if (q.dma)
-    launch(dense_tile_kernel<DT, 128, 128, 2, 2, true>, dim3((uint32_t)grid), dim3(256), 0, st, p);
+    launch(dense_tile_kernel<DT, 128, 128, 2, 2>, dim3((uint32_t)grid), dim3(256), 0, st, p);
   else
-    launch(dense_tile_kernel<DT, 128, 128, 2, 2, false>, dim3((uint32_t)grid), dim3(256), 0, st, p);
+    launch(dense_ragged_kernel<DT>, dim3((uint32_t)grid), dim3(256), 0, st, p);
   if (int rc = launch_status(what)) return rc;
   if (p.part != nullptr) {
     launch(dense_join_kernel, dim3((uint32_t)grid_for(p.M * cdiv(p.N, 4), 256)), dim3(256), 0, st, p);
