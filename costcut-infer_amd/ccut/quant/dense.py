@@ -24,7 +24,7 @@ _HALF = (torch.bfloat16, torch.float16)
 _pack = DENSE_ARGS.pack
 MAX_ROWS, MAX_SIDE, MAX_EXPERTS = 1 << 20, 1 << 20, 1024
 # batches above this many rows may split K over workgroups and need scratch for the partial sums
-_UNSPLIT_ROWS = 64
+_UNSPLIT_ROWS = 16
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:

@@ -5,14 +5,16 @@
 // x [M, K], w [N, K] (grouped: w[e] for the rows offsets[e] .. offsets[e + 1] - 1),
 // products and everything after them in float32, y rounded once.
 //
-// Both kernels give the matrix instructions w as their first operand, so a lane
+// All kernels give the matrix instructions w as their first operand, so a lane
 // ends with four neighbouring columns of one row of y, and with the gate and up
 // rows of w in turn (16 by 16) also both halves of a gated value: the epilogue
 // needs no exchange.
 //
-// dense_few_kernel   up to 64 rows at once: w goes from memory to registers, the
-//                    waves of a workgroup share K and add up at the end.
-// dense_tile_kernel  tiles of rows and columns through LDS.
+// dense_few_kernel   up to 16 rows: w goes from memory to registers, the waves of a
+//                    workgroup share K and add up at the end.
+// dense_mid_kernel   small tiles of rows and columns through a ring of stages in LDS.
+// dense_tile_kernel  large tiles, the products interleaved with the next ones' reads.
+// dense_ragged_kernel  rows at any alignment.
 #include "ccq_common.h"
 
 #include <algorithm>
@@ -233,34 +235,30 @@ __device__ __forceinline__ u32x4 dn_load8(const uint16_t* row, int k, int K) {
 }
 
 // ------------------------------------------------------------- few rows --
-// A workgroup takes NF groups of 16 rows of w and up to 16 MT rows of x; its 8
-// waves take 32 U columns of K in turn, each multiplying what it loads, and
-// their sums are added at the end in the waves' order.  w is read once, straight
-// into the operand's registers: lane l holds 8 values of row l % 16 from column
-// 8 (l / 16) on, so 4 neighbouring loads of a wave fill whole lines.
-constexpr int FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES;
-
-template <int DT, int MT, int NF, int U, bool WHOLE>
-__global__ __launch_bounds__(FEW_THREADS) void dense_few_kernel(const DenseP p) {
+// A workgroup takes NF groups of 16 rows of w and up to 16 MT rows of x; its waves
+// take 32 U columns of K in turn, each multiplying what it loads, and their sums
+// are added at the end in the waves' order.  w is read once, straight into the
+// operand's registers, the next columns while these are multiplied: lane l holds 8
+// values of row l % 16 from column 8 (l / 16) on, so neighbouring loads of a wave
+// fill whole lines.
+template <int DT, int MT, int NF, int U, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
-  constexpr int BM = 16 * MT;
-  __shared__ f32x4 sums[FEW_WAVES][MT * NF][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int BM = 16 * MT, THREADS = 64 * WAVES, STEP = 32 * U;
+  __shared__ f32x4 sums[WAVES][MT * NF][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, k8 = (lane >> 4) * 8;
+  const int nt = blockIdx.x % p.ntiles, mt = blockIdx.x / p.ntiles;
   DnTile t;
-  int nt;
   if (p.offsets != nullptr) {
-    nt = blockIdx.x % p.ntiles;
-    t = dn_find_tile<BM>(p, [&](int) { return (int)blockIdx.x / p.ntiles; });
+    t = dn_find_tile<BM>(p, [&](int) { return mt; });
     if (t.expert < 0) return;
   } else {
-    nt = blockIdx.x % p.ntiles;
-    const int mt = blockIdx.x / p.ntiles;
     t = DnTile{0, (int64_t)mt * BM, (int)imin64(BM, p.M - (int64_t)mt * BM)};
   }
   const int columns = p.gated ? 8 * NF : 16 * NF, n0 = nt * columns;
   if (t.expert == p.E) {
-    dn_zero(p, t, n0, columns, FEW_THREADS);
+    dn_zero(p, t, n0, columns, THREADS);
     return;
   }
   const uint16_t* w[NF];
@@ -268,35 +266,69 @@ __global__ __launch_bounds__(FEW_THREADS) void dense_few_kernel(const DenseP p) 
   for (int f = 0; f < NF; ++f) {
     const int n = p.gated ? n0 + f / 2 * 16 + r : n0 + f * 16 + r;
     const int64_t row = (int64_t)min(n, p.N - 1) + (p.gated && f & 1 ? p.N : 0);
-    w[f] = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)t.expert * p.W + row) * p.K;
+    w[f] = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)t.expert * p.W + row) * p.K + k8;
   }
   const uint16_t* x[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
-    x[m] = reinterpret_cast<const uint16_t*>(p.x) + (t.row + min(16 * m + r, t.rows - 1)) * p.ldx;
+    x[m] = reinterpret_cast<const uint16_t*>(p.x) + (t.row + min(16 * m + r, t.rows - 1)) * p.ldx + k8;
   f32x4 acc[NF][MT];
 #pragma unroll
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int STEP = 32 * U;
-  for (int k0 = wave * STEP; k0 < p.K; k0 += FEW_WAVES * STEP) {
-    u32x4 wv[NF][U], xv[MT][U];
+  struct Step {
+    u32x4 w[NF][U], x[MT][U];
+  };
+  auto load = [&](Step& s, int k0) {
+    if (k0 + STEP <= p.K) {
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
+      for (int f = 0; f < NF; ++f)
 #pragma unroll
-      for (int u = 0; u < U; ++u) wv[f][u] = dn_load8<WHOLE>(w[f], k0 + 32 * u + k8, p.K);
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&s.w[f][u], w[f] + k0 + 32 * u, 16);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int u = 0; u < U; ++u) xv[m][u] = dn_load8<WHOLE>(x[m], k0 + 32 * u + k8, p.K);
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&s.x[m][u], x[m] + k0 + 32 * u, 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 32 * u;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) s.w[f][u] = dn_load8<WHOLE>(w[f], k, p.K - k8);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s.x[m][u] = dn_load8<WHOLE>(x[m], k, p.K - k8);
+      }
+    }
+  };
+  auto multiply = [&](const Step& s) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          acc[f][m] = dn_mfma(__builtin_bit_cast(Vec, wv[f][u]), __builtin_bit_cast(Vec, xv[m][u]), acc[f][m]);
+          acc[f][m] = dn_mfma(__builtin_bit_cast(Vec, s.w[f][u]), __builtin_bit_cast(Vec, s.x[m][u]), acc[f][m]);
+  };
+  constexpr int STRIDE = WAVES * STEP;
+  int k0 = wave * STEP;
+  if (k0 < p.K) {
+    Step a, b;
+    load(a, k0);
+    for (;;) {
+      if ((k0 += STRIDE) >= p.K) {
+        multiply(a);
+        break;
+      }
+      load(b, k0);
+      multiply(a);
+      if ((k0 += STRIDE) >= p.K) {
+        multiply(b);
+        break;
+      }
+      load(a, k0);
+      multiply(b);
+    }
   }
 #pragma unroll
   for (int f = 0; f < NF; ++f)
@@ -305,16 +337,16 @@ __global__ __launch_bounds__(FEW_THREADS) void dense_few_kernel(const DenseP p) 
   __syncthreads();
   // a pair of groups (gated: gate and up) and 16 rows at a time
   const int groups = p.gated ? NF / 2 : NF;
-  for (int i = threadIdx.x; i < groups * MT * 64; i += FEW_THREADS) {
+  for (int i = threadIdx.x; i < groups * MT * 64; i += THREADS) {
     const int l = i & 63, m = i / 64 % MT, f = i / (64 * MT);
     const int fg = p.gated ? 2 * f : f;
     f32x4 g = sums[0][fg * MT + m][l], u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 1; v < FEW_WAVES; ++v) g += sums[v][fg * MT + m][l];
-    if (p.gated) {
+    for (int v = 1; v < WAVES; ++v) g += sums[v][fg * MT + m][l];
+    if (NF > 1 && p.gated) {
       u = sums[0][(fg + 1) * MT + m][l];
 #pragma unroll
-      for (int v = 1; v < FEW_WAVES; ++v) u += sums[v][(fg + 1) * MT + m][l];
+      for (int v = 1; v < WAVES; ++v) u += sums[v][(fg + 1) * MT + m][l];
     }
     const int row = 16 * m + (l & 15);
     if (row < t.rows) dn_finish(p, t.row + row, t.expert, n0 + f * 16 + 4 * (l >> 4), g, u);
@@ -327,6 +359,18 @@ __global__ __launch_bounds__(FEW_THREADS) void dense_few_kernel(const DenseP p) 
 // pieces XORed with the row's low bits, so that the lanes which one cycle of an
 // operand's read serves lie in different banks (no conflicts in the counters).
 constexpr int DN_BK = 64;
+
+// Waits until at most `n` stages of L copies each are on their way (n >= N: N).
+template <int N, int L>
+__device__ __forceinline__ void wait_stages(int n) {
+  if constexpr (N > 0) {
+    if (n < N) {
+      wait_stages<N - 1, L>(n);
+      return;
+    }
+  }
+  wait_vmcnt<N * L>();
+}
 
 struct DnPlace {  // a workgroup's tile
   DnTile t;
@@ -368,40 +412,100 @@ __device__ __forceinline__ int64_t dn_wrow(const DenseP& p, int n0, int q) {
 // The sums of a wave's FN x FM groups to y, or to the splits' sums: group (i, j)
 // holds rows w0 + 16 i .. of the tile's w and row m0 + 16 j + lane % 16 of its x.
 // They go through the wave's own piece of LDS, 16 rows at a time, so that rows of y
-// are read and written in whole lines and the epilogue's code stands here once a
-// group of rows (in place it took the accumulators' registers).
+// are read and written in whole lines, a lane's columns and so its bias stay the
+// same, and the code stands here once, not once for each accumulator.
 template <int FN>
 constexpr int kScratch = 16 * (4 * FN + 1) * 16;  // bytes; a row's 4 FN quads and one, so that 16 rows start in 16 banks
-template <int FM, int FN>
-__device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
-                                         char* scratch) {
-  constexpr int LINE = 4 * FN + 1;
+constexpr int dn_pow2(int n) { return n <= 1 ? 1 : 2 * dn_pow2((n + 1) / 2); }
+
+template <int FM, int FN, class F>
+__device__ __forceinline__ void dn_rows(const f32x4 (&acc)[FN][FM], f32x4* own, F each) {
   const int lane = lane_id();
-  f32x4* own = reinterpret_cast<f32x4*>(scratch);
-  const bool paired = p.gated && p.part == nullptr;
-  const int quads = paired ? 2 * FN : 4 * FN;
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
 #pragma unroll
-    for (int i = 0; i < FN; ++i) own[(lane & 15) * LINE + 4 * i + (lane >> 4)] = acc[i][j];
+    for (int i = 0; i < FN; ++i) own[(lane & 15) * (4 * FN + 1) + 4 * i + (lane >> 4)] = acc[i][j];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    each(j);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+template <int G>
+__device__ __forceinline__ void dn_act_all(int act, f32x4 (&v)[G]) {
+  auto all = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = dn_act(decltype(a)::value, v[i][e]);
+  };
+  if (act == CCQ_ACT_SILU) all(std::integral_constant<int, CCQ_ACT_SILU>{});
+  else if (act == CCQ_ACT_GELU) all(std::integral_constant<int, CCQ_ACT_GELU>{});
+  else if (act == CCQ_ACT_GELU_TANH) all(std::integral_constant<int, CCQ_ACT_GELU_TANH>{});
+  else if (act == CCQ_ACT_RELU) all(std::integral_constant<int, CCQ_ACT_RELU>{});
+}
+
+template <int FM, int FN, bool PAIRED>
+__device__ __forceinline__ void dn_write_y(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
+                                           f32x4* own) {
+  constexpr int QUADS = PAIRED ? 2 * FN : 4 * FN, SIDE = dn_pow2(QUADS), STEP = 64 / SIDE, LINE = 4 * FN + 1;
+  constexpr int G = STEP < 16 ? 2 : 1;  // rows of y at once
+  const int lane = lane_id(), c = lane & (SIDE - 1), r0 = lane / SIDE;
+  const int n = w.n0 + (PAIRED ? w0 / 2 : w0) + 4 * c;
+  const int left = c < QUADS ? p.N - n : 0;
+  f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = bg;
+  if (p.bias != nullptr && left > 0) {
+    const int64_t at = (int64_t)w.t.expert * p.W + n;
+    bg = dn_load4(p.bias_dtype, p.bias, at, left);
+    if (PAIRED) bu = dn_load4(p.bias_dtype, p.bias, at + p.N, left);
+  }
+  const f32x4* from = own + r0 * LINE + (PAIRED ? (c & 3) + 8 * (c >> 2) : c);
+  dn_rows<FM, FN>(acc, own, [&](int j) {
+    const int row0 = m0 + 16 * j + r0;
 #pragma unroll 1
-    for (int at = lane; at < 16 * quads; at += 64) {
-      const int r = at / quads, c = at - r * quads, row = m0 + 16 * j + r;
-      if (row >= w.t.rows) break;
-      if (paired) {
-        const f32x4* q = own + r * LINE + (c & 3) + 8 * (c >> 2);
-        dn_finish(p, w.t.row + row, w.t.expert, w.n0 + w0 / 2 + 4 * c, q[0], q[4]);
-      } else if (p.part == nullptr) {
-        dn_finish(p, w.t.row + row, w.t.expert, w.n0 + w0 + 4 * c, own[r * LINE + c], f32x4{0.f, 0.f, 0.f, 0.f});
-      } else {
-        const int q = w0 + 4 * c, n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q);
-        if (n < p.N)
-          dn_store4(CCQ_F32, p.part, ((int64_t)w.split * p.M + w.t.row + row) * p.W + n + (p.gated && q & 16 ? p.N : 0),
-                    p.N - n, own[r * LINE + c]);
+    for (int i = 0; i < 16 / STEP; i += G) {
+      f32x4 g[G], r[G];
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const int row = row0 + (i + e) * STEP;
+        if (p.residual != nullptr && row < w.t.rows && left > 0)
+          r[e] = dn_load4(p.y_dtype, p.residual, (w.t.row + row) * p.ldr + n, left);
+        g[e] = from[(i + e) * STEP * LINE] + bg;
+      }
+      dn_act_all<G>(p.act, g);
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const int row = row0 + (i + e) * STEP;
+        if (PAIRED) g[e] *= from[(i + e) * STEP * LINE + 4] + bu;
+        if (row >= w.t.rows || left <= 0) continue;
+        if (p.residual != nullptr) g[e] += r[e];
+        dn_store4(p.y_dtype, p.y, (w.t.row + row) * p.ldy + n, left, g[e]);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  });
+}
+
+template <int FM, int FN>
+__device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
+                                         char* scratch) {
+  f32x4* own = reinterpret_cast<f32x4*>(scratch);
+  if (p.part != nullptr) {
+    constexpr int QUADS = 4 * FN, SIDE = dn_pow2(QUADS), STEP = 64 / SIDE;
+    const int lane = lane_id(), c = lane & (SIDE - 1), r0 = lane / SIDE, q = w0 + 4 * c;
+    const int n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q), left = c < QUADS ? p.N - n : 0;
+    float* part = p.part + ((int64_t)w.split * p.M + w.t.row) * p.W + n + (p.gated && q & 16 ? p.N : 0);
+    dn_rows<FM, FN>(acc, own, [&](int j) {
+#pragma unroll 1
+      for (int r = r0; r < 16; r += STEP) {
+        const int row = m0 + 16 * j + r;
+        if (row < w.t.rows && left > 0)
+          dn_store4(CCQ_F32, part, (int64_t)row * p.W, left, own[r * (4 * FN + 1) + c]);
+      }
+    });
+  } else if (p.gated) {
+    if constexpr (FN % 2 == 0) dn_write_y<FM, FN, true>(p, w, m0, w0, acc, own);
+  } else {
+    dn_write_y<FM, FN, false>(p, w, m0, w0, acc, own);
   }
 }
 
@@ -554,14 +658,96 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const Dense
   dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
-// The same product for rows at any alignment: stages pass through registers, two
-// of them in LDS.
-template <int DT>
-__global__ __launch_bounds__(256, 2) void dense_ragged_kernel(const DenseP p) {
+// Batches between: what bounds them is w's way from memory, so small tiles, K split
+// over workgroups, and a ring of D stages of 64 columns that are on their way while
+// one is multiplied.  Four waves, 2 x 2.
+template <int DT, int BM, int BN, int D>
+__global__ __launch_bounds__(256) void dense_mid_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
-  constexpr int B = 128, WAVES = 4, FM = 4, FN = 4, LOADS = B / 8 / WAVES, UNIT = B * 128;
-  __shared__ __align__(16) char lds[2][2 * UNIT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int WAVES = 4, TM = BM / 2, TN = BN / 2, FM = TM / 16, FN = TN / 16;
+  constexpr int LX = BM / (8 * WAVES), LW = BN / (8 * WAVES), STAGE = (BM + BN) * 128;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole copies");
+  __shared__ __align__(16) char lds[D * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int columns = p.gated ? BN / 2 : BN;
+  const DnPlace w = dn_place<BM>(p, columns);
+  if (w.t.expert < 0) return;
+  if (w.t.expert == p.E) {
+    dn_zero(p, w.t, w.n0, columns, 64 * WAVES);
+    return;
+  }
+  const int kfrom = w.split * p.kchunk, kto = min(p.K, kfrom + p.kchunk);
+  const int stages = (kto - kfrom + DN_BK - 1) / DN_BK;
+  const uint16_t* xb = reinterpret_cast<const uint16_t*>(p.x) + w.t.row * p.ldx + kfrom;
+  const uint16_t* wb = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)w.t.expert * p.W + w.n0) * p.K + kfrom;
+  const int piece = (lane & 7) ^ (lane >> 3);
+  uint32_t xo[LX], wo[LW];
+#pragma unroll
+  for (int i = 0; i < LX; ++i)
+    xo[i] = (uint32_t)(2 * (min(8 * (wave + WAVES * i) + (lane >> 3), w.t.rows - 1) * p.ldx + 8 * piece));
+#pragma unroll
+  for (int i = 0; i < LW; ++i) wo[i] = (uint32_t)(2 * (dn_wrow(p, w.n0, 8 * (wave + WAVES * i) + (lane >> 3)) * p.K + 8 * piece));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(&lds[0])) + wave * 1024;
+  auto copy = [&](int s, int slot) {
+    const uint16_t *xs = xb + s * DN_BK, *ws = wb + s * DN_BK;
+    const uint32_t to = lds0 + slot;
+    if ((s + 1) * DN_BK <= kto - kfrom) {
+#pragma unroll
+      for (int i = 0; i < LW; ++i) dma16(ws, wo[i], to + (BM / 8 + i * WAVES) * 1024);
+#pragma unroll
+      for (int i = 0; i < LX; ++i) dma16(xs, xo[i], to + i * WAVES * 1024);
+    } else {  // K ends inside: zeros from there on, in both operands (each copy has lanes before the end)
+      const bool valid = s * DN_BK + 8 * piece < kto - kfrom;
+#pragma unroll
+      for (int i = 0; i < LX + LW; ++i) {
+        const int at = i < LX ? i * WAVES : BM / 8 + (i - LX) * WAVES;
+        if (valid) dma16(i < LX ? xs : ws, i < LX ? xo[i < LX ? i : 0] : wo[i < LX ? 0 : i - LX], to + at * 1024);
+        else *reinterpret_cast<u32x4*>(&lds[slot + (wave + at) * 1024 + lane * 16]) = u32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int m0 = wave / 2 * TM, w0 = wave % 2 * TN;
+  const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;
+  const uint32_t xat = (m0 + (lane & 15)) * 128 + swz, wat = (BM + w0 + (lane & 15)) * 128 + swz;
+  for (int s = 0; s < D - 1 && s < stages; ++s) copy(s, s * STAGE);
+  int slot = 0, to = (D - 1) * STAGE;
+  for (int s = 0; s < stages; ++s) {
+    // stage s is there; as many behind it as there are may still be on their way
+    wait_stages<D - 2, LX + LW>(stages - 1 - s);
+    lds_barrier();
+    if (s + D - 1 < stages) copy(s + D - 1, to);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Vec xf[FM], wf[FN];
+#pragma unroll
+      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const Vec*>(&lds[slot + (xat ^ (64 * h)) + j * 2048]);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const Vec*>(&lds[slot + (wat ^ (64 * h)) + i * 2048]);
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = dn_mfma(wf[i], xf[j], acc[i][j]);
+    }
+    to = slot;
+    slot = slot + STAGE == D * STAGE ? 0 : slot + STAGE;
+  }
+  __syncthreads();
+  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
+}
+
+// The same product for rows at any alignment: stages pass through registers, two of
+// them on their way there, into two in LDS.
+template <int DT, int B>
+__global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
+  using Vec = typename DnVec<DT>::type;
+  constexpr int WAVES = 4, TM = B / 2, FM = TM / 16, FN = FM, LOADS = B / 8 / WAVES, UNIT = B * 128;
+  __shared__ __align__(16) char lds[2 * 2 * UNIT];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int columns = p.gated ? B / 2 : B;
   const DnPlace w = dn_place<B>(p, columns);
   if (w.t.expert < 0) return;
@@ -585,43 +771,59 @@ __global__ __launch_bounds__(256, 2) void dense_ragged_kernel(const DenseP p) {
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int m0 = wave / 2 * 64, w0 = wave % 2 * 64;
+  const int m0 = wave / 2 * TM, w0 = wave % 2 * TM;
   const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;
   const uint32_t xat = (m0 + (lane & 15)) * 128 + swz, wat = UNIT + (w0 + (lane & 15)) * 128 + swz;
-  u32x4 xv[LOADS], wv[LOADS];
-  auto load = [&](int s) {
+  struct Stage {
+    u32x4 x[LOADS], w[LOADS];
+  };
+  auto load = [&](Stage& v, int s) {
     const int k = kfrom + s * DN_BK + 8 * piece;
+    if (kfrom + (s + 1) * DN_BK <= kto) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      xv[i] = dn_load8<false>(x[i], k, kto);
-      wv[i] = dn_load8<false>(wr[i], k, kto);
+      for (int i = 0; i < LOADS; ++i) {
+        __builtin_memcpy(&v.w[i], wr[i] + k, 16);
+        __builtin_memcpy(&v.x[i], x[i] + k, 16);
+      }
+    } else if (s < stages) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        v.w[i] = dn_load8<false>(wr[i], k, kto);
+        v.x[i] = dn_load8<false>(x[i], k, kto);
+      }
     }
   };
-  load(0);
-  for (int s = 0; s < stages; ++s) {
-    char* to = &lds[s & 1][wave * 1024 + lane * 16];
+  auto turn = [&](Stage& v, int s, char* buffer) {  // v: stage s, then stage s + 2
+    char* to = buffer + wave * 1024 + lane * 16;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      *reinterpret_cast<u32x4*>(to + i * WAVES * 1024) = xv[i];
-      *reinterpret_cast<u32x4*>(to + UNIT + i * WAVES * 1024) = wv[i];
+      *reinterpret_cast<u32x4*>(to + i * WAVES * 1024) = v.x[i];
+      *reinterpret_cast<u32x4*>(to + UNIT + i * WAVES * 1024) = v.w[i];
     }
-    __syncthreads();
-    if (s + 1 < stages) load(s + 1);
+    lds_barrier();  // (all waves have multiplied stage s - 1, so stage s + 1 may take its buffer)
+    load(v, s + 2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       Vec xf[FM], wf[FN];
 #pragma unroll
-      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const Vec*>(&lds[s & 1][(xat ^ (64 * h)) + j * 2048]);
+      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const Vec*>(buffer + (xat ^ (64 * h)) + j * 2048);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const Vec*>(&lds[s & 1][(wat ^ (64 * h)) + i * 2048]);
+      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const Vec*>(buffer + (wat ^ (64 * h)) + i * 2048);
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = dn_mfma(wf[i], xf[j], acc[i][j]);
     }
+  };
+  Stage even, odd;
+  load(even, 0);
+  load(odd, 1);
+  for (int s = 0; s < stages; s += 2) {
+    turn(even, s, lds);
+    if (s + 1 < stages) turn(odd, s + 1, lds + 2 * UNIT);
   }
   __syncthreads();
-  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[0][wave * kScratch<FN>]);
+  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
 // The splits' sums added in order, and the epilogue.
@@ -642,51 +844,89 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const DenseP p) {
 }
 
 // ------------------------------------------------------------- dispatch --
-constexpr int64_t FEW_ROWS = 64;
+enum Kind { FEW, MID, TILE, RAGGED };
 
 struct Plan {
-  bool few, dma;
-  int bm, bn;       // of the tile, or 16 MT and 16 NF
+  Kind kind;
+  int bm, bn;       // of the tile; FEW: 16 rows, 16 NF columns
   int splits, kchunk;
 };
 
-// rows: of the batch, or of a group on average
+// What a stage of 64 columns takes in us, with up to one and two workgroups on a
+// CU, and what a tile takes besides.  From K = 4096 and 2048 over M = 32 .. 2048,
+// N = 2048 .. 14336 (M=256 K=N=4096: MID 64 x 64 in 2 splits 19.6 us, TILE 128 in 4
+// 20.0, in one 35.1; M=512: 23.9 at best, 27.4, 36.1; M=512 N=14336: MID 117, TILE
+// 128 75.5, 256 x 192 74.0, 256 86.0; M=1024: TILE 128 138, 256 96.5).
+struct Shape {
+  Kind kind;
+  int bm, bn;
+  float one, two, tile;
+};
+constexpr Shape kShapes[] = {
+    {MID, 32, 64, 0.25f, 0.40f, 2.f},   {MID, 64, 64, 0.33f, 0.50f, 2.f},   {MID, 128, 64, 0.50f, 0.76f, 2.f},
+    {TILE, 128, 128, 0.72f, 1.05f, 5.f}, {TILE, 256, 192, 1.05f, 0.f, 6.f}, {TILE, 256, 224, 1.32f, 0.f, 7.f},
+    {TILE, 256, 256, 1.45f, 0.f, 8.f},   {RAGGED, 64, 64, 0.6f, 0.9f, 3.f}, {RAGGED, 128, 128, 1.2f, 1.7f, 5.f},
+};
+
+float shape_time(const Shape& s, const DenseP& p, int splits) {
+  const int64_t stages = cdiv(cdiv(p.K, DN_BK), splits);
+  const int64_t groups = cdiv(p.M, s.bm) * cdiv(p.W, s.bn) * splits, round = s.two > 0.f ? 512 : 256;
+  const float full = s.two > 0.f ? s.two : s.one;
+  const int64_t rest = groups % round;
+  float t = (float)(groups / round) * (stages * full + s.tile);
+  if (rest > 0) t += stages * (rest <= 256 ? s.one : full) + s.tile;
+  // the partial sums' way out and back, and a launch
+  if (splits > 1) t += 3.f + (float)splits * p.M * p.W * 8 / 4e6f;
+  return t;
+}
+
+// rows: of the batch, or of an expert on average
 Plan make_plan(const DenseP& p, int64_t rows, bool dma) {
-  Plan q = {};
-  q.few = rows <= FEW_ROWS;
-  q.dma = dma;
-  q.splits = 1;
-  q.kchunk = p.K;
-  if (q.few) {
-    q.bm = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    q.bn = q.bm == 64 ? 64 : 32;
+  Plan q = {FEW, 16, 16, 1, p.K};
+  const bool grouped = p.offsets != nullptr;
+  if (grouped && (dma || rows > 16)) {
+    // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 140
+    // us, MID 64: 146; 1 to 6 rows as FEW), 64 up to 48 (32 skewed rows: 161, MID 32: 169; 64 rows: TILE 128 168, MID 64
+    // 180), TILE 256 from 200 on (256 rows: 238, TILE 128: 275; 128 rows: 216 and 186)
+    q.kind = !dma ? RAGGED : rows <= 48 ? MID : TILE;
+    q.bm = !dma ? (rows <= 64 ? 64 : 128) : rows <= 24 ? 32 : rows <= 48 ? 64 : rows < 200 ? 128 : 256;
+    q.bn = q.kind == MID ? 64 : q.bm;
     return q;
   }
-  const int64_t big = cdiv(p.M, 256) * cdiv(p.W, 256);
-  if (dma && rows > 128 && big >= 192) {
-    q.bm = q.bn = 256;
+  if (rows <= 16) {
+    // as many columns a workgroup as leave one for every second CU (M=1: K=2048 N=5632 16 columns 8.0 us, 32 7.3, 64 11.0;
+    // K=4096 N=14336 32, 31, 25.6; K=N=4096 8.3, 11.5, 17.5); groups of rows bring as many workgroups as experts
+    const int64_t sets = cdiv(p.W, 16) * (grouped ? std::min<int64_t>(p.M, p.E) : 1);
+    q.bn = sets >= 640 ? 64 : sets >= 320 || p.gated ? 32 : 16;
     return q;
   }
-  q.bm = q.bn = 128;
-  const int64_t tiles = cdiv(p.M, 128) * cdiv(p.W, 128);
-  if (p.offsets == nullptr && tiles < 256) {
+  float best = 0.f;
+  for (const Shape& s : kShapes) {
+    if (dma ? s.kind == RAGGED : s.kind != RAGGED) continue;
+    if (p.gated && s.bn == 224) continue;  // a wave's 112 rows are no whole pairs of gate and up
     const int64_t stages = cdiv(p.K, DN_BK);
-    int64_t s = std::min<int64_t>(std::min<int64_t>(cdiv(512, tiles), stages / 8), 16);
-    if (s > 1) {
-      q.kchunk = (int)(cdiv(stages, s) * DN_BK);
-      q.splits = (int)cdiv(p.K, q.kchunk);
+    for (int splits = 1; splits <= 16; ++splits) {
+      if (splits > 1 && (stages / splits < 4 || s.bm == 256)) break;
+      const float t = shape_time(s, p, splits);
+      if (best == 0.f || t < best) {
+        best = t;
+        q = {s.kind, s.bm, s.bn, 1, p.K};
+        if (splits > 1) {
+          q.kchunk = (int)(cdiv(stages, splits) * DN_BK);
+          q.splits = (int)cdiv(p.K, q.kchunk);
+        }
+      }
     }
   }
   return q;
 }
 
-template <int DT, int MT, int NF, int U>
-void launch_few(const DenseP& p, hipStream_t st) {
-  const dim3 grid((uint32_t)((int64_t)p.mtiles * p.ntiles));
+template <int DT, int NF, int U, int WAVES>
+void launch_few(const DenseP& p, dim3 grid, hipStream_t st) {
   if (p.K % 8 == 0)
-    launch(dense_few_kernel<DT, MT, NF, U, true>, grid, dim3(FEW_THREADS), 0, st, p);
+    launch(dense_few_kernel<DT, 1, NF, U, WAVES, true>, grid, dim3(64 * WAVES), 0, st, p);
   else
-    launch(dense_few_kernel<DT, MT, NF, U, false>, grid, dim3(FEW_THREADS), 0, st, p);
+    launch(dense_few_kernel<DT, 1, NF, U, WAVES, false>, grid, dim3(64 * WAVES), 0, st, p);
 }
 
 template <int DT>
@@ -696,23 +936,26 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
   p.mtiles = (int)(p.offsets == nullptr ? cdiv(p.M, q.bm) : imin64(p.M, p.E + 1) + p.M / q.bm);
   p.splits = q.splits;
   p.kchunk = q.kchunk;
-  const int64_t grid = (int64_t)p.mtiles * p.ntiles * q.splits;
-  CCQ_REQUIRE(grid < 1 << 22, "%s: %lld tiles, too many for one launch", what, (long long)grid);
-  if (q.few) {
-    if (q.bm == 16)
-      launch_few<DT, 1, 2, 4>(p, st);
-    else if (q.bm == 32)
-      launch_few<DT, 2, 2, 4>(p, st);
-    else
-      launch_few<DT, 4, 4, 2>(p, st);
-    return launch_status(what);
+  const int64_t groups = (int64_t)p.mtiles * p.ntiles * q.splits;
+  CCQ_REQUIRE(groups < 1 << 22, "%s: %lld tiles, too many for one launch", what, (long long)groups);
+  const dim3 grid((uint32_t)groups);
+  if (q.kind == FEW) {
+    if (q.bn == 16) launch_few<DT, 1, 4, 8>(p, grid, st);
+    else if (q.bn == 32) launch_few<DT, 2, 4, 8>(p, grid, st);
+    else launch_few<DT, 4, 2, 4>(p, grid, st);
+  } else if (q.kind == MID) {
+    if (q.bm == 32) launch(dense_mid_kernel<DT, 32, 64, 4>, grid, dim3(256), 0, st, p);
+    else if (q.bm == 64) launch(dense_mid_kernel<DT, 64, 64, 4>, grid, dim3(256), 0, st, p);
+    else launch(dense_mid_kernel<DT, 128, 64, 3>, grid, dim3(256), 0, st, p);
+  } else if (q.kind == TILE) {
+    if (q.bm == 128) launch(dense_tile_kernel<DT, 128, 128, 2, 2>, grid, dim3(256), 0, st, p);
+    else if (q.bn == 192) launch(dense_tile_kernel<DT, 256, 192, 4, 2>, grid, dim3(512), 0, st, p);
+    else if (q.bn == 224) launch(dense_tile_kernel<DT, 256, 224, 4, 2>, grid, dim3(512), 0, st, p);
+    else launch(dense_tile_kernel<DT, 256, 256, 4, 2>, grid, dim3(512), 0, st, p);
+  } else {
+    if (q.bm == 64) launch(dense_ragged_kernel<DT, 64>, grid, dim3(256), 0, st, p);
+    else launch(dense_ragged_kernel<DT, 128>, grid, dim3(256), 0, st, p);
   }
-  if (q.bm == 256)
-    launch(dense_tile_kernel<DT, 256, 256, 4, 2>, dim3((uint32_t)grid), dim3(512), 0, st, p);
-  else if (q.dma)
-    launch(dense_tile_kernel<DT, 128, 128, 2, 2>, dim3((uint32_t)grid), dim3(256), 0, st, p);
-  else
-    launch(dense_ragged_kernel<DT>, dim3((uint32_t)grid), dim3(256), 0, st, p);
   if (int rc = launch_status(what)) return rc;
   if (p.part != nullptr) {
     launch(dense_join_kernel, dim3((uint32_t)grid_for(p.M * cdiv(p.N, 4), 256)), dim3(256), 0, st, p);
