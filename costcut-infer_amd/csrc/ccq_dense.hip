@@ -644,12 +644,37 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const Dense
   if (whole >= 2) wait_vmcnt<LX + LW>();
   else wait_vmcnt<0>();
   lds_barrier();
-#pragma unroll
-  for (int r = 0; r < NR; ++r) read(even, r, xat, wat + UNIT);
   constexpr std::integral_constant<int, 0> none{};
   constexpr std::integral_constant<int, 1> full{};
   constexpr std::integral_constant<int, 2> end{};
   int s = 0;
+  if (m0 >= w.t.rows) {
+    // a wave whose rows are all behind the tile's end only copies: the others of a short tile have the matrix units
+    // to themselves
+    for (; s + 1 < stages; ++s) {
+      const int nx = ring(ux + 2 * UNIT), free = ring(ux + 4 * UNIT);
+      if (s + 2 < whole)
+#pragma unroll
+        for (int i = 0; i < LX; ++i) copy_x(i, s + 2, free);
+      else if (s + 2 < stages)
+#pragma unroll
+        for (int i = 0; i < LX; ++i) last_x(i, free);
+      if (s + 2 < whole) wait_vmcnt<LX>();
+      else wait_vmcnt<0>();
+      lds_barrier();
+      if (s + 2 < whole)
+#pragma unroll
+        for (int i = 0; i < LW; ++i) copy_w(i, s + 2, ux);
+      else if (s + 2 < stages)
+#pragma unroll
+        for (int i = 0; i < LW; ++i) last_w(i, ux);
+      ux = nx;
+    }
+    __syncthreads();
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(even, r, xat, wat + UNIT);
   for (; s + 2 < whole; ++s) stage(full, std::true_type{}, s);
   if (s + 2 < stages) stage(end, std::true_type{}, s++);
   if (s + 1 < stages) stage(none, std::true_type{}, s++);
