@@ -139,6 +139,29 @@ __device__ __forceinline__ void dn_store4(int dt, void* p, int64_t i, int n, f32
   }
 }
 
+struct f32x8 {
+  f32x4 lo, hi;
+};
+__device__ __forceinline__ f32x8 dn_floats8(int dt, u32x4 b) {
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t u = (b[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+    (e < 4 ? v.lo : v.hi)[e & 3] = dt == CCQ_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+  }
+  return v;
+}
+__device__ __forceinline__ u32x4 dn_bits8(int dt, const f32x8& v) {
+  u32x4 b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f32x4& h = e < 2 ? v.lo : v.hi;
+    const float a = h[2 * (e & 1)], c = h[2 * (e & 1) + 1];
+    b[e] = dt == CCQ_BF16 ? bf16x2_bits(a, c) : f32_to_f16_bits(a) | f32_to_f16_bits(c) << 16;
+  }
+  return b;
+}
+
 // Four columns of y from column n on, of row `row`, from sums g (and u, the up
 // half of a gated pair); e: the rows' expert.
 __device__ __forceinline__ void dn_finish(const DenseP& p, int64_t row, int e, int n, f32x4 g, f32x4 u) {
@@ -411,33 +434,35 @@ __device__ __forceinline__ int64_t dn_wrow(const DenseP& p, int n0, int q) {
 
 // The sums of a wave's FN x FM groups to y, or to the splits' sums: group (i, j)
 // holds rows w0 + 16 i .. of the tile's w and row m0 + 16 j + lane % 16 of its x.
-// They go through the wave's own piece of LDS, 16 rows at a time, so that rows of y
-// are read and written in whole lines, a lane's columns and so its bias stay the
-// same, and the code stands here once, not once for each accumulator.
+// Bias, activation and gate are applied where the sums are; then 16 rows at a time
+// go through the wave's own piece of LDS, so that y and the residual are accessed
+// 16 bytes a lane in whole lines (8 bytes a lane in 16 rows at once take 4 to 7
+// times as long: 14000 cycles of a 256 x 256 tile).
 template <int FN>
 constexpr int kScratch = 16 * (4 * FN + 1) * 16;  // bytes; a row's 4 FN quads and one, so that 16 rows start in 16 banks
 constexpr int dn_pow2(int n) { return n <= 1 ? 1 : 2 * dn_pow2((n + 1) / 2); }
 
-template <int FM, int FN, class F>
-__device__ __forceinline__ void dn_rows(const f32x4 (&acc)[FN][FM], f32x4* own, F each) {
+// row group j to the wave's LDS, behind what was read there before: every group of columns, or every second one
+template <int FM, int FN, int EVERY>
+__device__ __forceinline__ void dn_dump(const f32x4 (&acc)[FN][FM], f32x4* own, int j) {
   const int lane = lane_id();
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < FM; ++j) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i) own[(lane & 15) * (4 * FN + 1) + 4 * i + (lane >> 4)] = acc[i][j];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    each(j);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
+  for (int i = 0; i < FN; i += EVERY) own[(lane & 15) * (4 * (FN / EVERY) + 1) + 4 * (i / EVERY) + (lane >> 4)] = acc[i][j];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-template <int G>
-__device__ __forceinline__ void dn_act_all(int act, f32x4 (&v)[G]) {
+template <int FM, int FN>
+__device__ __forceinline__ void dn_act_all(int act, int every, f32x4 (&acc)[FN][FM]) {
   auto all = [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < G; ++i)
+    for (int i = 0; i < FN; ++i) {
+      if (i % 2 && every == 2) continue;  // (the up half's)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][e] = dn_act(decltype(a)::value, v[i][e]);
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = dn_act(decltype(a)::value, acc[i][j][e]);
+    }
   };
   if (act == CCQ_ACT_SILU) all(std::integral_constant<int, CCQ_ACT_SILU>{});
   else if (act == CCQ_ACT_GELU) all(std::integral_constant<int, CCQ_ACT_GELU>{});
@@ -445,67 +470,116 @@ __device__ __forceinline__ void dn_act_all(int act, f32x4 (&v)[G]) {
   else if (act == CCQ_ACT_RELU) all(std::integral_constant<int, CCQ_ACT_RELU>{});
 }
 
-template <int FM, int FN, bool PAIRED>
+// y's rows from the wave's LDS; EVERY 2: the groups of columns that a gated product leaves
+template <int FM, int FN, int EVERY>
 __device__ __forceinline__ void dn_write_y(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
                                            f32x4* own) {
-  constexpr int QUADS = PAIRED ? 2 * FN : 4 * FN, SIDE = dn_pow2(QUADS), STEP = 64 / SIDE, LINE = 4 * FN + 1;
-  constexpr int G = STEP < 16 ? 2 : 1;  // rows of y at once
+  constexpr int GROUPS = FN / EVERY, OCTS = 2 * GROUPS, SIDE = dn_pow2(OCTS), LINE = 4 * GROUPS + 1;
+  constexpr int STEP = 64 / SIDE < 16 ? 64 / SIDE : 16, TURNS = 16 / STEP;  // rows of an access, accesses of 16 rows
   const int lane = lane_id(), c = lane & (SIDE - 1), r0 = lane / SIDE;
-  const int n = w.n0 + (PAIRED ? w0 / 2 : w0) + 4 * c;
-  const int left = c < QUADS ? p.N - n : 0;
-  f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = bg;
-  if (p.bias != nullptr && left > 0) {
-    const int64_t at = (int64_t)w.t.expert * p.W + n;
-    bg = dn_load4(p.bias_dtype, p.bias, at, left);
-    if (PAIRED) bu = dn_load4(p.bias_dtype, p.bias, at + p.N, left);
+  const int n = w.n0 + w0 / EVERY + 8 * c;
+  const int left = c < OCTS && r0 < 16 ? p.N - n : 0;
+  const f32x4* from = own + (r0 & 15) * LINE + 2 * c;
+  if (p.y_dtype != CCQ_F32 && (p.N % 8 == 0 || w.n0 + w0 / EVERY + 16 * GROUPS <= p.N)) {  // whole eights
+    // the residual two row groups ahead: turns that wait for their own cost a tile 16 us
+    constexpr int AHEAD = FM < 2 ? FM : 2;
+    u32x4 res[AHEAD][TURNS];
+    auto ask = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int row = m0 + 16 * j + r0 + i * STEP;
+        if (row < w.t.rows && left > 0)
+          __builtin_memcpy(&res[j % AHEAD][i], reinterpret_cast<const uint16_t*>(p.residual) + (w.t.row + row) * p.ldr + n, 16);
+      }
+    };
+    auto rows = [&](auto residual) {
+      constexpr bool RES = decltype(residual)::value;
+      if constexpr (RES) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) ask(j);
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        dn_dump<FM, FN, EVERY>(acc, own, j);
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+          const int row = m0 + 16 * j + r0 + i * STEP;
+          f32x8 v = {from[i * STEP * LINE], from[i * STEP * LINE + 1]};
+          if constexpr (RES) {
+            const f32x8 r = dn_floats8(p.y_dtype, res[j % AHEAD][i]);
+            v.lo += r.lo;
+            v.hi += r.hi;
+          }
+          const u32x4 bits = dn_bits8(p.y_dtype, v);
+          if (row < w.t.rows && left > 0)
+            __builtin_memcpy(reinterpret_cast<uint16_t*>(p.y) + (w.t.row + row) * p.ldy + n, &bits, 16);
+        }
+        if constexpr (RES) {
+          if (j + AHEAD < FM) ask(j + AHEAD);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if (p.residual != nullptr) rows(std::true_type{});
+    else rows(std::false_type{});
+    return;
   }
-  const f32x4* from = own + r0 * LINE + (PAIRED ? (c & 3) + 8 * (c >> 2) : c);
-  dn_rows<FM, FN>(acc, own, [&](int j) {
-    const int row0 = m0 + 16 * j + r0;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    dn_dump<FM, FN, EVERY>(acc, own, j);
 #pragma unroll 1
-    for (int i = 0; i < 16 / STEP; i += G) {
-      f32x4 g[G], r[G];
-#pragma unroll
-      for (int e = 0; e < G; ++e) {
-        const int row = row0 + (i + e) * STEP;
-        if (p.residual != nullptr && row < w.t.rows && left > 0)
-          r[e] = dn_load4(p.y_dtype, p.residual, (w.t.row + row) * p.ldr + n, left);
-        g[e] = from[(i + e) * STEP * LINE] + bg;
-      }
-      dn_act_all<G>(p.act, g);
-#pragma unroll
-      for (int e = 0; e < G; ++e) {
-        const int row = row0 + (i + e) * STEP;
-        if (PAIRED) g[e] *= from[(i + e) * STEP * LINE + 4] + bu;
-        if (row >= w.t.rows || left <= 0) continue;
-        if (p.residual != nullptr) g[e] += r[e];
-        dn_store4(p.y_dtype, p.y, (w.t.row + row) * p.ldy + n, left, g[e]);
-      }
+    for (int i = 0; i < 2 * TURNS; ++i) {
+      const int row = m0 + 16 * j + r0 + (i >> 1) * STEP, at = n + 4 * (i & 1), some = left - 4 * (i & 1);
+      if (row >= w.t.rows || some <= 0) continue;
+      f32x4 v = from[(i >> 1) * STEP * LINE + (i & 1)];
+      if (p.residual != nullptr) v += dn_load4(p.y_dtype, p.residual, (w.t.row + row) * p.ldr + at, some);
+      dn_store4(p.y_dtype, p.y, (w.t.row + row) * p.ldy + at, some, v);
     }
-  });
+  }
 }
 
 template <int FM, int FN>
-__device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int m0, int w0, const f32x4 (&acc)[FN][FM],
+__device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int m0, int w0, f32x4 (&acc)[FN][FM],
                                          char* scratch) {
   f32x4* own = reinterpret_cast<f32x4*>(scratch);
+  const int lane = lane_id();
   if (p.part != nullptr) {
     constexpr int QUADS = 4 * FN, SIDE = dn_pow2(QUADS), STEP = 64 / SIDE;
-    const int lane = lane_id(), c = lane & (SIDE - 1), r0 = lane / SIDE, q = w0 + 4 * c;
+    const int c = lane & (SIDE - 1), r0 = lane / SIDE, q = w0 + 4 * c;
     const int n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q), left = c < QUADS ? p.N - n : 0;
     float* part = p.part + ((int64_t)w.split * p.M + w.t.row) * p.W + n + (p.gated && q & 16 ? p.N : 0);
-    dn_rows<FM, FN>(acc, own, [&](int j) {
-#pragma unroll 1
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      dn_dump<FM, FN, 1>(acc, own, j);
+#pragma unroll 2
       for (int r = r0; r < 16; r += STEP) {
         const int row = m0 + 16 * j + r;
         if (row < w.t.rows && left > 0)
           dn_store4(CCQ_F32, part, (int64_t)row * p.W, left, own[r * (4 * FN + 1) + c]);
       }
-    });
-  } else if (p.gated) {
-    if constexpr (FN % 2 == 0) dn_write_y<FM, FN, true>(p, w, m0, w0, acc, own);
-  } else {
-    dn_write_y<FM, FN, false>(p, w, m0, w0, acc, own);
+    }
+    return;
+  }
+  const int every = p.gated ? 2 : 1;
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int q = w0 + 16 * i, n = w.n0 + (p.gated ? (q >> 5) * 16 : q) + 4 * (lane >> 4);
+      if (n >= p.N) continue;
+      const f32x4 b = dn_load4(p.bias_dtype, p.bias, (int64_t)w.t.expert * p.W + n + (p.gated && i % 2 ? p.N : 0), p.N - n);
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] += b;
+    }
+  }
+  dn_act_all<FM, FN>(p.act, every, acc);
+  if (!p.gated) {
+    dn_write_y<FM, FN, 1>(p, w, m0, w0, acc, own);
+  } else if constexpr (FN % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < FN; i += 2)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] *= acc[i + 1][j];
+    dn_write_y<FM, FN, 2>(p, w, m0, w0, acc, own);
   }
 }
 
