@@ -182,53 +182,59 @@ __device__ __forceinline__ void dn_finish(const DenseP& p, int64_t row, int e, i
 // ------------------------------------------------------- groups of rows --
 // Row tile `tile` of BM rows of the experts' groups one behind the other, each
 // padded to whole tiles, and behind them the rows of no expert (expert E).
-// pick(tiles) is called with their number and gives the tile.  Every wave
-// finds out by itself: lane l counts the experts from l PER on.
+// pick(tiles) is called with their number and gives the tile.  Every wave finds it
+// by itself, 256 experts at a time: lane l looks at the four experts l, l + 64, ..
 struct DnTile {
   int expert;      // E: rows of no expert; -1: no such tile
   int64_t row;     // first row
   int rows;
 };
 
-__device__ __forceinline__ int64_t dn_offset(const DenseP& p, int e) {
-  return e > p.E ? p.M : imin64(p.M, e < 0 ? 0 : p.offsets[e] < 0 ? 0 : (int64_t)p.offsets[e]);
-}
 template <int BM, class Pick>
 __device__ __forceinline__ DnTile dn_find_tile(const DenseP& p, Pick pick) {
-  const int lane = lane_id();
-  const int per = (p.E + 64) / 64, e0 = lane * per;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int e = e0 + i;
-    if (e > p.E) break;
-    const int64_t rows = dn_offset(p, e + 1) - dn_offset(p, e);
-    if (rows > 0) mine += (int)((rows + BM - 1) / BM);
-  }
-  int upto = mine;
+  constexpr int SETS = 4;
+  const int lane = lane_id(), M = (int)p.M;
+  int first[SETS], rows[SETS], tiles[SETS], upto[SETS], all[SETS];
+  auto look = [&](int base) {
+    int next[SETS];
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(upto, m, 64);
-    upto += lane >= m ? o : 0;
-  }
-  const int total = __builtin_amdgcn_readlane(upto, 63);
-  const int tile = pick(total);
-  DnTile t = {-1, 0, 0};
-  if (tile < 0 || tile >= total) return t;
-  const uint64_t has = __ballot(tile < upto);
-  const int l = __builtin_ctzll(has);  // the first lane whose experts reach the tile
-  int at = tile - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
-  for (int i = 0; i < per; ++i) {
-    const int e = l * per + i;
-    if (e > p.E) break;
-    const int64_t first = dn_offset(p, e), rows = dn_offset(p, e + 1) - first;
-    const int n = rows > 0 ? (int)((rows + BM - 1) / BM) : 0;
-    if (at < n) {
-      t.expert = e;
-      t.row = first + (int64_t)at * BM;
-      t.rows = (int)imin64(BM, rows - (int64_t)at * BM);
-      return t;
+    for (int c = 0; c < SETS; ++c) {  // (all of the loads at once)
+      const int e = base + 64 * c + lane;
+      first[c] = p.offsets[min(e, p.E)];
+      next[c] = p.offsets[min(e + 1, p.E)];
     }
-    at -= n;
+    int sum = 0;
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+      const int e = base + 64 * c + lane;
+      first[c] = min(max(first[c], 0), M);
+      rows[c] = e > p.E ? 0 : (e == p.E ? M : min(max(next[c], 0), M)) - first[c];
+      tiles[c] = rows[c] > 0 ? (rows[c] + BM - 1) / BM : 0;
+      upto[c] = wave_scan(tiles[c]);
+      all[c] = __builtin_amdgcn_readlane(upto[c], 63);
+      sum += all[c];
+    }
+    return sum;
+  };
+  int total = look(0);
+  for (int base = 64 * SETS; base <= p.E; base += 64 * SETS) total += look(base);
+  int at = pick(total);
+  DnTile t = {-1, 0, 0};
+  if (at < 0 || at >= total) return t;
+  for (int base = 0; base <= p.E; base += 64 * SETS) {
+    if (p.E >= 64 * SETS) look(base);
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+      if (t.expert < 0 && at < all[c]) {
+        const int l = __builtin_ctzll(__ballot(at < upto[c]));  // the first lane whose experts reach the tile
+        at -= __builtin_amdgcn_readlane(upto[c], l) - __builtin_amdgcn_readlane(tiles[c], l);
+        t.expert = base + 64 * c + l;
+        t.row = __builtin_amdgcn_readlane(first[c], l) + (int64_t)at * BM;
+        t.rows = min(BM, __builtin_amdgcn_readlane(rows[c], l) - at * BM);
+      }
+      at -= all[c];
+    }
+    if (t.expert >= 0) break;
   }
   return t;
 }

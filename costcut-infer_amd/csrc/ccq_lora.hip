@@ -134,18 +134,6 @@ __device__ __forceinline__ int lr_rank(const LoraP& p, int adapter) {
   return p.rank != nullptr ? min(max(p.rank[adapter], 0), p.R) : p.R;
 }
 
-// inclusive sum over the lanes up to this one: within rows of 16 lanes, then
-// the rows' last lanes carried on
-__device__ __forceinline__ int lr_wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
 // -------------------------------------------------------------- the tile --
 // Tile `tile` of the tokens sorted by adapter (tokens in order within one),
 // each adapter's run padded to whole tiles of TM: its adapter (-1: there is no
@@ -187,7 +175,7 @@ __device__ void lr_find_tile(const LoraP& p, Pick pick, TileS<TM>& t, SortS& s) 
   // tiles before an adapter: each thread takes two neighbouring adapters
   const int n0 = 2 * tid < p.L ? (s.count[2 * tid] + TM - 1) / TM : 0;
   const int n1 = 2 * tid + 1 < p.L ? (s.count[2 * tid + 1] + TM - 1) / TM : 0;
-  int sum = lr_wave_scan(n0 + n1);
+  int sum = wave_scan(n0 + n1);
   if (lane == 63) s.sum[wave] = sum;
   __syncthreads();
 #pragma unroll
@@ -242,7 +230,7 @@ __device__ __forceinline__ int lr_find_tile_wave(const LoraP& p, int tile, int& 
   if (__ballot(n > 1) == 0) {
     start = __popcll(__ballot(head) & ((1ull << lane) - 1));
   } else {
-    start = lr_wave_scan(n) - n;
+    start = wave_scan(n) - n;
   }
   const uint64_t hit = __ballot(head && tile >= start && tile < start + n);
   adapter = -1;

@@ -48,17 +48,6 @@ __device__ __forceinline__ uint32_t pm_key(const PermP& p, int a) {
   return id >= 0 && id < p.E ? (uint32_t)id : (uint32_t)p.E;
 }
 
-// inclusive sum over the lanes up to this one
-__device__ __forceinline__ int pm_scan(int v) {
-  const int lane = lane_id();
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(v, m, 64);
-    v += lane >= m ? o : 0;
-  }
-  return v;
-}
-
 // s.total (counts by key) -> s.start (rows before a key), by all threads
 struct PermS {
   int total[PM_MAX_E + 1], start[PM_MAX_E + 1], before[PM_MAX_E + 1];
@@ -76,7 +65,7 @@ __device__ __forceinline__ void pm_starts(const PermP& p, PermS& s) {
     v[i] = e <= p.E ? s.total[e] : 0;
     sum += v[i];
   }
-  int at = pm_scan(sum);
+  int at = wave_scan(sum);
   if (lane == 63) s.sum[wave] = at;
   __syncthreads();
   at -= sum;
