@@ -32,11 +32,12 @@ struct DenseP {
   const void* bias;       // or null
   const void* residual;   // or null
   void* y;
-  float* part;            // [splits][M][W] sums of K's splits, or null
+  float* part;            // [splits][M][P] sums of K's splits, or null
   const int32_t* offsets; // grouped, or null
   int64_t ldx, ldr, ldy;
   int64_t M;              // rows in all
   int K, N, W;            // W: rows of w, N or 2N
+  int half, P;            // columns of a row of part: N (gated: of each half), to whole quads, in all
   int E;
   int gated, act, bias_dtype, y_dtype;
   int mtiles, ntiles;     // most row tiles, column tiles
@@ -552,16 +553,17 @@ __device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int 
   if (p.part != nullptr) {
     constexpr int QUADS = 4 * FN, SIDE = dn_pow2(QUADS), STEP = 64 / SIDE;
     const int c = lane & (SIDE - 1), r0 = lane / SIDE, q = w0 + 4 * c;
-    const int n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q), left = c < QUADS ? p.N - n : 0;
-    float* part = p.part + ((int64_t)w.split * p.M + w.t.row) * p.W + n + (p.gated && q & 16 ? p.N : 0);
+    const int n = w.n0 + (p.gated ? (q >> 5) * 16 + (q & 15) : q);
+    const bool own_columns = c < QUADS && n < p.half;
+    float* part = p.part + ((int64_t)w.split * p.M + w.t.row) * p.P + n + (p.gated && q & 16 ? p.half : 0);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       dn_dump<FM, FN, 1>(acc, own, j);
 #pragma unroll 2
       for (int r = r0; r < 16; r += STEP) {
         const int row = m0 + 16 * j + r;
-        if (row < w.t.rows && left > 0)
-          dn_store4(CCQ_F32, part, (int64_t)row * p.W, left, own[r * (4 * FN + 1) + c]);
+        if (row < w.t.rows && own_columns)
+          *reinterpret_cast<f32x4*>(part + (int64_t)row * p.P) = own[r * (4 * FN + 1) + c];
       }
     }
     return;
@@ -845,9 +847,9 @@ __global__ __launch_bounds__(256) void dense_mid_kernel(const DenseP p) {
   dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
-// The same product for rows at any alignment: stages pass through registers, two of
+// The same product for rows at any alignment: stages pass through registers, AHEAD of
 // them on their way there, into two in LDS.
-template <int DT, int B>
+template <int DT, int B, int AHEAD>
 __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
   constexpr int WAVES = 4, TM = B / 2, FM = TM / 16, FN = FM, LOADS = B / 8 / WAVES, UNIT = B * 128;
@@ -898,7 +900,8 @@ __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
       }
     }
   };
-  auto turn = [&](Stage& v, int s, char* buffer) {  // v: stage s, then stage s + 2
+  auto turn = [&](Stage& v, int s) {  // v: stage s, then stage s + AHEAD
+    char* buffer = lds + (s & 1) * 2 * UNIT;
     char* to = buffer + wave * 1024 + lane * 16;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -906,7 +909,7 @@ __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
       *reinterpret_cast<u32x4*>(to + UNIT + i * WAVES * 1024) = v.w[i];
     }
     lds_barrier();  // (all waves have multiplied stage s - 1, so stage s + 1 may take its buffer)
-    load(v, s + 2);
+    load(v, s + AHEAD);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       Vec xf[FM], wf[FN];
@@ -920,31 +923,42 @@ __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
         for (int j = 0; j < FM; ++j) acc[i][j] = dn_mfma(wf[i], xf[j], acc[i][j]);
     }
   };
-  Stage even, odd;
-  load(even, 0);
-  load(odd, 1);
-  for (int s = 0; s < stages; s += 2) {
-    turn(even, s, lds);
-    if (s + 1 < stages) turn(odd, s + 1, lds + 2 * UNIT);
-  }
+  Stage v[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(v[i], i);
+  for (int s = 0; s < stages; s += AHEAD)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (s + i < stages) turn(v[i], s + i);
   __syncthreads();
   dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
-// The splits' sums added in order, and the epilogue.
+// The splits' sums added in order, four of them on their way at once, and the
+// epilogue.
 __global__ __launch_bounds__(256) void dense_join_kernel(const DenseP p) {
-  const int quads = (p.N + 3) / 4;
-  const int64_t total = p.M * quads;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / quads;
-    const int n = (int)(i % quads) * 4;
+  const int quads = p.half / 4, total = (int)p.M * quads;
+  const int64_t split = p.M * p.P / 4;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const int row = i / quads, c = i - row * quads;
+    const f32x4* part = reinterpret_cast<const f32x4*>(p.part) + (int64_t)row * (p.P / 4) + c;
     f32x4 g = {0.f, 0.f, 0.f, 0.f}, u = g;
-    for (int s = 0; s < p.splits; ++s) {
-      const float* part = p.part + ((int64_t)s * p.M + row) * p.W;
-      g += dn_load4(CCQ_F32, part, n, p.N - n);
-      if (p.gated) u += dn_load4(CCQ_F32, part, n + p.N, p.N - n);
+    for (int s = 0; s < p.splits; s += 4, part += 4 * split) {
+      f32x4 a[4], b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s + k < p.splits) {
+          a[k] = part[k * split];
+          if (p.gated) b[k] = part[k * split + quads];
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s + k < p.splits) {
+          g += a[k];
+          if (p.gated) u += b[k];
+        }
     }
-    dn_finish(p, row, 0, n, g, u);
+    dn_finish(p, row, 0, 4 * c, g, u);
   }
 }
 
@@ -1058,12 +1072,12 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
     else if (q.bn == 224) launch(dense_tile_kernel<DT, 256, 224, 4, 2>, grid, dim3(512), 0, st, p);
     else launch(dense_tile_kernel<DT, 256, 256, 4, 2>, grid, dim3(512), 0, st, p);
   } else {
-    if (q.bm == 64) launch(dense_ragged_kernel<DT, 64>, grid, dim3(256), 0, st, p);
-    else launch(dense_ragged_kernel<DT, 128>, grid, dim3(256), 0, st, p);
+    if (q.bm == 64) launch(dense_ragged_kernel<DT, 64, 4>, grid, dim3(256), 0, st, p);
+    else launch(dense_ragged_kernel<DT, 128, 2>, grid, dim3(256), 0, st, p);
   }
   if (int rc = launch_status(what)) return rc;
   if (p.part != nullptr) {
-    launch(dense_join_kernel, dim3((uint32_t)grid_for(p.M * cdiv(p.N, 4), 256)), dim3(256), 0, st, p);
+    launch(dense_join_kernel, dim3((uint32_t)grid_for(p.M * p.half / 4, 256)), dim3(256), 0, st, p);
     return launch_status(what);
   }
   return 0;
@@ -1096,6 +1110,7 @@ DenseP make_params(const ccq_dense_args& a, bool grouped) {
   p.offsets = grouped ? a.offsets : nullptr;
   p.ldx = a.ldx, p.ldr = a.ldr, p.ldy = a.ldy, p.M = a.M;
   p.K = (int)a.K, p.N = (int)a.N, p.W = (int)(a.gated ? 2 * a.N : a.N);
+  p.half = (int)(cdiv(a.N, 4) * 4), p.P = a.gated ? 2 * p.half : p.half;
   p.E = grouped ? (int)a.num_experts : 1;  // (a batch's one "expert" is 0)
   p.gated = a.gated != 0, p.act = a.act, p.bias_dtype = a.bias_dtype, p.y_dtype = a.y_dtype;
   return p;
@@ -1118,7 +1133,7 @@ int run_dense(const char* what, const ccq_dense_args& a, bool grouped) {
   DenseP p = make_params(a, grouped);
   const Plan q = plan_of(a, p);
   if (q.splits > 1) {
-    const size_t need = (size_t)q.splits * p.M * p.W * 4;
+    const size_t need = (size_t)q.splits * p.M * p.P * 4;
     CCQ_REQUIRE(a.workspace != nullptr && aligned(a.workspace, 16) && a.workspace_bytes >= need,
                 "%s: workspace of %zu bytes needed", what, need);
     p.part = reinterpret_cast<float*>(a.workspace);
@@ -1137,7 +1152,7 @@ extern "C" size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args) {
   if (args == nullptr || args->M < 1 || check_dense("ccq_dense_linear", *args, false)) return 0;
   const DenseP p = make_params(*args, false);
   const Plan q = plan_of(*args, p);
-  return q.splits > 1 ? (size_t)q.splits * p.M * p.W * 4 : 0;
+  return q.splits > 1 ? (size_t)q.splits * p.M * p.P * 4 : 0;
 }
 
 extern "C" int ccq_dense_linear(const ccq_dense_args* args) {
