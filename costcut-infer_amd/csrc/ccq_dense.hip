@@ -12,8 +12,9 @@
 //
 // dense_few_kernel   up to 16 rows: w goes from memory to registers, the waves of a
 //                    workgroup share K and add up at the end.
-// dense_mid_kernel   small tiles of rows and columns through a ring of stages in LDS.
+// dense_mid_kernel   up to 32 rows, through a ring of stages in LDS.
 // dense_tile_kernel  large tiles, the products interleaved with the next ones' reads.
+// dense_ring_kernel  smaller ones, more stages on their way.
 // dense_ragged_kernel  rows at any alignment.
 #include "ccq_common.h"
 
@@ -765,9 +766,123 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const Dense
   dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
-// Batches between: what bounds them is w's way from memory, so small tiles, K split
-// over workgroups, and a ring of D stages of 64 columns that are on their way while
-// one is multiplied.  Four waves, 2 x 2.
+// Smaller tiles of the same form, with A whole stages on their way: they are
+// multiplied in a fraction of the time that a stage takes from memory, and what
+// counts is that every CU has one.  A stage's operands are read half by half while
+// the half before is multiplied; the barrier stands between the halves as above.
+// One workgroup a CU, K=4096: 64 x 64 0.31 us a stage, 128 x 128 0.41 to 0.47 (in the
+// form above, which leaves room for two: 0.50 to 0.72), 256 x 128 0.7 to 0.9.
+template <int DT, int BM, int BN, int WM, int WN, int A>
+__global__ __launch_bounds__(64 * WM * WN, 2) void dense_ring_kernel(const DenseP p) {
+  using Vec = typename DnVec<DT>::type;
+  constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  constexpr int LX = BM / (8 * WAVES), LW = BN / (8 * WAVES), LOADS = LX + LW, STAGE = (BM + BN) * 128, D = A + 1;
+  constexpr int NM = FM * FN, NR = FM + FN;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole copies");
+  __shared__ __align__(16) char lds[D * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int columns = p.gated ? BN / 2 : BN;
+  const DnPlace w = dn_place<BM>(p, columns);
+  if (w.t.expert < 0) return;
+  if (w.t.expert == p.E) {
+    dn_zero(p, w.t, w.n0, columns, 64 * WAVES);
+    return;
+  }
+  const int kfrom = w.split * p.kchunk, klen = min(p.K, kfrom + p.kchunk) - kfrom;
+  const int stages = (klen + DN_BK - 1) / DN_BK, whole = klen / DN_BK;
+  const uint16_t* xb = reinterpret_cast<const uint16_t*>(p.x) + w.t.row * p.ldx + kfrom;
+  const uint16_t* wb = reinterpret_cast<const uint16_t*>(p.w) + ((int64_t)w.t.expert * p.W + w.n0) * p.K + kfrom;
+  const int piece = (lane & 7) ^ (lane >> 3);
+  uint32_t xo[LX], wo[LW];
+#pragma unroll
+  for (int i = 0; i < LX; ++i)
+    xo[i] = (uint32_t)(2 * (min(8 * (wave + WAVES * i) + (lane >> 3), w.t.rows - 1) * p.ldx + 8 * piece));
+#pragma unroll
+  for (int i = 0; i < LW; ++i) wo[i] = (uint32_t)(2 * (dn_wrow(p, w.n0, 8 * (wave + WAVES * i) + (lane >> 3)) * p.K + 8 * piece));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(&lds[0])) + wave * 1024;
+  auto copy = [&](int i, int s, int slot) {
+    if (i < LW) dma16(wb + s * DN_BK, wo[i < LW ? i : 0], lds0 + slot + (BM / 8 + i * WAVES) * 1024);
+    else dma16(xb + s * DN_BK, xo[i < LW ? 0 : i - LW], lds0 + slot + (i - LW) * WAVES * 1024);
+  };
+  auto copy_last = [&](int slot) {  // K ends inside: zeros from there on, in both operands
+    const bool valid = (stages - 1) * DN_BK + 8 * piece < klen;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if (valid)
+        copy(i, stages - 1, slot);
+      else
+        *reinterpret_cast<u32x4*>(&lds[slot + (wave + (i < LW ? BM / 8 + i * WAVES : (i - LW) * WAVES)) * 1024 + lane * 16]) =
+            u32x4{0, 0, 0, 0};
+    }
+  };
+  f32x4 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Half {
+    Vec x[FM], w[FN];
+  };
+  Half even, odd;
+  const int m0 = wave / WN * TM, w0 = wave % WN * TN;
+  const uint32_t swz = ((lane >> 4) ^ (lane & 7)) * 16;
+  const uint32_t xat = (m0 + (lane & 15)) * 128 + swz, wat = (BM + w0 + (lane & 15)) * 128 + swz;
+  auto read = [&](Half& h, int r, int slot, uint32_t half) {
+    if (r == 0)
+      h.w[0] = *reinterpret_cast<const Vec*>(&lds[slot + (wat ^ half)]);
+    else if (r <= FM)
+      h.x[r - 1] = *reinterpret_cast<const Vec*>(&lds[slot + (xat ^ half) + (r - 1) * 2048]);
+    else
+      h.w[r - FM] = *reinterpret_cast<const Vec*>(&lds[slot + (wat ^ half) + (r - FM) * 2048]);
+  };
+#pragma unroll
+  for (int s = 0; s < D; ++s) {
+    if (s < whole) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) copy(i, s, s * STAGE);
+    } else if (s < stages) {
+      copy_last(s * STAGE);
+    }
+  }
+  if (stages >= D) wait_vmcnt<A * LOADS>();
+  else wait_vmcnt<0>();
+  lds_barrier();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(even, r, 0, 0);
+  int slot = 0;
+  for (int s = 0; s < stages; ++s) {
+    const int next = slot + STAGE == D * STAGE ? 0 : slot + STAGE;
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+#pragma unroll
+      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read(odd, r, slot, 64);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[q / FM][q % FM] = dn_mfma(even.w[q / FM], even.x[q % FM], acc[q / FM][q % FM]);
+    }
+    if (s + A < stages) wait_vmcnt<(A - 1) * LOADS>();  // stage s + 1 is there; those behind it may be on their way
+    else wait_vmcnt<0>();
+    lds_barrier();
+    const bool more = s + D < whole;
+    if (!more && s + D < stages) copy_last(slot);
+#pragma unroll
+    for (int q = 0; q < NM; ++q) {
+#pragma unroll
+      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read(even, r, next, 0);  // (behind the last stage: not used)
+#pragma unroll
+      for (int i = q * LOADS / NM; i < (q + 1) * LOADS / NM; ++i)
+        if (more) copy(i, s + D, slot);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[q / FM][q % FM] = dn_mfma(odd.w[q / FM], odd.x[q % FM], acc[q / FM][q % FM]);
+    }
+    slot = next;
+  }
+  __syncthreads();  // (the waves' scratch lies in the ring)
+  dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
+}
+
+// 32 rows: w's way from memory bounds them, so a simple loop, K split over
+// workgroups, and a ring of D stages that are on their way while one is multiplied.
+// Four waves, 2 x 2.
 template <int DT, int BM, int BN, int D>
 __global__ __launch_bounds__(256) void dense_mid_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
@@ -963,7 +1078,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const DenseP p) {
 }
 
 // ------------------------------------------------------------- dispatch --
-enum Kind { FEW, MID, TILE, RAGGED };
+enum Kind { FEW, MID, RING, TILE, RAGGED };
 
 struct Plan {
   Kind kind;
@@ -972,19 +1087,20 @@ struct Plan {
 };
 
 // What a stage of 64 columns takes in us, with up to one and two workgroups on a
-// CU, and what a tile takes besides.  From K = 4096 and 2048 over M = 32 .. 2048,
-// N = 2048 .. 14336 (M=256 K=N=4096: MID 64 x 64 in 2 splits 19.6 us, TILE 128 in 4
-// 20.0, in one 35.1; M=512: 23.9 at best, 27.4, 36.1; M=512 N=14336: MID 117, TILE
-// 128 75.5, 256 x 192 74.0, 256 86.0; M=1024: TILE 128 138, 256 96.5).
+// CU (0: there is room for one), and what a tile takes besides.  From K = 4096 and
+// 2048 over M = 32 .. 2048, N = 2048 .. 14336 (K=N=4096: M=256 RING 64 22.4 us, 128 29.5,
+// TILE 128 33.5; M=1024 52, 34, 36, RING 256 x 128 49; K=4096 N=14336: M=512 RING 256 x
+// 128 63, TILE 128 74.6, 256 x 192 74, 256 81; M=1024 TILE 128 138, 256 96.5).
 struct Shape {
   Kind kind;
   int bm, bn;
   float one, two, tile;
 };
 constexpr Shape kShapes[] = {
-    {MID, 32, 64, 0.25f, 0.40f, 2.f},   {MID, 64, 64, 0.33f, 0.50f, 2.f},   {MID, 128, 64, 0.50f, 0.76f, 2.f},
-    {TILE, 128, 128, 0.72f, 1.05f, 5.f}, {TILE, 256, 192, 1.05f, 0.f, 6.f}, {TILE, 256, 224, 1.32f, 0.f, 7.f},
-    {TILE, 256, 256, 1.45f, 0.f, 8.f},   {RAGGED, 64, 64, 0.6f, 0.9f, 3.f}, {RAGGED, 128, 128, 1.2f, 1.7f, 5.f},
+    {MID, 32, 64, 0.25f, 0.40f, 2.f},    {RING, 64, 64, 0.31f, 0.39f, 2.5f},   {RING, 128, 128, 0.46f, 0.f, 4.f},
+    {RING, 256, 128, 0.90f, 0.f, 5.f},   {TILE, 128, 128, 0.72f, 0.97f, 5.f},  {TILE, 256, 192, 1.05f, 0.f, 6.f},
+    {TILE, 256, 224, 1.30f, 0.f, 6.f},   {TILE, 256, 256, 1.42f, 0.f, 7.f},    {RAGGED, 64, 64, 0.6f, 0.9f, 3.f},
+    {RAGGED, 128, 128, 1.2f, 1.7f, 5.f},
 };
 
 float shape_time(const Shape& s, const DenseP& p, int splits) {
@@ -1007,7 +1123,7 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma) {
     // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 140
     // us, MID 64: 146; 1 to 6 rows as FEW), 64 up to 48 (32 skewed rows: 161, MID 32: 169; 64 rows: TILE 128 168, MID 64
     // 180), TILE 256 from 200 on (256 rows: 238, TILE 128: 275; 128 rows: 216 and 186)
-    q.kind = !dma ? RAGGED : rows <= 48 ? MID : TILE;
+    q.kind = !dma ? RAGGED : rows <= 24 ? MID : rows <= 48 ? RING : TILE;
     q.bm = !dma ? (rows <= 64 ? 64 : 128) : rows <= 24 ? 32 : rows <= 48 ? 64 : rows < 200 ? 128 : 256;
     q.bn = q.kind == MID ? 64 : q.bm;
     return q;
@@ -1063,9 +1179,11 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
     else if (q.bn == 32) launch_few<DT, 2, 4, 8>(p, grid, st);
     else launch_few<DT, 4, 2, 4>(p, grid, st);
   } else if (q.kind == MID) {
-    if (q.bm == 32) launch(dense_mid_kernel<DT, 32, 64, 4>, grid, dim3(256), 0, st, p);
-    else if (q.bm == 64) launch(dense_mid_kernel<DT, 64, 64, 4>, grid, dim3(256), 0, st, p);
-    else launch(dense_mid_kernel<DT, 128, 64, 3>, grid, dim3(256), 0, st, p);
+    launch(dense_mid_kernel<DT, 32, 64, 4>, grid, dim3(256), 0, st, p);
+  } else if (q.kind == RING) {
+    if (q.bm == 64) launch(dense_ring_kernel<DT, 64, 64, 2, 2, 3>, grid, dim3(256), 0, st, p);
+    else if (q.bm == 128) launch(dense_ring_kernel<DT, 128, 128, 2, 4, 2>, grid, dim3(512), 0, st, p);
+    else launch(dense_ring_kernel<DT, 256, 128, 4, 2, 2>, grid, dim3(512), 0, st, p);
   } else if (q.kind == TILE) {
     if (q.bm == 128) launch(dense_tile_kernel<DT, 128, 128, 2, 2>, grid, dim3(256), 0, st, p);
     else if (q.bn == 192) launch(dense_tile_kernel<DT, 256, 192, 4, 2>, grid, dim3(512), 0, st, p);
