@@ -173,6 +173,7 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_moe_unpermute": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
     "ccq_moe_unpermute_grad": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "ccq_dense_linear_workspace_size": (_sz, [ctypes.c_char_p]),  # DENSE_ARGS.pack(...)
+    "ccq_dense_linear_grouped_workspace_size": (_sz, [ctypes.c_char_p]),
     "ccq_dense_linear": (_int, [ctypes.c_char_p]),
     "ccq_dense_linear_grouped": (_int, [ctypes.c_char_p]),
 }

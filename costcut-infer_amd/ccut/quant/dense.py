@@ -23,8 +23,8 @@ __all__ = ["linear", "linear_grouped"]
 _HALF = (torch.bfloat16, torch.float16)
 _pack = DENSE_ARGS.pack
 MAX_ROWS, MAX_SIDE, MAX_EXPERTS = 1 << 20, 1 << 20, 1024
-# batches above this many rows may split K over workgroups and need scratch for the partial sums
-_UNSPLIT_ROWS = 16
+# batches of up to this many rows take no scratch
+_BARE_ROWS = 16
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -118,18 +118,20 @@ def _dense(x, offsets, w, bias, act, gated: bool, residual, out, out_dtype):
     if M == 0:
         return out
     handle = lib()
-    tail = (ldx, ldr, ldy, M, K, N, E, DTYPE_CODE[dtype], bcode, ycode, code, gated)
-    wp, op, stream = w.data_ptr(), 0, raw_stream(index)
+    wp, op = w.data_ptr(), 0
+    run, size = handle.ccq_dense_linear, handle.ccq_dense_linear_workspace_size
+    scratch = M > _BARE_ROWS
     if offsets is not None:
-        rc = handle.ccq_dense_linear_grouped(_pack(xp, wp, bp, rp, yp, offsets.data_ptr(), 0, stream, 0, *tail))
-    else:
-        sp = nbytes = 0
-        if M > _UNSPLIT_ROWS:
-            nbytes = handle.ccq_dense_linear_workspace_size(_pack(xp, wp, bp, rp, yp, op, 0, stream, 0, *tail))
-            if nbytes:  # this call's own, so that calls on several streams or in several graphs do not share it
-                scratch = empty_strided((nbytes,), (1,), torch.uint8)
-                sp = scratch.data_ptr()
-        rc = handle.ccq_dense_linear(_pack(xp, wp, bp, rp, yp, op, sp, stream, nbytes, *tail))
+        op, run, size = offsets.data_ptr(), handle.ccq_dense_linear_grouped, handle.ccq_dense_linear_grouped_workspace_size
+        scratch = (K | ldx) & 7 or (xp | wp) & 15  # (aligned groups take none)
+    sp = nbytes = 0
+    tail = (ldx, ldr, ldy, M, K, N, E, DTYPE_CODE[dtype], bcode, ycode, code, gated)
+    if scratch:
+        nbytes = size(_pack(xp, wp, bp, rp, yp, op, 0, 0, 0, *tail))
+        if nbytes:  # this call's own, so that calls on several streams or in several graphs do not share it
+            scratch = empty_strided((nbytes,), (1,), torch.uint8)
+            sp = scratch.data_ptr()
+    rc = run(_pack(xp, wp, bp, rp, yp, op, sp, raw_stream(index), nbytes, *tail))
     if rc:
         check(rc, "ccq_dense_linear" if offsets is None else "ccq_dense_linear_grouped")
     return out

@@ -962,12 +962,14 @@ __global__ __launch_bounds__(256) void dense_mid_kernel(const DenseP p) {
   dn_write<FM, FN>(p, w, m0, w0, acc, &lds[wave * kScratch<FN>]);
 }
 
-// The same product for rows at any alignment: stages pass through registers, AHEAD of
-// them on their way there, into two in LDS.
-template <int DT, int B, int AHEAD>
+// The same product for rows at any alignment: stages pass through registers, four of
+// them on their way there, into two in LDS.  Unaligned loads of 16 bytes cost a third
+// (K=2747 for 2752: 39 and 28 us at M=1274 N=1520), the registers the rest (RING 64: 20);
+// tiles of 128 are no faster (58).
+template <int DT>
 __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
-  constexpr int WAVES = 4, TM = B / 2, FM = TM / 16, FN = FM, LOADS = B / 8 / WAVES, UNIT = B * 128;
+  constexpr int B = 64, AHEAD = 4, WAVES = 4, TM = B / 2, FM = TM / 16, FN = FM, LOADS = B / 8 / WAVES, UNIT = B * 128;
   __shared__ __align__(16) char lds[2 * 2 * UNIT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int columns = p.gated ? B / 2 : B;
@@ -1077,6 +1079,26 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const DenseP p) {
   }
 }
 
+// Rows of x and w with K to whole pieces of 8 and zeros behind it, at aligned
+// addresses: what makes an unaligned product one for the kernels with LDS copies
+// (M=6628 K=657 N=2x1735 105 us on unaligned rows, 45 on aligned ones, the copy 6).
+struct PadP {
+  const uint16_t* from[2];
+  uint16_t* to[2];
+  int64_t rows[2], ld[2];  // rows 0: used as they are
+  int K, Kp;
+};
+__global__ __launch_bounds__(256) void dense_pad_kernel(const PadP p) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < p.rows[0] + p.rows[1]; r += (int64_t)gridDim.x * 4) {
+    const int which = r >= p.rows[0];
+    const int64_t row = which ? r - p.rows[0] : r;
+    const uint16_t* from = p.from[which] + row * p.ld[which];
+    uint16_t* to = p.to[which] + row * p.Kp;
+    for (int k = 8 * lane; k < p.Kp; k += 512) *reinterpret_cast<u32x4*>(to + k) = dn_load8<false>(from, k, p.K);
+  }
+}
+
 // ------------------------------------------------------------- dispatch --
 enum Kind { FEW, MID, RING, TILE, RAGGED };
 
@@ -1084,6 +1106,7 @@ struct Plan {
   Kind kind;
   int bm, bn;       // of the tile; FEW: 16 rows, 16 NF columns
   int splits, kchunk;
+  bool pad;         // x and w are copied to aligned rows first
 };
 
 // What a stage of 64 columns takes in us, with up to one and two workgroups on a
@@ -1099,13 +1122,12 @@ struct Shape {
 constexpr Shape kShapes[] = {
     {MID, 32, 64, 0.25f, 0.40f, 2.f},    {RING, 64, 64, 0.31f, 0.39f, 2.5f},   {RING, 128, 128, 0.46f, 0.f, 4.f},
     {RING, 256, 128, 0.90f, 0.f, 5.f},   {TILE, 128, 128, 0.72f, 0.97f, 5.f},  {TILE, 256, 192, 1.05f, 0.f, 6.f},
-    {TILE, 256, 224, 1.30f, 0.f, 6.f},   {TILE, 256, 256, 1.42f, 0.f, 7.f},    {RAGGED, 64, 64, 0.6f, 0.9f, 3.f},
-    {RAGGED, 128, 128, 1.2f, 1.7f, 5.f},
+    {TILE, 256, 224, 1.30f, 0.f, 6.f},   {TILE, 256, 256, 1.42f, 0.f, 7.f},    {RAGGED, 64, 64, 0.6f, 0.65f, 3.f},
 };
 
-float shape_time(const Shape& s, const DenseP& p, int splits) {
+float shape_time(const Shape& s, const DenseP& p, int64_t mtiles, int splits) {
   const int64_t stages = cdiv(cdiv(p.K, DN_BK), splits);
-  const int64_t groups = cdiv(p.M, s.bm) * cdiv(p.W, s.bn) * splits, round = s.two > 0.f ? 512 : 256;
+  const int64_t groups = mtiles * cdiv(p.W, s.bn) * splits, round = s.two > 0.f ? 512 : 256;
   const float full = s.two > 0.f ? s.two : s.one;
   const int64_t rest = groups % round;
   float t = (float)(groups / round) * (stages * full + s.tile);
@@ -1115,17 +1137,33 @@ float shape_time(const Shape& s, const DenseP& p, int splits) {
   return t;
 }
 
-// rows: of the batch, or of an expert on average
-Plan make_plan(const DenseP& p, int64_t rows, bool dma) {
-  Plan q = {FEW, 16, 16, 1, p.K};
+// rows: of the batch, or of an expert on average; dma: x and w are aligned; can_pad: they can be made so
+Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
+  Plan q = {FEW, 16, 16, 1, p.K, false};
   const bool grouped = p.offsets != nullptr;
-  if (grouped && (dma || rows > 16)) {
-    // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 140
-    // us, MID 64: 146; 1 to 6 rows as FEW), 64 up to 48 (32 skewed rows: 161, MID 32: 169; 64 rows: TILE 128 168, MID 64
-    // 180), TILE 256 from 200 on (256 rows: 238, TILE 128: 275; 128 rows: 216 and 186)
-    q.kind = !dma ? RAGGED : rows <= 24 ? MID : rows <= 48 ? RING : TILE;
-    q.bm = !dma ? (rows <= 64 ? 64 : 128) : rows <= 24 ? 32 : rows <= 48 ? 64 : rows < 200 ? 128 : 256;
-    q.bn = q.kind == MID ? 64 : q.bm;
+  const float pad_time = 3.f + (float)(p.M + (grouped ? (int64_t)p.E : 1) * p.W) * p.K * 4 / 4.5e6f;
+  // (few columns of few experts are too few tiles: T=2 of 2 of 35, K=2432 N=320 MID 11.8 us, FEW 7.6)
+  if (grouped && (rows > 16 || (dma && std::min<int64_t>(p.M, p.E) * cdiv(p.W, 64) >= 128))) {
+    // unaligned rows run at some 300 TFLOP/s, aligned ones at 700
+    q.pad = !dma && can_pad && 2.f * p.M * p.W * p.K * 1.9e-9f > pad_time;
+    // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 139
+    // us, RING 64: 143; 1 to 6 rows as FEW), RING 64 up to 48 (32 skewed rows: 161, MID 32: 169; 64 rows: TILE 128 160, RING 64
+    // 171), TILE 256 from 200 on (256 rows: 238, TILE 128: 275; 128 rows: 216 and 186)
+    q.kind = !dma && !q.pad ? RAGGED : rows <= 24 ? MID : rows <= 48 ? RING : TILE;
+    q.bm = q.kind == RAGGED ? 64 : rows <= 24 ? 32 : rows <= 48 ? 64 : rows < 200 ? 128 : 256;
+    q.bn = q.kind == TILE ? q.bm : 64;
+    if (q.kind == TILE) {
+      // where the products take longer than the weights' way from memory, the tiles' rounds count as in a batch (14
+      // experts of 534 rows, K=1872 N=1600: TILE 256 in two rounds 98 us, TILE 128 91; 36 of 316, K=528 N=2x528: 51, 38)
+      const Shape* best = nullptr;
+      float best_time = 0.f;
+      for (const Shape& s : kShapes) {
+        if (s.kind != TILE || s.bn == 224) continue;
+        const float t = shape_time(s, p, p.E * cdiv(rows, s.bm), 1);
+        if (best == nullptr || t < best_time) best = &s, best_time = t;
+      }
+      if (best_time > (float)p.E * p.W * p.K * 2 / 4.5e6f) q.bm = best->bm, q.bn = best->bn;
+    }
     return q;
   }
   if (rows <= 16) {
@@ -1137,15 +1175,16 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma) {
   }
   float best = 0.f;
   for (const Shape& s : kShapes) {
-    if (dma ? s.kind == RAGGED : s.kind != RAGGED) continue;
+    const bool pad = s.kind != RAGGED && !dma;
+    if ((pad && !can_pad) || (s.kind == RAGGED && dma)) continue;
     if (p.gated && s.bn == 224) continue;  // a wave's 112 rows are no whole pairs of gate and up
     const int64_t stages = cdiv(p.K, DN_BK);
     for (int splits = 1; splits <= 16; ++splits) {
       if (splits > 1 && (stages / splits < 4 || s.bm == 256)) break;
-      const float t = shape_time(s, p, splits);
+      const float t = shape_time(s, p, cdiv(p.M, s.bm), splits) + (pad ? pad_time : 0.f);
       if (best == 0.f || t < best) {
         best = t;
-        q = {s.kind, s.bm, s.bn, 1, p.K};
+        q = {s.kind, s.bm, s.bn, 1, p.K, pad};
         if (splits > 1) {
           q.kchunk = (int)(cdiv(stages, splits) * DN_BK);
           q.splits = (int)cdiv(p.K, q.kchunk);
@@ -1170,7 +1209,7 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
   p.ntiles = (int)cdiv(p.N, columns);
   p.mtiles = (int)(p.offsets == nullptr ? cdiv(p.M, q.bm) : imin64(p.M, p.E + 1) + p.M / q.bm);
   p.splits = q.splits;
-  p.kchunk = q.kchunk;
+  p.kchunk = q.splits > 1 ? q.kchunk : p.K;
   const int64_t groups = (int64_t)p.mtiles * p.ntiles * q.splits;
   CCQ_REQUIRE(groups < 1 << 22, "%s: %lld tiles, too many for one launch", what, (long long)groups);
   const dim3 grid((uint32_t)groups);
@@ -1190,8 +1229,7 @@ int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
     else if (q.bn == 224) launch(dense_tile_kernel<DT, 256, 224, 4, 2>, grid, dim3(512), 0, st, p);
     else launch(dense_tile_kernel<DT, 256, 256, 4, 2>, grid, dim3(512), 0, st, p);
   } else {
-    if (q.bm == 64) launch(dense_ragged_kernel<DT, 64, 4>, grid, dim3(256), 0, st, p);
-    else launch(dense_ragged_kernel<DT, 128, 2>, grid, dim3(256), 0, st, p);
+    launch(dense_ragged_kernel<DT>, grid, dim3(256), 0, st, p);
   }
   if (int rc = launch_status(what)) return rc;
   if (p.part != nullptr) {
@@ -1234,29 +1272,68 @@ DenseP make_params(const ccq_dense_args& a, bool grouped) {
   return p;
 }
 
-// LDS DMA: 16-byte pieces at 16-byte addresses, offsets from a tile's first row in 32 bits
-bool can_dma(const ccq_dense_args& a) {
-  const int64_t ldx = a.M > 1 ? a.ldx : a.K;
-  return a.K % 8 == 0 && ldx % 8 == 0 && aligned(a.x, 16) && aligned(a.w, 16) && 256 * ldx + a.K < 1ll << 31 &&
-         ((a.gated ? a.N : 0) + 256) * a.K < 1ll << 31;
+// LDS copies: 16-byte pieces at 16-byte addresses, offsets from a tile's first row in 32 bits
+bool in_reach(int64_t K, int64_t ldx, const ccq_dense_args& a) {
+  return 256 * ldx + K < 1ll << 31 && ((a.gated ? a.N : 0) + 256) * K < 1ll << 31;
 }
+bool x_aligned(const ccq_dense_args& a) { return a.K % 8 == 0 && (a.M <= 1 || a.ldx % 8 == 0) && aligned(a.x, 16); }
+bool w_aligned(const ccq_dense_args& a) { return a.K % 8 == 0 && aligned(a.w, 16); }
 
 Plan plan_of(const ccq_dense_args& a, const DenseP& p) {
-  return make_plan(p, p.offsets != nullptr ? cdiv(a.M, a.num_experts) : a.M, can_dma(a));
+  const int64_t Kp = cdiv(a.K, 8) * 8;
+  const bool dma = x_aligned(a) && w_aligned(a) && in_reach(a.K, a.M > 1 ? a.ldx : a.K, a);
+  return make_plan(p, p.offsets != nullptr ? cdiv(a.M, a.num_experts) : a.M, dma, in_reach(Kp, std::max(Kp, a.ldx), a));
 }
 
-int run_dense(const char* what, const ccq_dense_args& a, bool grouped) {
+// the splits' sums, then the aligned rows of x and of w
+struct Scratch {
+  size_t part, x, w;
+};
+Scratch scratch_of(const ccq_dense_args& a, const DenseP& p, const Plan& q) {
+  const size_t Kp = (size_t)cdiv(a.K, 8) * 8, L = p.offsets != nullptr ? (size_t)p.E : 1;
+  const auto whole = [](size_t n) { return (n + 255) / 256 * 256; };
+  return {q.splits > 1 ? whole((size_t)q.splits * p.M * p.P * 4) : 0, q.pad && !x_aligned(a) ? whole(p.M * Kp * 2) : 0,
+          q.pad && !w_aligned(a) ? whole(L * p.W * Kp * 2) : 0};
+}
+
+size_t workspace_of(const char* what, const ccq_dense_args* args, bool grouped) {
+  if (args == nullptr || args->M < 1 || check_dense(what, *args, grouped)) return 0;
+  const DenseP p = make_params(*args, grouped);
+  const Scratch s = scratch_of(*args, p, plan_of(*args, p));
+  return s.part + s.x + s.w;
+}
+
+int run_dense(const char* what, const ccq_dense_args* args, bool grouped) {
+  CCQ_REQUIRE(args != nullptr, "%s: null arguments", what);
+  const ccq_dense_args& a = *args;
   if (int rc = check_dense(what, a, grouped)) return rc;
   if (a.M == 0) return 0;
   DenseP p = make_params(a, grouped);
   const Plan q = plan_of(a, p);
-  if (q.splits > 1) {
-    const size_t need = (size_t)q.splits * p.M * p.P * 4;
-    CCQ_REQUIRE(a.workspace != nullptr && aligned(a.workspace, 16) && a.workspace_bytes >= need,
-                "%s: workspace of %zu bytes needed", what, need);
-    p.part = reinterpret_cast<float*>(a.workspace);
-  }
+  const Scratch s = scratch_of(a, p, q);
+  const size_t need = s.part + s.x + s.w;
+  CCQ_REQUIRE(need == 0 || (a.workspace != nullptr && aligned(a.workspace, 16) && a.workspace_bytes >= need),
+              "%s: workspace of %zu bytes needed", what, need);
+  char* at = reinterpret_cast<char*>(a.workspace);
   const hipStream_t st = as_stream(a.stream);
+  if (s.part) p.part = reinterpret_cast<float*>(at);
+  if (q.pad) {
+    PadP pad = {};
+    pad.K = p.K, pad.Kp = (int)(cdiv(a.K, 8) * 8);
+    if (s.x) {
+      pad.from[0] = reinterpret_cast<const uint16_t*>(a.x), pad.to[0] = reinterpret_cast<uint16_t*>(at + s.part);
+      pad.rows[0] = p.M, pad.ld[0] = a.ldx;
+      p.x = pad.to[0], p.ldx = pad.Kp;
+    }
+    if (s.w) {
+      pad.from[1] = reinterpret_cast<const uint16_t*>(a.w), pad.to[1] = reinterpret_cast<uint16_t*>(at + s.part + s.x);
+      pad.rows[1] = (grouped ? (int64_t)p.E : 1) * p.W, pad.ld[1] = p.K;
+      p.w = pad.to[1];
+    }
+    p.K = pad.Kp;
+    launch(dense_pad_kernel, dim3((uint32_t)std::min<int64_t>(cdiv(pad.rows[0] + pad.rows[1], 4), 8192)), dim3(256), 0, st, pad);
+    if (int rc = launch_status(what)) return rc;
+  }
   return a.dtype == CCQ_BF16 ? launch_dense<CCQ_BF16>(p, q, st, what) : launch_dense<CCQ_F16>(p, q, st, what);
 }
 
@@ -1267,18 +1344,15 @@ int run_dense(const char* what, const ccq_dense_args& a, bool grouped) {
 using namespace ccq;
 
 extern "C" size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args) {
-  if (args == nullptr || args->M < 1 || check_dense("ccq_dense_linear", *args, false)) return 0;
-  const DenseP p = make_params(*args, false);
-  const Plan q = plan_of(*args, p);
-  return q.splits > 1 ? (size_t)q.splits * p.M * p.P * 4 : 0;
+  return workspace_of("ccq_dense_linear", args, false);
 }
 
-extern "C" int ccq_dense_linear(const ccq_dense_args* args) {
-  CCQ_REQUIRE(args != nullptr, "ccq_dense_linear: null arguments");
-  return run_dense("ccq_dense_linear", *args, false);
+extern "C" int ccq_dense_linear(const ccq_dense_args* args) { return run_dense("ccq_dense_linear", args, false); }
+
+extern "C" size_t ccq_dense_linear_grouped_workspace_size(const ccq_dense_args* args) {
+  return workspace_of("ccq_dense_linear_grouped", args, true);
 }
 
 extern "C" int ccq_dense_linear_grouped(const ccq_dense_args* args) {
-  CCQ_REQUIRE(args != nullptr, "ccq_dense_linear_grouped: null arguments");
-  return run_dense("ccq_dense_linear_grouped", *args, true);
+  return run_dense("ccq_dense_linear_grouped", args, true);
 }

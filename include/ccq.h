@@ -804,10 +804,13 @@ typedef struct ccq_dense_args {
   int dtype, bias_dtype, y_dtype, act, gated;
 } ccq_dense_args;
 
-/* Workspace of ccq_dense_linear for these arguments (partial sums of K's
- * splits; no initial contents required), 0 where K is not split.  Calls sharing
- * one must not overlap in time. */
+/* Workspace of ccq_dense_linear and ccq_dense_linear_grouped for these arguments
+ * (partial sums of K's splits; aligned copies of rows of x and w that are not, where
+ * the product is large; no initial contents required), often 0, and always for up to
+ * 16 rows, or groups of rows aligned to 16 bytes.  Calls sharing one must not overlap
+ * in time. */
 size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args);
+size_t ccq_dense_linear_grouped_workspace_size(const ccq_dense_args* args);
 
 /* z = x w^T + bias; y = act(z) + residual, gated: y = act(z[:, :N]) * z[:, N:] +
  * residual; products, sums and the epilogue in float32, y rounded once. */
@@ -815,8 +818,7 @@ int ccq_dense_linear(const ccq_dense_args* args);
 
 /* ccq_dense_linear where rows offsets[e] .. offsets[e + 1] - 1 of x take w[e] and
  * bias[e] (offsets within [0, M] and rising, as ccq_moe_permute makes them; read
- * on the device); rows of y from offsets[num_experts] on are zeros.  Takes no
- * workspace. */
+ * on the device); rows of y from offsets[num_experts] on are zeros. */
 int ccq_dense_linear_grouped(const ccq_dense_args* args);
 
 #ifdef __cplusplus

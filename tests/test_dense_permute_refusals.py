@@ -65,9 +65,17 @@ def test_dense_workspace(lib):
 
     big = dict(M=100, K=8192, N=64, ldx=8192, ldy=64)
     need = lib.ccq_dense_linear_workspace_size(_args(**big))
-    assert need > 0 and need % (100 * 64 * 4) == 0
+    assert need >= 2 * 100 * 64 * 4
     for kw in (dict(), dict(workspace=P, workspace_bytes=need - 1), dict(workspace=P + 8, workspace_bytes=need)):
         assert lib.ccq_dense_linear(_args(**big, **kw)) == CCQ_EINVAL and "workspace" in last_error()
+    odd = dict(M=4000, K=515, N=700, ldx=515, ldy=700, num_experts=2)
+    for size, run in ((lib.ccq_dense_linear_workspace_size, lib.ccq_dense_linear),
+                      (lib.ccq_dense_linear_grouped_workspace_size, lib.ccq_dense_linear_grouped)):
+        need = size(_args(**odd))
+        assert need >= 4000 * 520 * 2
+        assert run(_args(**odd, workspace=P, workspace_bytes=need - 1)) == CCQ_EINVAL and "workspace" in last_error()
+    for M, K, N, E in ((1, 8, 1, 3), (5000, 64, 32, 3), (5000, 4096, 512, 1), (1 << 20, 8, 8, 1024)):  # aligned groups
+        assert lib.ccq_dense_linear_grouped_workspace_size(_args(M=M, K=K, N=N, ldx=K, ldy=N, num_experts=E)) == 0
     for M in range(1, 17):  # what the Python entry point counts on
         for K, N in ((64, 32), (14336, 16), (1 << 20, 1), (1405, 1407)):
             assert lib.ccq_dense_linear_workspace_size(_args(M=M, K=K, N=N, ldx=K, ldy=N)) == 0

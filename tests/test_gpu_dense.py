@@ -218,6 +218,40 @@ def test_group_sizes(gpu, counts):
             assert (y[kept:] == 0).all() and (wide[:, 0] == 7).all() and (wide[:, N + 1:] == 7).all()
 
 
+@pytest.mark.parametrize("M,K,N", [(1300, 1031, 900), (700, 2049, 1500), (2100, 257, 1700), (513, 4100, 700)])
+def test_large_unaligned(gpu, M, K, N):
+    """Products large enough to copy their unaligned rows first: odd K, and K of whole pieces at odd addresses."""
+    from ccut.quant import dense
+
+    for gated, dt in ((False, BF), (True, F16)):
+        c = _inputs(M, K, N // 2 if gated else N, dt, gated, "same", True, dt)
+        _run(gpu, c, gated, "silu")
+        K8 = K // 8 * 8
+        c = _inputs(M, K8, N, dt, False, None, False, dt)
+        ref, bound = od.linear(c["x"], c["w"])
+        for dx, dw in ((1, 0), (0, 3), (5, 8)):
+            x = torch.full((M * (K8 + 3) + 16,), float("nan"), dtype=dt, device=gpu)[dx:dx + M * (K8 + 3)].view(M, K8 + 3)[:, :K8]
+            w = torch.empty((N * K8 + 16,), dtype=dt, device=gpu)[dw:dw + N * K8].view(N, K8)
+            x.copy_(c["x"])
+            w.copy_(c["w"])
+            _close(dense.linear(x, w), ref, bound)
+
+
+@pytest.mark.parametrize("E,rows,K,N", [(3, 900, 515, 700), (2, 700, 1030, 1100)])
+def test_large_unaligned_groups(gpu, E, rows, K, N):
+    from ccut.quant import dense
+
+    counts = [rows, 0] + [rows // 3] * (E - 1)
+    offsets = torch.tensor([0] + torch.tensor(counts[:E]).cumsum(0).tolist(), dtype=torch.int32)
+    M = int(offsets[-1]) + 37
+    c = _inputs(M, K, N, F16, True, F32, False, F16, E=E)
+    c["x"][int(offsets[-1]):] = float("nan")
+    ref, bound = od.grouped(c["x"], offsets, c["w"], c["bias"], "gelu", True)
+    y = dense.linear_grouped(c["x"].to(gpu), offsets.to(gpu), c["w"].to(gpu), c["bias"].to(gpu), act="gelu", gated=True)
+    _close(y, ref, bound)
+    assert (y[int(offsets[-1]):] == 0).all()
+
+
 def test_repeated_calls_give_the_same_bits(gpu):
     from ccut.quant import dense
 
@@ -232,7 +266,7 @@ def test_graphs_and_streams(gpu):
     """Captured calls with scratch of their own, two graphs, replayed with eager work between, against eager results."""
     from ccut.quant import dense
 
-    shapes = [(100, 8192, 96), (90, 6000, 160), (4, 512, 64)]
+    shapes = [(100, 8192, 96), (90, 6000, 160), (4, 512, 64), (1300, 1031, 900)]
     cs = [{k: _up(v, gpu) for k, v in _inputs(M, K, N, BF, False, "same", False, BF).items()} for M, K, N in shapes]
     call = lambda c: dense.linear(c["x"], c["w"], c["bias"], act="silu")  # noqa: E731
     graphs, outs = [], []
