@@ -73,6 +73,7 @@ class ccq_lora_adapters(ctypes.Structure):
 
 RMS_NORM_ARGS = struct.Struct("@8P5q4if4x")  # ccq_rms_norm_args
 DENSE_ARGS = struct.Struct("@8PN7q5i4x")  # ccq_dense_args
+PERMUTE_ARGS = struct.Struct("@10PN6q2i")  # ccq_moe_permute_args
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # CCQ_ACT_*
 
 
@@ -169,9 +170,9 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_moe_f32_ffn": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _i64,
                                _i64, _i64, _vp, _sz, _vp]),
     "ccq_moe_permute_workspace_size": (_sz, [_i64, _i64, _i64]),
-    "ccq_moe_permute": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
-    "ccq_moe_unpermute": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
-    "ccq_moe_unpermute_grad": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "ccq_moe_permute": (_int, [ctypes.c_char_p]),  # PERMUTE_ARGS.pack(...)
+    "ccq_moe_unpermute": (_int, [ctypes.c_char_p]),
+    "ccq_moe_unpermute_grad": (_int, [ctypes.c_char_p]),
     "ccq_dense_linear_workspace_size": (_sz, [ctypes.c_char_p]),  # DENSE_ARGS.pack(...)
     "ccq_dense_linear_grouped_workspace_size": (_sz, [ctypes.c_char_p]),
     "ccq_dense_linear": (_int, [ctypes.c_char_p]),

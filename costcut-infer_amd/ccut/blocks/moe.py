@@ -24,7 +24,8 @@ import torch
 
 from ccut import _dev
 from ccut._dev import empty_strided, is_current, raw_stream
-from ccut._lib import ACTIVATIONS, call, ccq_fp8_experts, ccq_fp8row_experts, ccq_w4_experts, check, lib
+from ccut._lib import (ACTIVATIONS, PERMUTE_ARGS, call, ccq_fp8_experts, ccq_fp8row_experts, ccq_w4_experts, check,
+                       lib)
 from ccut.quant import awq, dense
 
 __all__ = [
@@ -668,6 +669,10 @@ def moe_ffn_fp8row(x, ids, weights, experts: Fp8RowExperts, out_dtype: torch.dty
 # ---------------------------------------------------------------------------
 
 MAX_ASSIGNMENTS, MAX_SLOTS, MAX_SORT_EXPERTS = 1 << 20, 64, 1024
+_BARE_ASSIGNMENTS = 4096  # batches of up to this many are sorted without scratch
+_CODE = _dev.DTYPE_CODE
+_pack = PERMUTE_ARGS.pack
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 
 
 class Permutation(NamedTuple):
@@ -681,29 +686,37 @@ class Permutation(NamedTuple):
 
 
 def _float_rows(t: torch.Tensor, what: str, index: int) -> tuple[torch.Tensor, int]:
-    if t.dtype not in _dev.DTYPE_CODE or t.dim() != 2 or t.shape[1] < 1 or t.get_device() != index:
+    shape = t.shape
+    if t.dtype not in _CODE or len(shape) != 2 or shape[1] < 1 or t.get_device() != index:
         raise ValueError(f"{what} must be float32, float16 or bfloat16 rows [n, H] on cuda:{index}, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-    if t.shape[0] <= 1:
-        return (t if t.stride(1) == 1 else t.contiguous()), t.shape[1]
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+                         f"{tuple(shape)} on {t.device}")
+    if t.is_contiguous():
+        return t, shape[1]
+    if shape[0] <= 1:
+        return (t if t.stride(1) == 1 else t.contiguous()), shape[1]
+    if t.stride(1) != 1 or t.stride(0) < shape[1]:
         t = t.contiguous()
     return t, t.stride(0)
 
 
-def _positions(plan: Permutation, index: int) -> torch.Tensor:
+def _positions(plan: Permutation, rows: torch.Tensor, index: int) -> torch.Tensor:
     p = plan.position
-    if p.dtype != torch.int32 or p.dim() != 2 or p.get_device() != index:
-        raise ValueError(f"plan.position must be int32 [T, k] on cuda:{index}, got {p.dtype} {tuple(p.shape)} on "
+    shape = p.shape
+    if p.dtype != _I32 or len(shape) != 2 or p.get_device() != index:
+        raise ValueError(f"plan.position must be int32 [T, k] on cuda:{index}, got {p.dtype} {tuple(shape)} on "
                          f"{p.device}")
+    T, k = shape
+    if not 1 <= k <= MAX_SLOTS or rows.shape[0] != T * k or T * k > MAX_ASSIGNMENTS:
+        raise ValueError(f"rows {tuple(rows.shape)} and position {tuple(shape)}: need T * k rows, k <= {MAX_SLOTS}, "
+                         f"T * k <= {MAX_ASSIGNMENTS}")
     return p if p.is_contiguous() else p.contiguous()
 
 
-def _routing_weights(weights: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
-    if weights.shape != position.shape or weights.device != position.device or not weights.is_floating_point():
+def _routing_weights(weights: torch.Tensor, position: torch.Tensor, index: int) -> torch.Tensor:
+    if weights.shape != position.shape or weights.get_device() != index or not weights.is_floating_point():
         raise ValueError(f"weights must be floats {tuple(position.shape)} on {position.device}, got {weights.dtype} "
                          f"{tuple(weights.shape)} on {weights.device}")
-    return weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
+    return weights if weights.dtype == _F32 and weights.is_contiguous() else weights.float().contiguous()
 
 
 def moe_permute(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, Permutation]:
@@ -719,29 +732,30 @@ def moe_permute(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[t
         with torch.cuda.device(index):
             return moe_permute(x, ids, num_experts)
     x2, ldx = _float_rows(x, "x", index)
-    T, H = x2.shape
-    if ids.dim() != 2 or ids.shape[0] != T or ids.get_device() != index:
-        raise ValueError(f"ids must be [{T}, k] on {x.device}, got {tuple(ids.shape)} on {ids.device}")
-    k = ids.shape[1]
-    if not 1 <= k <= MAX_SLOTS or T * k > MAX_ASSIGNMENTS or not 1 <= num_experts <= MAX_SORT_EXPERTS:
+    (T, H), dtype, shape = x2.shape, x2.dtype, ids.shape
+    if len(shape) != 2 or shape[0] != T or ids.get_device() != index:
+        raise ValueError(f"ids must be [{T}, k] on {x.device}, got {tuple(shape)} on {ids.device}")
+    k = shape[1]
+    n = T * k
+    if not 1 <= k <= MAX_SLOTS or n > MAX_ASSIGNMENTS or not 1 <= num_experts <= MAX_SORT_EXPERTS:
         raise ValueError(f"{T} tokens of {k} of {num_experts} experts: need 1 <= k <= {MAX_SLOTS}, T * k <= "
                          f"{MAX_ASSIGNMENTS}, 1 to {MAX_SORT_EXPERTS} experts")
-    if ids.dtype != torch.int64 or not ids.is_contiguous():
+    if ids.dtype != _I64 or not ids.is_contiguous():
         if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
             raise ValueError(f"ids must hold whole numbers, got {ids.dtype}")
-        ids = ids.to(torch.int64).contiguous()
-    rows = empty_strided((T * k, H), (H, 1), x.dtype)
-    position = empty_strided((T, k), (k, 1), torch.int32)
-    offsets = empty_strided((num_experts + 1,), (1,), torch.int32)
+        ids = ids.to(_I64).contiguous()
+    rows = empty_strided((n, H), (H, 1), dtype)
+    position = empty_strided((T, k), (k, 1), _I32)
+    offsets = empty_strided((num_experts + 1,), (1,), _I32)
     handle = lib()
-    nbytes = handle.ccq_moe_permute_workspace_size(T, k, num_experts)
-    sp = 0
-    if nbytes:  # this call's own, so that calls on several streams or in several graphs do not share it
+    sp = nbytes = 0
+    if n > _BARE_ASSIGNMENTS:  # this call's own, so that calls on several streams or in several graphs do not share it
+        nbytes = handle.ccq_moe_permute_workspace_size(T, k, num_experts)
         scratch = empty_strided((nbytes,), (1,), torch.uint8)
         sp = scratch.data_ptr()
-    rc = handle.ccq_moe_permute(x2.data_ptr(), _dev.DTYPE_CODE[x.dtype], ldx, ids.data_ptr(), rows.data_ptr(),
-                                position.data_ptr(), offsets.data_ptr(), T, k, num_experts, H, sp, nbytes,
-                                raw_stream(index))
+    rc = handle.ccq_moe_permute(_pack(x2.data_ptr(), ids.data_ptr(), rows.data_ptr(), position.data_ptr(),
+                                      offsets.data_ptr(), 0, 0, 0, sp, raw_stream(index), nbytes, ldx, H, T, k, H,
+                                      num_experts, _CODE[dtype], 0))
     if rc:
         check(rc, "ccq_moe_permute")
     return rows, Permutation(position, offsets)
@@ -758,22 +772,20 @@ def moe_unpermute(rows: torch.Tensor, plan: Permutation, weights: torch.Tensor |
         with torch.cuda.device(index):
             return moe_unpermute(rows, plan, weights, out_dtype)
     r2, ldr = _float_rows(rows, "rows", index)
-    position = _positions(plan, index)
-    T, k = position.shape
-    H = r2.shape[1]
-    if not 1 <= k <= MAX_SLOTS or r2.shape[0] != T * k or T * k > MAX_ASSIGNMENTS:
-        raise ValueError(f"rows {tuple(rows.shape)} and position {tuple(position.shape)}: need T * k rows, k <= "
-                         f"{MAX_SLOTS}, T * k <= {MAX_ASSIGNMENTS}")
-    out_dtype = out_dtype or rows.dtype
-    if out_dtype not in _dev.DTYPE_CODE:
+    position = _positions(plan, r2, index)
+    (T, k), H = position.shape, r2.shape[1]
+    if out_dtype is None:
+        out_dtype = r2.dtype
+    ycode = _CODE.get(out_dtype)
+    if ycode is None:
         raise ValueError(f"y must be float32, float16 or bfloat16, got {out_dtype}")
     wp = 0
     if weights is not None:
-        weights = _routing_weights(weights, position)
+        weights = _routing_weights(weights, position, index)
         wp = weights.data_ptr()
     y = empty_strided((T, H), (H, 1), out_dtype)
-    rc = lib().ccq_moe_unpermute(r2.data_ptr(), _dev.DTYPE_CODE[rows.dtype], ldr, T * k, position.data_ptr(), wp,
-                                 y.data_ptr(), _dev.DTYPE_CODE[out_dtype], T, k, H, raw_stream(index))
+    rc = lib().ccq_moe_unpermute(_pack(0, 0, r2.data_ptr(), position.data_ptr(), 0, wp, y.data_ptr(), 0, 0,
+                                       raw_stream(index), 0, 0, ldr, T, k, H, 0, _CODE[r2.dtype], ycode))
     if rc:
         check(rc, "ccq_moe_unpermute")
     return y
@@ -797,21 +809,17 @@ def moe_unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, plan: Permutati
         with torch.cuda.device(index):
             return moe_unpermute_backward(dy, rows, plan, weights)
     r2, ldr = _float_rows(rows, "rows", index)
-    g2, ldy = _float_rows(dy, "dy", index)
-    position = _positions(plan, index)
-    T, k = position.shape
-    H = r2.shape[1]
-    if not 1 <= k <= MAX_SLOTS or r2.shape[0] != T * k or T * k > MAX_ASSIGNMENTS:
-        raise ValueError(f"rows {tuple(rows.shape)} and position {tuple(position.shape)}: need T * k rows, k <= "
-                         f"{MAX_SLOTS}, T * k <= {MAX_ASSIGNMENTS}")
-    if dy.dtype != rows.dtype or tuple(dy.shape) != (T, H):
-        raise ValueError(f"dy must be {rows.dtype} [{T}, {H}], got {dy.dtype} {tuple(dy.shape)}")
-    weights = _routing_weights(weights, position)
-    d_rows = empty_strided((T * k, H), (H, 1), rows.dtype)
-    d_weights = empty_strided((T, k), (k, 1), torch.float32)
-    rc = lib().ccq_moe_unpermute_grad(g2.data_ptr(), ldy, r2.data_ptr(), ldr, _dev.DTYPE_CODE[rows.dtype], T * k,
-                                      position.data_ptr(), weights.data_ptr(), d_rows.data_ptr(), d_weights.data_ptr(),
-                                      T, k, H, raw_stream(index))
+    g2, ldx = _float_rows(dy, "dy", index)
+    position = _positions(plan, r2, index)
+    (T, k), H, dtype = position.shape, r2.shape[1], r2.dtype
+    if g2.dtype != dtype or tuple(g2.shape) != (T, H):
+        raise ValueError(f"dy must be {dtype} [{T}, {H}], got {dy.dtype} {tuple(dy.shape)}")
+    weights = _routing_weights(weights, position, index)
+    d_rows = empty_strided((T * k, H), (H, 1), dtype)
+    d_weights = empty_strided((T, k), (k, 1), _F32)
+    rc = lib().ccq_moe_unpermute_grad(_pack(g2.data_ptr(), 0, r2.data_ptr(), position.data_ptr(), 0, weights.data_ptr(),
+                                            d_rows.data_ptr(), d_weights.data_ptr(), 0, raw_stream(index), 0, ldx, ldr,
+                                            T, k, H, 0, _CODE[dtype], 0))
     if rc:
         check(rc, "ccq_moe_unpermute_grad")
     return d_rows, d_weights

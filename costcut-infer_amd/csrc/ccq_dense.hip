@@ -68,18 +68,19 @@ __device__ __forceinline__ float dn_rcp(float v) { return __builtin_amdgcn_rcpf(
 // z Phi(z): Phi(-|z|) = exp(-x^2) erfcx(x) / 2 with x = |z| / sqrt 2 and erfcx
 // a polynomial in t = 1 / (1 + 0.33 x) without a constant term, fitted over
 // x <= 10 to 9.4e-8 of its value (beyond, exp(-x^2) is 0 in float32).  Both tails
-// keep their relative accuracy, and it takes a third of erff's instructions.
+// keep their relative accuracy, and it takes a third of erff's instructions.  The
+// factors 1 / sqrt 2 and 1 / 2 are in the constants: 0.33 / sqrt 2, the coefficients'
+// halves, log2(e) / 2.
 __device__ __forceinline__ float dn_gelu(float z) {
-  const float x = fabsf(z) * 0.707106781f;
-  const float t = dn_rcp(fmaf(0.33f, x, 1.f));
-  float q = fmaf(t, -0.1353449f, 0.46023397f);
-  q = fmaf(t, q, -0.35114448f);
-  q = fmaf(t, q, 0.40849535f);
-  q = fmaf(t, q, 0.04722303f);
-  q = fmaf(t, q, 0.20122319f);
-  q = fmaf(t, q, 0.18295605f);
-  q = fmaf(t, q, 0.1863578f);
-  q = q * t * 0.5f * dn_exp(-x * x);
+  const float t = dn_rcp(fmaf(0.233345238f, fabsf(z), 1.f));
+  float q = fmaf(t, -0.06767245f, 0.230116985f);
+  q = fmaf(t, q, -0.17557224f);
+  q = fmaf(t, q, 0.204247675f);
+  q = fmaf(t, q, 0.023611515f);
+  q = fmaf(t, q, 0.100611595f);
+  q = fmaf(t, q, 0.091478025f);
+  q = fmaf(t, q, 0.0931789f);
+  q = q * t * __builtin_amdgcn_exp2f(z * z * -0.72134752f);
   return z * (z >= 0.f ? 1.f - q : q);
 }
 

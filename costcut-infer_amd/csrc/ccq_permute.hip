@@ -401,12 +401,12 @@ int row_threads(int64_t bytes) {
 
 int64_t esize(int dt) { return dt == CCQ_F32 ? 4 : 2; }
 
-int check_sizes(const char* what, int dtype, int64_t T, int64_t k, int64_t H) {
-  CCQ_REQUIRE(dtype == CCQ_F32 || dtype == CCQ_F16 || dtype == CCQ_BF16, "%s: dtype %d", what, dtype);
-  CCQ_REQUIRE(k >= 1 && k <= PM_MAX_K, "%s: k=%lld, 1 to %d", what, (long long)k, PM_MAX_K);
-  CCQ_REQUIRE(T >= 0 && T <= PM_MAX_N && T * k <= PM_MAX_N, "%s: T=%lld tokens of %lld experts: at most 2^20 in all", what, (long long)T,
-              (long long)k);
-  CCQ_REQUIRE(H >= 1 && H <= 1 << 20, "%s: H=%lld, 1 to 2^20", what, (long long)H);
+int check_sizes(const char* what, const ccq_moe_permute_args& a) {
+  CCQ_REQUIRE(a.dtype == CCQ_F32 || a.dtype == CCQ_F16 || a.dtype == CCQ_BF16, "%s: dtype %d", what, a.dtype);
+  CCQ_REQUIRE(a.k >= 1 && a.k <= PM_MAX_K, "%s: k=%lld, 1 to %d", what, (long long)a.k, PM_MAX_K);
+  CCQ_REQUIRE(a.T >= 0 && a.T <= PM_MAX_N && a.T * a.k <= PM_MAX_N,
+              "%s: T=%lld tokens of %lld experts: at most 2^20 in all", what, (long long)a.T, (long long)a.k);
+  CCQ_REQUIRE(a.H >= 1 && a.H <= 1 << 20, "%s: H=%lld, 1 to 2^20", what, (long long)a.H);
   return 0;
 }
 
@@ -435,61 +435,62 @@ extern "C" size_t ccq_moe_permute_workspace_size(int64_t T, int64_t k, int64_t n
   return (size_t)p.chunks * (num_experts + 1) * 4;
 }
 
-extern "C" int ccq_moe_permute(const void* x, int dtype, int64_t ldx, const int64_t* ids, void* rows, int32_t* position,
-                               int32_t* offsets, int64_t T, int64_t k, int64_t num_experts, int64_t H, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+extern "C" int ccq_moe_permute(const ccq_moe_permute_args* args) {
   const char* what = "ccq_moe_permute";
-  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
-  CCQ_REQUIRE(num_experts >= 1 && num_experts <= PM_MAX_E, "%s: num_experts=%lld, 1 to %d", what, (long long)num_experts,
-              PM_MAX_E);
-  CCQ_REQUIRE(T <= 1 || ldx >= H, "%s: row stride %lld of rows of %lld", what, (long long)ldx, (long long)H);
-  CCQ_REQUIRE(offsets != nullptr && (T == 0 || (x && ids && rows && position)), "%s: null pointer", what);
-  const size_t e = (size_t)esize(dtype);
-  CCQ_REQUIRE(aligned(x, e) && aligned(rows, e) && aligned(ids, 8) && aligned(position, 4) && aligned(offsets, 4),
+  CCQ_REQUIRE(args != nullptr, "%s: null arguments", what);
+  const ccq_moe_permute_args& a = *args;
+  if (int rc = check_sizes(what, a)) return rc;
+  CCQ_REQUIRE(a.num_experts >= 1 && a.num_experts <= PM_MAX_E, "%s: num_experts=%lld, 1 to %d", what,
+              (long long)a.num_experts, PM_MAX_E);
+  CCQ_REQUIRE(a.T <= 1 || a.ldx >= a.H, "%s: row stride %lld of rows of %lld", what, (long long)a.ldx, (long long)a.H);
+  CCQ_REQUIRE(a.offsets != nullptr && (a.T == 0 || (a.x && a.ids && a.rows && a.position)), "%s: null pointer", what);
+  const size_t e = (size_t)esize(a.dtype);
+  CCQ_REQUIRE(aligned(a.x, e) && aligned(a.rows, e) && aligned(a.ids, 8) && aligned(a.position, 4) && aligned(a.offsets, 4),
               "%s: pointers must be aligned to their elements", what);
-  const size_t need = ccq_moe_permute_workspace_size(T, k, num_experts);
-  CCQ_REQUIRE(need == 0 || (workspace != nullptr && aligned(workspace, 16) && workspace_bytes >= need),
+  const size_t need = ccq_moe_permute_workspace_size(a.T, a.k, a.num_experts);
+  CCQ_REQUIRE(need == 0 || (a.workspace != nullptr && aligned(a.workspace, 16) && a.workspace_bytes >= need),
               "%s: workspace of %zu bytes needed", what, need);
-  PermP p = {x, ids, rows, position, offsets, reinterpret_cast<int32_t*>(workspace), ldx * (int64_t)e, T};
-  plan_permute(p, T, k);
-  p.k = (int)k;
-  p.E = (int)num_experts;
-  p.H = (int)H;
+  PermP p = {a.x, a.ids, a.rows, a.position, a.offsets, reinterpret_cast<int32_t*>(a.workspace), a.ldx * (int64_t)e, a.T};
+  plan_permute(p, a.T, a.k);
+  p.k = (int)a.k;
+  p.E = (int)a.num_experts;
+  p.H = (int)a.H;
   p.esize = (int)e;
-  p.row_threads = row_threads(H * (int64_t)e);
-  const dim3 grid((uint32_t)(cdiv(T, p.tokens) + 1));
+  p.row_threads = row_threads(a.H * (int64_t)e);
+  const dim3 grid((uint32_t)(cdiv(a.T, p.tokens) + 1));
+  const hipStream_t st = as_stream(a.stream);
   if (need) {
-    launch(permute_count_kernel, dim3((uint32_t)p.chunks), dim3(PM_THREADS), 0, as_stream(stream), p);
+    launch(permute_count_kernel, dim3((uint32_t)p.chunks), dim3(PM_THREADS), 0, st, p);
     if (int rc = launch_status(what)) return rc;
-    launch(permute_kernel<true>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+    launch(permute_kernel<true>, grid, dim3(PM_THREADS), 0, st, p);
   } else {
-    launch(permute_kernel<false>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+    launch(permute_kernel<false>, grid, dim3(PM_THREADS), 0, st, p);
   }
   return launch_status(what);
 }
 
-extern "C" int ccq_moe_unpermute(const void* rows, int dtype, int64_t ldr, int64_t num_rows, const int32_t* position,
-                                 const float* weights, void* y, int y_dtype, int64_t T, int64_t k, int64_t H,
-                                 void* stream) {
+extern "C" int ccq_moe_unpermute(const ccq_moe_permute_args* args) {
   const char* what = "ccq_moe_unpermute";
-  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
-  CCQ_REQUIRE(y_dtype == CCQ_F32 || y_dtype == CCQ_F16 || y_dtype == CCQ_BF16, "%s: y_dtype %d", what, y_dtype);
-  CCQ_REQUIRE(num_rows >= 0 && (num_rows <= 1 || ldr >= H), "%s: %lld rows of %lld, stride %lld", what,
-              (long long)num_rows, (long long)H, (long long)ldr);
-  if (T == 0) return 0;
-  CCQ_REQUIRE((rows || num_rows == 0) && position && y, "%s: null pointer", what);
-  CCQ_REQUIRE(aligned(rows, (size_t)esize(dtype)) && aligned(position, 4) && aligned(weights, 4) &&
-                  aligned(y, (size_t)esize(y_dtype)),
+  CCQ_REQUIRE(args != nullptr, "%s: null arguments", what);
+  const ccq_moe_permute_args& a = *args;
+  if (int rc = check_sizes(what, a)) return rc;
+  CCQ_REQUIRE(a.y_dtype == CCQ_F32 || a.y_dtype == CCQ_F16 || a.y_dtype == CCQ_BF16, "%s: y_dtype %d", what, a.y_dtype);
+  CCQ_REQUIRE(a.T * a.k <= 1 || a.ldr >= a.H, "%s: row stride %lld of rows of %lld", what, (long long)a.ldr, (long long)a.H);
+  if (a.T == 0) return 0;
+  CCQ_REQUIRE(a.rows && a.position && a.y, "%s: null pointer", what);
+  CCQ_REQUIRE(aligned(a.rows, (size_t)esize(a.dtype)) && aligned(a.position, 4) && aligned(a.weights, 4) &&
+                  aligned(a.y, (size_t)esize(a.y_dtype)),
               "%s: pointers must be aligned to their elements", what);
-  UnpermP p = {rows, position, weights, nullptr, y, nullptr, ldr, 0, num_rows, T, (int)k, (int)H, y_dtype,
-               row_threads(H * esize(dtype))};
-  const dim3 grid((uint32_t)cdiv(T, PM_THREADS / p.row_threads));
-  if (dtype == CCQ_BF16)
-    launch(unpermute_kernel<CCQ_BF16>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
-  else if (dtype == CCQ_F16)
-    launch(unpermute_kernel<CCQ_F16>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+  const UnpermP p = {a.rows, a.position, a.weights, nullptr, a.y, nullptr, a.ldr, 0, a.T * a.k, a.T, (int)a.k, (int)a.H,
+                     a.y_dtype, row_threads(a.H * esize(a.dtype))};
+  const dim3 grid((uint32_t)cdiv(a.T, PM_THREADS / p.row_threads));
+  const hipStream_t st = as_stream(a.stream);
+  if (a.dtype == CCQ_BF16)
+    launch(unpermute_kernel<CCQ_BF16>, grid, dim3(PM_THREADS), 0, st, p);
+  else if (a.dtype == CCQ_F16)
+    launch(unpermute_kernel<CCQ_F16>, grid, dim3(PM_THREADS), 0, st, p);
   else
-    launch(unpermute_kernel<CCQ_F32>, grid, dim3(PM_THREADS), 0, as_stream(stream), p);
+    launch(unpermute_kernel<CCQ_F32>, grid, dim3(PM_THREADS), 0, st, p);
   return launch_status(what);
 }
 
@@ -508,24 +509,24 @@ void launch_grad(int dtype, const UnpermP& p, hipStream_t st) {
 }  // namespace
 }  // namespace ccq
 
-extern "C" int ccq_moe_unpermute_grad(const void* dy, int64_t ldy, const void* rows, int64_t ldr, int dtype,
-                                      int64_t num_rows, const int32_t* position, const float* weights, void* d_rows,
-                                      float* d_weights, int64_t T, int64_t k, int64_t H, void* stream) {
+extern "C" int ccq_moe_unpermute_grad(const ccq_moe_permute_args* args) {
   const char* what = "ccq_moe_unpermute_grad";
-  if (int rc = check_sizes(what, dtype, T, k, H)) return rc;
-  CCQ_REQUIRE(num_rows >= 0 && (num_rows <= 1 || ldr >= H) && (T <= 1 || ldy >= H),
-              "%s: %lld rows of %lld, strides %lld and %lld", what, (long long)num_rows, (long long)H, (long long)ldr,
-              (long long)ldy);
-  if (T == 0) return 0;
-  CCQ_REQUIRE(dy && rows && position && weights && d_rows && d_weights, "%s: null pointer", what);
-  const size_t e = (size_t)esize(dtype);
-  CCQ_REQUIRE(aligned(dy, e) && aligned(rows, e) && aligned(d_rows, e) && aligned(position, 4) && aligned(weights, 4) &&
-                  aligned(d_weights, 4),
+  CCQ_REQUIRE(args != nullptr, "%s: null arguments", what);
+  const ccq_moe_permute_args& a = *args;
+  if (int rc = check_sizes(what, a)) return rc;
+  CCQ_REQUIRE((a.T * a.k <= 1 || a.ldr >= a.H) && (a.T <= 1 || a.ldx >= a.H), "%s: row strides %lld and %lld of rows of %lld",
+              what, (long long)a.ldr, (long long)a.ldx, (long long)a.H);
+  if (a.T == 0) return 0;
+  CCQ_REQUIRE(a.x && a.rows && a.position && a.weights && a.y && a.d_weights, "%s: null pointer", what);
+  const size_t e = (size_t)esize(a.dtype);
+  CCQ_REQUIRE(aligned(a.x, e) && aligned(a.rows, e) && aligned(a.y, e) && aligned(a.position, 4) && aligned(a.weights, 4) &&
+                  aligned(a.d_weights, 4),
               "%s: pointers must be aligned to their elements", what);
-  const UnpermP p = {rows, position, weights, dy, d_rows, d_weights, ldr, ldy, num_rows, T, (int)k, (int)H, dtype, 0};
-  if (T >= 1024)
-    launch_grad<1>(dtype, p, as_stream(stream));
+  const UnpermP p = {a.rows, a.position, a.weights, a.x, a.y, a.d_weights, a.ldr, a.ldx, a.T * a.k, a.T, (int)a.k, (int)a.H,
+                     a.dtype, 0};
+  if (a.T >= 1024)
+    launch_grad<1>(a.dtype, p, as_stream(a.stream));
   else
-    launch_grad<4>(dtype, p, as_stream(stream));
+    launch_grad<4>(a.dtype, p, as_stream(a.stream));
   return launch_status(what);
 }

@@ -746,34 +746,47 @@ int ccq_moe_f32_ffn(const float* x, const int64_t* ids, const float* weights,
  * the batches that one kernel sorts.  Calls sharing one must not overlap. */
 size_t ccq_moe_permute_workspace_size(int64_t T, int64_t k, int64_t num_experts);
 
+/* Arguments of the three calls below, in one block for callers that pay for each
+ * argument of a call.  x [T, H] (the tokens, or the gradient of the sum) with row
+ * stride ldx, rows [T k, H] with row stride ldr, both of dtype (CCQ_F32 | CCQ_F16 |
+ * CCQ_BF16), ids [T, k] int64, position [T, k], offsets [num_experts + 1], weights
+ * and d_weights [T, k]; strides in elements, any element alignment.  T k <= 2^20,
+ * k <= 64, H <= 2^20, num_experts <= 1024. */
+typedef struct ccq_moe_permute_args {
+  const void* x;
+  const int64_t* ids;
+  void* rows;
+  int32_t* position;
+  int32_t* offsets;
+  const float* weights;
+  void* y;
+  float* d_weights;
+  void* workspace;
+  void* stream;
+  size_t workspace_bytes;
+  int64_t ldx, ldr, T, k, H, num_experts;
+  int dtype, y_dtype;
+} ccq_moe_permute_args;
+
 /* The assignments (token t, slot s), a = t k + s, in the order of (expert, a),
- * those with ids outside [0, num_experts) behind all others:
- * position [T, k] the row of each assignment, ~row for those left out;
- * offsets [num_experts + 1] the first row of each expert, and the end;
- * rows [T k, H] the tokens' rows in that order, zeros from row
- * offsets[num_experts] on.  x [T, H] of dtype (CCQ_F32 | CCQ_F16 | CCQ_BF16) with
- * row stride ldx, ids [T, k] int64.  T k <= 2^20, k <= 64, H <= 2^20,
- * num_experts <= 1024; any element alignment; rows must not overlap x. */
-int ccq_moe_permute(const void* x, int dtype, int64_t ldx, const int64_t* ids, void* rows, int32_t* position,
-                    int32_t* offsets, int64_t T, int64_t k, int64_t num_experts, int64_t H, void* workspace,
-                    size_t workspace_bytes, void* stream);
+ * those with ids outside [0, num_experts) behind all others: writes position, the row
+ * of each assignment, ~row for those left out; offsets, the first row of each expert,
+ * and the end; and rows (dense), the tokens' rows in that order, zeros from row
+ * offsets[num_experts] on.  rows must not overlap x.  Takes the workspace. */
+int ccq_moe_permute(const ccq_moe_permute_args* args);
 
 /* y[t] = sum over s of weights[t, s] * rows[position[t, s]] (weights null: 1
- * each), float32 sums in slot order, y [T, H] of y_dtype rounded once; positions
- * outside [0, num_rows) contribute nothing.  rows [num_rows, H] of dtype, row
- * stride ldr.  Without weights also the gradient of x in ccq_moe_permute, rows
- * being that of its rows. */
-int ccq_moe_unpermute(const void* rows, int dtype, int64_t ldr, int64_t num_rows, const int32_t* position,
-                      const float* weights, void* y, int y_dtype, int64_t T, int64_t k, int64_t H, void* stream);
+ * each), float32 sums in slot order, y [T, H] of y_dtype (dense) rounded once;
+ * positions outside [0, T k) contribute nothing.  Without weights also the gradient of
+ * x in ccq_moe_permute, rows being that of its rows. */
+int ccq_moe_unpermute(const ccq_moe_permute_args* args);
 
-/* The gradients of ccq_moe_unpermute from dy [T, H]: d_rows [num_rows, H] (dense)
- * in row position[t, s] weights[t, s] * dy[t] rounded once, zeros in row r where
- * the position is ~r; d_weights [T, k] the float32 products of rows and dy, 0
- * where the position is negative.  rows, dy and d_rows of dtype, row strides ldr
- * and ldy; each row of d_rows is written by the position that names it. */
-int ccq_moe_unpermute_grad(const void* dy, int64_t ldy, const void* rows, int64_t ldr, int dtype, int64_t num_rows,
-                           const int32_t* position, const float* weights, void* d_rows, float* d_weights, int64_t T,
-                           int64_t k, int64_t H, void* stream);
+/* The gradients of ccq_moe_unpermute from x, that of its y: y [T k, H] (dense, of
+ * dtype), the gradient of rows, weights[t, s] * x[t] rounded once in row position[t, s],
+ * zeros in row r where the position is ~r (each row is written by the position that
+ * names it); d_weights, the float32 products of rows and x, 0 where the position is
+ * negative. */
+int ccq_moe_unpermute_grad(const ccq_moe_permute_args* args);
 
 /* ------------------------------------------------------------------------
  * Linears with 16-bit weights, the epilogue in the product's kernel

@@ -83,59 +83,81 @@ def test_dense_workspace(lib):
     assert lib.ccq_dense_linear_workspace_size(None) == 0
 
 
+PERMUTE_FIELDS = ("x", "ids", "rows", "position", "offsets", "weights", "y", "d_weights", "workspace", "stream",
+                  "workspace_bytes", "ldx", "ldr", "T", "k", "H", "num_experts", "dtype", "y_dtype")
+
+
+def _permute(**kw):
+    from ccut._lib import PERMUTE_ARGS
+
+    a = dict(x=P, ids=P, rows=P, position=P, offsets=P, weights=P, y=P, d_weights=P, workspace=0, stream=0,
+             workspace_bytes=0, ldx=16, ldr=16, T=4, k=2, H=16, num_experts=3, dtype=2, y_dtype=2)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return PERMUTE_ARGS.pack(*(a[f] for f in PERMUTE_FIELDS))
+
+
 def test_empty_calls(lib):
     assert lib.ccq_dense_linear(_args(M=0)) == 0 and lib.ccq_dense_linear_grouped(_args(M=0)) == 0
-    assert lib.ccq_moe_unpermute(P, 0, 16, 0, P, None, P, 0, 0, 2, 16, None) == 0
-    assert lib.ccq_moe_unpermute_grad(P, 16, P, 16, 0, 0, P, P, P, P, 0, 2, 16, None) == 0
+    assert lib.ccq_moe_unpermute(_permute(T=0, y=0)) == 0 and lib.ccq_moe_unpermute_grad(_permute(T=0, y=0)) == 0
 
 
-def _permute(lib, **kw):
-    a = dict(x=P, dtype=2, ldx=16, ids=P, rows=P, position=P, offsets=P, T=4, k=2, E=3, H=16, ws=None, ws_bytes=0)
-    a.update(kw)
-    return lib.ccq_moe_permute(*a.values(), None)
+SIZES = [(dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(k=0), "k="), (dict(k=65), "k="), (dict(T=-1), "T="),
+         (dict(T=1 << 20), "T="), (dict(T=1 << 60), "T="), (dict(H=0), "H="),
+         (dict(H=(1 << 20) + 1, ldx=1 << 21, ldr=1 << 21), "H=")]
+
+
+@pytest.mark.parametrize("kw,word", SIZES)
+def test_permute_sizes(lib, kw, word):
+    from ccut._lib import CCQ_EINVAL, last_error
+
+    for fn in (lib.ccq_moe_permute, lib.ccq_moe_unpermute, lib.ccq_moe_unpermute_grad):
+        assert fn(_permute(**kw)) == CCQ_EINVAL and word in last_error()
+        assert fn(None) == CCQ_EINVAL
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(dtype=3), "dtype"), (dict(k=0), "k="), (dict(k=65), "k="), (dict(T=-1), "T="), (dict(T=1 << 20), "T="),
-    (dict(T=1 << 60), "T="), (dict(H=0), "H="), (dict(H=(1 << 20) + 1, ldx=1 << 21), "H="), (dict(E=0), "num_experts"),
-    (dict(E=1025), "num_experts"), (dict(ldx=15), "stride"), (dict(x=None), "null"), (dict(ids=None), "null"),
-    (dict(rows=None), "null"), (dict(position=None), "null"), (dict(offsets=None), "null"), (dict(T=0, offsets=None), "null"),
-    (dict(x=P + 1), "aligned"), (dict(dtype=0, rows=P + 2), "aligned"), (dict(ids=P + 4), "aligned"),
-    (dict(position=P + 2), "aligned"), (dict(offsets=P + 2), "aligned"), (dict(T=1 << 15), "workspace"),
-    (dict(T=1 << 15, ws=P, ws_bytes=16), "workspace"), (dict(T=1 << 15, ws=P + 8, ws_bytes=1 << 30), "workspace"),
+    (dict(num_experts=0), "num_experts"), (dict(num_experts=1025), "num_experts"), (dict(ldx=15), "stride"),
+    (dict(x=0), "null"), (dict(ids=0), "null"), (dict(rows=0), "null"), (dict(position=0), "null"), (dict(offsets=0), "null"),
+    (dict(T=0, offsets=0), "null"), (dict(x=P + 1), "aligned"), (dict(dtype=0, rows=P + 2), "aligned"),
+    (dict(ids=P + 4), "aligned"), (dict(position=P + 2), "aligned"), (dict(offsets=P + 2), "aligned"),
+    (dict(T=1 << 15), "workspace"), (dict(T=1 << 15, workspace=P, workspace_bytes=16), "workspace"),
+    (dict(T=1 << 15, workspace=P + 8, workspace_bytes=1 << 30), "workspace"),
 ])
 def test_permute(lib, kw, word):
     from ccut._lib import CCQ_EINVAL, last_error
 
-    assert _permute(lib, **kw) == CCQ_EINVAL and word in last_error()
+    assert lib.ccq_moe_permute(_permute(**kw)) == CCQ_EINVAL and word in last_error()
+
+
+def test_permute_workspace(lib):
+    """What the Python entry point counts on."""
+    for T, k in ((1, 1), (64, 64), (4096, 1), (512, 8), (585, 7)):
+        assert lib.ccq_moe_permute_workspace_size(T, k, 1024) == 0
+    for T, k in ((4097, 1), (1 << 20, 1), (1 << 14, 64), (586, 7)):
+        assert lib.ccq_moe_permute_workspace_size(T, k, 1) > 0
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(dtype=-1), "dtype"), (dict(y_dtype=3), "y_dtype"), (dict(k=0), "k="), (dict(T=1 << 20), "T="), (dict(H=0), "H="),
-    (dict(ldr=15), "stride"), (dict(R=-1), "rows"), (dict(rows=None), "null"), (dict(position=None), "null"),
-    (dict(y=None), "null"), (dict(rows=P + 1), "aligned"), (dict(position=P + 2), "aligned"), (dict(w=P + 2), "aligned"),
+    (dict(y_dtype=3), "y_dtype"), (dict(ldr=15), "stride"), (dict(rows=0), "null"), (dict(position=0), "null"),
+    (dict(y=0), "null"), (dict(rows=P + 1), "aligned"), (dict(position=P + 2), "aligned"), (dict(weights=P + 2), "aligned"),
     (dict(y=P + 1), "aligned"),
 ])
 def test_unpermute(lib, kw, word):
     from ccut._lib import CCQ_EINVAL, last_error
 
-    a = dict(rows=P, dtype=2, ldr=16, R=8, position=P, w=P, y=P, y_dtype=2, T=4, k=2, H=16)
-    a.update(kw)
-    assert lib.ccq_moe_unpermute(*a.values(), None) == CCQ_EINVAL and word in last_error()
+    assert lib.ccq_moe_unpermute(_permute(**kw)) == CCQ_EINVAL and word in last_error()
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(dtype=7), "dtype"), (dict(k=65), "k="), (dict(T=-2), "T="), (dict(H=0), "H="), (dict(ldr=15), "stride"),
-    (dict(ldy=15), "stride"), (dict(dy=None), "null"), (dict(rows=None), "null"), (dict(w=None), "null"),
-    (dict(d_rows=None), "null"), (dict(d_w=None), "null"), (dict(position=None), "null"), (dict(dy=P + 1), "aligned"),
-    (dict(d_rows=P + 1), "aligned"), (dict(d_w=P + 2), "aligned"),
+    (dict(ldr=15), "stride"), (dict(ldx=15), "stride"), (dict(x=0), "null"), (dict(rows=0), "null"), (dict(weights=0), "null"),
+    (dict(y=0), "null"), (dict(d_weights=0), "null"), (dict(position=0), "null"), (dict(x=P + 1), "aligned"),
+    (dict(y=P + 1), "aligned"), (dict(d_weights=P + 2), "aligned"),
 ])
 def test_unpermute_grad(lib, kw, word):
     from ccut._lib import CCQ_EINVAL, last_error
 
-    a = dict(dy=P, ldy=16, rows=P, ldr=16, dtype=2, R=8, position=P, w=P, d_rows=P, d_w=P, T=4, k=2, H=16)
-    a.update(kw)
-    assert lib.ccq_moe_unpermute_grad(*a.values(), None) == CCQ_EINVAL and word in last_error()
+    assert lib.ccq_moe_unpermute_grad(_permute(**kw)) == CCQ_EINVAL and word in last_error()
 
 
 def test_host_tensors_are_refused(lib):
