@@ -669,7 +669,7 @@ def moe_ffn_fp8row(x, ids, weights, experts: Fp8RowExperts, out_dtype: torch.dty
 # ---------------------------------------------------------------------------
 
 MAX_ASSIGNMENTS, MAX_SLOTS, MAX_SORT_EXPERTS = 1 << 20, 64, 1024
-_BARE_ASSIGNMENTS = 4096  # batches of up to this many are sorted without scratch
+_BARE_ASSIGNMENTS = 2048  # batches of up to this many are sorted without scratch
 _CODE = _dev.DTYPE_CODE
 _pack = PERMUTE_ARGS.pack
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32

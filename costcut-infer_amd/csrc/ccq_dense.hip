@@ -1143,8 +1143,10 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
   Plan q = {FEW, 16, 16, 1, p.K, false};
   const bool grouped = p.offsets != nullptr;
   const float pad_time = 3.f + (float)(p.M + (grouped ? (int64_t)p.E : 1) * p.W) * p.K * 4 / 4.5e6f;
-  // (few columns of few experts are too few tiles: T=2 of 2 of 35, K=2432 N=320 MID 11.8 us, FEW 7.6)
-  if (grouped && (rows > 16 || (dma && std::min<int64_t>(p.M, p.E) * cdiv(p.W, 64) >= 128))) {
+  // (few tiles do not fill the card: 10 of K=2432, T=2 N=320, MID 12.4 us, FEW 6.1; 96 of K=2048, T=4 N=2x768, 11.3
+  // and 8.7; 192, T=8, 11.9 and 12.5; 256 of K=768 7.6 and 8.1; 384, T=16, 20.9 and 22.8; 128 of K=4096 18.6 and 14.8, 512
+  // 55.5 and 54.1)
+  if (grouped && (rows > 16 || (dma && std::min<int64_t>(p.M, p.E) * cdiv(p.W, 64) >= 160))) {
     // unaligned rows run at some 300 TFLOP/s, aligned ones at 700
     q.pad = !dma && can_pad && 2.f * p.M * p.W * p.K * 1.9e-9f > pad_time;
     // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 139

@@ -132,9 +132,9 @@ def test_permute(lib, kw, word):
 
 def test_permute_workspace(lib):
     """What the Python entry point counts on."""
-    for T, k in ((1, 1), (64, 64), (4096, 1), (512, 8), (585, 7)):
+    for T, k in ((1, 1), (32, 64), (2048, 1), (256, 8), (292, 7)):
         assert lib.ccq_moe_permute_workspace_size(T, k, 1024) == 0
-    for T, k in ((4097, 1), (1 << 20, 1), (1 << 14, 64), (586, 7)):
+    for T, k in ((2049, 1), (1 << 20, 1), (1 << 14, 64), (293, 7)):
         assert lib.ccq_moe_permute_workspace_size(T, k, 1) > 0
 
 
