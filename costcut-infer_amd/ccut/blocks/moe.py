@@ -713,9 +713,9 @@ def _positions(plan: Permutation, rows: torch.Tensor, index: int) -> torch.Tenso
 
 
 def _routing_weights(weights: torch.Tensor, position: torch.Tensor, index: int) -> torch.Tensor:
-    if weights.shape != position.shape or weights.get_device() != index or not weights.is_floating_point():
-        raise ValueError(f"weights must be floats {tuple(position.shape)} on {position.device}, got {weights.dtype} "
-                         f"{tuple(weights.shape)} on {weights.device}")
+    if weights is None or weights.shape != position.shape or weights.get_device() != index or not weights.is_floating_point():
+        got = "None" if weights is None else f"{weights.dtype} {tuple(weights.shape)} on {weights.device}"
+        raise ValueError(f"weights must be floats {tuple(position.shape)} on {position.device}, got {got}")
     return weights if weights.dtype == _F32 and weights.is_contiguous() else weights.float().contiguous()
 
 
@@ -726,7 +726,8 @@ def moe_permute(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[t
     are converted) on the device -> ``(rows [T * k, H], Permutation)``.
     Assignments whose id is outside ``[0, num_experts)`` are left out; as many
     rows of zeros stand at the end.  ``T * k <= 2^20``, ``k <= 64``, at most
-    1024 experts."""
+    1024 experts.  Values only, here and in :func:`moe_unpermute`: their
+    gradients are the calls named ``_backward``."""
     index = x.get_device()
     if not is_current(index):
         with torch.cuda.device(index):

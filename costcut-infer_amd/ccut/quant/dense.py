@@ -106,6 +106,10 @@ def _dense(x, offsets, w, bias, act, gated: bool, residual, out, out_dtype):
             raise ValueError("out must hold its rows one after the other, each of them dense")
         if rows_overlap(yp, ycode, ldy, N, xp, DTYPE_CODE[dtype], ldx, K, M):
             raise ValueError("out overlaps x")
+        end = yp + ((M - 1) * ldy + N) * out.element_size()
+        for t in (w, bias, offsets):
+            if t is not None and M and t.data_ptr() < end and yp < t.data_ptr() + t.numel() * t.element_size():
+                raise ValueError("out overlaps w, bias or offsets")
     rp = ldr = 0
     if residual is not None:
         if residual.dtype != out_dtype or residual.shape != y_shape or residual.get_device() != index:
@@ -146,8 +150,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *
     ``"relu"``, ``"gelu"``, ``"gelu_tanh"`` or ``"silu"``; ``bias`` of any
     float type; ``residual`` of the output's type (``out_dtype``, default
     ``out``'s or x's) and shape.  ``out`` is written where given: it may be
-    ``residual``, but no other view of it or of ``x``.  Rows may have any
-    stride; ``w`` and ``bias`` that are not dense are copied."""
+    ``residual``, but no other view of it or of ``x``, and must not lie
+    around ``w`` or ``bias``.  Rows may have any stride; ``w`` and ``bias``
+    that are not dense are copied."""
     return _dense(x, None, w, bias, act, bool(gated), residual, out, out_dtype)
 
 
@@ -157,8 +162,10 @@ def linear_grouped(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, bias
     """:func:`linear` of rows sorted by expert: rows ``offsets[e]`` to
     ``offsets[e + 1]`` of ``x [rows, K]`` with ``w[e]`` of ``w [E, N, K]``
     (gated: ``[E, 2N, K]``) and ``bias[e]``.  ``offsets [E + 1]`` (int32, on
-    the device, rising, as ``moe_permute`` returns them; the host does not
-    read it).  Rows of the result from ``offsets[E]`` on are zeros."""
+    the device, rising from 0, as ``moe_permute`` returns them; the host does
+    not read it; a row that no pair of them covers before the last one is not
+    written).  Rows of the
+    result from ``offsets[E]`` on are zeros."""
     if offsets is None:
         raise ValueError("linear_grouped needs offsets")
     return _dense(x, offsets, w, bias, act, bool(gated), None, out, out_dtype)

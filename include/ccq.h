@@ -776,9 +776,9 @@ typedef struct ccq_moe_permute_args {
 int ccq_moe_permute(const ccq_moe_permute_args* args);
 
 /* y[t] = sum over s of weights[t, s] * rows[position[t, s]] (weights null: 1
- * each), float32 sums in slot order, y [T, H] of y_dtype (dense) rounded once;
- * positions outside [0, T k) contribute nothing.  Without weights also the gradient of
- * x in ccq_moe_permute, rows being that of its rows. */
+ * each), float32 sums in slot order, y [T, H] of y_dtype (dense, no part of
+ * rows) rounded once; positions outside [0, T k) contribute nothing.  Without
+ * weights also the gradient of x in ccq_moe_permute, rows being that of its rows. */
 int ccq_moe_unpermute(const ccq_moe_permute_args* args);
 
 /* The gradients of ccq_moe_unpermute from x, that of its y: y [T k, H] (dense, of
@@ -801,8 +801,8 @@ int ccq_moe_unpermute_grad(const ccq_moe_permute_args* args);
  * bias [W] of bias_dtype or null; residual [M, N] of y_dtype or null; y [M, N] of
  * y_dtype; row strides ldx, ldr, ldy in elements, w dense, any element alignment.
  * Grouped: w [num_experts, W, K], bias [num_experts, W], offsets
- * [num_experts + 1].  residual may be y; y must not overlap x or another view of
- * residual.  M, K, N <= 2^20, num_experts <= 1024. */
+ * [num_experts + 1].  residual may be y; y must not overlap x, w, bias, offsets or
+ * another view of residual.  M, K, N <= 2^20, num_experts <= 1024. */
 typedef struct ccq_dense_args {
   const void* x;
   const void* w;
@@ -830,8 +830,8 @@ size_t ccq_dense_linear_grouped_workspace_size(const ccq_dense_args* args);
 int ccq_dense_linear(const ccq_dense_args* args);
 
 /* ccq_dense_linear where rows offsets[e] .. offsets[e + 1] - 1 of x take w[e] and
- * bias[e] (offsets within [0, M] and rising, as ccq_moe_permute makes them; read
- * on the device); rows of y from offsets[num_experts] on are zeros. */
+ * bias[e] (offsets rising from 0 within [0, M], as ccq_moe_permute makes them;
+ * read on the device); rows of y from offsets[num_experts] on are zeros. */
 int ccq_dense_linear_grouped(const ccq_dense_args* args);
 
 #ifdef __cplusplus

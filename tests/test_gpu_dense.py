@@ -303,13 +303,69 @@ def test_graphs_and_streams(gpu):
         assert torch.equal(y, call(cs[0]))
 
 
+@pytest.mark.parametrize("M,K,ldx", [(300, 128, (1 << 23) - 8), (300, 128, (1 << 23) + 8), (12, 128, (1 << 28) + 8),
+                                     (40, 128, (1 << 23) + 8)])
+def test_rows_far_apart(gpu, M, K, ldx):
+    """Rows of x whose distance in a tile fits 32 bits by a little, and does not."""
+    from ccut.quant import dense
+
+    c = _inputs(M, K, 72, BF, False, None, False, BF)
+    far = torch.empty((M - 1) * ldx + K, dtype=BF, device=gpu).as_strided((M, K), (ldx, 1))
+    far.copy_(c["x"])
+    ref, bound = od.linear(c["x"], c["w"], None, "silu")
+    _close(dense.linear(far, c["w"].to(gpu), act="silu"), ref, bound)
+    del far
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_weights_beyond_32_bits(gpu, rows):
+    """The last of experts whose weights take 4.6 GiB, its rows and y behind 2^31 elements' worth of others."""
+    from ccut.quant import dense
+
+    E, K, N = 37, 4096, 8192
+    c = _inputs(rows, K, N, BF, True, None, False, BF)
+    w = torch.empty((E, 2 * N, K), dtype=BF, device=gpu)
+    w[E - 1] = c["w"].to(gpu)
+    offsets = torch.zeros(E + 1, dtype=torch.int32, device=gpu)
+    offsets[E] = rows
+    y = dense.linear_grouped(c["x"].to(gpu), offsets, w, act="silu", gated=True)
+    ref, bound = od.linear(c["x"], c["w"], None, "silu", True)
+    _close(y, ref, bound)
+    del w
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M", [4, 40])
+def test_gated_halves_beyond_32_bits(gpu, M):
+    """The up half of w more than 2^31 elements behind the gate's."""
+    from ccut.quant import dense
+
+    K, N = 4096, (1 << 19) + 40
+    g = torch.Generator().manual_seed(M)
+    x, ws = torch.randn((M, K), generator=g).to(BF), (torch.randn((2, 24, K), generator=g) * K ** -0.5).to(BF)
+    w = torch.zeros((2, N, K), dtype=BF, device=gpu)
+    w[:, -24:] = ws.to(gpu)
+    y = dense.linear(x.to(gpu), w.view(2 * N, K), act="silu", gated=True)
+    ref, bound = od.linear(x, ws.reshape(48, K), None, "silu", True)
+    _close(y[:, -24:], ref, bound)
+    assert (y[:, :-24] == 0).all()
+    del w, y
+    torch.cuda.empty_cache()
+
+
 def test_refusals(gpu):
     from ccut.quant import dense
 
     x, w = torch.zeros((4, 64), dtype=BF, device=gpu), torch.zeros((32, 64), dtype=BF, device=gpu)
     b, off = torch.zeros(32, device=gpu), torch.zeros(4, dtype=torch.int32, device=gpu)
     w3 = torch.zeros((3, 32, 64), dtype=BF, device=gpu)
-    for call in (lambda: dense.linear(x.float(), w), lambda: dense.linear(x, w.half()), lambda: dense.linear(x, w.cpu()),
+    square = torch.zeros((64, 64), dtype=BF, device=gpu)
+    for call in (lambda: dense.linear(x, square, out=square[8:12]),
+                 lambda: dense.linear(x, square, torch.zeros(64, dtype=BF, device=gpu), out=square[:4]),
+                 lambda: dense.linear(x[:1], w, b, out=b.view(1, 32), out_dtype=F32),
+                 lambda: dense.linear_grouped(x[:1], off, w3, out=w3[2, 3:4, :32]),
+                 lambda: dense.linear(x.float(), w), lambda: dense.linear(x, w.half()), lambda: dense.linear(x, w.cpu()),
                  lambda: dense.linear(x[:, :32], w), lambda: dense.linear(x, w[0]), lambda: dense.linear(x, w3),
                  lambda: dense.linear(x, w[:31], gated=True), lambda: dense.linear(x, w, act="tanh"),
                  lambda: dense.linear(x, w, b[:16]), lambda: dense.linear(x, w, b.double()),

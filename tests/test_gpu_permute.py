@@ -311,6 +311,37 @@ def test_graphs(gpu):
                 assert torch.equal(o, y)
 
 
+@pytest.mark.parametrize("T,k,H", [(1 << 17, 8, 8200), (1 << 20, 1, 8200)])
+def test_rows_beyond_32_bits(gpu, T, k, H):
+    """Rows that take 16 GiB, there and back; the second has more pieces than a row of the grid."""
+    from ccut.blocks import moe
+
+    E = 40
+    g = torch.Generator(device=gpu).manual_seed(T)
+    x = torch.randint(-4, 5, (T, 1), generator=g, device=gpu).to(BF) + torch.arange(H, device=gpu).remainder(3).to(BF)
+    ids = torch.randint(0, E, (T, k), generator=g, device=gpu)
+    rows, plan = moe.moe_permute(x, ids, E)
+    at = torch.empty(T * k, dtype=torch.int64, device=gpu)
+    at[torch.sort(ids.view(-1), stable=True).indices] = torch.arange(T * k, device=gpu)
+    assert torch.equal(plan.position.view(-1).long(), at)
+    for s in range(k):
+        at = plan.position[:, s].long()
+        for t in range(0, T, 1 << 17):
+            assert torch.equal(rows[at[t:t + (1 << 17)]], x[t:t + (1 << 17)])
+    y = moe.moe_permute_backward(rows, plan)
+    for t in range(0, T, 1 << 17):  # (small whole numbers: exact)
+        assert torch.equal(y[t:t + (1 << 17)], x[t:t + (1 << 17)] * k)
+    del y
+    w = torch.ones((T, k), device=gpu)
+    d_rows, d_w = moe.moe_unpermute_backward(x, rows, plan, w)
+    for t in range(0, T * k, 1 << 17):
+        assert torch.equal(d_rows[t:t + (1 << 17)], rows[t:t + (1 << 17)])
+    some = torch.cat([torch.arange(5), torch.arange(T - 5, T)]).to(gpu)
+    assert torch.equal(d_w[some].cpu(), x[some].double().square().sum(1).float().cpu()[:, None].expand(-1, k))
+    del rows, d_rows, x
+    torch.cuda.empty_cache()
+
+
 def test_refusals(gpu):
     from ccut.blocks import moe
 
@@ -334,6 +365,7 @@ def test_refusals(gpu):
                  lambda: moe.moe_unpermute_backward(x[:5], rows, plan, w),
                  lambda: moe.moe_unpermute_backward(x, rows[:-2], plan, w),
                  lambda: moe.moe_unpermute_backward(x, rows, plan, w[:3]),
+                 lambda: moe.moe_unpermute_backward(x, rows, plan, None),
                  lambda: moe.moe_ffn_dense(x, ids, w, ex), lambda: moe.moe_ffn_dense(x.to(BF)[:, :8], ids, w, ex),
                  lambda: moe.DenseExperts(ex.w_gate_up, ex.w_down.half()),
                  lambda: moe.DenseExperts(ex.w_gate_up[:, :8], ex.w_down),
