@@ -163,9 +163,8 @@ def linear_grouped(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, bias
     ``offsets[e + 1]`` of ``x [rows, K]`` with ``w[e]`` of ``w [E, N, K]``
     (gated: ``[E, 2N, K]``) and ``bias[e]``.  ``offsets [E + 1]`` (int32, on
     the device, rising from 0, as ``moe_permute`` returns them; the host does
-    not read it; a row that no pair of them covers before the last one is not
-    written).  Rows of the
-    result from ``offsets[E]`` on are zeros."""
+    not read it).  Rows of the result from ``offsets[E]`` on are zeros; others
+    that no two of the offsets hold between them are not written."""
     if offsets is None:
         raise ValueError("linear_grouped needs offsets")
     return _dense(x, offsets, w, bias, act, bool(gated), None, out, out_dtype)

@@ -1114,14 +1114,15 @@ struct Plan {
 // CU (0: there is room for one), and what a tile takes besides.  From K = 4096 and
 // 2048 over M = 32 .. 2048, N = 2048 .. 14336 (K=N=4096: M=256 RING 64 22.4 us, 128 29.5,
 // TILE 128 33.5; M=1024 52, 34, 36, RING 256 x 128 49; K=4096 N=14336: M=512 RING 256 x
-// 128 63, TILE 128 74.6, 256 x 192 74, 256 81; M=1024 TILE 128 138, 256 96.5).
+// 128 63, TILE 128 74.6, 256 x 192 74, 256 81; M=1024 TILE 128 138, 256 96.5; M=172 K=11376
+// N=9808: RING 64 131 us, 128 in three splits 101, 256 x 128 in three 84).
 struct Shape {
   Kind kind;
   int bm, bn;
   float one, two, tile;
 };
 constexpr Shape kShapes[] = {
-    {MID, 32, 64, 0.25f, 0.40f, 2.f},    {RING, 64, 64, 0.31f, 0.39f, 2.5f},   {RING, 128, 128, 0.46f, 0.f, 4.f},
+    {MID, 32, 64, 0.25f, 0.40f, 2.f},    {RING, 64, 64, 0.35f, 0.45f, 2.5f},   {RING, 128, 128, 0.46f, 0.f, 4.f},
     {RING, 256, 128, 0.90f, 0.f, 5.f},   {TILE, 128, 128, 0.72f, 0.97f, 5.f},  {TILE, 256, 192, 1.05f, 0.f, 6.f},
     {TILE, 256, 224, 1.30f, 0.f, 6.f},   {TILE, 256, 256, 1.42f, 0.f, 7.f},    {RAGGED, 64, 64, 0.6f, 0.65f, 3.f},
 };
@@ -1134,7 +1135,7 @@ float shape_time(const Shape& s, const DenseP& p, int64_t mtiles, int splits) {
   float t = (float)(groups / round) * (stages * full + s.tile);
   if (rest > 0) t += stages * (rest <= 256 ? s.one : full) + s.tile;
   // the partial sums' way out and back, and a launch
-  if (splits > 1) t += 3.f + (float)splits * p.M * p.W * 8 / 4e6f;
+  if (splits > 1) t += 4.f + (float)splits * p.M * p.W * 8 / 4e6f;
   return t;
 }
 
@@ -1183,7 +1184,7 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
     if (p.gated && s.bn == 224) continue;  // a wave's 112 rows are no whole pairs of gate and up
     const int64_t stages = cdiv(p.K, DN_BK);
     for (int splits = 1; splits <= 16; ++splits) {
-      if (splits > 1 && (stages / splits < 4 || s.bm == 256)) break;
+      if (splits > 1 && (stages / splits < 4 || (s.kind == TILE && s.bm == 256))) break;
       const float t = shape_time(s, p, cdiv(p.M, s.bm), splits) + (pad ? pad_time : 0.f);
       if (best == 0.f || t < best) {
         best = t;
