@@ -1139,6 +1139,26 @@ float shape_time(const Shape& s, const DenseP& p, int64_t mtiles, int splits) {
   return t;
 }
 
+// The same for rows grouped by expert, whose workgroups end one by one: each expert
+// leaves 0.6 of a tile more than its rows fill, and the last round counts half a round
+// more.  The weights' way from memory costs every shape alike.  Over 150 products (8 to
+// 256 experts of 1/2 to 450 rows, K = 304 .. 14336) its choice takes 1.1 % more than the
+// best one (8 experts, 4096 -> 2 x 14336: 1024 rows TILE 256 x 192 403 us,
+// TILE 128 588; 8, 14336 -> 4096: 384 rows RING 128 173, RING 64 232; 128, 2048 -> 2 x 768: 48
+// rows each TILE 128 155, RING 64 173; 16 rows MID 139, TILE 128 147; 8, 2048 -> 784: 576 rows
+// RING 64 14.4, TILE 128 28).
+constexpr Shape kGroupShapes[] = {
+    {MID, 32, 64, 0.30f, 0.46f, 1.f},    {RING, 64, 64, 0.36f, 0.50f, 2.f},  {RING, 128, 128, 0.45f, 0.f, 4.5f},
+    {TILE, 128, 128, 0.67f, 0.93f, 3.5f}, {TILE, 256, 192, 0.88f, 0.f, 6.f}, {TILE, 256, 256, 1.16f, 0.f, 8.f},
+};
+float group_time(const Shape& s, const DenseP& p) {
+  const float experts = (float)std::min<int64_t>(p.M, p.E), stages = (float)cdiv(p.K, DN_BK);
+  const float groups = std::max(experts, (float)p.M / s.bm + 0.6f * experts) * cdiv(p.W, s.bn);
+  const float round = s.two > 0.f ? 512 : 256, whole = stages * (s.two > 0.f ? s.two : s.one) + s.tile;
+  if (groups <= round) return groups <= 256 ? stages * s.one + s.tile : whole;
+  return (groups / round + 0.5f) * whole;
+}
+
 // rows: of the batch, or of an expert on average; dma: x and w are aligned; can_pad: they can be made so
 Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
   Plan q = {FEW, 16, 16, 1, p.K, false};
@@ -1150,23 +1170,15 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
   if (grouped && (rows > 16 || (dma && std::min<int64_t>(p.M, p.E) * cdiv(p.W, 64) >= 160))) {
     // unaligned rows run at some 300 TFLOP/s, aligned ones at 700
     q.pad = !dma && can_pad && 2.f * p.M * p.W * p.K * 1.9e-9f > pad_time;
-    // by the rows of an expert on average (128 experts, 2048 -> 2 x 768, and 64, 1408 -> 2048): MID 32 up to 24 (16 rows: 139
-    // us, RING 64: 143; 1 to 6 rows as FEW), RING 64 up to 48 (32 skewed rows: 161, MID 32: 169; 64 rows: TILE 128 160, RING 64
-    // 171), TILE 256 from 200 on (256 rows: 238, TILE 128: 275; 128 rows: 216 and 186)
-    q.kind = !dma && !q.pad ? RAGGED : rows <= 24 ? MID : rows <= 48 ? RING : TILE;
-    q.bm = q.kind == RAGGED ? 64 : rows <= 24 ? 32 : rows <= 48 ? 64 : rows < 200 ? 128 : 256;
-    q.bn = q.kind == TILE ? q.bm : 64;
-    if (q.kind == TILE) {
-      // where the products take longer than the weights' way from memory, the tiles' rounds count as in a batch (14
-      // experts of 534 rows, K=1872 N=1600: TILE 256 in two rounds 98 us, TILE 128 91; 36 of 316, K=528 N=2x528: 51, 38)
-      const Shape* best = nullptr;
-      float best_time = 0.f;
-      for (const Shape& s : kShapes) {
-        if (s.kind != TILE || s.bn == 224) continue;
-        const float t = shape_time(s, p, p.E * cdiv(rows, s.bm), 1);
-        if (best == nullptr || t < best_time) best = &s, best_time = t;
-      }
-      if (best_time > (float)p.E * p.W * p.K * 2 / 4.5e6f) q.bm = best->bm, q.bn = best->bn;
+    if (!dma && !q.pad) {
+      q.kind = RAGGED, q.bm = q.bn = 64;
+      return q;
+    }
+    float best = 0.f;
+    for (const Shape& s : kGroupShapes) {
+      if (s.kind == RING && s.bm == 128 && rows < 32) continue;  // (67 experts of 17 rows, K=4064 N=2x576: 154 us, MID 130)
+      const float t = group_time(s, p);
+      if (best == 0.f || t < best) best = t, q.kind = s.kind, q.bm = s.bm, q.bn = s.bn;
     }
     return q;
   }
