@@ -84,7 +84,7 @@ def test_many_tiles(gpu, M, K, N, gated):
     _run(gpu, c, gated, "silu" if gated else None)
 
 
-@pytest.mark.parametrize("M,K,N", [(65, 8192, 64), (128, 14336, 128), (93, 4097, 131), (200, 5000, 300)])
+@pytest.mark.parametrize("M,K,N", [(65, 8192, 64), (128, 14336, 128), (93, 4097, 131), (200, 5000, 300), (135, 6664, 5524)])
 def test_long_inner(gpu, M, K, N):
     for gated, dt in ((False, BF), (True, F16)):
         _run(gpu, _inputs(M, K, N, dt, gated, "same", True, dt), gated, "relu")
@@ -196,6 +196,24 @@ def test_grouped(gpu, T, k, E, K, N, dt):
         y = dense.linear_grouped(c["x"].to(gpu), offsets.to(gpu), c["w"].to(gpu), _up(c["bias"], gpu), act=act, gated=gated)
         _close(y, ref, bound)
         assert (y[int(offsets[-1]):] == 0).all()
+
+
+@pytest.mark.parametrize("M,E,K,W", [(4536, 70, 136, 130), (1746, 16, 136, 912), (4134, 70, 280, 258), (4403, 40, 144, 1052),
+                                     (4286, 40, 136, 1468)])
+@pytest.mark.parametrize("gated,act,bias", [(False, "relu", "same"), (True, "silu", F32)])
+def test_tiles_of_groups(gpu, M, E, K, W, gated, act, bias):
+    """Sizes for each shape of tile, experts of uneven rows, K's last stage cut short, rows of no expert."""
+    from ccut.quant import dense
+
+    g = torch.Generator().manual_seed(M)
+    cuts = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(0, M - 50, (E,), generator=g).sort().values])
+    offsets = cuts.to(torch.int32)
+    c = _inputs(M, K, W // 2 if gated else W, BF, gated, bias, False, BF, E=E)
+    c["x"][int(offsets[-1]):] = float("nan")  # not read
+    ref, bound = od.grouped(c["x"].nan_to_num(0.0), offsets, c["w"], c["bias"], act, gated)
+    y = dense.linear_grouped(c["x"].to(gpu), offsets.to(gpu), c["w"].to(gpu), _up(c["bias"], gpu), act=act, gated=gated)
+    _close(y, ref, bound)
+    assert (y[int(offsets[-1]):] == 0).all()
 
 
 @pytest.mark.parametrize("counts", [[0, 0, 0], [0, 5, 0], [200, 0, 1], [1, 1, 1], [16, 32, 64], [17, 33, 65], [0, 0, 700],
