@@ -12,7 +12,7 @@
 //
 // dense_few_kernel   up to 16 rows: w goes from memory to registers, the waves of a
 //                    workgroup share K and add up at the end.
-// dense_mid_kernel   up to 32 rows, through a ring of stages in LDS.
+// dense_mid_kernel   tiles of 32 rows, through a ring of stages in LDS.
 // dense_tile_kernel  large tiles, the products interleaved with the next ones' reads.
 // dense_ring_kernel  smaller ones, more stages on their way.
 // dense_ragged_kernel  rows at any alignment.
