@@ -274,7 +274,17 @@ __device__ __forceinline__ u32x4 dn_load8(const uint16_t* row, int k, int K) {
 // values of row l % 16 from column 8 (l / 16) on, so neighbouring loads of a wave
 // fill whole lines.  M=1 K=2048 N=5632 7.2 us among others; M=16 K=4096 N=2x14336
 // 48.9 us, 4.8 TB/s.
-template <int DT, int MT, int NF, int U, int WAVES, bool WHOLE>
+//
+// Loads of 16 bytes at odd elements run at half the rate of those at dwords, so where
+// rows start at odd ones (ROWS == ODD) their lanes load the dwords around their eight
+// values: four from the one that holds the first, and the one that holds the last (a
+// lane at an even element loads its own last dword again), moved by a value when they
+// are multiplied.  A dword that holds a value of a row lies in the row's allocation.
+// M=8 K=2049: N=8192 20.7 us by loads at odd elements, 11.1 by dwords (K=2050 10.7);
+// N=20480 52 and 32.
+enum Rows { WHOLE, EVEN, ODD };  // K in whole eights; rows from whole dwords on; any
+
+template <int DT, int MT, int NF, int U, int WAVES, Rows ROWS>
 __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
   constexpr int BM = 16 * MT, THREADS = 64 * WAVES, STEP = 32 * U;
@@ -310,11 +320,39 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(const DenseP p) {
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  struct Step {
+  struct Pieces {
     u32x4 w[NF][U], x[MT][U];
   };
+  struct OddPieces : Pieces {
+    uint32_t wl[NF][U], xl[MT][U];  // the dwords of the last values
+  };
+  using Step = std::conditional_t<ROWS == ODD, OddPieces, Pieces>;
+  const auto odd = [](const uint16_t* row) { return (uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1; };
   auto load = [&](Step& s, int k0) {
-    if (k0 + STEP <= p.K) {
+    if constexpr (ROWS == ODD) {
+      const auto full = [&](u32x4& v, uint32_t& last, const uint16_t* row, int k) {
+        const uint32_t o = odd(row);
+        __builtin_memcpy(&v, row + k - o, 16);
+        __builtin_memcpy(&last, row + k + 6 + o, 4);
+      };
+      const auto tail = [&](u32x4& v, uint32_t& last, const uint16_t* row, int k) {
+        v = dn_load8<false>(row, k, p.K - k8);
+        last = v[3] >> 16;
+        if (odd(row)) v = u32x4{v[0] << 16, v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16};
+      };
+      const auto all = [&](const auto& one) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+          for (int u = 0; u < U; ++u) one(s.w[f][u], s.wl[f][u], w[f], k0 + 32 * u);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int u = 0; u < U; ++u) one(s.x[m][u], s.xl[m][u], x[m], k0 + 32 * u);
+      };
+      if (k0 + STEP <= p.K) all(full);
+      else all(tail);
+    } else if (k0 + STEP <= p.K) {
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -328,20 +366,29 @@ __global__ __launch_bounds__(64 * WAVES) void dense_few_kernel(const DenseP p) {
       for (int u = 0; u < U; ++u) {
         const int k = k0 + 32 * u;
 #pragma unroll
-        for (int f = 0; f < NF; ++f) s.w[f][u] = dn_load8<WHOLE>(w[f], k, p.K - k8);
+        for (int f = 0; f < NF; ++f) s.w[f][u] = dn_load8<ROWS == WHOLE>(w[f], k, p.K - k8);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) s.x[m][u] = dn_load8<WHOLE>(x[m], k, p.K - k8);
+        for (int m = 0; m < MT; ++m) s.x[m][u] = dn_load8<ROWS == WHOLE>(x[m], k, p.K - k8);
       }
     }
   };
   auto multiply = [&](const Step& s) {
+    const auto value = [&](const u32x4& v, uint32_t last, const uint16_t* row) {
+      const uint32_t by = 16 * odd(row);
+      return __builtin_bit_cast(Vec, u32x4{__builtin_amdgcn_alignbit(v[1], v[0], by), __builtin_amdgcn_alignbit(v[2], v[1], by),
+                                           __builtin_amdgcn_alignbit(v[3], v[2], by), __builtin_amdgcn_alignbit(last, v[3], by)});
+    };
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          acc[f][m] = dn_mfma(__builtin_bit_cast(Vec, s.w[f][u]), __builtin_bit_cast(Vec, s.x[m][u]), acc[f][m]);
+        for (int m = 0; m < MT; ++m) {
+          if constexpr (ROWS == ODD)
+            acc[f][m] = dn_mfma(value(s.w[f][u], s.wl[f][u], w[f]), value(s.x[m][u], s.xl[m][u], x[m]), acc[f][m]);
+          else
+            acc[f][m] = dn_mfma(__builtin_bit_cast(Vec, s.w[f][u]), __builtin_bit_cast(Vec, s.x[m][u]), acc[f][m]);
+        }
   };
   constexpr int STRIDE = WAVES * STEP;
   int k0 = wave * STEP;
@@ -1214,10 +1261,13 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
 
 template <int DT, int NF, int U, int WAVES>
 void launch_few(const DenseP& p, dim3 grid, hipStream_t st) {
-  if (p.K % 8 == 0)
-    launch(dense_few_kernel<DT, 1, NF, U, WAVES, true>, grid, dim3(64 * WAVES), 0, st, p);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w);
+  if (at & 2 || p.K & 1 || (p.M > 1 && p.ldx & 1))
+    launch(dense_few_kernel<DT, 1, NF, U, WAVES, ODD>, grid, dim3(64 * WAVES), 0, st, p);
+  else if (p.K % 8 != 0)
+    launch(dense_few_kernel<DT, 1, NF, U, WAVES, EVEN>, grid, dim3(64 * WAVES), 0, st, p);
   else
-    launch(dense_few_kernel<DT, 1, NF, U, WAVES, false>, grid, dim3(64 * WAVES), 0, st, p);
+    launch(dense_few_kernel<DT, 1, NF, U, WAVES, WHOLE>, grid, dim3(64 * WAVES), 0, st, p);
 }
 
 template <int DT>

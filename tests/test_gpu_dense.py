@@ -113,6 +113,29 @@ def test_strides_and_alignment(gpu, M):
             assert (o[rest] == 7.0).all()
 
 
+@pytest.mark.parametrize("M", [1, 5, 16, 40])
+@pytest.mark.parametrize("K", [7, 31, 257, 511, 1024, 2049])
+def test_odd_elements(gpu, M, K):
+    """Rows of x and w that start at odd and even elements, NaN around them."""
+    from ccut.quant import dense
+
+    N = 70
+    for shift, pad in ((0, 0), (1, 0), (0, 1), (1, 2), (3, 1), (2, 0)):
+        c = _inputs(M, K, N, BF, False, None, False, BF, seed=shift)
+        x = torch.full((M * (K + pad) + 16,), float("nan"), dtype=BF, device=gpu)[shift:shift + M * (K + pad)]
+        x = x.view(M, K + pad)[:, :K].copy_(c["x"])
+        w = torch.full((N * K + 16,), float("nan"), dtype=BF, device=gpu)[3 - shift:3 - shift + N * K].view(N, K)
+        w.copy_(c["w"])
+        ref, bound = od.linear(c["x"], c["w"])
+        _close(dense.linear(x, w), ref, bound)
+        if M > 1:
+            offsets = torch.tensor([0, M // 2, M], dtype=torch.int32, device=gpu)
+            y = dense.linear_grouped(x, offsets, w.view(2, N // 2, K))
+            left, right = od.linear(c["x"][:M // 2], c["w"][:N // 2]), od.linear(c["x"][M // 2:], c["w"][N // 2:])
+            _close(y[:M // 2], *left)
+            _close(y[M // 2:], *right)
+
+
 def test_transposed_and_leading_dimensions(gpu):
     from ccut.quant import dense
 
