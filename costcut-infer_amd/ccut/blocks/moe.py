@@ -887,7 +887,12 @@ def moe_ffn_dense(x: torch.Tensor, ids, weights, experts: DenseExperts, out_dtyp
     ``quant.dense.linear_grouped`` twice, :func:`moe_unpermute`).  ``x
     [T, H]`` of the experts' type; the rows between the steps are of that
     type too.  ``shared`` ([T, H], the shared expert's output): ``shared_gate
-    * shared`` is added to the sum, in float32."""
+    * shared`` is added to the sum, in float32.  Works on x's device; ``ids``,
+    ``weights`` and ``shared`` from elsewhere are copied there."""
+    index = x.get_device()
+    if not is_current(index):
+        with torch.cuda.device(index):
+            return moe_ffn_dense(x, ids, weights, experts, out_dtype, shared=shared, shared_gate=shared_gate)
     if x.dtype != experts.w_down.dtype or x.dim() != 2 or x.shape[1] != experts.hidden:
         raise ValueError(f"x must be {experts.w_down.dtype} [T, {experts.hidden}], got {x.dtype} {tuple(x.shape)}")
     rows, plan = moe_permute(x, _dev.to_device(ids), experts.num_experts)
@@ -905,5 +910,9 @@ def moe_forward_dense(x: torch.Tensor, router_logits, experts: DenseExperts, top
                       out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Routed MoE layer on 16-bit experts: ``topk_softmax`` then
     :func:`moe_ffn_dense`."""
+    index = x.get_device()
+    if not is_current(index):
+        with torch.cuda.device(index):
+            return moe_forward_dense(x, router_logits, experts, top_k, norm_topk_prob, out_dtype)
     w, ids = topk_softmax(router_logits, top_k, norm_topk_prob)
     return moe_ffn_dense(x, ids, w, experts, out_dtype)

@@ -1,0 +1,69 @@
+"""The layer of 16-bit experts and its container on the host: what reaches the
+kernels' entry points, and what is refused before (runs without a GPU)."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+class _Rows:
+    """Rows on a device that this machine does not have."""
+
+    dtype, shape = BF, (4, 8)
+
+    def __init__(self, index):
+        self.index = index
+
+    def dim(self):
+        return 2
+
+    def get_device(self):
+        return self.index
+
+
+@pytest.mark.parametrize("forward", [False, True])
+@pytest.mark.parametrize("current", [0, 1])
+def test_layer_works_on_its_rows_device(monkeypatch, current, forward):
+    """Routing and weights that are converted on the way go to the rows' device, whichever is current."""
+    from ccut.blocks import moe
+
+    state, seen = [current], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state[0] = state[0], self.index
+
+        def __exit__(self, *exc):
+            state[0] = self.before
+
+    def on_current(name, result):
+        def step(*args, **kw):
+            seen.append((name, state[0]))
+            return result
+
+        return step
+
+    plan = SimpleNamespace(offsets=None)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(moe, "is_current", lambda index: index == state[0])
+    monkeypatch.setattr(moe._dev, "to_device", on_current("to_device", None))
+    monkeypatch.setattr(moe, "topk_softmax", on_current("topk", (None, None)))
+    monkeypatch.setattr(moe, "moe_permute", on_current("permute", (None, plan)))
+    monkeypatch.setattr(moe.dense, "linear_grouped", on_current("linear", None))
+    monkeypatch.setattr(moe, "moe_unpermute", on_current("unpermute", "y"))
+    ex = moe.DenseExperts(torch.zeros((3, 12, 8), dtype=BF), torch.zeros((3, 8, 6), dtype=BF))
+    if forward:
+        assert moe.moe_forward_dense(_Rows(1), None, ex, 2) == "y"
+    else:
+        assert moe.moe_ffn_dense(_Rows(1), None, None, ex) == "y"
+    assert [name for name, _ in seen] == ["topk"] * forward + ["to_device", "permute", "linear", "linear", "to_device",
+                                                               "unpermute"]
+    assert all(index == 1 for _, index in seen) and state[0] == current
