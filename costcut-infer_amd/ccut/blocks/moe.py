@@ -831,7 +831,9 @@ class DenseExperts:
     """All experts of one MoE layer in 16 bits, resident in HBM: ``w_gate_up
     [E, 2I, H]`` (each expert's gate rows, then its up rows), ``w_down
     [E, H, I]``, both float16 or both bfloat16, and where the model has them
-    the biases ``b_gate_up [E, 2I]`` and ``b_down [E, H]``."""
+    the biases ``b_gate_up [E, 2I]`` and ``b_down [E, H]``.  Strided ones
+    (experts stored ``[E, in, out]``, as transposed views) are made dense
+    here, once: the products would copy them at every call."""
 
     w_gate_up: torch.Tensor
     w_down: torch.Tensor
@@ -852,6 +854,10 @@ class DenseExperts:
         for b, w, what in ((self.b_gate_up, gu, "b_gate_up"), (self.b_down, d, "b_down")):
             if b is not None and b.shape != w.shape[:-1]:
                 raise ValueError(f"{what} must be {tuple(w.shape[:-1])}, got {tuple(b.shape)}")
+        for name in ("w_gate_up", "w_down", "b_gate_up", "b_down"):
+            t = getattr(self, name)
+            if t is not None:
+                setattr(self, name, t.contiguous())
 
     @staticmethod
     def from_stacks(gate, up, down, act: str = "silu") -> "DenseExperts":

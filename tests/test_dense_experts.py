@@ -67,3 +67,21 @@ def test_layer_works_on_its_rows_device(monkeypatch, current, forward):
     assert [name for name, _ in seen] == ["topk"] * forward + ["to_device", "permute", "linear", "linear", "to_device",
                                                                "unpermute"]
     assert all(index == 1 for _, index in seen) and state[0] == current
+
+
+def test_strided_weights_are_made_dense_once():
+    """Experts stored [E, in, out] come as transposed views: the container holds dense rows, so that no call copies
+    them; dense ones are kept as they are."""
+    from ccut.blocks import moe
+
+    g = torch.Generator().manual_seed(0)
+    gu, d = torch.randn((3, 8, 12), generator=g).to(BF), torch.randn((3, 6, 8), generator=g).to(BF)
+    bgu, bd = torch.randn((12, 3), generator=g), torch.randn((3, 16), generator=g)[:, ::2]
+    ex = moe.DenseExperts(gu.transpose(1, 2), d.transpose(1, 2), bgu.t(), bd)
+    for t, ref in ((ex.w_gate_up, gu.transpose(1, 2)), (ex.w_down, d.transpose(1, 2)), (ex.b_gate_up, bgu.t()),
+                   (ex.b_down, bd)):
+        assert t.is_contiguous() and torch.equal(t, ref)
+    again = moe.DenseExperts(ex.w_gate_up, ex.w_down, ex.b_gate_up, ex.b_down)
+    assert again.w_gate_up is ex.w_gate_up and again.w_down is ex.w_down
+    assert again.b_gate_up is ex.b_gate_up and again.b_down is ex.b_down
+    assert moe.DenseExperts(ex.w_gate_up, ex.w_down).b_down is None
