@@ -901,6 +901,8 @@ def moe_ffn_dense(x: torch.Tensor, ids, weights, experts: DenseExperts, out_dtyp
             return moe_ffn_dense(x, ids, weights, experts, out_dtype, shared=shared, shared_gate=shared_gate)
     if x.dtype != experts.w_down.dtype or x.dim() != 2 or x.shape[1] != experts.hidden:
         raise ValueError(f"x must be {experts.w_down.dtype} [T, {experts.hidden}], got {x.dtype} {tuple(x.shape)}")
+    if out_dtype is not None and out_dtype not in _CODE:
+        raise ValueError(f"y must be float32, float16 or bfloat16, got {out_dtype}")
     rows, plan = moe_permute(x, _dev.to_device(ids), experts.num_experts)
     h = dense.linear_grouped(rows, plan.offsets, experts.w_gate_up, experts.b_gate_up, act=experts.act, gated=True)
     down = dense.linear_grouped(h, plan.offsets, experts.w_down, experts.b_down)

@@ -85,3 +85,25 @@ def test_strided_weights_are_made_dense_once():
     assert again.w_gate_up is ex.w_gate_up and again.w_down is ex.w_down
     assert again.b_gate_up is ex.b_gate_up and again.b_down is ex.b_down
     assert moe.DenseExperts(ex.w_gate_up, ex.w_down).b_down is None
+
+
+@pytest.mark.parametrize("shared", [None, "rows"])
+@pytest.mark.parametrize("out_dtype", [torch.int32, torch.float64, torch.bool])
+def test_layer_refuses_other_types_of_y(monkeypatch, out_dtype, shared):
+    """With and without the shared expert's rows, before anything is computed."""
+    from ccut.blocks import moe
+
+    x = _Rows(0)
+    monkeypatch.setattr(moe, "is_current", lambda index: True)
+    plan = SimpleNamespace(offsets=None)
+    monkeypatch.setattr(moe._dev, "to_device", lambda *args: None)
+    monkeypatch.setattr(moe, "moe_permute", lambda *args: (None, plan))
+    monkeypatch.setattr(moe.dense, "linear_grouped", lambda *args, **kw: None)
+    monkeypatch.setattr(moe, "moe_unpermute", lambda rows, plan, weights, dtype: torch.zeros((4, 8), dtype=dtype))
+    monkeypatch.setattr(moe, "_shared_rows", lambda *args: None)
+    monkeypatch.setattr(moe, "shared_expert_add", lambda *args: None)
+    ex = moe.DenseExperts(torch.zeros((3, 12, 8), dtype=BF), torch.zeros((3, 8, 6), dtype=BF))
+    with pytest.raises(ValueError, match="y must be"):
+        moe.moe_ffn_dense(x, None, None, ex, out_dtype, shared=shared)
+    for ok in (None, F32, F16, BF):
+        assert moe.moe_ffn_dense(x, None, None, ex, ok, shared="rows").dtype == (ok or BF)
