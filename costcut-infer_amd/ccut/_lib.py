@@ -175,6 +175,7 @@ SIGNATURES: dict[str, tuple] = {
     "ccq_moe_unpermute_grad": (_int, [ctypes.c_char_p]),
     "ccq_dense_linear_workspace_size": (_sz, [ctypes.c_char_p]),  # DENSE_ARGS.pack(...)
     "ccq_dense_linear_grouped_workspace_size": (_sz, [ctypes.c_char_p]),
+    "ccq_dense_linear_kernel": (_int, [ctypes.c_char_p, _int, *[ctypes.POINTER(_int)] * 4]),
     "ccq_dense_linear": (_int, [ctypes.c_char_p]),
     "ccq_dense_linear_grouped": (_int, [ctypes.c_char_p]),
 }

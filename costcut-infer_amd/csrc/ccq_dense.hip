@@ -1149,7 +1149,7 @@ __global__ __launch_bounds__(256) void dense_pad_kernel(const PadP p) {
 }
 
 // ------------------------------------------------------------- dispatch --
-enum Kind { FEW, MID, RING, TILE, RAGGED };
+enum Kind { FEW, MID, RING, TILE, RAGGED };  // (numbered as ccq_dense_linear_kernel returns them)
 
 struct Plan {
   Kind kind;
@@ -1412,6 +1412,24 @@ using namespace ccq;
 
 extern "C" size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args) {
   return workspace_of("ccq_dense_linear", args, false);
+}
+
+extern "C" int ccq_dense_linear_kernel(const ccq_dense_args* args, int grouped, int* tile_rows, int* tile_cols, int* splits,
+                                       int* copies) {
+  const char* what = grouped ? "ccq_dense_linear_grouped" : "ccq_dense_linear";
+  Plan q = {};
+  int kernel = -1, copied = 0;
+  if (args != nullptr && args->M >= 1 && check_dense(what, *args, grouped != 0) == 0) {
+    const DenseP p = make_params(*args, grouped != 0);
+    q = plan_of(*args, p);
+    const Scratch s = scratch_of(*args, p, q);
+    kernel = q.kind, copied = (s.x ? 1 : 0) | (s.w ? 2 : 0);
+  }
+  if (tile_rows) *tile_rows = q.bm;
+  if (tile_cols) *tile_cols = q.bn;
+  if (splits) *splits = q.splits;
+  if (copies) *copies = copied;
+  return kernel;
 }
 
 extern "C" int ccq_dense_linear(const ccq_dense_args* args) { return run_dense("ccq_dense_linear", args, false); }

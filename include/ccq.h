@@ -825,6 +825,15 @@ typedef struct ccq_dense_args {
 size_t ccq_dense_linear_workspace_size(const ccq_dense_args* args);
 size_t ccq_dense_linear_grouped_workspace_size(const ccq_dense_args* args);
 
+/* The kernel that ccq_dense_linear (grouped != 0: ccq_dense_linear_grouped) runs
+ * for these arguments (for tests and profiles): 0 16 rows with K split over a
+ * workgroup's waves, 1 tiles of 32 rows, 2 smaller and 3 larger tiles, 4 tiles of
+ * rows at any alignment; -1 for arguments it refuses, and for no rows.  tile_rows,
+ * tile_cols, splits and copies (may be NULL): a workgroup's rows and columns of w, the
+ * workgroups that share K, and what is copied to aligned rows first (1 x, 2 w, 3 both). */
+int ccq_dense_linear_kernel(const ccq_dense_args* args, int grouped, int* tile_rows, int* tile_cols,
+                            int* splits, int* copies);
+
 /* z = x w^T + bias; y = act(z) + residual, gated: y = act(z[:, :N]) * z[:, N:] +
  * residual; products, sums and the epilogue in float32, y rounded once. */
 int ccq_dense_linear(const ccq_dense_args* args);

@@ -1,0 +1,155 @@
+"""``quant.dense.linear`` and ``linear_grouped`` on each of their kernels, tiles,
+splits of K and aligned copies: sizes for each, the rule's choice (host code: no
+GPU is needed), and the products on the GPU.
+
+The products are of small whole numbers, so every sum in float32 is exact in any
+order and the results have to be equal: one term lost or taken twice shows,
+however long K is.  With |x|, |w| <= 2 sums stay within 4 K < 2^24."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+FEW, MID, RING, TILE, RAGGED = range(5)
+X, W, BOTH = 1, 2, 3  # what is copied to aligned rows
+
+
+def _route(lib, M, K, rows, gated=False, E=0, dx=0, dw=0, pad=0):
+    """(kernel, rows and columns of a workgroup, splits, copies) of ``rows`` rows of w, x and w ``dx`` and ``dw``
+    elements behind a 256-byte boundary, x's rows ``pad`` elements apart."""
+    from ccut._lib import DENSE_ARGS
+
+    N = rows // 2 if gated else rows
+    got = [ctypes.c_int() for _ in range(4)]
+    args = DENSE_ARGS.pack(256 + 2 * dx, 256 + 2 * dw, 0, 0, 256, 256, 0, 0, 0, K + pad, N, N, M, K, N, E, 2, 0, 2, 0, gated)
+    kernel = lib.ccq_dense_linear_kernel(args, E > 0, *map(ctypes.byref, got))
+    return kernel, *(v.value for v in got)
+
+
+def _whole(g, shape, largest=2):
+    return torch.randint(-largest, largest + 1, shape, generator=g)
+
+
+def _amid_nan(t, gpu, dt, shift=0, pad=0):
+    """``t [rows, width]`` on the GPU, ``shift`` elements into a buffer of NaN, its rows ``pad`` elements apart."""
+    rows, width = t.shape
+    buf = torch.full((rows * (width + pad) + shift + 64,), float("nan"), dtype=dt, device=gpu)
+    return buf[shift:shift + rows * (width + pad)].view(rows, width + pad)[:, :width].copy_(t)
+
+
+def _finish(z, bias, N, gated, act, residual):
+    z = z.double()
+    if bias is not None:
+        z = z + bias
+    g = z[:, :N].clamp_min(0) if act == "relu" else z[:, :N]
+    if gated:
+        g = g * z[:, N:]
+    if residual is not None:
+        g = g + residual
+    assert g.abs().max() < 2 ** 24  # exact in float32
+    return g
+
+
+def _check(gpu, M, K, rows, gated, dt, ydt, act=None, bias=False, residual=False, E=0, dx=0, dw=0, pad=0):
+    from ccut.quant import dense
+
+    g = torch.Generator().manual_seed(M * 31 + K * 7 + rows + gated)
+    N = rows // 2 if gated else rows
+    rows = 2 * N if gated else N
+    L = max(E, 1)
+    x, w = _whole(g, (M, K)).float(), _whole(g, (L, rows, K)).float()
+    b = _whole(g, (L, rows), 5) if bias else None
+    r = _whole(g, (M, N), 9) if residual else None
+    xd = _amid_nan(x, gpu, dt, dx, pad)
+    wd = _amid_nan(w.view(L * rows, K), gpu, dt, dw).view(L, rows, K)
+    bd = b.float().to(gpu) if bias else None
+    want = torch.zeros((M, N), dtype=torch.float64)
+    if E:
+        # uneven groups, empty ones, rows of no expert behind them (NaN: they do not count)
+        cuts = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(0, M - 50, (E,), generator=g).sort().values])
+        cuts[E // 2] = cuts[E // 2 + 1]
+        for e in range(E):
+            n, m = int(cuts[e]), int(cuts[e + 1])
+            if n < m:
+                want[n:m] = _finish(x[n:m] @ w[e].t(), b[e] if bias else None, N, gated, act, None)
+        xd[int(cuts[E]):] = float("nan")
+        y = dense.linear_grouped(xd, cuts.to(torch.int32).to(gpu), wd, bd, act=act, gated=gated, out_dtype=ydt)
+    else:
+        want = _finish(x @ w[0].t(), b[0] if bias else None, N, gated, act, r)
+        y = dense.linear(xd, wd[0], bd[0] if bias else None, act=act, gated=gated,
+                         residual=r.to(ydt).to(gpu) if residual else None, out_dtype=ydt)
+    want = want.float().to(ydt)
+    same = y.cpu() == want
+    assert same.all(), f"{(~same).sum()} of {same.numel()} differ, the first at {(~same).nonzero()[0].tolist()}"
+
+
+# ---- rows at any alignment: products large enough to copy x, w or both to aligned rows first
+COPIED = [
+    (2100, 257, 1700, 0, {}, (RING, 128, 128, 1, BOTH)), (2000, 520, 1900, 0, dict(dx=1), (RING, 128, 128, 1, X)),
+    (2000, 520, 1900, 0, dict(dw=3), (RING, 128, 128, 1, W)), (2000, 520, 1900, 0, dict(pad=3), (RING, 128, 128, 1, X)),
+    (1500, 1032, 2000, 0, dict(dx=5, dw=2), (RING, 128, 128, 1, BOTH)), (2600, 1416, 2200, 0, dict(dw=1), (RING, 256, 128, 1, W)),
+    (700, 2049, 1500, 0, dict(dx=1, dw=1), (RING, 64, 64, 1, BOTH)),
+    (4000, 515, 700, 2, {}, (RING, 128, 128, 1, BOTH)), (4000, 520, 700, 2, dict(dx=3), (RING, 128, 128, 1, X)),
+    (4000, 520, 700, 2, dict(dw=1), (RING, 128, 128, 1, W)), (2500, 1030, 900, 3, dict(pad=5), (RING, 128, 128, 1, BOTH)),
+    (6628, 657, 1736, 5, dict(dx=1, dw=1), (TILE, 256, 256, 1, BOTH)),
+]
+
+
+@pytest.fixture(scope="module")
+def lib(built_lib):
+    from ccut import _lib
+
+    return _lib.lib()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,E,at,route", COPIED)
+def test_choice_copied(lib, M, K, rows, E, at, route, gated):
+    assert _route(lib, M, K, rows, gated, E, **at) == route
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,E,at,route", COPIED)
+def test_copied(gpu, M, K, rows, E, at, route, gated):
+    _check(gpu, M, K, rows, gated, F16 if gated else BF, F32 if gated else BF, "relu" if gated else None, bias=True,
+           residual=not E, E=E, **at)
+
+
+@pytest.mark.gpu
+def test_copies_in_graphs(gpu):
+    """Two captured calls whose scratch holds the aligned copies, a batch's and experts': replays with eager calls
+    between them against these."""
+    from ccut.quant import dense
+
+    g = torch.Generator().manual_seed(2)
+    offsets = torch.tensor([0, 2900, 3950], dtype=torch.int32, device=gpu)
+    state = []
+    for M, K, rows, E in ((2100, 257, 1700, 0), (4000, 515, 700, 2)):
+        x = _whole(g, (M, K)).to(BF).to(gpu)
+        w = _whole(g, (E, rows, K) if E else (rows, K)).to(BF).to(gpu)
+        call = (lambda x=x, w=w: dense.linear_grouped(x, offsets, w)) if E else (lambda x=x, w=w: dense.linear(x, w))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+        state.append((graph, y, call, x))
+    for _ in range(4):
+        want = []
+        for _, y, call, x in state:
+            x.copy_(_whole(g, x.shape))
+            want.append(call())
+            y.fill_(float("nan"))
+        for graph, *_ in state:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, y, _, _), ref in zip(state, want):
+            assert torch.equal(y, ref)
