@@ -153,3 +153,35 @@ def test_copies_in_graphs(gpu):
         torch.cuda.synchronize()
         for (_, y, _, _), ref in zip(state, want):
             assert torch.equal(y, ref)
+
+
+# ---- tiles whose ring of stages goes round several times: K of ten stages or more, the last one whole or cut short,
+# and (groups) experts of uneven rows, so that waves behind a short tile's end only copy.  The second route is the
+# gated product's, where another one is taken.
+WIDE = (TILE, 256, 224, 1, 0), (TILE, 256, 256, 1, 0)
+TILED = [
+    (513, 640, 12416, 0, [(TILE, 128, 128, 1, 0)]), (513, 712, 12410, 0, [(TILE, 128, 128, 1, 0)]),
+    (530, 648, 14300, 0, [(TILE, 256, 192, 1, 0)]), (900, 2048, 9000, 0, [(TILE, 256, 192, 1, 0)]),
+    (900, 648, 12416, 0, WIDE), (777, 712, 14200, 0, WIDE), (2050, 640, 6272, 0, WIDE), (40, 712, 9000, 0, [(RING, 64, 64, 1, 0)]),
+    (1000, 648, 2050, 0, [(RING, 128, 128, 1, 0)]), (600, 1288, 9000, 0, [(RING, 256, 128, 1, 0)]),
+    (60, 1288, 8100, 0, [(MID, 32, 64, 1, 0)]),
+    (300, 712, 450, 128, [(TILE, 128, 128, 1, 0)]), (3000, 712, 1468, 12, [(TILE, 128, 128, 1, 0)]),
+    (4403, 712, 1052, 40, [(TILE, 256, 192, 1, 0)]), (4403, 640, 1052, 40, [(TILE, 256, 192, 1, 0)]),
+    (4286, 712, 1468, 40, [(TILE, 256, 256, 1, 0)]), (2500, 648, 1468, 40, [(TILE, 256, 256, 1, 0)]),
+    (4134, 712, 258, 70, [(RING, 128, 128, 1, 0)]), (2500, 1288, 1468, 8, [(RING, 128, 128, 1, 0)]),
+    (1746, 712, 130, 70, [(RING, 64, 64, 1, 0)]), (1000, 648, 130, 70, [(MID, 32, 64, 1, 0)]),
+]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,E,routes", TILED)
+def test_choice_tiled(lib, M, K, rows, E, routes, gated):
+    assert _route(lib, M, K, rows, gated, E) == routes[-1 if gated else 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ydt", [BF, F32])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,E,routes", TILED)
+def test_tiled(gpu, M, K, rows, E, routes, gated, ydt):
+    _check(gpu, M, K, rows, gated, BF, ydt, "relu" if gated else None, bias=True, residual=not E, E=E)
