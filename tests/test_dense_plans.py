@@ -185,3 +185,28 @@ def test_choice_tiled(lib, M, K, rows, E, routes, gated):
 @pytest.mark.parametrize("M,K,rows,E,routes", TILED)
 def test_tiled(gpu, M, K, rows, E, routes, gated, ydt):
     _check(gpu, M, K, rows, gated, BF, ydt, "relu" if gated else None, bias=True, residual=not E, E=E)
+
+
+# ---- K shared by several workgroups, its parts whole and cut short
+SPLIT = [
+    (64, 4096, 4096, {}, (RING, 64, 64, 4, 0)), (64, 4104, 4100, {}, (RING, 64, 64, 6, 0)),
+    (40, 14336, 4096, {}, (RING, 64, 64, 8, 0)), (128, 4104, 4100, {}, (RING, 128, 128, 5, 0)),
+    (172, 4096, 4096, {}, (RING, 128, 128, 4, 0)), (300, 7176, 2050, {}, (RING, 128, 128, 5, 0)),
+    (400, 14336, 1024, {}, (RING, 128, 128, 8, 0)), (172, 7176, 9000, {}, (RING, 256, 128, 3, 0)),
+    (90, 14336, 12416, {}, (TILE, 128, 128, 5, 0)), (20, 14336, 256, {}, (MID, 32, 64, 16, 0)),
+    (50, 14329, 520, dict(dx=1), (RAGGED, 64, 64, 16, 0)), (172, 10001, 1024, dict(dw=1, pad=2), (RAGGED, 64, 64, 10, 0)),
+]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,at,route", SPLIT)
+def test_choice_split(lib, M, K, rows, at, route, gated):
+    assert _route(lib, M, K, rows, gated, **at) == route
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ydt", [BF, F32])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,rows,at,route", SPLIT)
+def test_split(gpu, M, K, rows, at, route, gated, ydt):
+    _check(gpu, M, K, rows, gated, F16, ydt, "relu" if gated else None, bias=True, residual=True, **at)
