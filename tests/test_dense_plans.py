@@ -31,7 +31,7 @@ def _route(lib, M, K, rows, gated=False, E=0, dx=0, dw=0, pad=0):
 
 
 def _whole(g, shape, largest=2):
-    return torch.randint(-largest, largest + 1, shape, generator=g)
+    return torch.randint(-largest, largest + 1, shape, generator=g, dtype=torch.int8)
 
 
 def _amid_nan(t, gpu, dt, shift=0, pad=0):
@@ -210,3 +210,48 @@ def test_choice_split(lib, M, K, rows, at, route, gated):
 @pytest.mark.parametrize("M,K,rows,at,route", SPLIT)
 def test_split(gpu, M, K, rows, at, route, gated, ydt):
     _check(gpu, M, K, rows, gated, F16, ydt, "relu" if gated else None, bias=True, residual=True, **at)
+
+
+# ---- up to 16 rows: 16, 32 and 64 columns a workgroup, rows in whole eights, at dwords and at odd elements, K of less
+# than one step of the waves, of whole steps and cut short (a step is 256 columns, of 64 columns a workgroup 128; four
+# and two waves take steps in turn)
+COLUMNS = [(70, 0, 16), (5200, 0, 32), (10300, 0, 64), (72, 3, 16), (2000, 3, 32), (4100, 3, 64)]
+
+
+@pytest.mark.parametrize("rows,E,columns", COLUMNS)
+def test_choice_few(lib, rows, E, columns):
+    for K in (257, 1030, 4999, 2056):
+        if E and K % 8 == 0 and rows > 2000:  # (aligned groups of that many tiles take others)
+            continue
+        assert _route(lib, 13, K, rows, False, E) == (FEW, 16, columns, 1, 0)
+        assert _route(lib, 13, K, rows, True, E) == (FEW, 16, max(columns, 32), 1, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [257, 1024, 1030, 2049, 2056, 4999])
+@pytest.mark.parametrize("rows,E,columns", COLUMNS)
+def test_few(gpu, rows, E, columns, K):
+    for i, (dx, dw, pad) in enumerate(((0, 0, 0), (1, 0, 0), (0, 1, 2), (3, 1, 1), (2, 2, 2))):
+        for gated in (False, True):
+            if E:
+                _check_few_groups(gpu, K, rows, gated, E, dx, dw, pad)
+            else:
+                _check(gpu, (1, 5, 16)[i % 3], K, rows, gated, BF, (BF, F32)[i % 2], "relu" if gated else None,
+                       bias=True, residual=i != 1, dx=dx, dw=dw, pad=pad)
+
+
+def _check_few_groups(gpu, K, rows, gated, E, dx, dw, pad):
+    """13 rows: nine and two of the outer experts', two of none."""
+    from ccut.quant import dense
+
+    g = torch.Generator().manual_seed(K + rows + gated)
+    N = rows // 2 if gated else rows
+    x, w, b = _whole(g, (13, K)).float(), _whole(g, (E, rows, K)).float(), _whole(g, (E, rows), 5)
+    offsets = torch.tensor([0, 9] + [9] * (E - 2) + [11], dtype=torch.int32)
+    want = torch.zeros((13, N), dtype=torch.float64)
+    for e, n, m in ((0, 0, 9), (E - 1, 9, 11)):
+        want[n:m] = _finish(x[n:m] @ w[e].t(), b[e], N, gated, "relu", None)
+    xd, wd = _amid_nan(x, gpu, F16, dx, pad), _amid_nan(w.view(E * rows, K), gpu, F16, dw).view(E, rows, K)
+    xd[11:] = float("nan")
+    y = dense.linear_grouped(xd, offsets.to(gpu), wd, b.float().to(gpu), act="relu", gated=gated, out_dtype=F32)
+    assert torch.equal(y.cpu(), want.float())
