@@ -1259,6 +1259,14 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
   return q;
 }
 
+// tiles of a product: of groups as many as any offsets can make
+int64_t col_tiles(const DenseP& p, const Plan& q) { return cdiv(p.N, p.gated ? q.bn / 2 : q.bn); }
+int64_t row_tiles(const DenseP& p, const Plan& q) {
+  return p.offsets == nullptr ? cdiv(p.M, q.bm) : imin64(p.M, p.E + 1) + p.M / q.bm;
+}
+int64_t workgroups(const DenseP& p, const Plan& q) { return row_tiles(p, q) * col_tiles(p, q) * q.splits; }
+constexpr int64_t DN_MAX_TILES = 1 << 22;  // (of 512 threads, so that a launch stays below 2^32 of them)
+
 template <int DT, int NF, int U, int WAVES>
 void launch_few(const DenseP& p, dim3 grid, hipStream_t st) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w);
@@ -1272,14 +1280,11 @@ void launch_few(const DenseP& p, dim3 grid, hipStream_t st) {
 
 template <int DT>
 int launch_dense(DenseP p, const Plan& q, hipStream_t st, const char* what) {
-  const int columns = p.gated ? q.bn / 2 : q.bn;
-  p.ntiles = (int)cdiv(p.N, columns);
-  p.mtiles = (int)(p.offsets == nullptr ? cdiv(p.M, q.bm) : imin64(p.M, p.E + 1) + p.M / q.bm);
+  p.ntiles = (int)col_tiles(p, q);
+  p.mtiles = (int)row_tiles(p, q);
   p.splits = q.splits;
   p.kchunk = q.splits > 1 ? q.kchunk : p.K;
-  const int64_t groups = (int64_t)p.mtiles * p.ntiles * q.splits;
-  CCQ_REQUIRE(groups < 1 << 22, "%s: %lld tiles, too many for one launch", what, (long long)groups);
-  const dim3 grid((uint32_t)groups);
+  const dim3 grid((uint32_t)workgroups(p, q));
   if (q.kind == FEW) {
     if (q.bn == 16) launch_few<DT, 1, 4, 8>(p, grid, st);
     else if (q.bn == 32) launch_few<DT, 2, 4, 8>(p, grid, st);
@@ -1366,7 +1371,9 @@ Scratch scratch_of(const ccq_dense_args& a, const DenseP& p, const Plan& q) {
 size_t workspace_of(const char* what, const ccq_dense_args* args, bool grouped) {
   if (args == nullptr || args->M < 1 || check_dense(what, *args, grouped)) return 0;
   const DenseP p = make_params(*args, grouped);
-  const Scratch s = scratch_of(*args, p, plan_of(*args, p));
+  const Plan q = plan_of(*args, p);
+  if (workgroups(p, q) >= DN_MAX_TILES) return 0;
+  const Scratch s = scratch_of(*args, p, q);
   return s.part + s.x + s.w;
 }
 
@@ -1377,6 +1384,8 @@ int run_dense(const char* what, const ccq_dense_args* args, bool grouped) {
   if (a.M == 0) return 0;
   DenseP p = make_params(a, grouped);
   const Plan q = plan_of(a, p);
+  CCQ_REQUIRE(workgroups(p, q) < DN_MAX_TILES, "%s: M=%lld, N=%lld in %lld tiles, fewer than 2^22 tiles fit a launch", what,
+              (long long)a.M, (long long)a.N, (long long)workgroups(p, q));
   const Scratch s = scratch_of(a, p, q);
   const size_t need = s.part + s.x + s.w;
   CCQ_REQUIRE(need == 0 || (a.workspace != nullptr && aligned(a.workspace, 16) && a.workspace_bytes >= need),
@@ -1421,9 +1430,11 @@ extern "C" int ccq_dense_linear_kernel(const ccq_dense_args* args, int grouped, 
   int kernel = -1, copied = 0;
   if (args != nullptr && args->M >= 1 && check_dense(what, *args, grouped != 0) == 0) {
     const DenseP p = make_params(*args, grouped != 0);
-    q = plan_of(*args, p);
-    const Scratch s = scratch_of(*args, p, q);
-    kernel = q.kind, copied = (s.x ? 1 : 0) | (s.w ? 2 : 0);
+    const Plan plan = plan_of(*args, p);
+    if (workgroups(p, plan) < DN_MAX_TILES) {
+      const Scratch s = scratch_of(*args, p, plan);
+      q = plan, kernel = q.kind, copied = (s.x ? 1 : 0) | (s.w ? 2 : 0);
+    }
   }
   if (tile_rows) *tile_rows = q.bm;
   if (tile_cols) *tile_cols = q.bn;

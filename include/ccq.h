@@ -802,7 +802,9 @@ int ccq_moe_unpermute_grad(const ccq_moe_permute_args* args);
  * y_dtype; row strides ldx, ldr, ldy in elements, w dense, any element alignment.
  * Grouped: w [num_experts, W, K], bias [num_experts, W], offsets
  * [num_experts + 1].  residual may be y; y must not overlap x, w, bias, offsets or
- * another view of residual.  M, K, N <= 2^20, num_experts <= 1024. */
+ * another view of residual.  M, K, N <= 2^20, num_experts <= 1024, and fewer than
+ * 2^22 tiles (of 16 to 256 rows, an expert's last one counted whole, by 64 to 256 rows
+ * of w, fewer where w has under 10240): larger products are refused. */
 typedef struct ccq_dense_args {
   const void* x;
   const void* w;

@@ -107,3 +107,19 @@ def test_layer_refuses_other_types_of_y(monkeypatch, out_dtype, shared):
         moe.moe_ffn_dense(x, None, None, ex, out_dtype, shared=shared)
     for ok in (None, F32, F16, BF):
         assert moe.moe_ffn_dense(x, None, None, ex, ok, shared="rows").dtype == (ok or BF)
+
+
+@pytest.mark.parametrize("grouped,size", [
+    (True, dict(M=16384, K=8, N=1 << 20, ldx=8, num_experts=1024)), (True, dict(M=25600, K=9, N=1 << 20, ldx=9, num_experts=128)),
+    (False, dict(M=1 << 20, K=8, N=1 << 20, ldx=8)), (False, dict(M=1 << 20, K=9, N=1 << 20, ldx=9)),
+])
+def test_products_of_too_many_tiles_are_refused_before_any_launch(built_lib, grouped, size):
+    """Also those whose rows would be copied to aligned ones first."""
+    from ccut._lib import CCQ_EINVAL, DENSE_ARGS, last_error, lib
+
+    a = dict(ldy=1 << 20, num_experts=0, ldr=0) | size
+    tail = (a["ldx"], a["ldr"], a["ldy"], a["M"], a["K"], a["N"], a["num_experts"], 2, 0, 2, 0, 0)
+    args = DENSE_ARGS.pack(256, 256, 0, 0, 256, 256, 256, 0, 1 << 50, *tail)
+    run = lib().ccq_dense_linear_grouped if grouped else lib().ccq_dense_linear
+    assert run(args) == CCQ_EINVAL and "2^22 tiles" in last_error()
+    assert lib().ccq_dense_linear_kernel(args, grouped, None, None, None, None) == -1
