@@ -650,10 +650,11 @@ __device__ __forceinline__ void dn_write(const DenseP& p, const DnPlace& w, int 
 // (64 of them at once fill the address unit and hold up the waves that issue
 // them): w of the stage after the next follows the barrier, its x, into the ring's
 // fifth unit, the first half of the next stage, so x is two stages ahead.
-// 256 x 256, 4096 x 14336 x 4096: 327 us, 1470 TFLOP/s; the matrix unit is busy in
-// 76 % of the cycles, at 1.75 GHz of 2.4: power bounds it.  (Two whole stages, the
-// copies at once: 423 us; spread: 344; 32x32x16 products: 347 us, fewer cycles at
-// a lower clock.)
+// 256 x 256, 4096 x 14336 x 4096: 327 to 332 us, 1470 TFLOP/s; the matrix unit is
+// busy in 76 % of the cycles, and the clock falls to 1.75 GHz of 2.4 under this load.
+// That is no limit of the card: a library's plain product of these sizes takes 294 to
+// 308 us, for a reason that the counters do not name.  (Two whole stages, the copies at
+// once: 423 us; spread: 344; 32x32x16 products: 347 us, fewer cycles at a lower clock.)
 template <int DT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
@@ -1012,9 +1013,10 @@ __global__ __launch_bounds__(256) void dense_mid_kernel(const DenseP p) {
 }
 
 // The same product for rows at any alignment: stages pass through registers, four of
-// them on their way there, into two in LDS.  Unaligned loads of 16 bytes cost a third
-// (K=2747 for 2752: 39 and 28 us at M=1274 N=1520), the registers the rest (RING 64: 20);
-// tiles of 128 are no faster (58).
+// them on their way there, into two in LDS.  Its loads are of 16 bytes at any element
+// (dense_few_kernel's dwords were not tried here): they cost a third (K=2747 for 2752: 38
+// and 28 us at M=1274 N=1520), the registers the rest (RING 64: 20); tiles of 128 are no
+// faster (58).
 template <int DT>
 __global__ __launch_bounds__(256) void dense_ragged_kernel(const DenseP p) {
   using Vec = typename DnVec<DT>::type;
@@ -1234,8 +1236,10 @@ Plan make_plan(const DenseP& p, int64_t rows, bool dma, bool can_pad) {
     return q;
   }
   if (rows <= 16) {
-    // as many columns a workgroup as leave one for every second CU (M=1: K=2048 N=5632 16 columns 8.0 us, 32 7.3, 64 11.0;
-    // K=4096 N=14336 32, 31, 25.6; K=N=4096 8.3, 11.5, 17.5); groups of rows bring as many workgroups as experts
+    // as many columns a workgroup as leave one for every second CU, where there are that many (M=1: K=2048 N=5632 16
+    // columns 8.0 us, 32 7.3, 64 11.0; K=4096 N=14336 32, 31, 25.6; K=N=4096 8.3, 11.5, 17.5); groups of rows bring as many
+    // workgroups as experts.  K is not split, so narrow outputs with long K leave CUs idle (M=16 K=14336 N=1024 27 us,
+    // M=17 on MID in 16 splits 12; K=7168 N=64 14 and 11)
     const int64_t sets = cdiv(p.W, 16) * (grouped ? std::min<int64_t>(p.M, p.E) : 1);
     q.bn = sets >= 640 ? 64 : sets >= 320 || p.gated ? 32 : 16;
     return q;
